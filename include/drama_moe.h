@@ -361,6 +361,43 @@ int dr_gemv_q8_bf16s(const int8_t* w, const dr_bf16* s, const float* x, const fl
                      int k, const float* nw, float eps, dr_stream_t st);
 
 /* ===================================================================================== */
+/* Around the blocks, for one row or many -- no reference counterpart                      */
+/* ===================================================================================== */
+
+/* gate_mode of the block norms */
+#define DR_GATE_NONE 0
+#define DR_GATE_ROW 1  /* gate f32 [rows]: one logit per row */
+#define DR_GATE_ELEM 2 /* gate f32 [rows, ldg]: one logit per element */
+
+/* The norms behind a block and before the next one, with the gate and the residual scale, per row:
+ *   n  = b * rsqrt(mean(b^2) + eps) * pw           (pw NULL: n = b)
+ *   xo = xscale * x + bscale * cs * sigmoid(gate) * n
+ *   hn = bf16(xo * rsqrt(mean(xo^2) + eps) * nw)
+ * b: the block's output, f32 (dr_block_norm) or bf16 (dr_block_norm_bf16); NULL: there is none, xo =
+ * xscale * x (the norm before the first block).  x f32: the residual stream; NULL: none.  pw, cs, nw
+ * f32 [h]; cs NULL: 1.  xo f32 and hn bf16: either may be NULL.  Row r of b, x, gate (DR_GATE_ELEM),
+ * xo, hn starts r * ldb, ldx, ldg, ldo, ldh elements in; columns past h are neither read nor written.
+ * xo may be x or b, and hn the bf16 b, at the same stride.  Sums, norms and the gate are fp32.  16-byte
+ * addresses and strides of whole 16 bytes (8 for bf16) take the wide path; any others work.
+ * Unsupported: h < 1, h > 16384, rows < 0, a stride below h, an unknown gate_mode or one without gate,
+ * hn without nw, neither xo nor hn, neither b nor x -> -1.  rows == 0 does nothing. */
+int dr_block_norm(const float* b, int ldb, const float* x, int ldx, const float* pw, const float* gate, int gate_mode,
+                  int ldg, const float* cs, float bscale, float xscale, const float* nw, float eps, float* xo, int ldo,
+                  dr_bf16* hn, int ldh, int rows, int h, dr_stream_t st);
+int dr_block_norm_bf16(const dr_bf16* b, int ldb, const float* x, int ldx, const float* pw, const float* gate,
+                       int gate_mode, int ldg, const float* cs, float bscale, float xscale, const float* nw, float eps,
+                       float* xo, int ldo, dr_bf16* hn, int ldh, int rows, int h, dr_stream_t st);
+/* The same with b the output of a prefill's MoE layer, summed here instead of by dr_moe_combine:
+ * b[r] = sigmoid(sgate[r]) * shared[r] + sum_k wts[r, k] * y[slot_of[r, k]] (k ascending), y, slot_of, wts,
+ * sgate and shared as there (rows of h elements); shared NULL: none (sgate is then not read).  xo and hn
+ * must not overlap y or shared.  Also unsupported: topk < 1 or > 32, a missing y, slot_of or wts, shared
+ * without sgate -> -1. */
+int dr_moe_combine_norm(const float* y, const int* slot_of, const float* wts, const float* sgate, const float* shared,
+                        int topk, const float* x, int ldx, const float* pw, const float* gate, int gate_mode, int ldg,
+                        const float* cs, float bscale, float xscale, const float* nw, float eps, float* xo, int ldo,
+                        dr_bf16* hn, int ldh, int rows, int h, dr_stream_t st);
+
+/* ===================================================================================== */
 /* Fused multi-layer decode step (persistent kernel) -- no single reference symbol: it    */
 /* replaces the per-layer chain dr_router_topk + dr_moe_decode that src/engine.rs:1001-   */
 /* 1007 records for every MoE layer of a decode step (src/ffi.rs:41-46).                  */

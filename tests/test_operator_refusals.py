@@ -1,0 +1,47 @@
+"""Calls that the operators around and of the MoE block refuse with -1 before any launch (CPU: shapes are
+checked before any pointer is used)."""
+import ctypes
+
+import pytest
+
+import dramamoe as D
+
+P = 0x1000  # an aligned address that is never dereferenced
+
+
+def expect(name, base, cases):
+    f = D.lib().raw(name)
+    for change in cases:
+        args = list(base)
+        for pos, bad in change.items():
+            args[pos] = bad
+        assert f(*args) == -1, (name, change)
+
+
+# (x, ldx, pw, gate, gate_mode, ldg, cs, bscale, xscale, nw, eps, xo, ldo, hn, ldh, rows, h, st)
+NORM_TAIL = [P, 64, P, P, 2, 64, P, 1.0, 1.0, P, 1e-6, P, 64, P, 64, 2, 64, None]
+
+
+@pytest.mark.parametrize("name", ["dr_block_norm", "dr_block_norm_bf16"])
+def test_block_norm_refusals(name):
+    base = [P, 64] + NORM_TAIL
+    expect(name, base, [
+        {18: 0}, {18: 16385, 1: 20000, 3: 20000, 7: 20000, 14: 20000, 16: 20000}, {17: -1},
+        {1: 63}, {3: 63}, {7: 63}, {14: 63}, {16: 63}, {1: -64},
+        {6: 3}, {6: -1}, {5: None}, {5: None, 6: 1}, {11: None}, {13: None, 15: None}, {0: None, 2: None},
+    ])
+
+
+def test_block_norm_of_no_rows_does_nothing():
+    for name, head in (("dr_block_norm", [P, 64]), ("dr_block_norm_bf16", [P, 64]), ("dr_moe_combine_norm", [P, P, P, P, P, 8])):
+        args = head + NORM_TAIL
+        args[-3] = 0
+        assert D.lib().raw(name)(*args) == 0
+
+
+def test_combine_norm_refusals():
+    base = [P, P, P, P, P, 8] + NORM_TAIL
+    expect("dr_moe_combine_norm", base, [
+        {5: 0}, {5: 33}, {0: None}, {1: None}, {2: None}, {3: None}, {22: 0}, {22: 16385}, {21: -1}, {7: 63}, {18: 63},
+        {10: 7}, {15: None}, {17: None, 19: None},
+    ])
