@@ -397,6 +397,43 @@ int dr_moe_combine_norm(const float* y, const int* slot_of, const float* wts, co
                         const float* cs, float bscale, float xscale, const float* nw, float eps, float* xo, int ldo,
                         dr_bf16* hn, int ldh, int rows, int h, dr_stream_t st);
 
+/* A whole MoE layer for a few rows (1 <= rows <= 64) of any size: router, experts, shared expert and
+ * residual.  x bf16 [rows, h] is the normalised input (hn of dr_block_norm or dr_moe_combine_norm):
+ *   l = R x[r], idx[r] = the topk experts by (l desc, index asc), wts[r] their softmax weights
+ *   renormalised to sum 1, sgate[r] = l_E: the bits of dr_gemm followed by dr_moe_topk;
+ *   y[r] = res[r] + sigmoid(sgate[r]) * SD (silu(SG x) * (SU x)) + sum_k wts[r, k] * D_k (silu(G_k x) * (U_k x)).
+ * router bf16 [e + 1, h] (row e: the shared expert's gate; [e, h] without a shared expert); experts as
+ * dr_moe_decode, dr_moe_decode_bf16s, dr_moe_decode_fp8 and dr_moe_decode_fp8_bf16s; the four shared
+ * pointers all NULL: no shared expert (sgate is then not written and may be NULL).  Each expert is
+ * fetched once for all rows that picked it (up to 16 at a time).  x enters exactly, activations,
+ * sums and the combine are fp32.  res f32 [rows, h] may be NULL; y f32 [rows, h] may be res, and overlaps nothing else.
+ * ws: dr_moe_layer_rows_ws(rows, e, h, i, topk) bytes, its first 1024 zero before the first call and
+ * then owned by the library; it serves calls of any size it is large enough for.  Calls that share ws must
+ * not overlap (two graphs that may run at once need one each).
+ * Every pointer but idx, wts, sgate and the scales of the shared expert is a multiple of 16 bytes.
+ * Unsupported: rows < 1 or > 64, e > 256, topk < 1, > 32 or > e, h or i < 128, > 8192 or no multiple of
+ * 128, some but not all shared pointers, a missing or misaligned buffer -> -1 (ws size: 0). */
+size_t dr_moe_layer_rows_ws(int rows, int e, int h, int i, int topk);
+int dr_moe_layer_rows(const dr_bf16* router, const uint8_t* gu_q, const dr_half* gu_sm, const uint8_t* d_q,
+                      const dr_half* d_sm, const int8_t* sgu_q, const dr_half* sgu_s, const int8_t* sd_q,
+                      const dr_half* sd_s, const dr_bf16* x, const float* res, int* idx, float* wts, float* sgate,
+                      void* ws, float* y, int rows, int e, int h, int i, int topk, dr_stream_t st);
+int dr_moe_layer_rows_bf16s(const dr_bf16* router, const uint8_t* gu_q, const dr_bf16* gu_sm, const uint8_t* d_q,
+                            const dr_bf16* d_sm, const int8_t* sgu_q, const dr_bf16* sgu_s, const int8_t* sd_q,
+                            const dr_bf16* sd_s, const dr_bf16* x, const float* res, int* idx, float* wts,
+                            float* sgate, void* ws, float* y, int rows, int e, int h, int i, int topk,
+                            dr_stream_t st);
+int dr_moe_layer_rows_fp8(const dr_bf16* router, const uint8_t* gu_w, const float* gu_s, const uint8_t* d_w,
+                          const float* d_s, const int8_t* sgu_q, const dr_half* sgu_s, const int8_t* sd_q,
+                          const dr_half* sd_s, const dr_bf16* x, const float* res, int* idx, float* wts,
+                          float* sgate, void* ws, float* y, int rows, int e, int h, int i, int topk,
+                          dr_stream_t st);
+int dr_moe_layer_rows_fp8_bf16s(const dr_bf16* router, const uint8_t* gu_w, const dr_bf16* gu_s, const uint8_t* d_w,
+                                const dr_bf16* d_s, const int8_t* sgu_q, const dr_bf16* sgu_s, const int8_t* sd_q,
+                                const dr_bf16* sd_s, const dr_bf16* x, const float* res, int* idx, float* wts,
+                                float* sgate, void* ws, float* y, int rows, int e, int h, int i, int topk,
+                                dr_stream_t st);
+
 /* ===================================================================================== */
 /* Fused multi-layer decode step (persistent kernel) -- no single reference symbol: it    */
 /* replaces the per-layer chain dr_router_topk + dr_moe_decode that src/engine.rs:1001-   */

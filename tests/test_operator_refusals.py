@@ -45,3 +45,25 @@ def test_combine_norm_refusals():
         {5: 0}, {5: 33}, {0: None}, {1: None}, {2: None}, {3: None}, {22: 0}, {22: 16385}, {21: -1}, {7: 63}, {18: 63},
         {10: 7}, {15: None}, {17: None, 19: None},
     ])
+
+
+MOE = ["dr_moe_layer_rows", "dr_moe_layer_rows_bf16s", "dr_moe_layer_rows_fp8", "dr_moe_layer_rows_fp8_bf16s"]
+
+
+@pytest.mark.parametrize("name", MOE)
+def test_moe_layer_rows_refusals(name):
+    # router, gu_q, gu_s, d_q, d_s, sgu_q, sgu_s, sd_q, sd_s, x, res, idx, wts, sgate, ws, y, rows, e, h, i, topk, st
+    base = [P] * 16 + [4, 16, 2048, 512, 8, None]
+    bad = [{16: 0}, {16: 65}, {17: 0}, {17: 257}, {17: 7}, {18: 0}, {18: 2050}, {18: 64}, {18: 8320}, {19: 0}, {19: 500}, {19: 64},
+           {19: 8320}, {20: 0}, {20: 33, 17: 64}, {20: 17}]
+    bad += [{q: None} for q in (0, 1, 2, 3, 4, 9, 11, 12, 13, 14, 15)] + [{q: None} for q in (5, 6, 7, 8)]
+    bad += [{q: P + 8} for q in (0, 1, 2, 3, 4, 5, 7, 9, 10, 14, 15)]
+    expect(name, base, bad)
+
+
+def test_moe_layer_rows_ws():
+    f = D.lib().cdll.dr_moe_layer_rows_ws
+    assert f(1, 256, 2048, 512, 8) >= 1024 + 9 * (512 * 6 + 2048 * 4)
+    assert f(64, 256, 2048, 512, 8) > f(1, 256, 2048, 512, 8)
+    for bad in ((0, 256, 2048, 512, 8), (65, 256, 2048, 512, 8), (4, 256, 2050, 512, 8), (4, 4, 2048, 512, 8), (4, 256, 2048, 500, 8)):
+        assert f(*bad) == 0
