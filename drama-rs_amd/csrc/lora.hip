@@ -1,0 +1,185 @@
+// An int8 projection shared by all rows with each row's own low-rank adapter:
+//   y[r] = res[r] + W x[r] + s_a B_a (A_a x[r]),   a = adapter[r].
+//
+// Two launches.  k_lora_down: t[r] = s_a A_a x[r] (fp32), a block per 16 rows and distinct adapter among them, so
+// rows that share an adapter share its fetch whatever their order.  k_lora_gemm: W x on
+// v_mfma_f32_16x16x32_bf16 (int8 is exact in bf16, the scales enter the fp32 sums), with B_a t and the residual
+// added to each output before its one store.
+#include "common.hpp"
+
+using namespace drm;
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+DEV f32x4 mfma(const uint4& a, const uint4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+struct Lora {
+  const int8_t* w;
+  const uint16_t* s;
+  const uint16_t* x;
+  const int* adapter;
+  const uint16_t *la, *lb;
+  const int* rank;
+  const float* lscale;
+  const float* res;
+  float *t, *y;
+  size_t ldx, ldy;
+  int adapters, rmax, rows, n, k;
+};
+
+constexpr int LR_NW = 8, LR_NT = LR_NW * 64;
+
+// adapter of row r, -1 for none (an id outside 0 .. adapters - 1, an adapter without rank)
+DEV int adapter_of(const Lora& a, int r) {
+  if (!a.adapter || r >= a.rows) return -1;
+  const int v = a.adapter[r];
+  return v >= 0 && v < a.adapters && a.rank[v] > 0 ? v : -1;
+}
+DEV int rank_of(const Lora& a, int v) { return a.rank[v] < a.rmax ? a.rank[v] : a.rmax; }
+
+// ---- t = s_a A_a x --------------------------------------------------------------------------
+// Block: 16 rows (blockIdx.x), 16 ranks (blockIdx.z), the distinct adapters blockIdx.y, + gridDim.y, ... of
+// those rows.  The eight waves take 128 inputs each in turn.
+__global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
+  __shared__ f32x4 red[LR_NW][64];
+  const int lane = lane_id(), wave = wave_id(), c16 = lane & 15, g = lane >> 4;
+  const int r0 = blockIdx.x * 16, j0 = blockIdx.z * 16;
+  const int mine = adapter_of(a, r0 + c16);
+  // row c16 is the first of its adapter: no earlier row of the 16 has it
+  bool first = mine >= 0;
+#pragma unroll
+  for (int q = 0; q < 15; ++q) first = first && !(q < c16 && __builtin_amdgcn_readlane(mine, q) == mine);
+  uint32_t firsts = (uint32_t)__ballot(first) & 0xffffu;
+  for (int q = 0; q < (int)blockIdx.y && firsts; ++q) firsts &= firsts - 1;
+  while (firsts) {
+    const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctz(firsts));
+    for (int q = 0; q < (int)gridDim.y && firsts; ++q) firsts &= firsts - 1;
+    const int rk = rank_of(a, ad);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (j0 < rk) {
+      const uint16_t* xr = a.x + (size_t)(r0 + c16 < a.rows ? r0 + c16 : a.rows - 1) * a.ldx + 8 * g;
+      const uint16_t* ar = a.la + ((size_t)ad * a.rmax + (j0 + c16 < rk ? j0 + c16 : rk - 1)) * a.k + 8 * g;
+      for (int c = wave * 128; c < a.k; c += LR_NW * 128) {
+        uint4 xv[4], av[4];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) xv[f] = ld16(xr + c + 32 * f), av[f] = ld16(ar + c + 32 * f);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc = mfma(xv[f], av[f], acc);
+      }
+    }
+    __syncthreads();
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      const int l = threadIdx.x & 63, q = threadIdx.x >> 6, row = r0 + 4 * (l >> 4) + q, j = j0 + (l & 15);
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < LR_NW; ++w) v += red[w][l][q];
+      if (j < a.rmax && adapter_of(a, row) == ad) a.t[(size_t)row * a.rmax + j] = j < rk ? a.lscale[ad] * v : 0.f;
+    }
+  }
+}
+
+// ---- y = res + W x + B t -----------------------------------------------------------------------
+DEV uint32_t pk8(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
+  const float a = (float)(int8_t)(v >> (8 * i)), b = (float)(int8_t)(v >> (8 * i + 8));
+  return (__float_as_uint(b) & 0xffff0000u) | (__float_as_uint(a) >> 16);
+}
+DEV uint4 frag8(uint32_t a, uint32_t b) { return make_uint4(pk8(a, 0), pk8(a, 2), pk8(b, 0), pk8(b, 2)); }
+
+// Few rows: a block owns 16 columns and up to MT 16-row tiles; its eight waves take 128 inputs each in turn and
+// add their sums through LDS.  Column l % 16 of the weights in lane l, 16 inputs (16 (l / 16)) of each 64.
+template <class SH, int MT>
+__global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
+  __shared__ f32x4 red[LR_NW][MT][64];
+  const int lane = lane_id(), wave = wave_id(), c16 = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, r0 = blockIdx.y * 16 * MT;
+  const size_t n = n0 + c16 < a.n ? n0 + c16 : a.n - 1;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint8_t* wr = reinterpret_cast<const uint8_t*>(a.w) + n * a.k + 16 * g;
+  for (int c = wave * 128; c < a.k; c += LR_NW * 128) {
+    const uint4 w0 = ld16(wr + c), w1 = ld16(wr + c + 64);
+    const float sc = SH::scale(a.s, n, c, a.k);
+    const uint4 b0 = frag8(w0.x, w0.y), b1 = frag8(w0.z, w0.w), b2 = frag8(w1.x, w1.y), b3 = frag8(w1.z, w1.w);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = r0 + 16 * m + c16;
+      const uint16_t* xr = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + c + 16 * g;
+      f32x4 p = {0.f, 0.f, 0.f, 0.f};
+      p = mfma(ld16(xr), b0, p), p = mfma(ld16(xr + 8), b1, p);
+      p = mfma(ld16(xr + 64), b2, p), p = mfma(ld16(xr + 72), b3, p);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[m][q] = __builtin_fmaf(sc, p[q], acc[m][q]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) red[wave][m][lane] = acc[m];
+  __syncthreads();
+  for (int q = threadIdx.x; q < 256 * MT; q += LR_NT) {
+    const int l = q & 63, e = q >> 6 & 3, m = q >> 8, row = r0 + 16 * m + 4 * (l >> 4) + e, col = n0 + (l & 15);
+    if (row >= a.rows || col >= a.n) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LR_NW; ++w) v += red[w][m][l][e];
+    const int ad = adapter_of(a, row);
+    if (ad >= 0) {
+      const int rk = rank_of(a, ad);
+      const uint16_t* b = a.lb + ((size_t)ad * a.n + col) * a.rmax;
+      const float* t = a.t + (size_t)row * a.rmax;
+      float d = 0.f;
+      for (int j = 0; j < rk; ++j) d = __builtin_fmaf(bf16f(b[j]), t[j], d);
+      v += d;
+    }
+    float* o = a.y + row * a.ldy + col;
+    *o = a.res ? a.res[row * a.ldy + col] + v : v;
+  }
+}
+
+bool lora_shape_ok(int rows, int n, int k, int rmax) {
+  return rows >= 0 && rows <= (1 << 20) && n >= 1 && k >= 128 && k <= 16384 && k % 128 == 0 && rmax >= 8 && rmax <= 128 && rmax % 8 == 0;
+}
+
+template <class SH>
+int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
+  if (!lora_shape_ok(a.rows, a.n, a.k, a.rmax) || ldx < a.k || ldx % 8 || ldy < a.n || a.adapters < 0) return -1;
+  if (a.rows == 0) return 0;
+  if (!a.w || !a.s || !a.x || !a.y || ((uintptr_t)a.w & 15) || ((uintptr_t)a.x & 15)) return -1;
+  if (a.adapters == 0) a.adapter = nullptr;
+  if (a.adapter && (!a.la || !a.lb || !a.rank || !a.lscale || !a.t || ((uintptr_t)a.la & 15) || ((uintptr_t)a.lb & 15) || ((uintptr_t)a.t & 15)))
+    return -1;
+  a.ldx = ldx, a.ldy = ldy;
+  if (a.t) a.t += 64;  // the first 256 bytes of the workspace hold counters
+  const long long tiles = ((long long)a.rows + 15) / 16;
+  if (a.adapter)
+    hipLaunchKernelGGL(k_lora_down, dim3((unsigned)tiles, 16, (a.rmax + 15) / 16), dim3(LR_NT), 0, st, a);
+  const dim3 g((a.n + 15) / 16, (unsigned)((tiles + 3) / 4));
+  hipLaunchKernelGGL((k_lora_gemm_rows<SH, 4>), g, dim3(LR_NT), 0, st, a);
+  return 0;
+}
+
+}  // namespace
+
+API size_t dr_gemm_q8_lora_ws(int rows, int n, int k, int rmax) {
+  return lora_shape_ok(rows, n, k, rmax) ? (((size_t)rows * rmax * 4 + 255) & ~(size_t)255) + 256 : 0;
+}
+
+API int dr_gemm_q8_lora(const int8_t* w, const uint16_t* s, const uint16_t* x, int ldx, const int* adapter, const uint16_t* la,
+                        const uint16_t* lb, const int* rank, const float* lscale, int adapters, int rmax, void* ws,
+                        const float* res, float* y, int ldy, int rows, int n, int k, hipStream_t st) {
+  return gemm_lora<Q8G128F16>(Lora{w, s, x, adapter, la, lb, rank, lscale, res, static_cast<float*>(ws), y, 0, 0, adapters, rmax, rows, n, k},
+                              ldx, ldy, st);
+}
+
+API int dr_gemm_q8_lora_bf16s(const int8_t* w, const uint16_t* s, const uint16_t* x, int ldx, const int* adapter,
+                              const uint16_t* la, const uint16_t* lb, const int* rank, const float* lscale, int adapters, int rmax,
+                              void* ws, const float* res, float* y, int ldy, int rows, int n, int k, hipStream_t st) {
+  return gemm_lora<Q8RowBF16>(Lora{w, s, x, adapter, la, lb, rank, lscale, res, static_cast<float*>(ws), y, 0, 0, adapters, rmax, rows, n, k},
+                              ldx, ldy, st);
+}

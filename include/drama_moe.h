@@ -397,6 +397,28 @@ int dr_moe_combine_norm(const float* y, const int* slot_of, const float* wts, co
                         const float* cs, float bscale, float xscale, const float* nw, float eps, float* xo, int ldo,
                         dr_bf16* hn, int ldh, int rows, int h, dr_stream_t st);
 
+/* An int8 projection shared by all rows, each row with its own low-rank adapter:
+ *   y[r] = res[r] + W x[r] + lscale[a] * B_a (A_a x[r]),  a = adapter[r].
+ * w i8 [n, k] with scales as dr_gemv_q8 (f16 per 128 inputs) or, _bf16s, dr_gemv_q8_bf16s (bf16 per row); x bf16, row r
+ * at r * ldx; res and y f32, row r at r * ldy (res NULL: none; y may be res and overlaps nothing else).
+ * adapter i32 [rows] on the device: rows may come in any order; a row whose id lies outside 0 .. adapters - 1 or whose
+ * adapter has rank[a] < 1 has none; NULL: no row has one.  la bf16 [adapters, rmax, k] (A_a), lb bf16
+ * [adapters, n, rmax] (B_a), rank i32 [adapters] (above rmax: rmax), lscale f32 [adapters]; ranks past rank[a] are
+ * not read.  x, A, B and W enter exactly, A_a x and all sums are fp32.
+ * ws: dr_gemm_q8_lora_ws(rows, n, k, rmax) bytes of scratch, its first 256 zero before the first call and then owned by
+ * the library.  Calls that share ws must not overlap (two graphs that may run at once need one each).
+ * w, x, la, lb and ws are multiples of 16 bytes.  rows == 0 does nothing.
+ * Unsupported: rows < 0 or > 1048576, n < 1, k < 128, > 16384 or no multiple of 128, ldx < k or no multiple of 8,
+ * ldy < n, rmax < 8, > 128 or no multiple of 8 (without adapters too), adapters < 0, a missing or misaligned buffer -> -1 (ws size: 0). */
+size_t dr_gemm_q8_lora_ws(int rows, int n, int k, int rmax);
+int dr_gemm_q8_lora(const int8_t* w, const dr_half* s, const dr_bf16* x, int ldx, const int* adapter,
+                    const dr_bf16* la, const dr_bf16* lb, const int* rank, const float* lscale, int adapters, int rmax,
+                    void* ws, const float* res, float* y, int ldy, int rows, int n, int k, dr_stream_t st);
+int dr_gemm_q8_lora_bf16s(const int8_t* w, const dr_bf16* s, const dr_bf16* x, int ldx, const int* adapter,
+                          const dr_bf16* la, const dr_bf16* lb, const int* rank, const float* lscale, int adapters,
+                          int rmax, void* ws, const float* res, float* y, int ldy, int rows, int n, int k,
+                          dr_stream_t st);
+
 /* A whole MoE layer for a few rows (1 <= rows <= 64) of any size: router, experts, shared expert and
  * residual.  x bf16 [rows, h] is the normalised input (hn of dr_block_norm or dr_moe_combine_norm):
  *   l = R x[r], idx[r] = the topk experts by (l desc, index asc), wts[r] their softmax weights

@@ -67,3 +67,23 @@ def test_moe_layer_rows_ws():
     assert f(64, 256, 2048, 512, 8) > f(1, 256, 2048, 512, 8)
     for bad in ((0, 256, 2048, 512, 8), (65, 256, 2048, 512, 8), (4, 256, 2050, 512, 8), (4, 4, 2048, 512, 8), (4, 256, 2048, 500, 8)):
         assert f(*bad) == 0
+
+
+@pytest.mark.parametrize("name", ["dr_gemm_q8_lora", "dr_gemm_q8_lora_bf16s"])
+def test_gemm_q8_lora_refusals(name):
+    # w, s, x, ldx, adapter, la, lb, rank, lscale, adapters, rmax, ws, res, y, ldy, rows, n, k, st
+    base = [P, P, P, 256, P, P, P, P, P, 4, 16, P, P, P, 100, 3, 100, 256, None]
+    bad = [{15: -1}, {15: (1 << 20) + 1}, {16: 0}, {17: 0}, {17: 64}, {17: 200}, {17: 16512, 3: 16512}, {3: 248}, {3: 260}, {14: 99}, {10: 0},
+           {10: 12}, {10: 136}, {9: -1}]
+    bad += [{q: None} for q in (0, 1, 2, 5, 6, 7, 8, 11, 13)] + [{q: P + 8} for q in (0, 2, 5, 6, 11)]
+    expect(name, base, bad)
+    none = list(base)
+    none[15] = 0
+    assert D.lib().raw(name)(*none) == 0
+
+
+def test_gemm_q8_lora_ws():
+    f = D.lib().cdll.dr_gemm_q8_lora_ws
+    assert f(5, 100, 256, 16) >= 256 + 5 * 16 * 4
+    for bad in ((-1, 100, 256, 16), (5, 0, 256, 16), (5, 100, 200, 16), (5, 100, 256, 12)):
+        assert f(*bad) == 0
