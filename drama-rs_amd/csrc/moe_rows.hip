@@ -42,23 +42,31 @@ struct MoeRows {
 };
 
 // ---- weight formats --------------------------------------------------------------------------
-// One wave's part of a 16-row tile: 256 inputs of each row, lane l holding 16-byte pieces of row l % 16
-// (g = l / 16).  Fragment f of x (two for each group of 64 inputs) covers inputs 64 (f / 2) + xoff(g) + 8 (f % 2) .. + 8.
-// half: only the chunk's first 128 inputs exist.
+// One wave's part of a 16-row tile: 256 inputs of each row (chunk c), lane l holding 16-byte pieces of row
+// l % 16 (g = l / 16).  Fragment f of x (two for each group of 64 inputs) covers inputs 64 (f / 2) + xoff(g) + 8 (f % 2) .. + 8.
+// The loads go through buffer resources of one expert's matrix, so a piece past the row's inputs (half: only
+// the chunk's first 128 exist) and a tile that does not exist (off: nothing left to prefetch) read zeros without a
+// fetch, and the code in flight stays free of branches, which keeps the load counter exact.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+DEV Rsrc rsrc(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+constexpr uint32_t NOWHERE = 0x80000000u;  // past every matrix
+DEV uint4 buf16(const Rsrc& r, uint32_t off) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); }
 
 template <class SC>
 struct RowsQ4 {
   static constexpr bool perm = true;  // fragment order 0 4 1 5 2 6 3 7
-  uint4 w[2];
-  uint2 s[2];
+  static constexpr int cost = 1;      // relative bytes of a tile
+  uint4 w[2], s;
+  static DEV size_t q_bytes(int N, int K) { return (size_t)N * K / 2; }
+  static DEV size_t s_bytes(int N, int K) { return (size_t)N * K / 16; }
   static DEV int xoff(int g) { return 32 * (g & 1) + 16 * (g >> 1); }
-  DEV void load(const uint8_t* Q, const void* S, size_t expert, int n, int N, int K, int c, bool half) {
-    const size_t row = expert * N + n;
-    const uint8_t* p = Q + row * (K / 2) + c * 128 + 16 * (lane_id() >> 4);
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(S) + row * (K / 64) + c * 4;
-    w[0] = ld16(p), s[0] = ld8(q);
-    w[1] = make_uint4(0, 0, 0, 0), s[1] = make_uint2(0, 0);
-    if (!half) w[1] = ld16(p + 64), s[1] = ld8(q + 2);
+  DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
+    const uint32_t p = off ? NOWHERE : n * (K / 2) + c * 128 + 16 * (lane_id() >> 4);
+    w[0] = buf16(Q, p);
+    w[1] = buf16(Q, half ? NOWHERE : p + 64);
+    s = buf16(S, off ? NOWHERE : (n * (K / 64) + c * 4) * 4);
   }
   // nibbles of a word as 16 + q in bf16: the nibble is the top four mantissa bits of a number in [16, 32)
   static DEV uint4 frag(uint32_t v) {
@@ -67,9 +75,10 @@ struct RowsQ4 {
   }
   // xsum: lane's sum of x over group l / 16 of row l % 16
   template <int NP>
-  DEV void mac(const uint4 (&x)[NP][8], float xsum, f32x4& out) const {
+  DEV void mac(const uint4 (&x)[NP][8], float xsum, bool half, f32x4& out) const {
     const int g = lane_id() >> 4;
-    const uint32_t own = (g & 2) ? ((g & 1) ? s[1].y : s[1].x) : ((g & 1) ? s[0].y : s[0].x);
+    const uint32_t sw[4] = {s.x, s.y, half ? 0u : s.z, half ? 0u : s.w};
+    const uint32_t own = (g & 2) ? ((g & 1) ? sw[3] : sw[2]) : ((g & 1) ? sw[1] : sw[0]);
     const float2 o = SC::pair(own);
     out = __builtin_amdgcn_mfma_f32_16x16x4f32(xsum, o.y - 16.f * o.x, out, 0, 0, 0);
 #pragma unroll
@@ -83,7 +92,7 @@ struct RowsQ4 {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < NP; ++q) a = mfma(x[q][4 * p + 2 * h], b0, a), a = mfma(x[q][4 * p + 2 * h + 1], b1, a);
-        const float sc = SC::pair(h ? s[p].y : s[p].x).x;
+        const float sc = SC::pair(sw[2 * p + h]).x;
 #pragma unroll
         for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
       }
@@ -91,82 +100,72 @@ struct RowsQ4 {
   }
 };
 
-struct Rows8 {  // one byte per weight: 64 inputs of a row per 16-byte load of four lanes
+// One byte per weight: 64 inputs of a row per 16-byte load of four lanes, scales per 128 inputs.  D: the
+// format's conversions
+template <class D>
+struct Rows8 {
   static constexpr bool perm = false;
+  static constexpr int cost = 2;
   uint4 w[4];
-  float s[2];
+  uint32_t s[2];
+  static DEV size_t q_bytes(int N, int K) { return (size_t)N * K; }
   static DEV int xoff(int g) { return 16 * g; }
-  DEV void load_bytes(const uint8_t* row, int c, bool half) {
-    const uint8_t* p = row + c * 256 + 16 * (lane_id() >> 4);
-    w[0] = ld16(p), w[1] = ld16(p + 64);
-    w[2] = w[3] = make_uint4(0, 0, 0, 0);
-    if (!half) w[2] = ld16(p + 128), w[3] = ld16(p + 192);
-  }
-};
-
-template <int SF>
-struct RowsFP8 : Rows8 {
-  DEV void load(const uint8_t* Q, const void* S, size_t expert, int n, int N, int K, int c, bool half) {
-    load_bytes(Q + (expert * N + n) * (size_t)K, c, half);
-    const size_t b = (expert * (N / 128) + (n >> 7)) * (size_t)(K / 128) + 2 * c;
-    s[0] = blk_scale<SF>(S, b);
-    s[1] = half ? 0.f : blk_scale<SF>(S, b + 1);
-  }
-  static DEV uint4 frag(uint32_t a, uint32_t b) {
-    auto cv = [](uint32_t v, auto hi) {
-      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, decltype(hi)::value));
-    };
-    constexpr std::integral_constant<bool, false> lo{};
-    constexpr std::integral_constant<bool, true> hi{};
-    return make_uint4(cv(a, lo), cv(a, hi), cv(b, lo), cv(b, hi));
+  DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
+    const uint32_t p = off ? NOWHERE : n * K + c * 256 + 16 * (lane_id() >> 4);
+    w[0] = buf16(Q, p), w[1] = buf16(Q, off ? NOWHERE : p + 64);
+    w[2] = buf16(Q, half ? NOWHERE : p + 128), w[3] = buf16(Q, half ? NOWHERE : p + 192);
+    s[0] = D::scale_raw(S, n, 2 * c, K, off);
+    s[1] = D::scale_raw(S, n, 2 * c + 1, K, off || half);
   }
   template <int NP>
-  DEV void mac(const uint4 (&x)[NP][8], float, f32x4& out) const {
+  DEV void mac(const uint4 (&x)[NP][8], float, bool, f32x4& out) const {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint4& v = w[2 * p + h];
-        const uint4 b0 = frag(v.x, v.y), b1 = frag(v.z, v.w);
+        const uint4 b0 = D::frag(v.x, v.y), b1 = D::frag(v.z, v.w);
 #pragma unroll
         for (int q = 0; q < NP; ++q) a = mfma(x[q][4 * p + 2 * h], b0, a), a = mfma(x[q][4 * p + 2 * h + 1], b1, a);
       }
+      const float sc = D::scale_cvt(s[p]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(s[p], a[r], out[r]);
+      for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
     }
+  }
+};
+DEV uint32_t buf_half(const Rsrc& S, uint32_t off) { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(S, off, 0, 0); }
+
+template <int SF>
+struct RowsFP8 : Rows8<RowsFP8<SF>> {
+  static DEV size_t s_bytes(int N, int K) { return (size_t)(N / 128) * (K / 128) * (SF ? 2 : 4); }
+  static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
+    const uint32_t i = (n >> 7) * (K / 128) + b;
+    if constexpr (SF) return buf_half(S, off ? NOWHERE : 2 * i);
+    else return __builtin_amdgcn_raw_buffer_load_b32(S, off ? NOWHERE : 4 * i, 0, 0);
+  }
+  static DEV float scale_cvt(uint32_t r) { return blk_cvt<SF>(r); }
+  static DEV uint4 frag(uint32_t a, uint32_t b) {
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true)));
   }
 };
 
 template <class SH>
-struct RowsQ8 : Rows8 {
-  DEV void load(const uint8_t* Q, const void* S, size_t, int n, int, int K, int c, bool half) {
-    load_bytes(Q + (size_t)n * K, c, half);
-    const uint16_t* sp = reinterpret_cast<const uint16_t*>(S);
-    s[0] = SH::scale(sp, n, c * 256, K);
-    s[1] = half ? 0.f : SH::scale(sp, n, c * 256 + 128, K);
+struct RowsQ8 : Rows8<RowsQ8<SH>> {
+  static DEV size_t s_bytes(int N, int K) { return (size_t)N * (SH::per_row ? 1 : K / 128) * 2; }
+  static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
+    return buf_half(S, off ? NOWHERE : 2 * (SH::per_row ? n : n * (K / 128) + b));
   }
+  static DEV float scale_cvt(uint32_t r) { return SH::cvt(r); }
   static DEV uint32_t pk(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
     const float a = (float)(int8_t)(v >> (8 * i)), b = (float)(int8_t)(v >> (8 * i + 8));
     return (__float_as_uint(b) & 0xffff0000u) | (__float_as_uint(a) >> 16);
   }
   static DEV uint4 frag(uint32_t a, uint32_t b) { return make_uint4(pk(a, 0), pk(a, 2), pk(b, 0), pk(b, 2)); }
-  template <int NP>
-  DEV void mac(const uint4 (&x)[NP][8], float, f32x4& out) const {
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4& v = w[2 * p + h];
-        const uint4 b0 = frag(v.x, v.y), b1 = frag(v.z, v.w);
-#pragma unroll
-        for (int q = 0; q < NP; ++q) a = mfma(x[q][4 * p + 2 * h], b0, a), a = mfma(x[q][4 * p + 2 * h + 1], b1, a);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(s[p], a[r], out[r]);
-    }
-  }
 };
 
 // A lane's fragments of 256 inputs of its row (planes `plane` elements apart); inputs past the chunk are zero
@@ -273,129 +272,181 @@ __global__ void __launch_bounds__(MR_NT) k_moe_rows_router(MoeRows a) {
 }
 
 // ---- experts ----------------------------------------------------------------------------------
-// MODE 0: gate_up (unit: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (unit: rows 32 t, K = i).
-// The units of all experts that were picked, ascending, then of the shared expert, are dealt to the blocks in
-// even, contiguous runs.  KS waves share a tile's inputs (256 each, a wave taking more than one chunk where
-// K is larger), the others take further tiles.
+// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (rows 32 t, K = i).
+// The tiles of all experts that were picked, ascending, then of the shared expert, are dealt to the blocks in
+// contiguous runs of even cost (a tile costs its passes of 16 rows, twice that where the shared expert's bytes are
+// twice the others').  KS waves share a tile's inputs, 256 each and further chunks in turn where K is larger than that;
+// the other RG = 8 / KS groups of waves take further tiles.  A wave's x fragments stay in registers for all tiles of an expert
+// (one pass, one chunk), a tile's next weights are requested as soon as the present ones are used, and the KS
+// sums meet in LDS, behind a barrier that leaves the loads in flight.
 template <int MODE, class F, class FS>
-__global__ void __launch_bounds__(MR_NT) k_moe_rows_experts(MoeRows a, int KS) {
+__global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_experts(MoeRows a, int KS) {
   constexpr int NP = MODE == 0 ? 1 : 3;
-  __shared__ uint16_t s_pick[MR_PAIRS];
-  __shared__ uint32_t s_mask[8];
-  __shared__ int s_list[MR_ROWS], s_n;
-  __shared__ f32x4 red[2][MR_NW][2][64];
-  const int lane = lane_id(), wave = wave_id();
+  __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert
+  __shared__ int s_cnt[257], s_e[257], s_off[258], s_cum[258], s_tot[8][3], s_first;
+  __shared__ float red[2][MR_NW][2][4][64];
+  const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x;
   const int pairs = a.rows * a.topk;
   const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 32;
   const int N = MODE == 0 ? 2 * a.i : a.h, second = MODE == 0 ? a.i : 16;
-  const int nch = (K + 255) / 256, RG = MR_NW / KS, wk = wave % KS, rg = wave / KS;
-  if (threadIdx.x < 8) s_mask[threadIdx.x] = 0;
-  __syncthreads();
-  for (int p = threadIdx.x; p < pairs; p += MR_NT) {
-    const int e = a.idx[p];
-    s_pick[p] = (uint16_t)e;
-    atomicOr(&s_mask[e >> 5 & 7], 1u << (e & 31));
-  }
-  __syncthreads();
-  int D = 0;
+  const int nch = (K + 255) / 256, RG = MR_NW / KS, wk = wave % KS, rg = wave / KS, cpw = (nch + KS - 1) / KS;
+  // rows of each expert
+  constexpr int PPT = MR_PAIRS / MR_NT;
+  int pe[PPT], pp[PPT];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) D += __builtin_popcount(s_mask[q]);
-  const long long U = (long long)(D + a.shared) * tiles;
-  int u = (int)(U * blockIdx.x / gridDim.x);
-  const int u1 = (int)(U * (blockIdx.x + 1) / gridDim.x);
+  for (int q = 0; q < PPT; ++q) pe[q] = tid + MR_NT * q < pairs ? a.idx[tid + MR_NT * q] & 255 : -1;
+  if (tid < 257) s_cnt[tid] = 0;
+  lds_barrier();
+#pragma unroll
+  for (int q = 0; q < PPT; ++q)
+    if (pe[q] >= 0) pp[q] = atomicAdd(&s_cnt[pe[q]], 1);
+  lds_barrier();
+  // exclusive sums over the experts (thread e) of their rows, of being picked and of their cost
+  {
+    int v[3] = {0, 0, 0}, own[3];
+    if (tid <= 256) {
+      const bool sh = tid == 256;
+      v[0] = sh ? (a.shared ? a.rows : 0) : s_cnt[tid];
+      v[1] = v[0] > 0;
+      v[2] = (v[0] + 15) / 16 * tiles * (sh && FS::cost > F::cost ? 2 : 1);
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      own[q] = v[q];
+      for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(v[q], o);
+        if (lane >= o) v[q] += up;
+      }
+      if (lane == 63) s_tot[wave][q] = v[q];
+    }
+    lds_barrier();
+    int base[3] = {0, 0, 0};
+    for (int w = 0; w < wave; ++w)
+#pragma unroll
+      for (int q = 0; q < 3; ++q) base[q] += s_tot[w][q];
+    if (tid <= 256 && own[1]) {
+      const int d = base[1] + v[1] - 1;
+      s_e[d] = tid, s_off[d] = base[0] + v[0] - own[0], s_cum[d] = base[2] + v[2] - own[2];
+      s_cnt[tid] = s_off[d];  // from here on: where the expert's rows start
+    }
+    if (tid == 256) {
+      const int D = base[1] + v[1];
+      s_off[D] = base[0] + v[0], s_cum[D] = base[2] + v[2], s_tot[0][0] = D;
+    }
+    lds_barrier();
+  }
+  const int D = s_tot[0][0];
+  const int lo = (int)((long long)s_cum[D] * blockIdx.x / gridDim.x), hi = (int)((long long)s_cum[D] * (blockIdx.x + 1) / gridDim.x);
+  if (tid < D && s_cum[tid] <= lo && lo < s_cum[tid + 1]) s_first = tid;
+#pragma unroll
+  for (int q = 0; q < PPT; ++q)
+    if (pe[q] >= 0) s_list[s_cnt[pe[q]] + pp[q]] = tid + MR_NT * q;
+  if (a.shared && tid < a.rows) s_list[pairs + tid] = pairs + tid;
+  lds_barrier();
+  if (lo >= hi) return;
   int par = 0;
-  while (u < u1) {
-    const int d = u / tiles, t0 = u - d * tiles, t1 = t0 + (u1 - u) < tiles ? t0 + (u1 - u) : tiles;
-    u += t1 - t0;
-    const bool sh = d == D;
-    int e = 0;
-    if (!sh) {  // the d-th set bit
-      int left = d;
-      for (int q = 0; q < 8; ++q) {
-        uint32_t m = s_mask[q];
-        const int c = __builtin_popcount(m);
-        if (left >= c) {
-          left -= c;
-          continue;
-        }
-        for (; left > 0; --left) m &= m - 1;
-        e = 32 * q + __builtin_ctz(m);
-        break;
-      }
-    }
-    __syncthreads();  // the previous segment's list has been read
-    if (wave == 0) {
-      int n = 0;
-      if (sh) {
-        n = a.rows;
-        if (lane < n) s_list[lane] = pairs + lane;
-      } else {
-        for (int b = 0; b < pairs; b += 64) {
-          const bool hit = b + lane < pairs && s_pick[b + lane] == e;
-          const unsigned long long m = __ballot(hit);
-          if (hit) s_list[n + __builtin_popcountll(m & ((1ull << lane) - 1))] = b + lane;
-          n += __builtin_popcountll(m);
-        }
-      }
-      if (lane == 0) s_n = n;
-    }
-    __syncthreads();
-    const int cnt = s_n;
-    auto segment = [&](auto fmt, const uint8_t* Q, const void* S) __attribute__((always_inline)) {
+  const size_t plane = (size_t)(pairs + a.rows) * a.i;
+  for (int d = s_first; d < D && s_cum[d] < hi; ++d) {
+    const int e = __builtin_amdgcn_readfirstlane(s_e[d]), off = s_off[d], cnt = s_off[d + 1] - off;
+    const int cum = s_cum[d], tc = (s_cum[d + 1] - cum) / tiles;
+    const int t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0, t1 = (hi - cum + tc - 1) / tc < tiles ? (hi - cum + tc - 1) / tc : tiles;
+    if (t0 >= t1) continue;
+    const int passes = (cnt + 15) / 16;
+    const bool sh = e == 256;
+    auto segment = [&](auto fmt, const void* Qp, const void* Sp) __attribute__((always_inline)) {
       using Fm = decltype(fmt);
-      for (int t = t0; t < t1; t += RG) {
-        const int tile = t + rg;
-        const int n0 = (MODE == 0 ? 16 : 32) * tile + (lane & 15);
-        for (int p0 = 0; p0 < cnt; p0 += 16) {
-          f32x4 o0 = {0.f, 0.f, 0.f, 0.f}, o1 = o0;
-          if (tile < t1) {
-            const int pr = s_list[p0 + (lane & 15) < cnt ? p0 + (lane & 15) : cnt - 1];
-            const uint16_t* xr;
-            if constexpr (MODE == 0) xr = a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K;
-            else xr = a.act + (size_t)pr * K;
-            const size_t plane = (size_t)(pairs + a.rows) * a.i;
-            for (int c = wk; c < nch; c += KS) {
-              const bool half = c * 256 + 128 >= K;
-              Fm w0, w1;
-              w0.load(Q, S, e, n0, N, K, c, half), w1.load(Q, S, e, n0 + second, N, K, c, half);
-              uint4 x[NP][8];
-              load_x<Fm, NP>(xr, plane, c, half, x);
-              const float xs = group_sum<Fm, NP>(x);
-              w0.mac(x, xs, o0), w1.mac(x, xs, o1);
+      const Rsrc Q = rsrc(Qp, (uint32_t)Fm::q_bytes(N, K)), S = rsrc(Sp, (uint32_t)Fm::s_bytes(N, K));
+      const bool keep_x = passes == 1 && cpw == 1;
+      Fm w0, w1;
+      uint4 x[NP][8];
+      float xs = 0.f;
+      auto half_of = [&](int c) { return c * 256 + 128 >= K; };
+      auto load_w = [&](Fm& w, int add, int t, int ci) __attribute__((always_inline)) {
+        const int c = wk + KS * ci, tile = t + rg;
+        const bool none = tile >= t1 || c >= nch;
+        w.load(Q, S, (MODE == 0 ? 16 : 32) * tile + (lane & 15) + add, K, c, none || half_of(c), none);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      auto fetch_x = [&](int p, int ci) __attribute__((always_inline)) {
+        const int m = 16 * p + (lane & 15), pr = s_list[off + (m < cnt ? m : cnt - 1)], c = wk + KS * ci < nch ? wk + KS * ci : 0;
+        const uint16_t* xr;
+        if constexpr (MODE == 0) xr = a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K;
+        else xr = a.act + (size_t)pr * K;
+        load_x<Fm, NP>(xr, plane, c, half_of(c), x);
+      };
+      // position of the tile being computed and of the one in flight
+      int t = t0, p = 0, ci = 0, nt = t0, np = 0, nci = 0;
+      auto next = [&]() {
+        if (++nci < cpw) return;
+        nci = 0;
+        if (++np < passes) return;
+        np = 0, nt += RG;
+      };
+      f32x4 o0, o1;
+      if (keep_x) fetch_x(0, 0);
+      load_w(w0, 0, t, 0), load_w(w1, second, t, 0);
+      if (keep_x) xs = group_sum<Fm, NP>(x);
+      while (t < t1) {
+        if (!keep_x) fetch_x(p, ci), xs = group_sum<Fm, NP>(x);
+        next();
+        if (ci == 0) o0 = o1 = f32x4{0.f, 0.f, 0.f, 0.f};
+        const bool hf = half_of(wk + KS * ci);
+        w0.mac(x, xs, hf, o0);
+        load_w(w0, 0, nt, nci);
+        w1.mac(x, xs, hf, o1);
+        load_w(w1, second, nt, nci);
+        if (ci == cpw - 1) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) red[par][wave][0][r][lane] = o0[r], red[par][wave][1][r][lane] = o1[r];
+          lds_barrier();
+          const int tile = t + rg, m0 = 16 * p, nr = cnt - m0 < 16 ? cnt - m0 : 16;
+          auto finish = [&](auto ks) __attribute__((always_inline)) {
+            constexpr int KK = decltype(ks)::value;
+            // register r of lane l: row 4 (l / 16) + r of x, column l % 16.  gate_up: 4 of the 8 waves, by turns (KK = 8)
+            const int base = rg * KK;
+#pragma unroll
+            for (int q0 = 0; q0 < (MODE == 0 ? 4 : 8); q0 += KK) {
+              const int q = q0 + (KK == 8 && MODE == 0 ? wave - 4 * par : wk), r = q & 3;
+              if (KK == 8 && MODE == 0 && (q < 0 || q > 3)) continue;
+              if (KK == 8 && MODE == 0 && q0 > 0) continue;
+              const int row = 4 * (lane >> 4) + r;
+              const bool live = row < nr && tile < t1;
+              const int pr = s_list[off + (live ? m0 + row : 0)];
+              if constexpr (MODE == 0) {
+                float g = 0.f, v = 0.f;
+#pragma unroll
+                for (int k = 0; k < KK; ++k) g += red[par][base + k][0][r][lane], v += red[par][base + k][1][r][lane];
+                if (live) {
+                  const float act = g / (1.f + expf(-g)) * v;
+                  uint16_t* o = a.act + (size_t)pr * a.i + 16 * tile + (lane & 15);
+                  const float hi8 = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi8;
+                  const float mi8 = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi8;
+                  o[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
+                  o[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
+                  o[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
+                }
+              } else {
+                const int b = q >> 2;
+                float v = 0.f;
+#pragma unroll
+                for (int k = 0; k < KK; ++k) v += red[par][base + k][b][r][lane];
+                if (live) a.yp[(size_t)pr * a.h + 32 * tile + 16 * b + (lane & 15)] = v;
+              }
             }
-          }
-          red[par][wave][0][lane] = o0, red[par][wave][1][lane] = o1;
-          __syncthreads();
-          // thread q of a row group's 64 KS: D register r of lane l is row 4 (l / 16) + r of x, column l % 16
-          const int np = cnt - p0 < 16 ? cnt - p0 : 16;
-          for (int q = threadIdx.x % (64 * KS); q < (MODE == 0 ? 256 : 512); q += 64 * KS) {
-            const int l = q & 63, r = q >> 6 & 3, row = 4 * (l >> 4) + r;
-            if (row >= np || tile >= t1) continue;
-            const int pr = s_list[p0 + row];
-            if constexpr (MODE == 0) {
-              float g = 0.f, v = 0.f;
-              for (int k = 0; k < KS; ++k) g += red[par][rg * KS + k][0][l][r], v += red[par][rg * KS + k][1][l][r];
-              const float act = g / (1.f + expf(-g)) * v;
-              uint16_t* o = a.act + (size_t)pr * a.i + 16 * tile + (l & 15);
-              const size_t plane = (size_t)(pairs + a.rows) * a.i;
-              const float hi = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi;
-              const float mi = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi;
-              o[0] = (uint16_t)(__float_as_uint(hi) >> 16);
-              o[plane] = (uint16_t)(__float_as_uint(mi) >> 16);
-              o[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
-            } else {
-              const int half = q >> 8;
-              float v = 0.f;
-              for (int k = 0; k < KS; ++k) v += red[par][rg * KS + k][half][l][r];
-              a.yp[(size_t)pr * a.h + 32 * tile + 16 * half + (l & 15)] = v;
-            }
-          }
+          };
+          if (KS == 8) finish(std::integral_constant<int, 8>{});
+          else if (KS == 4) finish(std::integral_constant<int, 4>{});
+          else if (KS == 2) finish(std::integral_constant<int, 2>{});
+          else finish(std::integral_constant<int, 1>{});
           par ^= 1;
         }
+        t = nt, p = np, ci = nci;
       }
     };
-    if (sh) segment(FS{}, reinterpret_cast<const uint8_t*>(MODE == 0 ? a.sgu_q : a.sd_q), MODE == 0 ? a.sgu_s : a.sd_s);
-    else segment(F{}, MODE == 0 ? a.gu_q : a.d_q, MODE == 0 ? a.gu_s : a.d_s);
+    if (sh) segment(FS{}, MODE == 0 ? a.sgu_q : a.sd_q, MODE == 0 ? a.sgu_s : a.sd_s);
+    else
+      segment(F{}, (MODE == 0 ? a.gu_q : a.d_q) + e * F::q_bytes(N, K),
+              reinterpret_cast<const char*>(MODE == 0 ? a.gu_s : a.d_s) + e * F::s_bytes(N, K));
   }
 }
 
