@@ -14,7 +14,7 @@ using namespace drm;
 namespace {
 
 constexpr int MR_NW = 8, MR_NT = MR_NW * 64, MR_ROWS = 64, MR_TOPK = 32, MR_PAIRS = MR_ROWS * MR_TOPK;
-constexpr int MR_GRID = 512;  // two blocks per CU
+constexpr int MR_GRID = 256;  // a block per CU
 constexpr int MR_SETS = 8;    // row sets of the router
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -42,47 +42,49 @@ struct MoeRows {
 };
 
 // ---- weight formats --------------------------------------------------------------------------
-// One wave's part of a 16-row tile: 256 inputs of each row (chunk c), lane l holding 16-byte pieces of row
+// One wave's part of a 16-row tile: chunk c of 128 HF inputs of each row, lane l holding 16-byte pieces of row
 // l % 16 (g = l / 16).  Fragment f of x (two for each group of 64 inputs) covers inputs 64 (f / 2) + xoff(g) + 8 (f % 2) .. + 8.
-// The loads go through buffer resources of one expert's matrix, so a piece past the row's inputs (half: only
-// the chunk's first 128 exist) and a tile that does not exist (off: nothing left to prefetch) read zeros without a
+// The loads go through buffer resources of one expert's matrix, so a piece past the row's inputs (half: of
+// the two only the chunk's first 128 exist) and a tile that does not exist (off: nothing left to prefetch) read zeros without a
 // fetch, and the code in flight stays free of branches, which keeps the load counter exact.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 DEV Rsrc rsrc(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
 }
 constexpr uint32_t NOWHERE = 0x80000000u;  // past every matrix
+DEV uint2 buf8(const Rsrc& r, uint32_t off) { return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0)); }
 DEV uint4 buf16(const Rsrc& r, uint32_t off) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); }
 
-template <class SC>
+template <class SC, int HF>
 struct RowsQ4 {
   static constexpr bool perm = true;  // fragment order 0 4 1 5 2 6 3 7
-  static constexpr int cost = 1;      // relative bytes of a tile
-  uint4 w[2], s;
+  uint4 w[HF];
+  uint2 s[HF];
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K / 2; }
   static DEV size_t s_bytes(int N, int K) { return (size_t)N * K / 16; }
   static DEV int xoff(int g) { return 32 * (g & 1) + 16 * (g >> 1); }
   DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
-    const uint32_t p = off ? NOWHERE : n * (K / 2) + c * 128 + 16 * (lane_id() >> 4);
+    const uint32_t p = off ? NOWHERE : n * (K / 2) + c * (64 * HF) + 16 * (lane_id() >> 4);
+    const uint32_t q = off ? NOWHERE : (n * (K / 64) + c * (2 * HF)) * 4;
     w[0] = buf16(Q, p);
-    w[1] = buf16(Q, half ? NOWHERE : p + 64);
-    s = buf16(S, off ? NOWHERE : (n * (K / 64) + c * 4) * 4);
+    if constexpr (HF == 2) w[1] = buf16(Q, half ? NOWHERE : p + 64);
+    s[0] = buf8(S, q);
+    if constexpr (HF == 2) s[1] = buf8(S, half ? NOWHERE : q + 8);
   }
   // nibbles of a word as 16 + q in bf16: the nibble is the top four mantissa bits of a number in [16, 32)
   static DEV uint4 frag(uint32_t v) {
     constexpr uint32_t m = 0x00780078u, b = 0x41804180u;
     return make_uint4(((v << 3) & m) | b, ((v >> 1) & m) | b, ((v >> 5) & m) | b, ((v >> 9) & m) | b);
   }
-  // xsum: lane's sum of x over group l / 16 of row l % 16
+  // xsum: lane's sum of x over group l / 16 of row l % 16 (0 past the chunk's groups)
   template <int NP>
-  DEV void mac(const uint4 (&x)[NP][8], float xsum, bool half, f32x4& out) const {
+  DEV void mac(const uint4 (&x)[NP][4 * HF], float xsum, f32x4& out) const {
     const int g = lane_id() >> 4;
-    const uint32_t sw[4] = {s.x, s.y, half ? 0u : s.z, half ? 0u : s.w};
-    const uint32_t own = (g & 2) ? ((g & 1) ? sw[3] : sw[2]) : ((g & 1) ? sw[1] : sw[0]);
-    const float2 o = SC::pair(own);
+    const uint2 ow = HF == 2 && (g & 2) ? s[HF - 1] : s[0];
+    const float2 o = SC::pair(g & 1 ? ow.y : ow.x);
     out = __builtin_amdgcn_mfma_f32_16x16x4f32(xsum, o.y - 16.f * o.x, out, 0, 0, 0);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
+    for (int p = 0; p < HF; ++p) {
       // lanes g = 0, 1 hold group 2 p, g = 2, 3 group 2 p + 1: two words of each change places
       const auto s02 = __builtin_amdgcn_permlane32_swap(w[p].x, w[p].z, false, false);
       const auto s13 = __builtin_amdgcn_permlane32_swap(w[p].y, w[p].w, false, false);
@@ -92,7 +94,7 @@ struct RowsQ4 {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < NP; ++q) a = mfma(x[q][4 * p + 2 * h], b0, a), a = mfma(x[q][4 * p + 2 * h + 1], b1, a);
-        const float sc = SC::pair(sw[2 * p + h]).x;
+        const float sc = SC::pair(h ? s[p].y : s[p].x).x;
 #pragma unroll
         for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
       }
@@ -102,25 +104,26 @@ struct RowsQ4 {
 
 // One byte per weight: 64 inputs of a row per 16-byte load of four lanes, scales per 128 inputs.  D: the
 // format's conversions
-template <class D>
+template <class D, int HF>
 struct Rows8 {
   static constexpr bool perm = false;
-  static constexpr int cost = 2;
-  uint4 w[4];
-  uint32_t s[2];
+  uint4 w[2 * HF];
+  uint32_t s[HF];
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K; }
   static DEV int xoff(int g) { return 16 * g; }
   DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
-    const uint32_t p = off ? NOWHERE : n * K + c * 256 + 16 * (lane_id() >> 4);
+    const uint32_t p = off ? NOWHERE : n * K + c * (128 * HF) + 16 * (lane_id() >> 4);
     w[0] = buf16(Q, p), w[1] = buf16(Q, off ? NOWHERE : p + 64);
-    w[2] = buf16(Q, half ? NOWHERE : p + 128), w[3] = buf16(Q, half ? NOWHERE : p + 192);
-    s[0] = D::scale_raw(S, n, 2 * c, K, off);
-    s[1] = D::scale_raw(S, n, 2 * c + 1, K, off || half);
+    s[0] = D::scale_raw(S, n, HF * c, K, off);
+    if constexpr (HF == 2) {
+      w[2] = buf16(Q, half ? NOWHERE : p + 128), w[3] = buf16(Q, half ? NOWHERE : p + 192);
+      s[1] = D::scale_raw(S, n, 2 * c + 1, K, half);
+    }
   }
   template <int NP>
-  DEV void mac(const uint4 (&x)[NP][8], float, bool, f32x4& out) const {
+  DEV void mac(const uint4 (&x)[NP][4 * HF], float, f32x4& out) const {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
+    for (int p = 0; p < HF; ++p) {
       f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -137,8 +140,8 @@ struct Rows8 {
 };
 DEV uint32_t buf_half(const Rsrc& S, uint32_t off) { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(S, off, 0, 0); }
 
-template <int SF>
-struct RowsFP8 : Rows8<RowsFP8<SF>> {
+template <int SF, int HF>
+struct RowsFP8 : Rows8<RowsFP8<SF, HF>, HF> {
   static DEV size_t s_bytes(int N, int K) { return (size_t)(N / 128) * (K / 128) * (SF ? 2 : 4); }
   static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
     const uint32_t i = (n >> 7) * (K / 128) + b;
@@ -154,8 +157,8 @@ struct RowsFP8 : Rows8<RowsFP8<SF>> {
   }
 };
 
-template <class SH>
-struct RowsQ8 : Rows8<RowsQ8<SH>> {
+template <class SH, int HF>
+struct RowsQ8 : Rows8<RowsQ8<SH, HF>, HF> {
   static DEV size_t s_bytes(int N, int K) { return (size_t)N * (SH::per_row ? 1 : K / 128) * 2; }
   static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
     return buf_half(S, off ? NOWHERE : 2 * (SH::per_row ? n : n * (K / 128) + b));
@@ -168,37 +171,37 @@ struct RowsQ8 : Rows8<RowsQ8<SH>> {
   static DEV uint4 frag(uint32_t a, uint32_t b) { return make_uint4(pk(a, 0), pk(a, 2), pk(b, 0), pk(b, 2)); }
 };
 
-// A lane's fragments of 256 inputs of its row (planes `plane` elements apart); inputs past the chunk are zero
-template <class F, int NP>
-DEV void load_x(const uint16_t* row, size_t plane, int c, bool half, uint4 (&x)[NP][8]) {
+// A lane's fragments of its row's chunk c (planes `plane` elements apart); inputs past the row are zero
+template <class F, int NP, int HF>
+DEV void load_x(const uint16_t* row, size_t plane, int c, bool half, uint4 (&x)[NP][4 * HF]) {
 #pragma unroll
   for (int q = 0; q < NP; ++q) {
-    const uint16_t* p = row + q * plane + c * 256 + F::xoff(lane_id() >> 4);
+    const uint16_t* p = row + q * plane + c * (128 * HF) + F::xoff(lane_id() >> 4);
 #pragma unroll
-    for (int f = 0; f < 8; ++f) {
+    for (int f = 0; f < 4 * HF; ++f) {
       uint4 v = make_uint4(0, 0, 0, 0);
       if (f < 4 || !half) v = ld16(p + 64 * (f >> 1) + 8 * (f & 1));
-      if constexpr (F::perm)
-        v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
       x[q][f] = v;
     }
   }
 }
-template <class F, int NP>
-DEV float group_sum(const uint4 (&x)[NP][8]) {
+// the fragments in the weights' order, and the lane's group sum (RowsQ4)
+template <class F, int NP, int HF>
+DEV float order_x(uint4 (&x)[NP][4 * HF]) {
   if constexpr (!F::perm) return 0.f;
   float own = 0.f;
 #pragma unroll
-  for (int G = 0; G < 4; ++G) {
+  for (int G = 0; G < 2 * HF; ++G) {
     float t = 0.f;
 #pragma unroll
     for (int q = NP - 1; q >= 0; --q)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint4& v = x[q][2 * G + j];
+        uint4& v = x[q][2 * G + j];
         t += ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) +
              ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
+        v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
       }
     t = xsum_step<32>(xsum_step<16>(t));
     own = (lane_id() >> 4) == G ? t : own;
@@ -272,24 +275,26 @@ __global__ void __launch_bounds__(MR_NT) k_moe_rows_router(MoeRows a) {
 }
 
 // ---- experts ----------------------------------------------------------------------------------
-// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (rows 32 t, K = i).
-// The tiles of all experts that were picked, ascending, then of the shared expert, are dealt to the blocks in
-// contiguous runs of even cost (a tile costs its passes of 16 rows, twice that where the shared expert's bytes are
-// twice the others').  KS waves share a tile's inputs, 256 each and further chunks in turn where K is larger than that;
-// the other RG = 8 / KS groups of waves take further tiles.  A wave's x fragments stay in registers for all tiles of an expert
-// (one pass, one chunk), a tile's next weights are requested as soon as the present ones are used, and the KS
-// sums meet in LDS, behind a barrier that leaves the loads in flight.
+// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 64 t, K = i).
+// KS waves share a tile's inputs, a chunk each (cpw > 1: further chunks in turn); the other groups of waves (RG)
+// take further tiles, a step of the block being RG tiles.  The steps of all experts that were picked, ascending,
+// then of the shared expert, are dealt to the blocks in contiguous runs of even cost: a step's passes of 16 rows,
+// twice that where the shared expert's bytes are twice the others'.
+// A wave's x fragments stay in registers for all tiles of an expert (one pass, one chunk).  Two steps of weights
+// are in flight: a tile's registers take the tile two steps on as soon as it is used.  The KS sums meet in LDS, behind a
+// barrier that leaves the loads in flight.
 template <int MODE, class F, class FS>
-__global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_experts(MoeRows a, int KS) {
-  constexpr int NP = MODE == 0 ? 1 : 3;
+__global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS, int cpw, int fs_cost) {
+  constexpr int NP = MODE == 0 ? 1 : 3, HF = MODE == 0 ? 2 : 1, CH = 128 * HF, TL = MODE == 0 ? 2 : 4;
   __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert
   __shared__ int s_cnt[257], s_e[257], s_off[258], s_cum[258], s_tot[8][3], s_first;
-  __shared__ float red[2][MR_NW][2][4][64];
+  __shared__ float red[2][MR_NW][TL][4][64];
   const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x;
   const int pairs = a.rows * a.topk;
-  const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 32;
-  const int N = MODE == 0 ? 2 * a.i : a.h, second = MODE == 0 ? a.i : 16;
-  const int nch = (K + 255) / 256, RG = MR_NW / KS, wk = wave % KS, rg = wave / KS, cpw = (nch + KS - 1) / KS;
+  const int K = MODE == 0 ? a.h : a.i, RG = MR_NW / KS, tiles = MODE == 0 ? a.i / 16 : a.h / 64;
+  const int steps = (tiles + RG - 1) / RG;
+  const int N = MODE == 0 ? 2 * a.i : a.h;
+  const int nch = (K + CH - 1) / CH, wk = wave % KS, rg = wave / KS;
   // rows of each expert
   constexpr int PPT = MR_PAIRS / MR_NT;
   int pe[PPT], pp[PPT];
@@ -308,7 +313,7 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_experts(M
       const bool sh = tid == 256;
       v[0] = sh ? (a.shared ? a.rows : 0) : s_cnt[tid];
       v[1] = v[0] > 0;
-      v[2] = (v[0] + 15) / 16 * tiles * (sh && FS::cost > F::cost ? 2 : 1);
+      v[2] = (v[0] + 15) / 16 * steps * (sh ? fs_cost : 1);
     }
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
@@ -324,10 +329,11 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_experts(M
     for (int w = 0; w < wave; ++w)
 #pragma unroll
       for (int q = 0; q < 3; ++q) base[q] += s_tot[w][q];
+    lds_barrier();
     if (tid <= 256 && own[1]) {
       const int d = base[1] + v[1] - 1;
       s_e[d] = tid, s_off[d] = base[0] + v[0] - own[0], s_cum[d] = base[2] + v[2] - own[2];
-      s_cnt[tid] = s_off[d];  // from here on: where the expert's rows start
+      if (tid < 256) s_cnt[tid] = base[0] + v[0] - own[0];  // from here on: where the expert's rows start
     }
     if (tid == 256) {
       const int D = base[1] + v[1];
@@ -348,8 +354,8 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_experts(M
   const size_t plane = (size_t)(pairs + a.rows) * a.i;
   for (int d = s_first; d < D && s_cum[d] < hi; ++d) {
     const int e = __builtin_amdgcn_readfirstlane(s_e[d]), off = s_off[d], cnt = s_off[d + 1] - off;
-    const int cum = s_cum[d], tc = (s_cum[d + 1] - cum) / tiles;
-    const int t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0, t1 = (hi - cum + tc - 1) / tc < tiles ? (hi - cum + tc - 1) / tc : tiles;
+    const int cum = s_cum[d], tc = (s_cum[d + 1] - cum) / steps;
+    const int t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0, t1 = (hi - cum + tc - 1) / tc < steps ? (hi - cum + tc - 1) / tc : steps;
     if (t0 >= t1) continue;
     const int passes = (cnt + 15) / 16;
     const bool sh = e == 256;
@@ -357,14 +363,14 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_experts(M
       using Fm = decltype(fmt);
       const Rsrc Q = rsrc(Qp, (uint32_t)Fm::q_bytes(N, K)), S = rsrc(Sp, (uint32_t)Fm::s_bytes(N, K));
       const bool keep_x = passes == 1 && cpw == 1;
-      Fm w0, w1;
-      uint4 x[NP][8];
+      Fm w[2][TL];
+      uint4 x[NP][4 * HF];
       float xs = 0.f;
-      auto half_of = [&](int c) { return c * 256 + 128 >= K; };
-      auto load_w = [&](Fm& w, int add, int t, int ci) __attribute__((always_inline)) {
-        const int c = wk + KS * ci, tile = t + rg;
-        const bool none = tile >= t1 || c >= nch;
-        w.load(Q, S, (MODE == 0 ? 16 : 32) * tile + (lane & 15) + add, K, c, none || half_of(c), none);
+      auto half_of = [&](int c) { return HF == 2 && c * CH + 128 >= K; };
+      auto load_w = [&](Fm& f, int i, int t, int ci) __attribute__((always_inline)) {
+        const int c = wk + KS * ci, tile = t * RG + rg;
+        const bool none = t >= t1 || tile >= tiles || rg >= RG || c >= nch;
+        f.load(Q, S, MODE == 0 ? 16 * tile + (lane & 15) + i * a.i : 64 * tile + 16 * i + (lane & 15), K, c, none || half_of(c), none);
         __builtin_amdgcn_sched_barrier(0);
       };
       auto fetch_x = [&](int p, int ci) __attribute__((always_inline)) {
@@ -372,75 +378,88 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_experts(M
         const uint16_t* xr;
         if constexpr (MODE == 0) xr = a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K;
         else xr = a.act + (size_t)pr * K;
-        load_x<Fm, NP>(xr, plane, c, half_of(c), x);
+        load_x<Fm, NP, HF>(xr, plane, c, half_of(c), x);
       };
-      // position of the tile being computed and of the one in flight
-      int t = t0, p = 0, ci = 0, nt = t0, np = 0, nci = 0;
-      auto next = [&]() {
-        if (++nci < cpw) return;
-        nci = 0;
-        if (++np < passes) return;
-        np = 0, nt += RG;
+      // step, pass and chunk that is computed, the next and the one after
+      int t = t0, p = 0, ci = 0, t2 = t0, p2 = 0, c2 = 0;
+      auto next = [&](int& t, int& p, int& ci) {
+        if (++ci < cpw) return;
+        ci = 0;
+        if (++p < passes) return;
+        p = 0, ++t;
       };
-      f32x4 o0, o1;
-      if (keep_x) fetch_x(0, 0);
-      load_w(w0, 0, t, 0), load_w(w1, second, t, 0);
-      if (keep_x) xs = group_sum<Fm, NP>(x);
-      while (t < t1) {
-        if (!keep_x) fetch_x(p, ci), xs = group_sum<Fm, NP>(x);
-        next();
-        if (ci == 0) o0 = o1 = f32x4{0.f, 0.f, 0.f, 0.f};
-        const bool hf = half_of(wk + KS * ci);
-        w0.mac(x, xs, hf, o0);
-        load_w(w0, 0, nt, nci);
-        w1.mac(x, xs, hf, o1);
-        load_w(w1, second, nt, nci);
+      f32x4 o[TL];
+      auto body = [&](auto cur) __attribute__((always_inline)) {
+        constexpr int B = decltype(cur)::value;
+        if (!keep_x) fetch_x(p, ci), xs = order_x<Fm, NP, HF>(x);
+        next(t2, p2, c2);
+        if (ci == 0)
+#pragma unroll
+          for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < TL; ++i) w[B][i].template mac<NP>(x, xs, o[i]), load_w(w[B][i], i, t2, c2);
         if (ci == cpw - 1) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) red[par][wave][0][r][lane] = o0[r], red[par][wave][1][r][lane] = o1[r];
+          for (int i = 0; i < TL; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) red[par][wave][i][r][lane] = o[i][r];
           lds_barrier();
-          const int tile = t + rg, m0 = 16 * p, nr = cnt - m0 < 16 ? cnt - m0 : 16;
+          const int tile = t * RG + rg, m0 = 16 * p, nr = tile < tiles && rg < RG ? (cnt - m0 < 16 ? cnt - m0 : 16) : 0;
+          // register r of lane l: row 4 (l / 16) + r of x, column l % 16; the KS waves share the registers
           auto finish = [&](auto ks) __attribute__((always_inline)) {
             constexpr int KK = decltype(ks)::value;
-            // register r of lane l: row 4 (l / 16) + r of x, column l % 16.  gate_up: 4 of the 8 waves, by turns (KK = 8)
-            const int base = rg * KK;
+            const int base = rg * KS;
+            auto total = [&](int i, int r) {
+              float v = 0.f;
 #pragma unroll
-            for (int q0 = 0; q0 < (MODE == 0 ? 4 : 8); q0 += KK) {
-              const int q = q0 + (KK == 8 && MODE == 0 ? wave - 4 * par : wk), r = q & 3;
-              if (KK == 8 && MODE == 0 && (q < 0 || q > 3)) continue;
-              if (KK == 8 && MODE == 0 && q0 > 0) continue;
-              const int row = 4 * (lane >> 4) + r;
-              const bool live = row < nr && tile < t1;
+              for (int k = 0; k < KK; ++k) {
+                const float q = red[par][base + (k < KS ? k : 0)][i][r][lane];
+                v += k < KS ? q : 0.f;
+              }
+              return v;
+            };
+            for (int q = MODE == 0 && KS == 8 ? wk ^ (4 * par) : wk; q < (MODE == 0 ? 4 : 4 * TL); q += KS) {
+              const int r = q & 3, row = 4 * (lane >> 4) + r;
+              if (r >= nr) continue;
+              const bool live = row < nr;
               const int pr = s_list[off + (live ? m0 + row : 0)];
               if constexpr (MODE == 0) {
-                float g = 0.f, v = 0.f;
-#pragma unroll
-                for (int k = 0; k < KK; ++k) g += red[par][base + k][0][r][lane], v += red[par][base + k][1][r][lane];
+                const float g = total(0, r), v = total(1, r);
                 if (live) {
                   const float act = g / (1.f + expf(-g)) * v;
-                  uint16_t* o = a.act + (size_t)pr * a.i + 16 * tile + (lane & 15);
+                  uint16_t* dst = a.act + (size_t)pr * a.i + 16 * tile + (lane & 15);
                   const float hi8 = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi8;
                   const float mi8 = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi8;
-                  o[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
-                  o[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
-                  o[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
+                  dst[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
+                  dst[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
+                  dst[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
                 }
               } else {
-                const int b = q >> 2;
-                float v = 0.f;
-#pragma unroll
-                for (int k = 0; k < KK; ++k) v += red[par][base + k][b][r][lane];
-                if (live) a.yp[(size_t)pr * a.h + 32 * tile + 16 * b + (lane & 15)] = v;
+                const float v = total(q >> 2, r);
+                if (live) a.yp[(size_t)pr * a.h + 64 * tile + 16 * (q >> 2) + (lane & 15)] = v;
               }
             }
           };
-          if (KS == 8) finish(std::integral_constant<int, 8>{});
-          else if (KS == 4) finish(std::integral_constant<int, 4>{});
+          if (KS > 4) finish(std::integral_constant<int, 8>{});
+          else if (KS > 2) finish(std::integral_constant<int, 4>{});
           else if (KS == 2) finish(std::integral_constant<int, 2>{});
           else finish(std::integral_constant<int, 1>{});
           par ^= 1;
         }
-        t = nt, p = np, ci = nci;
+        next(t, p, ci);
+      };
+#pragma unroll
+      for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t2, c2);
+      if (keep_x) fetch_x(0, 0);
+      next(t2, p2, c2);
+#pragma unroll
+      for (int i = 0; i < TL; ++i) load_w(w[1][i], i, t2, c2);
+      if (keep_x) xs = order_x<Fm, NP, HF>(x);
+      while (true) {
+        body(std::integral_constant<int, 0>{});
+        if (t >= t1) break;
+        body(std::integral_constant<int, 1>{});
+        if (t >= t1) break;
       }
     };
     if (sh) segment(FS{}, MODE == 0 ? a.sgu_q : a.sd_q, MODE == 0 ? a.sgu_s : a.sd_s);
@@ -490,12 +509,17 @@ struct WsLayout {
   }
 };
 
-int waves_on_k(int K) {
-  const int nch = (K + 255) / 256;
-  return nch >= 8 ? 8 : nch >= 4 ? 4 : nch >= 2 ? 2 : 1;
-}
+// The waves that share a tile's K inputs and the chunks each takes: a wave per chunk up to all eight.
+struct Split {
+  int ks, cpw;
+  Split(int K, int ch) {
+    const int nch = (K + ch - 1) / ch;
+    cpw = (nch + MR_NW - 1) / MR_NW;
+    ks = (nch + cpw - 1) / cpw;
+  }
+};
 
-template <class F, class FS>
+template <class F2, class F1, class SH, bool BYTES>
 int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   if (!rows_shape_ok(a.rows, a.e, a.h, a.i, a.topk)) return -1;
   const int given = (a.sgu_q != nullptr) + (a.sgu_s != nullptr) + (a.sd_q != nullptr) + (a.sd_s != nullptr);
@@ -516,8 +540,9 @@ int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   else if (a.rows <= 8) hipLaunchKernelGGL(k_moe_rows_router<2>, dim3(nb, (a.rows + 1) / 2), dim3(MR_NT), 0, st, a);
   else if (a.rows <= 32) hipLaunchKernelGGL(k_moe_rows_router<4>, dim3(nb, (a.rows + 3) / 4), dim3(MR_NT), 0, st, a);
   else hipLaunchKernelGGL(k_moe_rows_router<8>, dim3(nb, (a.rows + 7) / 8), dim3(MR_NT), 0, st, a);
-  hipLaunchKernelGGL((k_moe_rows_experts<0, F, FS>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, waves_on_k(a.h));
-  hipLaunchKernelGGL((k_moe_rows_experts<1, F, FS>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, waves_on_k(a.i));
+  const Split g(a.h, 256), d(a.i, 128);
+  hipLaunchKernelGGL((k_moe_rows_experts<0, F2, RowsQ8<SH, 2>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, g.ks, g.cpw, BYTES ? 1 : 2);
+  hipLaunchKernelGGL((k_moe_rows_experts<1, F1, RowsQ8<SH, 1>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, d.ks, d.cpw, BYTES ? 1 : 2);
   hipLaunchKernelGGL(k_moe_rows_combine, dim3(a.rows, (a.h + 1023) / 1024), dim3(256), 0, st, a);
   return 0;
 }
@@ -528,16 +553,17 @@ API size_t dr_moe_layer_rows_ws(int rows, int e, int h, int i, int topk) {
   return rows_shape_ok(rows, e, h, i, topk) ? WsLayout(rows, e, h, i, topk).bytes : 0;
 }
 
-#define MOE_ROWS_ENTRY(NAME, S, F, FS)                                                                              \
+#define MOE_ROWS_ENTRY(NAME, S, F2, F1, SH, BYTES)                                                                        \
   API int NAME(const uint16_t* router, const uint8_t* gu_q, const S* gu_s, const uint8_t* d_q, const S* d_s,              \
                const int8_t* sgu_q, const uint16_t* sgu_s, const int8_t* sd_q, const uint16_t* sd_s, const uint16_t* x,   \
                const float* res, int* idx, float* wts, float* sgate, void* ws, float* y, int rows, int e, int h, int i,   \
                int topk, hipStream_t st) {                                                                                \
     const MoeRows a{router, gu_q, d_q, gu_s, d_s, sgu_q, sd_q, sgu_s, sd_s, x, res, idx, wts, sgate, y, nullptr, nullptr, \
                     nullptr, nullptr, rows, e, h, i, topk, 0};                                                            \
-    return moe_rows<F, FS>(a, ws, st);                                                                                    \
+    return moe_rows<F2, F1, SH, BYTES>(a, ws, st);                                                                        \
   }
-MOE_ROWS_ENTRY(dr_moe_layer_rows, uint16_t, RowsQ4<ScaleF16>, RowsQ8<Q8G128F16>)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_bf16s, uint16_t, RowsQ4<ScaleBF16>, RowsQ8<Q8RowBF16>)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8, float, RowsFP8<0>, RowsQ8<Q8G128F16>)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8_bf16s, uint16_t, RowsFP8<1>, RowsQ8<Q8RowBF16>)
+#define ROWS_ARG(...) __VA_ARGS__
+MOE_ROWS_ENTRY(dr_moe_layer_rows, uint16_t, ROWS_ARG(RowsQ4<ScaleF16, 2>), ROWS_ARG(RowsQ4<ScaleF16, 1>), Q8G128F16, false)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_bf16s, uint16_t, ROWS_ARG(RowsQ4<ScaleBF16, 2>), ROWS_ARG(RowsQ4<ScaleBF16, 1>), Q8RowBF16, false)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8, float, ROWS_ARG(RowsFP8<0, 2>), ROWS_ARG(RowsFP8<0, 1>), Q8G128F16, true)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8_bf16s, uint16_t, ROWS_ARG(RowsFP8<1, 2>), ROWS_ARG(RowsFP8<1, 1>), Q8RowBF16, true)
