@@ -72,8 +72,11 @@ struct RowsQ4 {
     if constexpr (HF == 2) s[1] = buf8(S, half ? NOWHERE : q + 8);
   }
   // nibbles of a word as 16 + q in bf16: the nibble is the top four mantissa bits of a number in [16, 32)
+  // (the two constants in registers, so that each pair of nibbles is a shift and one v_and_or_b32)
   static DEV uint4 frag(uint32_t v) {
-    constexpr uint32_t m = 0x00780078u, b = 0x41804180u;
+    uint32_t m = 0x00780078u, b = 0x41804180u;
+    asm("" : "+s"(m));
+    asm("" : "+v"(b));
     return make_uint4(((v << 3) & m) | b, ((v >> 1) & m) | b, ((v >> 5) & m) | b, ((v >> 9) & m) | b);
   }
   // xsum: lane's sum of x over group l / 16 of row l % 16 (0 past the chunk's groups)
@@ -171,19 +174,16 @@ struct RowsQ8 : Rows8<RowsQ8<SH, HF>, HF> {
   static DEV uint4 frag(uint32_t a, uint32_t b) { return make_uint4(pk(a, 0), pk(a, 2), pk(b, 0), pk(b, 2)); }
 };
 
-// A lane's fragments of its row's chunk c (planes `plane` elements apart); inputs past the row are zero
+// A lane's fragments of chunk c of the row at byte `row` (planes `plane` bytes apart); inputs past the row are zero
 template <class F, int NP, int HF>
-DEV void load_x(const uint16_t* row, size_t plane, int c, bool half, uint4 (&x)[NP][4 * HF]) {
+DEV void load_x(const Rsrc& X, uint32_t row, uint32_t plane, int c, bool half, uint4 (&x)[NP][4 * HF]) {
+  const uint32_t p = row + (c * (128 * HF) + F::xoff(lane_id() >> 4)) * 2;
 #pragma unroll
-  for (int q = 0; q < NP; ++q) {
-    const uint16_t* p = row + q * plane + c * (128 * HF) + F::xoff(lane_id() >> 4);
+  for (int q = 0; q < NP; ++q)
 #pragma unroll
-    for (int f = 0; f < 4 * HF; ++f) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (f < 4 || !half) v = ld16(p + 64 * (f >> 1) + 8 * (f & 1));
-      x[q][f] = v;
-    }
-  }
+    for (int f = 0; f < 4 * HF; ++f)
+      x[q][f] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(X, f >= 4 && half ? NOWHERE : p + 2 * (64 * (f >> 1) + 8 * (f & 1)),
+                                                                                 q * plane, 0));
 }
 // the fragments in the weights' order, and the lane's group sum (RowsQ4)
 template <class F, int NP, int HF>
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
   __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert
   __shared__ int s_cnt[257], s_e[257], s_off[258], s_cum[258], s_tot[8][3], s_first;
   __shared__ float red[2][MR_NW][TL][4][64];
-  const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
   const int pairs = a.rows * a.topk;
   const int K = MODE == 0 ? a.h : a.i, RG = MR_NW / KS, tiles = MODE == 0 ? a.i / 16 : a.h / 64;
   const int steps = (tiles + RG - 1) / RG;
@@ -362,104 +362,126 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
     auto segment = [&](auto fmt, const void* Qp, const void* Sp) __attribute__((always_inline)) {
       using Fm = decltype(fmt);
       const Rsrc Q = rsrc(Qp, (uint32_t)Fm::q_bytes(N, K)), S = rsrc(Sp, (uint32_t)Fm::s_bytes(N, K));
-      const bool keep_x = passes == 1 && cpw == 1;
+      const Rsrc X = MODE == 0 ? rsrc(a.x, (uint32_t)a.rows * K * 2) : rsrc(a.act, (uint32_t)(6 * plane));
       Fm w[2][TL];
       uint4 x[NP][4 * HF];
-      float xs = 0.f;
       auto half_of = [&](int c) { return HF == 2 && c * CH + 128 >= K; };
       auto load_w = [&](Fm& f, int i, int t, int ci) __attribute__((always_inline)) {
         const int c = wk + KS * ci, tile = t * RG + rg;
-        const bool none = t >= t1 || tile >= tiles || rg >= RG || c >= nch;
-        f.load(Q, S, MODE == 0 ? 16 * tile + (lane & 15) + i * a.i : 64 * tile + 16 * i + (lane & 15), K, c, none || half_of(c), none);
+        const bool none = (t >= t1) | (tile >= tiles) | (rg >= RG) | (c >= nch);
+        f.load(Q, S, MODE == 0 ? 16 * tile + (lane & 15) + i * a.i : 64 * tile + 16 * i + (lane & 15), K, c, none | half_of(c), none);
         __builtin_amdgcn_sched_barrier(0);
       };
       auto fetch_x = [&](int p, int ci) __attribute__((always_inline)) {
-        const int m = 16 * p + (lane & 15), pr = s_list[off + (m < cnt ? m : cnt - 1)], c = wk + KS * ci < nch ? wk + KS * ci : 0;
-        const uint16_t* xr;
-        if constexpr (MODE == 0) xr = a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K;
-        else xr = a.act + (size_t)pr * K;
-        load_x<Fm, NP, HF>(xr, plane, c, half_of(c), x);
+        const int m = 16 * p + (lane & 15), pr = s_list[off + (m < cnt ? m : cnt - 1)], c = wk + KS * ci;
+        const int row = MODE == 1 ? pr : sh ? pr - pairs : pr / a.topk;
+        load_x<Fm, NP, HF>(X, c < nch ? (uint32_t)(row * K * 2) : NOWHERE, (uint32_t)(2 * plane), c, half_of(c), x);
+        __builtin_amdgcn_sched_barrier(0);
       };
-      // step, pass and chunk that is computed, the next and the one after
-      int t = t0, p = 0, ci = 0, t2 = t0, p2 = 0, c2 = 0;
-      auto next = [&](int& t, int& p, int& ci) {
-        if (++ci < cpw) return;
-        ci = 0;
-        if (++p < passes) return;
-        p = 0, ++t;
-      };
-      f32x4 o[TL];
-      auto body = [&](auto cur) __attribute__((always_inline)) {
-        constexpr int B = decltype(cur)::value;
-        if (!keep_x) fetch_x(p, ci), xs = order_x<Fm, NP, HF>(x);
-        next(t2, p2, c2);
-        if (ci == 0)
+      // the KS sums of a step's tiles (pass p of t), and what becomes of them
+      auto finish = [&](const f32x4 (&o)[TL], int t, int p) __attribute__((always_inline)) {
 #pragma unroll
-          for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < TL; ++i)
 #pragma unroll
-        for (int i = 0; i < TL; ++i) w[B][i].template mac<NP>(x, xs, o[i]), load_w(w[B][i], i, t2, c2);
-        if (ci == cpw - 1) {
+          for (int r = 0; r < 4; ++r) red[par][wave][i][r][lane] = o[i][r];
+        lds_barrier();
+        const int tile = t * RG + rg, m0 = 16 * p, nr = tile < tiles && rg < RG ? (cnt - m0 < 16 ? cnt - m0 : 16) : 0;
+        // register r of lane l: row 4 (l / 16) + r of x, column l % 16; the KS waves share the registers
+        auto part = [&](auto ks) __attribute__((always_inline)) {
+          constexpr int KK = decltype(ks)::value;
+          const int base = rg * KS;
+          auto total = [&](int i, int r) {
+            float v = 0.f;
 #pragma unroll
-          for (int i = 0; i < TL; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) red[par][wave][i][r][lane] = o[i][r];
-          lds_barrier();
-          const int tile = t * RG + rg, m0 = 16 * p, nr = tile < tiles && rg < RG ? (cnt - m0 < 16 ? cnt - m0 : 16) : 0;
-          // register r of lane l: row 4 (l / 16) + r of x, column l % 16; the KS waves share the registers
-          auto finish = [&](auto ks) __attribute__((always_inline)) {
-            constexpr int KK = decltype(ks)::value;
-            const int base = rg * KS;
-            auto total = [&](int i, int r) {
-              float v = 0.f;
-#pragma unroll
-              for (int k = 0; k < KK; ++k) {
-                const float q = red[par][base + (k < KS ? k : 0)][i][r][lane];
-                v += k < KS ? q : 0.f;
-              }
-              return v;
-            };
-            for (int q = MODE == 0 && KS == 8 ? wk ^ (4 * par) : wk; q < (MODE == 0 ? 4 : 4 * TL); q += KS) {
-              const int r = q & 3, row = 4 * (lane >> 4) + r;
-              if (r >= nr) continue;
-              const bool live = row < nr;
-              const int pr = s_list[off + (live ? m0 + row : 0)];
-              if constexpr (MODE == 0) {
-                const float g = total(0, r), v = total(1, r);
-                if (live) {
-                  const float act = g / (1.f + expf(-g)) * v;
-                  uint16_t* dst = a.act + (size_t)pr * a.i + 16 * tile + (lane & 15);
-                  const float hi8 = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi8;
-                  const float mi8 = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi8;
-                  dst[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
-                  dst[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
-                  dst[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
-                }
-              } else {
-                const float v = total(q >> 2, r);
-                if (live) a.yp[(size_t)pr * a.h + 64 * tile + 16 * (q >> 2) + (lane & 15)] = v;
-              }
+            for (int k = 0; k < KK; ++k) {
+              const float q = red[par][base + (k < KS ? k : 0)][i][r][lane];
+              v += k < KS ? q : 0.f;
             }
+            return v;
           };
-          if (KS > 4) finish(std::integral_constant<int, 8>{});
-          else if (KS > 2) finish(std::integral_constant<int, 4>{});
-          else if (KS == 2) finish(std::integral_constant<int, 2>{});
-          else finish(std::integral_constant<int, 1>{});
-          par ^= 1;
-        }
-        next(t, p, ci);
+          for (int q = MODE == 0 && KS == 8 ? wk ^ (4 * par) : wk; q < (MODE == 0 ? 4 : 4 * TL); q += KS) {
+            const int r = q & 3, row = 4 * (lane >> 4) + r;
+            if (r >= nr) continue;
+            const bool live = row < nr;
+            const int pr = s_list[off + (live ? m0 + row : 0)];
+            if constexpr (MODE == 0) {
+              const float g = total(0, r), v = total(1, r);
+              if (live) {
+                const float act = g / (1.f + expf(-g)) * v;
+                uint16_t* dst = a.act + (size_t)pr * a.i + 16 * tile + (lane & 15);
+                const float hi8 = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi8;
+                const float mi8 = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi8;
+                dst[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
+                dst[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
+                dst[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
+              }
+            } else {
+              const float v = total(q >> 2, r);
+              if (live) a.yp[(size_t)pr * a.h + 64 * tile + 16 * (q >> 2) + (lane & 15)] = v;
+            }
+          }
+        };
+        if (KS > 4) part(std::integral_constant<int, 8>{});
+        else if (KS > 2) part(std::integral_constant<int, 4>{});
+        else if (KS == 2) part(std::integral_constant<int, 2>{});
+        else part(std::integral_constant<int, 1>{});
+        par ^= 1;
       };
+      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+      f32x4 o[TL];
+      if (passes == 1 && cpw == 1) {  // x stays
 #pragma unroll
-      for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t2, c2);
-      if (keep_x) fetch_x(0, 0);
-      next(t2, p2, c2);
+        for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t0, 0);
+        fetch_x(0, 0);
 #pragma unroll
-      for (int i = 0; i < TL; ++i) load_w(w[1][i], i, t2, c2);
-      if (keep_x) xs = order_x<Fm, NP, HF>(x);
-      while (true) {
-        body(std::integral_constant<int, 0>{});
-        if (t >= t1) break;
-        body(std::integral_constant<int, 1>{});
-        if (t >= t1) break;
+        for (int i = 0; i < TL; ++i) load_w(w[1][i], i, t0 + 1, 0);
+        const float xs = order_x<Fm, NP, HF>(x);
+        auto body = [&](Fm (&f)[TL], int t) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < TL; ++i) o[i] = z, f[i].template mac<NP>(x, xs, o[i]), load_w(f[i], i, t + 2, 0);
+          finish(o, t, 0);
+        };
+        for (int t = t0;;) {
+          body(w[0], t);
+          if (++t >= t1) break;
+          body(w[1], t);
+          if (++t >= t1) break;
+        }
+      } else {
+        // step, pass and chunk of the one ahead (x) and of the two ahead (weights)
+        int t = t0, p = 0, ci = 0, tx = t0, px = 0, cx = 0, tw = t0, pw = 0, cw = 0;
+        auto next = [&](int& t, int& p, int& ci) {
+          if (++ci < cpw) return;
+          ci = 0;
+          if (++p < passes) return;
+          p = 0, ++t;
+        };
+#pragma unroll
+        for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t0, 0);
+        fetch_x(0, 0);
+        next(tw, pw, cw), next(tx, px, cx);
+#pragma unroll
+        for (int i = 0; i < TL; ++i) load_w(w[1][i], i, tw, cw);
+        auto body = [&](Fm (&f)[TL]) __attribute__((always_inline)) {
+          const float xs = order_x<Fm, NP, HF>(x);
+          if (ci == 0)
+#pragma unroll
+            for (int i = 0; i < TL; ++i) o[i] = z;
+#pragma unroll
+          for (int i = 0; i < TL; ++i) f[i].template mac<NP>(x, xs, o[i]);
+          fetch_x(px, cx);
+          next(tx, px, cx), next(tw, pw, cw);
+#pragma unroll
+          for (int i = 0; i < TL; ++i) load_w(f[i], i, tw, cw);
+          if (ci == cpw - 1) finish(o, t, p);
+          next(t, p, ci);
+        };
+        for (;;) {
+          body(w[0]);
+          if (t >= t1) break;
+          body(w[1]);
+          if (t >= t1) break;
+        }
       }
     };
     if (sh) segment(FS{}, MODE == 0 ? a.sgu_q : a.sd_q, MODE == 0 ? a.sgu_s : a.sd_s);
