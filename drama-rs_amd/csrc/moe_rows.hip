@@ -15,6 +15,7 @@ namespace {
 
 constexpr int MR_NW = 8, MR_NT = MR_NW * 64, MR_ROWS = 64, MR_TOPK = 32, MR_PAIRS = MR_ROWS * MR_TOPK;
 constexpr int MR_GRID = 256;  // a block per CU
+constexpr int MR_ITEMS = 256 + MR_PAIRS / 16 + MR_ROWS / 16;  // passes of 16 rows, the experts' and the shared expert's
 constexpr int MR_SETS = 8;    // row sets of the router
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -42,34 +43,48 @@ struct MoeRows {
 };
 
 // ---- weight formats --------------------------------------------------------------------------
-// One wave's part of a 16-row tile: chunk c of 128 HF inputs of each row, lane l holding 16-byte pieces of row
-// l % 16 (g = l / 16).  Fragment f of x (two for each group of 64 inputs) covers inputs 64 (f / 2) + xoff(g) + 8 (f % 2) .. + 8.
-// The loads go through buffer resources of one expert's matrix, so a piece past the row's inputs (half: of
-// the two only the chunk's first 128 exist) and a tile that does not exist (off: nothing left to prefetch) read zeros without a
+// One wave's part of a 16-row tile: chunk c of 256 inputs of each row.  For the product lane l has row l % 16 and
+// (g = l / 16) fragment f (two for each group of 64 inputs) the inputs 64 (f / 2) + xoff(g) + 8 (f % 2) .. + 8.
+// A load takes 128 bytes of 8 rows, a whole line each (16 rows of 64 bytes would ask for every line twice: 5 to 10% of
+// the kernels' time); rows of a pair of loads change places in pair_up.
+// The loads go through buffer resources of one expert's matrix, so a piece past the row's inputs (half: only the
+// chunk's first 128 exist) and a tile that does not exist (off: nothing left to prefetch) read zeros without a
 // fetch, and the code in flight stays free of branches, which keeps the load counter exact.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 DEV Rsrc rsrc(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
 }
 constexpr uint32_t NOWHERE = 0x80000000u;  // past every matrix
-DEV uint2 buf8(const Rsrc& r, uint32_t off) { return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0)); }
 DEV uint4 buf16(const Rsrc& r, uint32_t off) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); }
 
-template <class SC, int HF>
+// Where lane l's piece of a row pair's loads lies: row l % 8 (+ 8 in the second load), bytes 16 (4 (l / 8 % 2) + l / 16) of the 128
+DEV int pair_row() { return lane_id() & 7; }
+DEV int pair_byte() { return ((lane_id() >> 1) & 4) * 16 + (lane_id() >> 4) * 16; }
+// a: rows 0 .. 7, b: rows 8 .. 15 -> a: bytes 16 g of the first 64 of row l % 16, b: of the second 64.  Lanes 8 .. 15 of each 16 of a
+// take lanes 0 .. 7 of b, and the other way round.
+DEV void pair_up(uint4& a, uint4& b) {
+  auto sw = [](uint32_t& p, uint32_t& q) {
+    const int o = (int)p, n = (int)q;
+    p = (uint32_t)__builtin_amdgcn_update_dpp(o, n, 0x128, 0xF, 0xC, false);  // row_ror:8 into lanes 8 .. 15
+    q = (uint32_t)__builtin_amdgcn_update_dpp(n, o, 0x128, 0xF, 0x3, false);  // into lanes 0 .. 7
+  };
+  sw(a.x, b.x), sw(a.y, b.y), sw(a.z, b.z), sw(a.w, b.w);
+}
+
+template <class SC>
 struct RowsQ4 {
   static constexpr bool perm = true;  // fragment order 0 4 1 5 2 6 3 7
-  uint4 w[HF];
-  uint2 s[HF];
+  uint4 w[2], s;
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K / 2; }
   static DEV size_t s_bytes(int N, int K) { return (size_t)N * K / 16; }
   static DEV int xoff(int g) { return 32 * (g & 1) + 16 * (g >> 1); }
+  // n: the tile's first row
   DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
-    const uint32_t p = off ? NOWHERE : n * (K / 2) + c * (64 * HF) + 16 * (lane_id() >> 4);
-    const uint32_t q = off ? NOWHERE : (n * (K / 64) + c * (2 * HF)) * 4;
-    w[0] = buf16(Q, p);
-    if constexpr (HF == 2) w[1] = buf16(Q, half ? NOWHERE : p + 64);
-    s[0] = buf8(S, q);
-    if constexpr (HF == 2) s[1] = buf8(S, half ? NOWHERE : q + 8);
+    const bool none = off || (half && (lane_id() & 8));
+    const uint32_t p = (n + pair_row()) * (K / 2) + c * 128 + pair_byte();
+    w[0] = buf16(Q, none ? NOWHERE : p);
+    w[1] = buf16(Q, none ? NOWHERE : p + 4 * K);
+    s = buf16(S, off ? NOWHERE : ((n + (lane_id() & 15)) * (K / 64) + c * 4) * 4);
   }
   // nibbles of a word as 16 + q in bf16: the nibble is the top four mantissa bits of a number in [16, 32)
   // (the two constants in registers, so that each pair of nibbles is a shift and one v_and_or_b32)
@@ -81,13 +96,15 @@ struct RowsQ4 {
   }
   // xsum: lane's sum of x over group l / 16 of row l % 16 (0 past the chunk's groups)
   template <int NP>
-  DEV void mac(const uint4 (&x)[NP][4 * HF], float xsum, f32x4& out) const {
+  DEV void mac(const uint4 (&x)[NP][8], float xsum, bool half, f32x4& out) {
     const int g = lane_id() >> 4;
-    const uint2 ow = HF == 2 && (g & 2) ? s[HF - 1] : s[0];
-    const float2 o = SC::pair(g & 1 ? ow.y : ow.x);
+    const uint32_t sw[4] = {s.x, s.y, half ? 0u : s.z, half ? 0u : s.w};
+    const uint32_t lo = g & 1 ? sw[1] : sw[0], hi = g & 1 ? sw[3] : sw[2];
+    const float2 o = SC::pair(g & 2 ? hi : lo);
     out = __builtin_amdgcn_mfma_f32_16x16x4f32(xsum, o.y - 16.f * o.x, out, 0, 0, 0);
+    pair_up(w[0], w[1]);
 #pragma unroll
-    for (int p = 0; p < HF; ++p) {
+    for (int p = 0; p < 2; ++p) {
       // lanes g = 0, 1 hold group 2 p, g = 2, 3 group 2 p + 1: two words of each change places
       const auto s02 = __builtin_amdgcn_permlane32_swap(w[p].x, w[p].z, false, false);
       const auto s13 = __builtin_amdgcn_permlane32_swap(w[p].y, w[p].w, false, false);
@@ -97,7 +114,7 @@ struct RowsQ4 {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < NP; ++q) a = mfma(x[q][4 * p + 2 * h], b0, a), a = mfma(x[q][4 * p + 2 * h + 1], b1, a);
-        const float sc = SC::pair(h ? s[p].y : s[p].x).x;
+        const float sc = SC::pair(sw[2 * p + h]).x;
 #pragma unroll
         for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
       }
@@ -107,26 +124,25 @@ struct RowsQ4 {
 
 // One byte per weight: 64 inputs of a row per 16-byte load of four lanes, scales per 128 inputs.  D: the
 // format's conversions
-template <class D, int HF>
+template <class D>
 struct Rows8 {
   static constexpr bool perm = false;
-  uint4 w[2 * HF];
-  uint32_t s[HF];
+  uint4 w[4];
+  uint32_t s[2];
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K; }
   static DEV int xoff(int g) { return 16 * g; }
   DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
-    const uint32_t p = off ? NOWHERE : n * K + c * (128 * HF) + 16 * (lane_id() >> 4);
-    w[0] = buf16(Q, p), w[1] = buf16(Q, off ? NOWHERE : p + 64);
-    s[0] = D::scale_raw(S, n, HF * c, K, off);
-    if constexpr (HF == 2) {
-      w[2] = buf16(Q, half ? NOWHERE : p + 128), w[3] = buf16(Q, half ? NOWHERE : p + 192);
-      s[1] = D::scale_raw(S, n, 2 * c + 1, K, half);
-    }
+    const uint32_t p = (n + pair_row()) * K + c * 256 + pair_byte();
+    w[0] = buf16(Q, off ? NOWHERE : p), w[1] = buf16(Q, off ? NOWHERE : p + 8 * K);
+    w[2] = buf16(Q, half ? NOWHERE : p + 128), w[3] = buf16(Q, half ? NOWHERE : p + 128 + 8 * K);
+    s[0] = D::scale_raw(S, n + (lane_id() & 15), 2 * c, K, off);
+    s[1] = D::scale_raw(S, n + (lane_id() & 15), 2 * c + 1, K, half);
   }
   template <int NP>
-  DEV void mac(const uint4 (&x)[NP][4 * HF], float, f32x4& out) const {
+  DEV void mac(const uint4 (&x)[NP][8], float, bool, f32x4& out) {
 #pragma unroll
-    for (int p = 0; p < HF; ++p) {
+    for (int p = 0; p < 2; ++p) {
+      pair_up(w[2 * p], w[2 * p + 1]);
       f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -143,8 +159,8 @@ struct Rows8 {
 };
 DEV uint32_t buf_half(const Rsrc& S, uint32_t off) { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(S, off, 0, 0); }
 
-template <int SF, int HF>
-struct RowsFP8 : Rows8<RowsFP8<SF, HF>, HF> {
+template <int SF>
+struct RowsFP8 : Rows8<RowsFP8<SF>> {
   static DEV size_t s_bytes(int N, int K) { return (size_t)(N / 128) * (K / 128) * (SF ? 2 : 4); }
   static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
     const uint32_t i = (n >> 7) * (K / 128) + b;
@@ -160,8 +176,8 @@ struct RowsFP8 : Rows8<RowsFP8<SF, HF>, HF> {
   }
 };
 
-template <class SH, int HF>
-struct RowsQ8 : Rows8<RowsQ8<SH, HF>, HF> {
+template <class SH>
+struct RowsQ8 : Rows8<RowsQ8<SH>> {
   static DEV size_t s_bytes(int N, int K) { return (size_t)N * (SH::per_row ? 1 : K / 128) * 2; }
   static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
     return buf_half(S, off ? NOWHERE : 2 * (SH::per_row ? n : n * (K / 128) + b));
@@ -175,23 +191,23 @@ struct RowsQ8 : Rows8<RowsQ8<SH, HF>, HF> {
 };
 
 // A lane's fragments of chunk c of the row at byte `row` (planes `plane` bytes apart); inputs past the row are zero
-template <class F, int NP, int HF>
-DEV void load_x(const Rsrc& X, uint32_t row, uint32_t plane, int c, bool half, uint4 (&x)[NP][4 * HF]) {
-  const uint32_t p = row + (c * (128 * HF) + F::xoff(lane_id() >> 4)) * 2;
+template <class F, int NP>
+DEV void load_x(const Rsrc& X, uint32_t row, uint32_t plane, int c, bool half, uint4 (&x)[NP][8]) {
+  const uint32_t p = row + (c * 256 + F::xoff(lane_id() >> 4)) * 2;
 #pragma unroll
   for (int q = 0; q < NP; ++q)
 #pragma unroll
-    for (int f = 0; f < 4 * HF; ++f)
+    for (int f = 0; f < 8; ++f)
       x[q][f] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(X, f >= 4 && half ? NOWHERE : p + 2 * (64 * (f >> 1) + 8 * (f & 1)),
                                                                                  q * plane, 0));
 }
 // the fragments in the weights' order, and the lane's group sum (RowsQ4)
-template <class F, int NP, int HF>
-DEV float order_x(uint4 (&x)[NP][4 * HF]) {
+template <class F, int NP>
+DEV float order_x(uint4 (&x)[NP][8]) {
   if constexpr (!F::perm) return 0.f;
   float own = 0.f;
 #pragma unroll
-  for (int G = 0; G < 2 * HF; ++G) {
+  for (int G = 0; G < 4; ++G) {
     float t = 0.f;
 #pragma unroll
     for (int q = NP - 1; q >= 0; --q)
@@ -275,45 +291,50 @@ __global__ void __launch_bounds__(MR_NT) k_moe_rows_router(MoeRows a) {
 }
 
 // ---- experts ----------------------------------------------------------------------------------
-// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 64 t, K = i).
+// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 32 t, K = i).
 // KS waves share a tile's inputs, a chunk each (cpw > 1: further chunks in turn); the other groups of waves (RG)
-// take further tiles, a step of the block being RG tiles.  The steps of all experts that were picked, ascending,
-// then of the shared expert, are dealt to the blocks in contiguous runs of even cost: a step's passes of 16 rows,
-// twice that where the shared expert's bytes are twice the others'.
-// A wave's x fragments stay in registers for all tiles of an expert (one pass, one chunk).  Two steps of weights
+// take further tiles, a step of the block being RG tiles.  Items are passes of up to 16 rows of an expert, ascending,
+// then of the shared expert (whose rows are all); their steps are dealt to the blocks in contiguous runs of even
+// cost, the shared expert's counting twice where its bytes are twice the others'.  (All passes of an expert as one
+// item fetch its weights once but x again for every tile and pass: 64 rows 202 us against 152.)
+// A wave's x fragments stay in registers for all tiles of an item (where it has one chunk).  Two steps of weights
 // are in flight: a tile's registers take the tile two steps on as soon as it is used.  The KS sums meet in LDS, behind a
 // barrier that leaves the loads in flight.
 template <int MODE, class F, class FS>
 __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS, int cpw, int fs_cost) {
-  constexpr int NP = MODE == 0 ? 1 : 3, HF = MODE == 0 ? 2 : 1, CH = 128 * HF, TL = MODE == 0 ? 2 : 4;
+  constexpr int NP = MODE == 0 ? 1 : 3, TL = 2;
   __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert
-  __shared__ int s_cnt[257], s_e[257], s_off[258], s_cum[258], s_tot[8][3], s_first;
+  __shared__ uint32_t s_rows[256][2];
+  __shared__ int s_start[256], s_e[MR_ITEMS], s_off[MR_ITEMS], s_num[MR_ITEMS], s_cum[MR_ITEMS + 1], s_tot[8][3], s_first;
   __shared__ float red[2][MR_NW][TL][4][64];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
   const int pairs = a.rows * a.topk;
-  const int K = MODE == 0 ? a.h : a.i, RG = MR_NW / KS, tiles = MODE == 0 ? a.i / 16 : a.h / 64;
+  const int K = MODE == 0 ? a.h : a.i, RG = MR_NW / KS, tiles = MODE == 0 ? a.i / 16 : a.h / 32;
   const int steps = (tiles + RG - 1) / RG;
   const int N = MODE == 0 ? 2 * a.i : a.h;
-  const int nch = (K + CH - 1) / CH, wk = wave % KS, rg = wave / KS;
-  // rows of each expert
+  const int nch = (K + 255) / 256, wk = wave % KS, rg = wave / KS;
+  // rows of each expert as a 64-bit mask (a row picks an expert once), so that every block has the same passes
   constexpr int PPT = MR_PAIRS / MR_NT;
-  int pe[PPT], pp[PPT];
+  int pe[PPT];
 #pragma unroll
   for (int q = 0; q < PPT; ++q) pe[q] = tid + MR_NT * q < pairs ? a.idx[tid + MR_NT * q] & 255 : -1;
-  if (tid < 257) s_cnt[tid] = 0;
+  if (tid < 256) s_rows[tid][0] = s_rows[tid][1] = 0;
   lds_barrier();
 #pragma unroll
   for (int q = 0; q < PPT; ++q)
-    if (pe[q] >= 0) pp[q] = atomicAdd(&s_cnt[pe[q]], 1);
+    if (pe[q] >= 0) {
+      const int r = (tid + MR_NT * q) / a.topk;
+      atomicOr(&s_rows[pe[q]][r >> 5], 1u << (r & 31));
+    }
   lds_barrier();
-  // exclusive sums over the experts (thread e) of their rows, of being picked and of their cost
+  // sums over the experts (thread e) of their rows, their passes and their cost
   {
     int v[3] = {0, 0, 0}, own[3];
     if (tid <= 256) {
       const bool sh = tid == 256;
-      v[0] = sh ? (a.shared ? a.rows : 0) : s_cnt[tid];
-      v[1] = v[0] > 0;
-      v[2] = (v[0] + 15) / 16 * steps * (sh ? fs_cost : 1);
+      v[0] = sh ? (a.shared ? a.rows : 0) : __builtin_popcount(s_rows[tid][0]) + __builtin_popcount(s_rows[tid][1]);
+      v[1] = (v[0] + 15) / 16;
+      v[2] = v[1] * steps * (sh ? fs_cost : 1);
     }
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
@@ -330,15 +351,15 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
 #pragma unroll
       for (int q = 0; q < 3; ++q) base[q] += s_tot[w][q];
     lds_barrier();
-    if (tid <= 256 && own[1]) {
-      const int d = base[1] + v[1] - 1;
-      s_e[d] = tid, s_off[d] = base[0] + v[0] - own[0], s_cum[d] = base[2] + v[2] - own[2];
-      if (tid < 256) s_cnt[tid] = base[0] + v[0] - own[0];  // from here on: where the expert's rows start
+    if (tid <= 256) {
+      const int off = base[0] + v[0] - own[0], cum = base[2] + v[2] - own[2];
+      for (int p = 0; p < own[1]; ++p) {
+        const int d = base[1] + v[1] - own[1] + p;
+        s_e[d] = tid, s_off[d] = off + 16 * p, s_num[d] = own[0] - 16 * p < 16 ? own[0] - 16 * p : 16, s_cum[d] = cum + own[2] / own[1] * p;
+      }
+      if (tid < 256) s_start[tid] = off;
     }
-    if (tid == 256) {
-      const int D = base[1] + v[1];
-      s_off[D] = base[0] + v[0], s_cum[D] = base[2] + v[2], s_tot[0][0] = D;
-    }
+    if (tid == 256) s_cum[base[1] + v[1]] = base[2] + v[2], s_tot[0][0] = base[1] + v[1];
     lds_barrier();
   }
   const int D = s_tot[0][0];
@@ -346,46 +367,50 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
   if (tid < D && s_cum[tid] <= lo && lo < s_cum[tid + 1]) s_first = tid;
 #pragma unroll
   for (int q = 0; q < PPT; ++q)
-    if (pe[q] >= 0) s_list[s_cnt[pe[q]] + pp[q]] = tid + MR_NT * q;
+    if (pe[q] >= 0) {
+      const int r = (tid + MR_NT * q) / a.topk;
+      const uint32_t lo32 = s_rows[pe[q]][0], hi32 = s_rows[pe[q]][1], below = (1u << (r & 31)) - 1;
+      s_list[s_start[pe[q]] + (r < 32 ? __builtin_popcount(lo32 & below) : __builtin_popcount(lo32) + __builtin_popcount(hi32 & below))] =
+          tid + MR_NT * q;
+    }
   if (a.shared && tid < a.rows) s_list[pairs + tid] = pairs + tid;
   lds_barrier();
   if (lo >= hi) return;
   int par = 0;
   const size_t plane = (size_t)(pairs + a.rows) * a.i;
   for (int d = s_first; d < D && s_cum[d] < hi; ++d) {
-    const int e = __builtin_amdgcn_readfirstlane(s_e[d]), off = s_off[d], cnt = s_off[d + 1] - off;
+    const int e = __builtin_amdgcn_readfirstlane(s_e[d]), off = s_off[d], cnt = s_num[d];
     const int cum = s_cum[d], tc = (s_cum[d + 1] - cum) / steps;
     const int t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0, t1 = (hi - cum + tc - 1) / tc < steps ? (hi - cum + tc - 1) / tc : steps;
     if (t0 >= t1) continue;
-    const int passes = (cnt + 15) / 16;
     const bool sh = e == 256;
     auto segment = [&](auto fmt, const void* Qp, const void* Sp) __attribute__((always_inline)) {
       using Fm = decltype(fmt);
       const Rsrc Q = rsrc(Qp, (uint32_t)Fm::q_bytes(N, K)), S = rsrc(Sp, (uint32_t)Fm::s_bytes(N, K));
       const Rsrc X = MODE == 0 ? rsrc(a.x, (uint32_t)a.rows * K * 2) : rsrc(a.act, (uint32_t)(6 * plane));
       Fm w[2][TL];
-      uint4 x[NP][4 * HF];
-      auto half_of = [&](int c) { return HF == 2 && c * CH + 128 >= K; };
+      uint4 x[NP][8];
+      auto half_of = [&](int c) { return c * 256 + 128 >= K; };
       auto load_w = [&](Fm& f, int i, int t, int ci) __attribute__((always_inline)) {
         const int c = wk + KS * ci, tile = t * RG + rg;
         const bool none = (t >= t1) | (tile >= tiles) | (rg >= RG) | (c >= nch);
-        f.load(Q, S, MODE == 0 ? 16 * tile + (lane & 15) + i * a.i : 64 * tile + 16 * i + (lane & 15), K, c, none | half_of(c), none);
+        f.load(Q, S, MODE == 0 ? 16 * tile + i * a.i : 32 * tile + 16 * i, K, c, none | half_of(c), none);
         __builtin_amdgcn_sched_barrier(0);
       };
-      auto fetch_x = [&](int p, int ci) __attribute__((always_inline)) {
-        const int m = 16 * p + (lane & 15), pr = s_list[off + (m < cnt ? m : cnt - 1)], c = wk + KS * ci;
+      auto fetch_x = [&](int ci) __attribute__((always_inline)) {
+        const int m = lane & 15, pr = s_list[off + (m < cnt ? m : cnt - 1)], c = wk + KS * ci;
         const int row = MODE == 1 ? pr : sh ? pr - pairs : pr / a.topk;
-        load_x<Fm, NP, HF>(X, c < nch ? (uint32_t)(row * K * 2) : NOWHERE, (uint32_t)(2 * plane), c, half_of(c), x);
+        load_x<Fm, NP>(X, c < nch ? (uint32_t)(row * K * 2) : NOWHERE, (uint32_t)(2 * plane), c, half_of(c), x);
         __builtin_amdgcn_sched_barrier(0);
       };
-      // the KS sums of a step's tiles (pass p of t), and what becomes of them
-      auto finish = [&](const f32x4 (&o)[TL], int t, int p) __attribute__((always_inline)) {
+      // the KS sums of step t's tiles, and what becomes of them
+      auto finish = [&](const f32x4 (&o)[TL], int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < TL; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) red[par][wave][i][r][lane] = o[i][r];
         lds_barrier();
-        const int tile = t * RG + rg, m0 = 16 * p, nr = tile < tiles && rg < RG ? (cnt - m0 < 16 ? cnt - m0 : 16) : 0;
+        const int tile = t * RG + rg, nr = tile < tiles && rg < RG ? cnt : 0;
         // register r of lane l: row 4 (l / 16) + r of x, column l % 16; the KS waves share the registers
         auto part = [&](auto ks) __attribute__((always_inline)) {
           constexpr int KK = decltype(ks)::value;
@@ -403,7 +428,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
             const int r = q & 3, row = 4 * (lane >> 4) + r;
             if (r >= nr) continue;
             const bool live = row < nr;
-            const int pr = s_list[off + (live ? m0 + row : 0)];
+            const int pr = s_list[off + (live ? row : 0)];
             if constexpr (MODE == 0) {
               const float g = total(0, r), v = total(1, r);
               if (live) {
@@ -417,7 +442,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
               }
             } else {
               const float v = total(q >> 2, r);
-              if (live) a.yp[(size_t)pr * a.h + 64 * tile + 16 * (q >> 2) + (lane & 15)] = v;
+              if (live) a.yp[(size_t)pr * a.h + 32 * tile + 16 * (q >> 2) + (lane & 15)] = v;
             }
           }
         };
@@ -429,17 +454,17 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
       };
       const f32x4 z = {0.f, 0.f, 0.f, 0.f};
       f32x4 o[TL];
-      if (passes == 1 && cpw == 1) {  // x stays
+      if (cpw == 1) {  // x stays
 #pragma unroll
         for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t0, 0);
-        fetch_x(0, 0);
+        fetch_x(0);
 #pragma unroll
         for (int i = 0; i < TL; ++i) load_w(w[1][i], i, t0 + 1, 0);
-        const float xs = order_x<Fm, NP, HF>(x);
+        const float xs = order_x<Fm, NP>(x);
         auto body = [&](Fm (&f)[TL], int t) __attribute__((always_inline)) {
 #pragma unroll
-          for (int i = 0; i < TL; ++i) o[i] = z, f[i].template mac<NP>(x, xs, o[i]), load_w(f[i], i, t + 2, 0);
-          finish(o, t, 0);
+          for (int i = 0; i < TL; ++i) o[i] = z, f[i].template mac<NP>(x, xs, half_of(wk), o[i]), load_w(f[i], i, t + 2, 0);
+          finish(o, t);
         };
         for (int t = t0;;) {
           body(w[0], t);
@@ -448,33 +473,30 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
           if (++t >= t1) break;
         }
       } else {
-        // step, pass and chunk of the one ahead (x) and of the two ahead (weights)
-        int t = t0, p = 0, ci = 0, tx = t0, px = 0, cx = 0, tw = t0, pw = 0, cw = 0;
-        auto next = [&](int& t, int& p, int& ci) {
-          if (++ci < cpw) return;
-          ci = 0;
-          if (++p < passes) return;
-          p = 0, ++t;
+        // step and chunk, and those of the one ahead (x) and the two ahead (weights)
+        int t = t0, ci = 0, tx = t0, cx = 0, tw = t0, cw = 0;
+        auto next = [&](int& t, int& ci) {
+          if (++ci == cpw) ci = 0, ++t;
         };
 #pragma unroll
         for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t0, 0);
-        fetch_x(0, 0);
-        next(tw, pw, cw), next(tx, px, cx);
+        fetch_x(0);
+        next(tw, cw), next(tx, cx);
 #pragma unroll
         for (int i = 0; i < TL; ++i) load_w(w[1][i], i, tw, cw);
         auto body = [&](Fm (&f)[TL]) __attribute__((always_inline)) {
-          const float xs = order_x<Fm, NP, HF>(x);
+          const float xs = order_x<Fm, NP>(x);
           if (ci == 0)
 #pragma unroll
             for (int i = 0; i < TL; ++i) o[i] = z;
 #pragma unroll
-          for (int i = 0; i < TL; ++i) f[i].template mac<NP>(x, xs, o[i]);
-          fetch_x(px, cx);
-          next(tx, px, cx), next(tw, pw, cw);
+          for (int i = 0; i < TL; ++i) f[i].template mac<NP>(x, xs, half_of(wk + KS * ci), o[i]);
+          fetch_x(cx);
+          next(tx, cx), next(tw, cw);
 #pragma unroll
           for (int i = 0; i < TL; ++i) load_w(f[i], i, tw, cw);
-          if (ci == cpw - 1) finish(o, t, p);
-          next(t, p, ci);
+          if (ci == cpw - 1) finish(o, t);
+          next(t, ci);
         };
         for (;;) {
           body(w[0]);
@@ -534,14 +556,14 @@ struct WsLayout {
 // The waves that share a tile's K inputs and the chunks each takes: a wave per chunk up to all eight.
 struct Split {
   int ks, cpw;
-  Split(int K, int ch) {
-    const int nch = (K + ch - 1) / ch;
+  Split(int K) {
+    const int nch = (K + 255) / 256;
     cpw = (nch + MR_NW - 1) / MR_NW;
     ks = (nch + cpw - 1) / cpw;
   }
 };
 
-template <class F2, class F1, class SH, bool BYTES>
+template <class F, class SH, bool BYTES>
 int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   if (!rows_shape_ok(a.rows, a.e, a.h, a.i, a.topk)) return -1;
   const int given = (a.sgu_q != nullptr) + (a.sgu_s != nullptr) + (a.sd_q != nullptr) + (a.sd_s != nullptr);
@@ -562,9 +584,9 @@ int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   else if (a.rows <= 8) hipLaunchKernelGGL(k_moe_rows_router<2>, dim3(nb, (a.rows + 1) / 2), dim3(MR_NT), 0, st, a);
   else if (a.rows <= 32) hipLaunchKernelGGL(k_moe_rows_router<4>, dim3(nb, (a.rows + 3) / 4), dim3(MR_NT), 0, st, a);
   else hipLaunchKernelGGL(k_moe_rows_router<8>, dim3(nb, (a.rows + 7) / 8), dim3(MR_NT), 0, st, a);
-  const Split g(a.h, 256), d(a.i, 128);
-  hipLaunchKernelGGL((k_moe_rows_experts<0, F2, RowsQ8<SH, 2>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, g.ks, g.cpw, BYTES ? 1 : 2);
-  hipLaunchKernelGGL((k_moe_rows_experts<1, F1, RowsQ8<SH, 1>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, d.ks, d.cpw, BYTES ? 1 : 2);
+  const Split g(a.h), d(a.i);
+  hipLaunchKernelGGL((k_moe_rows_experts<0, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, g.ks, g.cpw, BYTES ? 1 : 2);
+  hipLaunchKernelGGL((k_moe_rows_experts<1, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, d.ks, d.cpw, BYTES ? 1 : 2);
   hipLaunchKernelGGL(k_moe_rows_combine, dim3(a.rows, (a.h + 1023) / 1024), dim3(256), 0, st, a);
   return 0;
 }
@@ -575,17 +597,16 @@ API size_t dr_moe_layer_rows_ws(int rows, int e, int h, int i, int topk) {
   return rows_shape_ok(rows, e, h, i, topk) ? WsLayout(rows, e, h, i, topk).bytes : 0;
 }
 
-#define MOE_ROWS_ENTRY(NAME, S, F2, F1, SH, BYTES)                                                                        \
+#define MOE_ROWS_ENTRY(NAME, S, F, SH, BYTES)                                                                             \
   API int NAME(const uint16_t* router, const uint8_t* gu_q, const S* gu_s, const uint8_t* d_q, const S* d_s,              \
                const int8_t* sgu_q, const uint16_t* sgu_s, const int8_t* sd_q, const uint16_t* sd_s, const uint16_t* x,   \
                const float* res, int* idx, float* wts, float* sgate, void* ws, float* y, int rows, int e, int h, int i,   \
                int topk, hipStream_t st) {                                                                                \
     const MoeRows a{router, gu_q, d_q, gu_s, d_s, sgu_q, sd_q, sgu_s, sd_s, x, res, idx, wts, sgate, y, nullptr, nullptr, \
                     nullptr, nullptr, rows, e, h, i, topk, 0};                                                            \
-    return moe_rows<F2, F1, SH, BYTES>(a, ws, st);                                                                        \
+    return moe_rows<F, SH, BYTES>(a, ws, st);                                                                             \
   }
-#define ROWS_ARG(...) __VA_ARGS__
-MOE_ROWS_ENTRY(dr_moe_layer_rows, uint16_t, ROWS_ARG(RowsQ4<ScaleF16, 2>), ROWS_ARG(RowsQ4<ScaleF16, 1>), Q8G128F16, false)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_bf16s, uint16_t, ROWS_ARG(RowsQ4<ScaleBF16, 2>), ROWS_ARG(RowsQ4<ScaleBF16, 1>), Q8RowBF16, false)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8, float, ROWS_ARG(RowsFP8<0, 2>), ROWS_ARG(RowsFP8<0, 1>), Q8G128F16, true)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8_bf16s, uint16_t, ROWS_ARG(RowsFP8<1, 2>), ROWS_ARG(RowsFP8<1, 1>), Q8RowBF16, true)
+MOE_ROWS_ENTRY(dr_moe_layer_rows, uint16_t, RowsQ4<ScaleF16>, Q8G128F16, false)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_bf16s, uint16_t, RowsQ4<ScaleBF16>, Q8RowBF16, false)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8, float, RowsFP8<0>, Q8G128F16, true)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8_bf16s, uint16_t, RowsFP8<1>, Q8RowBF16, true)
