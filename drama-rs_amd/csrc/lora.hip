@@ -2,8 +2,8 @@
 //   y[r] = res[r] + W x[r] + s_a B_a (A_a x[r]),   a = adapter[r].
 //
 // Two launches.  k_lora_down: t[r] = s_a A_a x[r] (fp32), a block per 16 rows and distinct adapter among them, so
-// rows that share an adapter share its fetch whatever their order.  k_lora_gemm: W x on
-// v_mfma_f32_16x16x32_bf16 (int8 is exact in bf16, the scales enter the fp32 sums), with B_a t and the residual
+// rows that share an adapter share its fetch whatever their order.  k_lora_gemm_rows (few rows) and k_lora_gemm_tiles:
+// W x on v_mfma_f32_16x16x32_bf16 (int8 is exact in bf16, the scales enter the fp32 sums), with B_a t and the residual
 // added to each output before its one store.
 #include "common.hpp"
 
@@ -30,6 +30,8 @@ struct Lora {
   float *t, *y;
   size_t ldx, ldy;
   int adapters, rmax, rows, n, k;
+  uint16_t* planes;  // t as three bf16 planes [rows, rp] whose sum it is, zero past the rank (k_lora_gemm_tiles), or null
+  int rp;            // rmax rounded up to the 32 of an MFMA
 };
 
 constexpr int LR_NW = 8, LR_NT = LR_NW * 64;
@@ -80,7 +82,21 @@ __global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
       float v = 0.f;
 #pragma unroll
       for (int w = 0; w < LR_NW; ++w) v += red[w][l][q];
-      if (j < a.rmax && adapter_of(a, row) == ad) a.t[(size_t)row * a.rmax + j] = j < rk ? a.lscale[ad] * v : 0.f;
+      if (adapter_of(a, row) == ad) {
+        v = j < rk ? a.lscale[ad] * v : 0.f;
+        if (!a.planes) {
+          if (j < a.rmax) a.t[(size_t)row * a.rmax + j] = v;
+        } else {
+          // 8 mantissa bits each, the last exact: hi + mid + lo = v
+          const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u), r1 = v - hi;
+          const float mi = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi;
+          uint16_t* p = a.planes + (size_t)row * a.rp + j;
+          const size_t plane = (size_t)a.rows * a.rp;
+          p[0] = (uint16_t)(__float_as_uint(hi) >> 16);
+          p[plane] = (uint16_t)(__float_as_uint(mi) >> 16);
+          p[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
+        }
+      }
     }
   }
 }
@@ -142,6 +158,175 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
   }
 }
 
+// Many rows: a block of 2 x 2 waves owns 32 MT rows x 32 NT columns, a wave 16 MT x 16 NT of them.  Slices of 64 inputs
+// go through two LDS buffers (x as it is, W converted to bf16 on its way there, once per block), a slice's
+// global loads in flight for the whole of the slice before; the barrier between slices leaves them in flight.  Row r's 16-byte
+// piece j lies at j ^ (r % 8), so the fragment reads meet no bank twice.
+// 8 XCDs take the tiles in 8 contiguous runs, down columns of 8 row tiles, so that an XCD's blocks share x and W in its L2.
+constexpr int LG_K = 64;
+template <class SH, int MT, int NT>
+__global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int tn) {
+  constexpr int BM = 32 * MT, BN = 32 * NT, PX = BM * 8 / 256, PW = BN * 4 / 256;
+  static_assert(PX * 256 == BM * 8 && PW * 256 == BN * 4, "pieces per thread");
+  __shared__ uint4 lx[2][BM * 8], lw[2][BN * 8];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
+  // tile of this block
+  const int total = tm * tn, per = (total + 7) / 8, q = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || q >= total) return;
+  const int band = q / (8 * tn), bh = tm - 8 * band < 8 ? tm - 8 * band : 8, in = q - band * 8 * tn;
+  const int m0 = (8 * band + in % bh) * BM, n0 = in / bh * BN;
+  const uint16_t* xp[PX];
+  const uint8_t* wp[PW];
+#pragma unroll
+  for (int i = 0; i < PX; ++i) {
+    const int r = m0 + (tid + 256 * i) / 8;
+    xp[i] = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + 8 * (tid & 7);
+  }
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    const int n = n0 + (tid + 256 * i) / 4;
+    wp[i] = reinterpret_cast<const uint8_t*>(a.w) + (size_t)(n < a.n ? n : a.n - 1) * a.k + 16 * (tid & 3);
+  }
+  uint4 xv[PX], wv[PW];
+  auto load = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PX; ++i) xv[i] = ld16(xp[i] + k);
+#pragma unroll
+    for (int i = 0; i < PW; ++i) wv[i] = ld16(wp[i] + k);
+  };
+  auto store = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PX; ++i) {
+      const int r = (tid + 256 * i) / 8, j = tid & 7;
+      lx[b][r * 8 + (j ^ (r & 7))] = xv[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int r = (tid + 256 * i) / 4, j = 2 * (tid & 3);
+      lw[b][r * 8 + (j ^ (r & 7))] = frag8(wv[i].x, wv[i].y);
+      lw[b][r * 8 + ((j + 1) ^ (r & 7))] = frag8(wv[i].z, wv[i].w);
+    }
+  };
+  const int wm = (wave >> 1) * 16 * MT, wn = (wave & 1) * 16 * NT;
+  f32x4 acc[MT][NT], sum[MT][NT];
+  const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = sum[m][n] = z;
+  size_t col[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int c = n0 + wn + 16 * n + c16;
+    col[n] = c < a.n ? c : a.n - 1;
+  }
+  const int steps = a.k / LG_K;  // even: k is a multiple of 128
+  load(0);
+  store(0);
+  load(LG_K);
+  lds_barrier();
+  auto step = [&](auto odd, int s) __attribute__((always_inline)) {
+    constexpr int B = decltype(odd)::value;
+    if (s + 1 < steps) {
+      store(B ^ 1);
+      load(s + 2 < steps ? (s + 2) * LG_K : (s + 1) * LG_K);
+    }
+    float sc[NT];
+    if constexpr (B == 1 && !SH::per_row) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[n] = SH::scale(a.s, col[n], s * LG_K, a.k);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      uint4 xf[MT], wf[NT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int r = wm + 16 * m + c16;
+        xf[m] = lx[B][r * 8 + ((4 * kk + g) ^ (r & 7))];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int r = wn + 16 * n + c16;
+        wf[n] = lw[B][r * 8 + ((4 * kk + g) ^ (r & 7))];
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = mfma(xf[m], wf[n], acc[m][n]);
+    }
+    if constexpr (B == 1 && !SH::per_row) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[m][n][r] = __builtin_fmaf(sc[n], acc[m][n][r], sum[m][n][r]);
+          acc[m][n] = z;
+        }
+    }
+    lds_barrier();
+  };
+  for (int s = 0; s < steps; s += 2) {
+    step(std::integral_constant<int, 0>{}, s);
+    step(std::integral_constant<int, 1>{}, s + 1);
+  }
+  if constexpr (SH::per_row) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float sc = SH::scale(a.s, col[n], 0, a.k);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[m][n][r] = sc * acc[m][n][r];
+    }
+  }
+  // B t: for each 16 rows their distinct adapters, rows of others zero
+  if (a.adapter) {
+    const size_t plane = (size_t)a.rows * a.rp;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = m0 + wm + 16 * m + c16, mine = adapter_of(a, row);
+      uint32_t left = (uint32_t)__ballot(mine >= 0) & 0xffffu;
+      while (left) {
+        const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
+        left &= ~(uint32_t)__ballot(mine == ad);
+        const int rk = rank_of(a, ad);
+        const uint16_t* tp = a.planes + (size_t)(mine == ad ? row : 0) * a.rp + 8 * g;
+        for (int j = 0; j < rk; j += 32) {
+          uint4 tf[3];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) tf[p] = mine == ad ? ld16(tp + p * plane + j) : make_uint4(0, 0, 0, 0);
+          const int on = rk - j - 8 * g;  // of this lane's 8 ranks, those below rk
+          const uint32_t k0 = on >= 2 ? 0xffffffffu : on == 1 ? 0xffffu : 0u, k1 = on >= 4 ? 0xffffffffu : on == 3 ? 0xffffu : 0u;
+          const uint32_t k2 = on >= 6 ? 0xffffffffu : on == 5 ? 0xffffu : 0u, k3 = on >= 8 ? 0xffffffffu : on == 7 ? 0xffffu : 0u;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint4 b = make_uint4(0, 0, 0, 0);
+            if (on > 0) b = ld16(a.lb + ((size_t)ad * a.n + col[n]) * a.rmax + j + 8 * g);
+            b = make_uint4(b.x & k0, b.y & k1, b.z & k2, b.w & k3);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) sum[m][n] = mfma(tf[p], b, sum[m][n]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = m0 + wm + 16 * m + 4 * g + r;
+      if (row >= a.rows) continue;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int c = n0 + wn + 16 * n + c16;
+        if (c >= a.n) continue;
+        const size_t o = row * a.ldy + c;
+        a.y[o] = a.res ? a.res[o] + sum[m][n][r] : sum[m][n][r];
+      }
+    }
+}
+
 bool lora_shape_ok(int rows, int n, int k, int rmax) {
   return rows >= 0 && rows <= (1 << 20) && n >= 1 && k >= 128 && k <= 16384 && k % 128 == 0 && rmax >= 8 && rmax <= 128 && rmax % 8 == 0;
 }
@@ -156,30 +341,42 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
     return -1;
   a.ldx = ldx, a.ldy = ldy;
   if (a.t) a.t += 64;  // the first 256 bytes of the workspace hold counters
-  const long long tiles = ((long long)a.rows + 15) / 16;
-  if (a.adapter)
-    hipLaunchKernelGGL(k_lora_down, dim3((unsigned)tiles, 16, (a.rmax + 15) / 16), dim3(LR_NT), 0, st, a);
-  const dim3 g((a.n + 15) / 16, (unsigned)((tiles + 3) / 4));
-  hipLaunchKernelGGL((k_lora_gemm_rows<SH, 4>), g, dim3(LR_NT), 0, st, a);
+  const int tiles = (a.rows + 15) / 16;
+  const bool few = a.rows <= 64;
+  a.rp = (a.rmax + 31) & ~31;
+  a.planes = few || !a.adapter ? nullptr : reinterpret_cast<uint16_t*>(a.t);
+  if (a.adapter) hipLaunchKernelGGL(k_lora_down, dim3(tiles, few ? 16 : 2, few ? (a.rmax + 15) / 16 : a.rp / 16), dim3(LR_NT), 0, st, a);
+  if (few) {
+    hipLaunchKernelGGL((k_lora_gemm_rows<SH, 4>), dim3((a.n + 15) / 16, 1), dim3(LR_NT), 0, st, a);
+    return 0;
+  }
+  auto go = [&](auto mt, auto nt) {
+    constexpr int M = decltype(mt)::value, N = decltype(nt)::value;
+    const long long tm = (a.rows + 32ll * M - 1) / (32 * M), tn = (a.n + 32ll * N - 1) / (32 * N), per = (tm * tn + 7) / 8;
+    hipLaunchKernelGGL((k_lora_gemm_tiles<SH, M, N>), dim3((unsigned)(8 * per)), dim3(256), 0, st, a, (int)tm, (int)tn);
+  };
+  if ((long long)((a.rows + 127) / 128) * ((a.n + 127) / 128) >= 256) go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+  else go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
   return 0;
 }
 
 }  // namespace
 
 API size_t dr_gemm_q8_lora_ws(int rows, int n, int k, int rmax) {
-  return lora_shape_ok(rows, n, k, rmax) ? (((size_t)rows * rmax * 4 + 255) & ~(size_t)255) + 256 : 0;
+  // counters, then t: fp32 of rmax ranks or three bf16 planes of rmax rounded up to 32
+  return lora_shape_ok(rows, n, k, rmax) ? 256 + (((size_t)rows * ((rmax + 31) & ~31) * 6 + 255) & ~(size_t)255) : 0;
 }
 
 API int dr_gemm_q8_lora(const int8_t* w, const uint16_t* s, const uint16_t* x, int ldx, const int* adapter, const uint16_t* la,
                         const uint16_t* lb, const int* rank, const float* lscale, int adapters, int rmax, void* ws,
                         const float* res, float* y, int ldy, int rows, int n, int k, hipStream_t st) {
-  return gemm_lora<Q8G128F16>(Lora{w, s, x, adapter, la, lb, rank, lscale, res, static_cast<float*>(ws), y, 0, 0, adapters, rmax, rows, n, k},
+  return gemm_lora<Q8G128F16>(Lora{w, s, x, adapter, la, lb, rank, lscale, res, static_cast<float*>(ws), y, 0, 0, adapters, rmax, rows, n, k, nullptr, 0},
                               ldx, ldy, st);
 }
 
 API int dr_gemm_q8_lora_bf16s(const int8_t* w, const uint16_t* s, const uint16_t* x, int ldx, const int* adapter,
                               const uint16_t* la, const uint16_t* lb, const int* rank, const float* lscale, int adapters, int rmax,
                               void* ws, const float* res, float* y, int ldy, int rows, int n, int k, hipStream_t st) {
-  return gemm_lora<Q8RowBF16>(Lora{w, s, x, adapter, la, lb, rank, lscale, res, static_cast<float*>(ws), y, 0, 0, adapters, rmax, rows, n, k},
+  return gemm_lora<Q8RowBF16>(Lora{w, s, x, adapter, la, lb, rank, lscale, res, static_cast<float*>(ws), y, 0, 0, adapters, rmax, rows, n, k, nullptr, 0},
                               ldx, ldy, st);
 }
