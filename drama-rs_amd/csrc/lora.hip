@@ -280,36 +280,65 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
         for (int r = 0; r < 4; ++r) sum[m][n][r] = sc * acc[m][n][r];
     }
   }
-  // B t: for each 16 rows their distinct adapters, rows of others zero
+  // the residual, all of it in flight beside the adapters (y may be res: its loads could not pass the stores)
+  f32x4 rv[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = m0 + wm + 16 * m + 4 * g + r;
+        rv[m][n][r] = a.res ? gld<float>(a.res + (size_t)(row < a.rows ? row : a.rows - 1) * a.ldy + col[n]) : 0.f;
+      }
+  // B t: the distinct adapters of the wave's rows, the t of other rows zero; B's fragments serve all row tiles
   if (a.adapter) {
     const size_t plane = (size_t)a.rows * a.rp;
+    int mine[MT];
+    uint32_t left[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int row = m0 + wm + 16 * m + c16, mine = adapter_of(a, row);
-      uint32_t left = (uint32_t)__ballot(mine >= 0) & 0xffffu;
-      while (left) {
-        const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
-        left &= ~(uint32_t)__ballot(mine == ad);
-        const int rk = rank_of(a, ad);
-        const uint16_t* tp = a.planes + (size_t)(mine == ad ? row : 0) * a.rp + 8 * g;
-        for (int j = 0; j < rk; j += 32) {
-          uint4 tf[3];
+      mine[m] = adapter_of(a, m0 + wm + 16 * m + c16);
+      left[m] = (uint32_t)__ballot(mine[m] >= 0) & 0xffffu;
+    }
 #pragma unroll
-          for (int p = 0; p < 3; ++p) tf[p] = mine == ad ? ld16(tp + p * plane + j) : make_uint4(0, 0, 0, 0);
+    for (int f = 0; f < MT; ++f)
+      while (left[f]) {
+        const int ad = __builtin_amdgcn_readlane(mine[f], __builtin_ctz(left[f]));
+        bool has[MT];
+#pragma unroll
+        for (int m = f; m < MT; ++m) {
+          const uint32_t b = (uint32_t)__ballot(mine[m] == ad) & 0xffffu;
+          has[m] = b != 0, left[m] &= ~b;
+        }
+        const int rk = rank_of(a, ad);
+        for (int j = 0; j < rk; j += 32) {
+          uint4 tf[MT][3], b[NT];
           const int on = rk - j - 8 * g;  // of this lane's 8 ranks, those below rk
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            b[n] = make_uint4(0, 0, 0, 0);
+            if (on > 0) b[n] = ld16(a.lb + ((size_t)ad * a.n + col[n]) * a.rmax + j + 8 * g);
+          }
+#pragma unroll
+          for (int m = f; m < MT; ++m) {
+            const uint16_t* tp = a.planes + (size_t)(mine[m] == ad ? m0 + wm + 16 * m + c16 : 0) * a.rp + 8 * g + j;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) tf[m][p] = has[m] && mine[m] == ad ? ld16(tp + p * plane) : make_uint4(0, 0, 0, 0);
+          }
           const uint32_t k0 = on >= 2 ? 0xffffffffu : on == 1 ? 0xffffu : 0u, k1 = on >= 4 ? 0xffffffffu : on == 3 ? 0xffffu : 0u;
           const uint32_t k2 = on >= 6 ? 0xffffffffu : on == 5 ? 0xffffu : 0u, k3 = on >= 8 ? 0xffffffffu : on == 7 ? 0xffffu : 0u;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (on > 0) b = ld16(a.lb + ((size_t)ad * a.n + col[n]) * a.rmax + j + 8 * g);
-            b = make_uint4(b.x & k0, b.y & k1, b.z & k2, b.w & k3);
+          for (int n = 0; n < NT; ++n) b[n] = make_uint4(b[n].x & k0, b[n].y & k1, b[n].z & k2, b[n].w & k3);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) sum[m][n] = mfma(tf[p], b, sum[m][n]);
-          }
+          for (int m = f; m < MT; ++m)
+            if (has[m])
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int p = 0; p < 3; ++p) sum[m][n] = mfma(tf[m][p], b[n], sum[m][n]);
         }
       }
-    }
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -320,9 +349,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int c = n0 + wn + 16 * n + c16;
-        if (c >= a.n) continue;
-        const size_t o = row * a.ldy + c;
-        a.y[o] = a.res ? a.res[o] + sum[m][n][r] : sum[m][n][r];
+        if (c < a.n) a.y[row * a.ldy + c] = rv[m][n][r] + sum[m][n][r];
       }
     }
 }
