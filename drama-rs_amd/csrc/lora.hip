@@ -104,57 +104,92 @@ __global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
 // ---- y = res + W x + B t -----------------------------------------------------------------------
 DEV uint32_t pk8(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
   const float a = (float)(int8_t)(v >> (8 * i)), b = (float)(int8_t)(v >> (8 * i + 8));
-  return (__float_as_uint(b) & 0xffff0000u) | (__float_as_uint(a) >> 16);
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // the upper halves
 }
 DEV uint4 frag8(uint32_t a, uint32_t b) { return make_uint4(pk8(a, 0), pk8(a, 2), pk8(b, 0), pk8(b, 2)); }
 
-// Few rows: a block owns 16 columns and up to MT 16-row tiles; its eight waves take 128 inputs each in turn and
+// Few rows: a block owns 16 columns and MT 16-row tiles; its eight waves take 128 inputs each in turn and
 // add their sums through LDS.  Column l % 16 of the weights in lane l, 16 inputs (16 (l / 16)) of each 64.
 template <class SH, int MT>
 __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
-  __shared__ f32x4 red[LR_NW][MT][64];
-  const int lane = lane_id(), wave = wave_id(), c16 = lane & 15, g = lane >> 4;
+  __shared__ float red[LR_NW][MT][4][64];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16, r0 = blockIdx.y * 16 * MT;
   const size_t n = n0 + c16 < a.n ? n0 + c16 : a.n - 1;
+  // the rows and columns of this thread's outputs: output o = tid + 512 i is row 16 (o / 256) + 4 (o / 16 % 4) + o / 64 % 4 of
+  // the block; what the epilogue needs of them is requested ahead of the product
+  constexpr int OPT = (256 * MT + LR_NT - 1) / LR_NT;
+  int row[OPT], ad[OPT], rk[OPT];
+  float base[OPT];
+  const int col = n0 + c16;
+#pragma unroll
+  for (int i = 0; i < OPT; ++i) {
+    const int o = threadIdx.x + LR_NT * i;
+    row[i] = r0 + 16 * (o >> 8) + 4 * (o >> 4 & 3) + (o >> 6 & 3);
+    const bool live = o < 256 * MT && row[i] < a.rows && col < a.n;
+    if (!live) row[i] = -1;
+    base[i] = live && a.res ? a.res[row[i] * a.ldy + col] : 0.f;
+    ad[i] = live ? adapter_of(a, row[i]) : -1;
+    rk[i] = ad[i] >= 0 ? rank_of(a, ad[i]) : 0;
+  }
   f32x4 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
   const uint8_t* wr = reinterpret_cast<const uint8_t*>(a.w) + n * a.k + 16 * g;
+  const uint16_t* xr[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = r0 + 16 * m + c16;
+    xr[m] = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + 16 * g;
+  }
   for (int c = wave * 128; c < a.k; c += LR_NW * 128) {
     const uint4 w0 = ld16(wr + c), w1 = ld16(wr + c + 64);
     const float sc = SH::scale(a.s, n, c, a.k);
+    uint4 x[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) x[m][f] = ld16(xr[m] + c + 64 * (f >> 1) + 8 * (f & 1));
     const uint4 b0 = frag8(w0.x, w0.y), b1 = frag8(w0.z, w0.w), b2 = frag8(w1.x, w1.y), b3 = frag8(w1.z, w1.w);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int r = r0 + 16 * m + c16;
-      const uint16_t* xr = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + c + 16 * g;
       f32x4 p = {0.f, 0.f, 0.f, 0.f};
-      p = mfma(ld16(xr), b0, p), p = mfma(ld16(xr + 8), b1, p);
-      p = mfma(ld16(xr + 64), b2, p), p = mfma(ld16(xr + 72), b3, p);
+      p = mfma(x[m][0], b0, p), p = mfma(x[m][1], b1, p), p = mfma(x[m][2], b2, p), p = mfma(x[m][3], b3, p);
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[m][q] = __builtin_fmaf(sc, p[q], acc[m][q]);
     }
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m) red[wave][m][lane] = acc[m];
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) red[wave][m][q][lane] = acc[m][q];
   __syncthreads();
-  for (int q = threadIdx.x; q < 256 * MT; q += LR_NT) {
-    const int l = q & 63, e = q >> 6 & 3, m = q >> 8, row = r0 + 16 * m + 4 * (l >> 4) + e, col = n0 + (l & 15);
-    if (row >= a.rows || col >= a.n) continue;
+#pragma unroll
+  for (int i = 0; i < OPT; ++i) {
+    if (row[i] < 0) continue;
+    const int o = threadIdx.x + LR_NT * i;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < LR_NW; ++w) v += red[w][m][l][e];
-    const int ad = adapter_of(a, row);
-    if (ad >= 0) {
-      const int rk = rank_of(a, ad);
-      const uint16_t* b = a.lb + ((size_t)ad * a.n + col) * a.rmax;
-      const float* t = a.t + (size_t)row * a.rmax;
-      float d = 0.f;
-      for (int j = 0; j < rk; ++j) d = __builtin_fmaf(bf16f(b[j]), t[j], d);
-      v += d;
+    for (int w = 0; w < LR_NW; ++w) v += red[w][o >> 8][o >> 6 & 3][lane];
+    // eight ranks at a time; t is 0 past the rank, where B's padding must not count
+    const uint16_t* b = a.lb + ((size_t)(ad[i] < 0 ? 0 : ad[i]) * a.n + col) * a.rmax;
+    const float* t = a.t + (size_t)row[i] * a.rmax;
+    float d = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < rk[i]; j += 8) {
+      const uint4 q = ld16(b + j);
+      const float4 t0 = ldf4(t + j), t1 = ldf4(t + j + 4);
+      const int on = rk[i] - j;
+      d = __builtin_fmaf(bf16_lo(q.x), t0.x, d);
+      d = on > 1 ? __builtin_fmaf(bf16_hi(q.x), t0.y, d) : d;
+      d = on > 2 ? __builtin_fmaf(bf16_lo(q.y), t0.z, d) : d;
+      d = on > 3 ? __builtin_fmaf(bf16_hi(q.y), t0.w, d) : d;
+      d = on > 4 ? __builtin_fmaf(bf16_lo(q.z), t1.x, d) : d;
+      d = on > 5 ? __builtin_fmaf(bf16_hi(q.z), t1.y, d) : d;
+      d = on > 6 ? __builtin_fmaf(bf16_lo(q.w), t1.z, d) : d;
+      d = on > 7 ? __builtin_fmaf(bf16_hi(q.w), t1.w, d) : d;
     }
-    float* o = a.y + row * a.ldy + col;
-    *o = a.res ? a.res[row * a.ldy + col] + v : v;
+    a.y[row[i] * a.ldy + col] = base[i] + (v + d);
   }
 }
 
@@ -374,7 +409,11 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
   a.planes = few || !a.adapter ? nullptr : reinterpret_cast<uint16_t*>(a.t);
   if (a.adapter) hipLaunchKernelGGL(k_lora_down, dim3(tiles, few ? 16 : 2, few ? (a.rmax + 15) / 16 : a.rp / 16), dim3(LR_NT), 0, st, a);
   if (few) {
-    hipLaunchKernelGGL((k_lora_gemm_rows<SH, 4>), dim3((a.n + 15) / 16, 1), dim3(LR_NT), 0, st, a);
+    const dim3 g((a.n + 15) / 16), b(LR_NT);
+    if (tiles == 1) hipLaunchKernelGGL((k_lora_gemm_rows<SH, 1>), g, b, 0, st, a);
+    else if (tiles == 2) hipLaunchKernelGGL((k_lora_gemm_rows<SH, 2>), g, b, 0, st, a);
+    else if (tiles == 3) hipLaunchKernelGGL((k_lora_gemm_rows<SH, 3>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((k_lora_gemm_rows<SH, 4>), g, b, 0, st, a);
     return 0;
   }
   auto go = [&](auto mt, auto nt) {
