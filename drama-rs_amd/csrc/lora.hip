@@ -45,12 +45,15 @@ DEV int adapter_of(const Lora& a, int r) {
 DEV int rank_of(const Lora& a, int v) { return a.rank[v] < a.rmax ? a.rank[v] : a.rmax; }
 
 // ---- t = s_a A_a x --------------------------------------------------------------------------
-// Block: 16 rows (blockIdx.x), 16 ranks (blockIdx.z), the distinct adapters blockIdx.y, + gridDim.y, ... of
-// those rows.  The eight waves take 128 inputs each in turn.
+// Block: 16 rows (blockIdx.x), 16 RT ranks (blockIdx.z), the distinct adapters blockIdx.y, + gridDim.y, ... of
+// those rows.  The eight waves take 128 inputs each in turn.  Bound by the latency of a short chain of loads (ids, ranks,
+// inputs) and, with many rows, by the requests of 16 rows a fetch (two turns in flight: 20 -> 31 us at 4096 rows).
+template <int RT>
 __global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
-  __shared__ f32x4 red[LR_NW][64];
-  const int lane = lane_id(), wave = wave_id(), c16 = lane & 15, g = lane >> 4;
-  const int r0 = blockIdx.x * 16, j0 = blockIdx.z * 16;
+  __shared__ float red[LR_NW][RT][4][64];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
+  const int r0 = blockIdx.x * 16, j0 = blockIdx.z * 16 * RT;
+  const uint16_t* xr = a.x + (size_t)(r0 + c16 < a.rows ? r0 + c16 : a.rows - 1) * a.ldx + 8 * g;
   const int mine = adapter_of(a, r0 + c16);
   // row c16 is the first of its adapter: no earlier row of the 16 has it
   bool first = mine >= 0;
@@ -61,41 +64,57 @@ __global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
   while (firsts) {
     const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctz(firsts));
     for (int q = 0; q < (int)gridDim.y && firsts; ++q) firsts &= firsts - 1;
+    const uint32_t rows = (uint32_t)__ballot(mine == ad) & 0xffffu;
     const int rk = rank_of(a, ad);
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const float scale = a.lscale[ad];
+    f32x4 acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (j0 < rk) {
-      const uint16_t* xr = a.x + (size_t)(r0 + c16 < a.rows ? r0 + c16 : a.rows - 1) * a.ldx + 8 * g;
-      const uint16_t* ar = a.la + ((size_t)ad * a.rmax + (j0 + c16 < rk ? j0 + c16 : rk - 1)) * a.k + 8 * g;
+      const uint16_t* ar[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int j = j0 + 16 * t + c16;
+        ar[t] = a.la + ((size_t)ad * a.rmax + (j < rk ? j : rk - 1)) * a.k + 8 * g;
+      }
       for (int c = wave * 128; c < a.k; c += LR_NW * 128) {
-        uint4 xv[4], av[4];
+        uint4 xv[4], av[RT][4];
 #pragma unroll
-        for (int f = 0; f < 4; ++f) xv[f] = ld16(xr + c + 32 * f), av[f] = ld16(ar + c + 32 * f);
+        for (int f = 0; f < 4; ++f) xv[f] = ld16(xr + c + 32 * f);
 #pragma unroll
-        for (int f = 0; f < 4; ++f) acc = mfma(xv[f], av[f], acc);
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) av[t][f] = ld16(ar[t] + c + 32 * f);
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) acc[t] = mfma(xv[f], av[t][f], acc[t]);
       }
     }
-    __syncthreads();
-    red[wave][lane] = acc;
-    __syncthreads();
-    if (threadIdx.x < 256) {
-      const int l = threadIdx.x & 63, q = threadIdx.x >> 6, row = r0 + 4 * (l >> 4) + q, j = j0 + (l & 15);
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) red[wave][t][q][lane] = acc[t][q];
+    lds_barrier();
+    for (int o = wave; o < 4 * RT; o += LR_NW) {
+      const int q = o & 3, t = o >> 2, i = 4 * g + q, row = r0 + i, j = j0 + 16 * t + c16;
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < LR_NW; ++w) v += red[w][l][q];
-      if (adapter_of(a, row) == ad) {
-        v = j < rk ? a.lscale[ad] * v : 0.f;
-        if (!a.planes) {
-          if (j < a.rmax) a.t[(size_t)row * a.rmax + j] = v;
-        } else {
-          // 8 mantissa bits each, the last exact: hi + mid + lo = v
-          const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u), r1 = v - hi;
-          const float mi = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi;
-          uint16_t* p = a.planes + (size_t)row * a.rp + j;
-          const size_t plane = (size_t)a.rows * a.rp;
-          p[0] = (uint16_t)(__float_as_uint(hi) >> 16);
-          p[plane] = (uint16_t)(__float_as_uint(mi) >> 16);
-          p[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
-        }
+      for (int w = 0; w < LR_NW; ++w) v += red[w][t][q][lane];
+      if (!(rows >> i & 1)) continue;
+      v = j < rk ? scale * v : 0.f;
+      if (!a.planes) {
+        if (j < a.rmax) a.t[(size_t)row * a.rmax + j] = v;
+      } else if (j < a.rp) {
+        // 8 mantissa bits each, the last exact: hi + mid + lo = v
+        const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u), r1 = v - hi;
+        const float mi = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi;
+        uint16_t* p = a.planes + (size_t)row * a.rp + j;
+        const size_t plane = (size_t)a.rows * a.rp;
+        p[0] = (uint16_t)(__float_as_uint(hi) >> 16);
+        p[plane] = (uint16_t)(__float_as_uint(mi) >> 16);
+        p[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
       }
     }
   }
@@ -194,22 +213,30 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
 }
 
 // Many rows: a block of 2 x 2 waves owns 32 MT rows x 32 NT columns, a wave 16 MT x 16 NT of them.  Slices of 64 inputs
-// go through two LDS buffers (x as it is, W converted to bf16 on its way there, once per block), a slice's
-// global loads in flight for the whole of the slice before; the barrier between slices leaves them in flight.  Row r's 16-byte
-// piece j lies at j ^ (r % 8), so the fragment reads meet no bank twice.
+// go through two LDS buffers, a slice's global loads in flight for the whole of the slice before; the barrier between slices
+// leaves them in flight.  The LDS reads set the pace (a wave tile of 64 x 64 in bf16 asks for 64 KB a slice, at ~64 bytes a
+// clock twice the time of its products), so W stays int8 there and is converted in the registers of the wave that
+// multiplies it, and the tile is as wide as the registers allow.
+// x: row r's 16-byte piece j lies at j ^ (r % 8), so the fragment reads meet no bank twice; W: four pieces a row in order, a
+// fragment pair being 1 KB in a row.  Lane (l % 16, g = l / 16) has the inputs 16 g .. 16 g + 15 of a slice, 8 a product.
 // 8 XCDs take the tiles in 8 contiguous runs, down columns of 8 row tiles, so that an XCD's blocks share x and W in its L2.
 constexpr int LG_K = 64;
 template <class SH, int MT, int NT>
 __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int tn) {
   constexpr int BM = 32 * MT, BN = 32 * NT, PX = BM * 8 / 256, PW = BN * 4 / 256;
   static_assert(PX * 256 == BM * 8 && PW * 256 == BN * 4, "pieces per thread");
-  __shared__ uint4 lx[2][BM * 8], lw[2][BN * 8];
+  __shared__ uint4 lx[2][BM * 8], lw[2][BN * 4];
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
   // tile of this block
   const int total = tm * tn, per = (total + 7) / 8, q = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || q >= total) return;
   const int band = q / (8 * tn), bh = tm - 8 * band < 8 ? tm - 8 * band : 8, in = q - band * 8 * tn;
   const int m0 = (8 * band + in % bh) * BM, n0 = in / bh * BN;
+  const int wm = (wave >> 1) * 16 * MT, wn = (wave & 1) * 16 * NT;
+  // adapters of the wave's rows, known before the product ends
+  int mine[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) mine[m] = adapter_of(a, m0 + wm + 16 * m + c16);
   const uint16_t* xp[PX];
   const uint8_t* wp[PW];
 #pragma unroll
@@ -236,20 +263,19 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
       lx[b][r * 8 + (j ^ (r & 7))] = xv[i];
     }
 #pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      const int r = (tid + 256 * i) / 4, j = 2 * (tid & 3);
-      lw[b][r * 8 + (j ^ (r & 7))] = frag8(wv[i].x, wv[i].y);
-      lw[b][r * 8 + ((j + 1) ^ (r & 7))] = frag8(wv[i].z, wv[i].w);
-    }
+    for (int i = 0; i < PW; ++i) lw[b][tid + 256 * i] = wv[i];
   };
-  const int wm = (wave >> 1) * 16 * MT, wn = (wave & 1) * 16 * NT;
-  f32x4 acc[MT][NT], sum[MT][NT];
+  // SH::per_row: the scale is applied once at the end; else the sums of a group (two slices) are scaled into `sum`
+  f32x4 acc[MT][NT], sum[SH::per_row ? 1 : MT][SH::per_row ? 1 : NT];
   const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) acc[m][n] = sum[m][n] = z;
-  size_t col[NT];
+    for (int n = 0; n < NT; ++n) {
+      acc[m][n] = z;
+      if constexpr (!SH::per_row) sum[m][n] = z;
+    }
+  int col[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int c = n0 + wn + 16 * n + c16;
@@ -271,33 +297,28 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
 #pragma unroll
       for (int n = 0; n < NT; ++n) sc[n] = SH::scale(a.s, col[n], s * LG_K, a.k);
     }
+    uint4 xf[2][MT];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      uint4 xf[MT], wf[NT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int r = wm + 16 * m + c16;
-        xf[m] = lx[B][r * 8 + ((4 * kk + g) ^ (r & 7))];
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int r = wn + 16 * n + c16;
-        wf[n] = lw[B][r * 8 + ((4 * kk + g) ^ (r & 7))];
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n] = mfma(xf[m], wf[n], acc[m][n]);
+    for (int m = 0; m < MT; ++m) {
+      const int r = wm + 16 * m + c16;
+      xf[0][m] = lx[B][r * 8 + ((2 * g) ^ (r & 7))], xf[1][m] = lx[B][r * 8 + ((2 * g + 1) ^ (r & 7))];
     }
-    if constexpr (B == 1 && !SH::per_row) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < NT; ++n) {
+      const uint4 v = lw[B][(wn + 16 * n + c16) * 4 + g];
+      const uint4 w0 = frag8(v.x, v.y), w1 = frag8(v.z, v.w);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+      for (int m = 0; m < MT; ++m) acc[m][n] = mfma(xf[0][m], w0, acc[m][n]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m][n] = mfma(xf[1][m], w1, acc[m][n]);
+      if constexpr (B == 1 && !SH::per_row) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum[m][n][r] = __builtin_fmaf(sc[n], acc[m][n][r], sum[m][n][r]);
           acc[m][n] = z;
         }
+      }
     }
     lds_barrier();
   };
@@ -305,37 +326,25 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
     step(std::integral_constant<int, 0>{}, s);
     step(std::integral_constant<int, 1>{}, s + 1);
   }
-  if constexpr (SH::per_row) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float sc = SH::scale(a.s, col[n], 0, a.k);
+  for (int n = 0; n < NT; ++n) {
+    const float sc = SH::per_row ? SH::scale(a.s, col[n], 0, a.k) : 1.f;
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m) {
+      if constexpr (SH::per_row) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum[m][n][r] = sc * acc[m][n][r];
+        for (int r = 0; r < 4; ++r) acc[m][n][r] *= sc;
+      } else {
+        acc[m][n] = sum[m][n];
+      }
     }
   }
-  // the residual, all of it in flight beside the adapters (y may be res: its loads could not pass the stores)
-  f32x4 rv[MT][NT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = m0 + wm + 16 * m + 4 * g + r;
-        rv[m][n][r] = a.res ? gld<float>(a.res + (size_t)(row < a.rows ? row : a.rows - 1) * a.ldy + col[n]) : 0.f;
-      }
   // B t: the distinct adapters of the wave's rows, the t of other rows zero; B's fragments serve all row tiles
   if (a.adapter) {
     const size_t plane = (size_t)a.rows * a.rp;
-    int mine[MT];
     uint32_t left[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      mine[m] = adapter_of(a, m0 + wm + 16 * m + c16);
-      left[m] = (uint32_t)__ballot(mine[m] >= 0) & 0xffffu;
-    }
+    for (int m = 0; m < MT; ++m) left[m] = (uint32_t)__ballot(mine[m] >= 0) & 0xffffu;
 #pragma unroll
     for (int f = 0; f < MT; ++f)
       while (left[f]) {
@@ -369,24 +378,30 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
           for (int m = f; m < MT; ++m)
             if (has[m])
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
+              for (int p = 0; p < 3; ++p)
 #pragma unroll
-                for (int p = 0; p < 3; ++p) sum[m][n] = mfma(tf[m][p], b[n], sum[m][n]);
+                for (int n = 0; n < NT; ++n) acc[m][n] = mfma(tf[m][p], b[n], acc[m][n]);
         }
       }
   }
+  // the residual of 16 rows in flight at a time (y may be res: its loads could not pass the stores)
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m) {
+    float rv[4][NT];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = m0 + wm + 16 * m + 4 * g + r;
-      if (row >= a.rows) continue;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int c = n0 + wn + 16 * n + c16;
-        if (c < a.n) a.y[row * a.ldy + c] = rv[m][n][r] + sum[m][n][r];
-      }
+      for (int n = 0; n < NT; ++n) rv[r][n] = a.res ? gld<float>(a.res + (size_t)(row < a.rows ? row : a.rows - 1) * a.ldy + col[n]) : 0.f;
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = m0 + wm + 16 * m + 4 * g + r;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (row < a.rows && n0 + wn + 16 * n + c16 < a.n) a.y[row * a.ldy + col[n]] = rv[r][n] + acc[m][n][r];
+    }
+  }
 }
 
 bool lora_shape_ok(int rows, int n, int k, int rmax) {
@@ -407,7 +422,8 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
   const bool few = a.rows <= 64;
   a.rp = (a.rmax + 31) & ~31;
   a.planes = few || !a.adapter ? nullptr : reinterpret_cast<uint16_t*>(a.t);
-  if (a.adapter) hipLaunchKernelGGL(k_lora_down, dim3(tiles, few ? 16 : 2, few ? (a.rmax + 15) / 16 : a.rp / 16), dim3(LR_NT), 0, st, a);
+  if (a.adapter && few) hipLaunchKernelGGL(k_lora_down<1>, dim3(tiles, 16, (a.rmax + 15) / 16), dim3(LR_NT), 0, st, a);
+  else if (a.adapter) hipLaunchKernelGGL(k_lora_down<2>, dim3(tiles, 2, a.rp / 32), dim3(LR_NT), 0, st, a);
   if (few) {
     const dim3 g((a.n + 15) / 16), b(LR_NT);
     if (tiles == 1) hipLaunchKernelGGL((k_lora_gemm_rows<SH, 1>), g, b, 0, st, a);
@@ -421,8 +437,13 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
     const long long tm = (a.rows + 32ll * M - 1) / (32 * M), tn = (a.n + 32ll * N - 1) / (32 * N), per = (tm * tn + 7) / 8;
     hipLaunchKernelGGL((k_lora_gemm_tiles<SH, M, N>), dim3((unsigned)(8 * per)), dim3(256), 0, st, a, (int)tm, (int)tn);
   };
-  if ((long long)((a.rows + 127) / 128) * ((a.n + 127) / 128) >= 256) go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-  else go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+  constexpr std::integral_constant<int, 2> i2{};
+  constexpr std::integral_constant<int, 4> i4{};
+  constexpr std::integral_constant<int, SH::per_row ? 8 : 4> wide{};
+  const long long m128 = (a.rows + 127) / 128;
+  if (m128 * ((a.n + 32 * wide.value - 1) / (32 * wide.value)) >= 256) go(i4, wide);
+  else if (m128 * ((a.n + 127) / 128) >= 256) go(i4, i4);
+  else go(i2, i2);
   return 0;
 }
 
