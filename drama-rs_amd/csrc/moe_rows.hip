@@ -3,7 +3,7 @@
 //   y = res + sigmoid(l_E) D_s (silu(G_s x) * (U_s x)) + sum_k w_k D_k (silu(G_k x) * (U_k x)).
 //
 // An expert is fetched once for all the rows that picked it.  Matrix products run on
-// v_mfma_f32_16x16x32_bf16 with A = 16 rows of x and B = 16 weight rows, converted exactly to bf16
+// v_mfma_f32_16x16x32_bf16 with A = up to 16 rows of x and B = 16 weight rows, converted exactly to bf16
 // in registers (int4: 16 + q, with the rest of q scale + min in one fp32 MFMA of the group sums of x), so x
 // enters exactly.  The activations are fp32; they travel as three bf16 planes of 8 mantissa
 // bits each (their sum is the fp32 value), three MFMAs per weight fragment, so nothing is rounded but the fp32 sums.
@@ -14,15 +14,27 @@ using namespace drm;
 namespace {
 
 constexpr int MR_NW = 8, MR_NT = MR_NW * 64, MR_ROWS = 64, MR_TOPK = 32, MR_PAIRS = MR_ROWS * MR_TOPK;
-constexpr int MR_GRID = 256;  // a block per CU
-constexpr int MR_ITEMS = 256 + MR_PAIRS / 16 + MR_ROWS / 16;  // passes of 16 rows, the experts' and the shared expert's
-constexpr int MR_SETS = 8;    // row sets of the router
+constexpr int MR_GRID = 256;             // a block per CU
+constexpr int MR_X = 120 * 1024;         // LDS bytes for rows of x
+constexpr int MR_ITEMS = MR_PAIRS + MR_ROWS;  // passes, the experts' and the shared expert's, of one row each at worst
+constexpr int MR_SETS = 8;               // row sets of the router
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 DEV f32x4 mfma(const uint4& a, const uint4& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+DEV uint32_t pick(bool c, uint32_t a, uint32_t b) { return c ? a : b; }
+
+// f(0), .., f(N - 1) with the index a constant, so that arrays it selects from live in registers
+template <int N, int I = 0, class Fn>
+DEV void static_for(Fn f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, I + 1>(f);
+  }
 }
 
 struct MoeRows {
@@ -63,7 +75,7 @@ DEV int pair_byte() { return ((lane_id() >> 1) & 4) * 16 + (lane_id() >> 4) * 16
 // a: rows 0 .. 7, b: rows 8 .. 15 -> a: bytes 16 g of the first 64 of row l % 16, b: of the second 64.  Lanes 8 .. 15 of each 16 of a
 // take lanes 0 .. 7 of b, and the other way round.
 DEV void pair_up(uint4& a, uint4& b) {
-  auto sw = [](uint32_t& p, uint32_t& q) {
+  auto sw = [](uint32_t& p, uint32_t& q) __attribute__((always_inline)) {
     const int o = (int)p, n = (int)q;
     p = (uint32_t)__builtin_amdgcn_update_dpp(o, n, 0x128, 0xF, 0xC, false);  // row_ror:8 into lanes 8 .. 15
     q = (uint32_t)__builtin_amdgcn_update_dpp(n, o, 0x128, 0xF, 0x3, false);  // into lanes 0 .. 7
@@ -94,31 +106,36 @@ struct RowsQ4 {
     asm("" : "+v"(b));
     return make_uint4(((v << 3) & m) | b, ((v >> 1) & m) | b, ((v >> 5) & m) | b, ((v >> 9) & m) | b);
   }
-  // xsum: lane's sum of x over group l / 16 of row l % 16 (0 past the chunk's groups)
-  template <int NP>
-  DEV void mac(const uint4 (&x)[NP][8], float xsum, bool half, f32x4& out) {
-    const int g = lane_id() >> 4;
-    const uint32_t sw[4] = {s.x, s.y, half ? 0u : s.z, half ? 0u : s.w};
-    const uint32_t lo = g & 1 ? sw[1] : sw[0], hi = g & 1 ? sw[3] : sw[2];
-    const float2 o = SC::pair(g & 2 ? hi : lo);
-    out = __builtin_amdgcn_mfma_f32_16x16x4f32(xsum, o.y - 16.f * o.x, out, 0, 0, 0);
+  // The tile's words in the order of the products: w[p].x, .y the fragments of group 2 p, .z, .w of group 2 p + 1
+  DEV void prep(bool half) {
     pair_up(w[0], w[1]);
+    if (half) s.z = s.w = 0;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       // lanes g = 0, 1 hold group 2 p, g = 2, 3 group 2 p + 1: two words of each change places
       const auto s02 = __builtin_amdgcn_permlane32_swap(w[p].x, w[p].z, false, false);
       const auto s13 = __builtin_amdgcn_permlane32_swap(w[p].y, w[p].w, false, false);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 b0 = frag(s02[h]), b1 = frag(s13[h]);
-        f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < NP; ++q) a = mfma(x[q][4 * p + 2 * h], b0, a), a = mfma(x[q][4 * p + 2 * h + 1], b1, a);
-        const float sc = SC::pair(sw[2 * p + h]).x;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
-      }
+      w[p] = make_uint4(s02[0], s13[0], s02[1], s13[1]);
     }
+  }
+  // what 16 + q leaves of q scale + min; xsum: the lane's sum of x over group l / 16 of row l % 16
+  DEV void rest(float xsum, f32x4& out) const {
+    const int g = lane_id() >> 4;
+    // (by value: a choice between members would keep them in memory)
+    const uint32_t lo = pick(g & 1, s.y, s.x), hi = pick(g & 1, s.w, s.z);
+    const float2 o = SC::pair(pick(g & 2, hi, lo));
+    out = __builtin_amdgcn_mfma_f32_16x16x4f32(xsum, o.y - 16.f * o.x, out, 0, 0, 0);
+  }
+  // group 2 p + h of the chunk
+  template <int NP>
+  DEV void group(int p, int h, const uint4 (&x)[NP][2], f32x4&, f32x4& out) const {
+    const uint4 b0 = frag(pick(h, w[p].z, w[p].x)), b1 = frag(pick(h, w[p].w, w[p].y));
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < NP; ++q) a = mfma(x[q][0], b0, a), a = mfma(x[q][1], b1, a);
+    const float sc = SC::pair(p ? pick(h, s.w, s.z) : pick(h, s.y, s.x)).x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
   }
 };
 
@@ -138,23 +155,19 @@ struct Rows8 {
     s[0] = D::scale_raw(S, n + (lane_id() & 15), 2 * c, K, off);
     s[1] = D::scale_raw(S, n + (lane_id() & 15), 2 * c + 1, K, half);
   }
+  DEV void prep(bool) { pair_up(w[0], w[1]), pair_up(w[2], w[3]); }
+  DEV void rest(float, f32x4&) const {}
   template <int NP>
-  DEV void mac(const uint4 (&x)[NP][8], float, bool, f32x4& out) {
+  DEV void group(int p, int h, const uint4 (&x)[NP][2], f32x4& a, f32x4& out) const {
+    const uint4& v = w[2 * p + h];
+    const uint4 b0 = D::frag(v.x, v.y), b1 = D::frag(v.z, v.w);
+    if (h == 0) a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      pair_up(w[2 * p], w[2 * p + 1]);
-      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < NP; ++q) a = mfma(x[q][0], b0, a), a = mfma(x[q][1], b1, a);
+    if (h == 0) return;
+    const float sc = D::scale_cvt(s[p]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4& v = w[2 * p + h];
-        const uint4 b0 = D::frag(v.x, v.y), b1 = D::frag(v.z, v.w);
-#pragma unroll
-        for (int q = 0; q < NP; ++q) a = mfma(x[q][4 * p + 2 * h], b0, a), a = mfma(x[q][4 * p + 2 * h + 1], b1, a);
-      }
-      const float sc = D::scale_cvt(s[p]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
-    }
+    for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
   }
 };
 DEV uint32_t buf_half(const Rsrc& S, uint32_t off) { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(S, off, 0, 0); }
@@ -185,45 +198,10 @@ struct RowsQ8 : Rows8<RowsQ8<SH>> {
   static DEV float scale_cvt(uint32_t r) { return SH::cvt(r); }
   static DEV uint32_t pk(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
     const float a = (float)(int8_t)(v >> (8 * i)), b = (float)(int8_t)(v >> (8 * i + 8));
-    return (__float_as_uint(b) & 0xffff0000u) | (__float_as_uint(a) >> 16);
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
   }
   static DEV uint4 frag(uint32_t a, uint32_t b) { return make_uint4(pk(a, 0), pk(a, 2), pk(b, 0), pk(b, 2)); }
 };
-
-// A lane's fragments of chunk c of the row at byte `row` (planes `plane` bytes apart); inputs past the row are zero
-template <class F, int NP>
-DEV void load_x(const Rsrc& X, uint32_t row, uint32_t plane, int c, bool half, uint4 (&x)[NP][8]) {
-  const uint32_t p = row + (c * 256 + F::xoff(lane_id() >> 4)) * 2;
-#pragma unroll
-  for (int q = 0; q < NP; ++q)
-#pragma unroll
-    for (int f = 0; f < 8; ++f)
-      x[q][f] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(X, f >= 4 && half ? NOWHERE : p + 2 * (64 * (f >> 1) + 8 * (f & 1)),
-                                                                                 q * plane, 0));
-}
-// the fragments in the weights' order, and the lane's group sum (RowsQ4)
-template <class F, int NP>
-DEV float order_x(uint4 (&x)[NP][8]) {
-  if constexpr (!F::perm) return 0.f;
-  float own = 0.f;
-#pragma unroll
-  for (int G = 0; G < 4; ++G) {
-    float t = 0.f;
-#pragma unroll
-    for (int q = NP - 1; q >= 0; --q)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint4& v = x[q][2 * G + j];
-        t += ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) +
-             ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
-        v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
-      }
-    t = xsum_step<32>(xsum_step<16>(t));
-    own = (lane_id() >> 4) == G ? t : own;
-  }
-  return own;
-}
 
 // ---- router -----------------------------------------------------------------------------------
 // Logits of TS rows (set blockIdx.y) in the canonical order of canon.hpp, wave w of block b taking router row
@@ -291,28 +269,45 @@ __global__ void __launch_bounds__(MR_NT) k_moe_rows_router(MoeRows a) {
 }
 
 // ---- experts ----------------------------------------------------------------------------------
-// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 32 t, K = i).
-// KS waves share a tile's inputs, a chunk each (cpw > 1: further chunks in turn); the other groups of waves (RG)
-// take further tiles, a step of the block being RG tiles.  Items are passes of up to 16 rows of an expert, ascending,
-// then of the shared expert (whose rows are all); their steps are dealt to the blocks in contiguous runs of even
-// cost, the shared expert's counting twice where its bytes are twice the others'.  (All passes of an expert as one
-// item fetch its weights once but x again for every tile and pass: 64 rows 202 us against 152.)
-// A wave's x fragments stay in registers for all tiles of an item (where it has one chunk).  Two steps of weights
-// are in flight: a tile's registers take the tile two steps on as soon as it is used.  The KS sums meet in LDS, behind a
-// barrier that leaves the loads in flight.
+// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 64 t, K = i).
+//
+// Items are passes of up to P rows of an expert, ascending, then of the shared expert (whose rows are all); their
+// tiles are dealt to the blocks in contiguous runs of even cost, the shared expert's counting twice where its bytes are
+// twice the others'.  A block stages the rows of its items in LDS (as many items at a time as R rows hold, most
+// often all), then each of its waves takes one tile after the other from a counter and multiplies all of its inputs, in chunks
+// of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights come in a ring of DEPTH chunks that
+// runs on across tiles and items.
+//
+// LDS: row slot s at s * RB, its planes Kp * 2 bytes apart (Kp: K rounded up to a chunk, zeros past K), pieces of 8 inputs
+// reordered for int4; RB is 16 bytes more than the planes, so that the 16 rows of a fragment meet different banks.
+// Then, for int4, the fp32 sums of each 64 inputs.
+template <int MODE>
+struct XLayout {
+  static constexpr int NP = MODE == 0 ? 1 : 3;
+  int Kp, RB, GS, R;  // padded inputs, row bytes, floats of sums a row, rows
+  __host__ __device__ XLayout(int K) {
+    Kp = (K + 255) & ~255;
+    RB = NP * Kp * 2 + 16;
+    GS = Kp / 64 + 4;
+    R = MR_X / (RB + 4 * GS);
+  }
+};
+
 template <int MODE, class F, class FS>
-__global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS, int cpw, int fs_cost) {
-  constexpr int NP = MODE == 0 ? 1 : 3, TL = 2;
-  __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert
+__global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs_cost) {
+  constexpr int NP = MODE == 0 ? 1 : 3, TL = MODE == 0 ? 2 : 4;
+  extern __shared__ uint4 xlds[];
+  __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert, then the shared expert's rows
+  __shared__ uint16_t s_e[MR_ITEMS], s_off[MR_ITEMS], s_num[MR_ITEMS];  // items: expert, first place in s_list, rows
+  __shared__ int s_cum[MR_ITEMS + 1];              // cost of the items before
   __shared__ uint32_t s_rows[256][2];
-  __shared__ int s_start[256], s_e[MR_ITEMS], s_off[MR_ITEMS], s_num[MR_ITEMS], s_cum[MR_ITEMS + 1], s_tot[8][3], s_first;
-  __shared__ float red[2][MR_NW][TL][4][64];
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
+  __shared__ int s_start[256], s_tot[8][3], s_first, s_ticket;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x, c16 = lane & 15, g = lane >> 4;
   const int pairs = a.rows * a.topk;
-  const int K = MODE == 0 ? a.h : a.i, RG = MR_NW / KS, tiles = MODE == 0 ? a.i / 16 : a.h / 32;
-  const int steps = (tiles + RG - 1) / RG;
-  const int N = MODE == 0 ? 2 * a.i : a.h;
-  const int nch = (K + 255) / 256, wk = wave % KS, rg = wave / KS;
+  const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 64, N = MODE == 0 ? 2 * a.i : a.h;
+  const int nch = (K + 255) / 256;
+  const XLayout<MODE> L(K);
+  const int P = L.R < 16 ? L.R : 16;
   // rows of each expert as a 64-bit mask (a row picks an expert once), so that every block has the same passes
   constexpr int PPT = MR_PAIRS / MR_NT;
   int pe[PPT];
@@ -330,11 +325,12 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
   // sums over the experts (thread e) of their rows, their passes and their cost
   {
     int v[3] = {0, 0, 0}, own[3];
+    const bool sh = tid == 256;
+    const int cost = tiles * (sh ? fs_cost : 1);
     if (tid <= 256) {
-      const bool sh = tid == 256;
       v[0] = sh ? (a.shared ? a.rows : 0) : __builtin_popcount(s_rows[tid][0]) + __builtin_popcount(s_rows[tid][1]);
-      v[1] = (v[0] + 15) / 16;
-      v[2] = v[1] * steps * (sh ? fs_cost : 1);
+      v[1] = (v[0] + P - 1) / P;
+      v[2] = v[1] * cost;
     }
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
@@ -352,19 +348,20 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
       for (int q = 0; q < 3; ++q) base[q] += s_tot[w][q];
     lds_barrier();
     if (tid <= 256) {
-      const int off = base[0] + v[0] - own[0], cum = base[2] + v[2] - own[2];
+      const int off = base[0] + v[0] - own[0], cum = base[2] + v[2] - own[2], d0 = base[1] + v[1] - own[1];
       for (int p = 0; p < own[1]; ++p) {
-        const int d = base[1] + v[1] - own[1] + p;
-        s_e[d] = tid, s_off[d] = off + 16 * p, s_num[d] = own[0] - 16 * p < 16 ? own[0] - 16 * p : 16, s_cum[d] = cum + own[2] / own[1] * p;
+        s_e[d0 + p] = tid, s_off[d0 + p] = off + P * p, s_num[d0 + p] = own[0] - P * p < P ? own[0] - P * p : P;
+        s_cum[d0 + p] = cum + cost * p;
       }
-      if (tid < 256) s_start[tid] = off;
+      if (!sh) s_start[tid] = off;
+      else s_cum[d0 + own[1]] = base[2] + v[2], s_tot[0][0] = d0 + own[1], s_tot[1][0] = d0;
     }
-    if (tid == 256) s_cum[base[1] + v[1]] = base[2] + v[2], s_tot[0][0] = base[1] + v[1];
     lds_barrier();
   }
-  const int D = s_tot[0][0];
+  const int D = s_tot[0][0], D0 = s_tot[1][0];  // items, those of the routed experts
   const int lo = (int)((long long)s_cum[D] * blockIdx.x / gridDim.x), hi = (int)((long long)s_cum[D] * (blockIdx.x + 1) / gridDim.x);
-  if (tid < D && s_cum[tid] <= lo && lo < s_cum[tid + 1]) s_first = tid;
+  for (int d = tid; d < D; d += MR_NT)
+    if (s_cum[d] <= lo && lo < s_cum[d + 1]) s_first = d;
 #pragma unroll
   for (int q = 0; q < PPT; ++q)
     if (pe[q] >= 0) {
@@ -376,140 +373,156 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int KS
   if (a.shared && tid < a.rows) s_list[pairs + tid] = pairs + tid;
   lds_barrier();
   if (lo >= hi) return;
-  int par = 0;
   const size_t plane = (size_t)(pairs + a.rows) * a.i;
-  for (int d = s_first; d < D && s_cum[d] < hi; ++d) {
-    const int e = __builtin_amdgcn_readfirstlane(s_e[d]), off = s_off[d], cnt = s_num[d];
-    const int cum = s_cum[d], tc = (s_cum[d + 1] - cum) / steps;
-    const int t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0, t1 = (hi - cum + tc - 1) / tc < steps ? (hi - cum + tc - 1) / tc : steps;
-    if (t0 >= t1) continue;
-    const bool sh = e == 256;
-    auto segment = [&](auto fmt, const void* Qp, const void* Sp) __attribute__((always_inline)) {
-      using Fm = decltype(fmt);
-      const Rsrc Q = rsrc(Qp, (uint32_t)Fm::q_bytes(N, K)), S = rsrc(Sp, (uint32_t)Fm::s_bytes(N, K));
-      const Rsrc X = MODE == 0 ? rsrc(a.x, (uint32_t)a.rows * K * 2) : rsrc(a.act, (uint32_t)(6 * plane));
-      Fm w[2][TL];
-      uint4 x[NP][8];
-      auto half_of = [&](int c) { return c * 256 + 128 >= K; };
-      auto load_w = [&](Fm& f, int i, int t, int ci) __attribute__((always_inline)) {
-        const int c = wk + KS * ci, tile = t * RG + rg;
-        const bool none = (t >= t1) | (tile >= tiles) | (rg >= RG) | (c >= nch);
-        f.load(Q, S, MODE == 0 ? 16 * tile + i * a.i : 32 * tile + 16 * i, K, c, none | half_of(c), none);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      auto fetch_x = [&](int ci) __attribute__((always_inline)) {
-        const int m = lane & 15, pr = s_list[off + (m < cnt ? m : cnt - 1)], c = wk + KS * ci;
-        const int row = MODE == 1 ? pr : sh ? pr - pairs : pr / a.topk;
-        load_x<Fm, NP>(X, c < nch ? (uint32_t)(row * K * 2) : NOWHERE, (uint32_t)(2 * plane), c, half_of(c), x);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      // the KS sums of step t's tiles, and what becomes of them
-      auto finish = [&](const f32x4 (&o)[TL], int t) __attribute__((always_inline)) {
+  char* xb = reinterpret_cast<char*>(xlds);
+  float* sums = reinterpret_cast<float*>(xb + (size_t)L.R * L.RB);
+  // the block's tiles [t0, t1) of item d
+  auto range = [&](int d, int& t0, int& t1) __attribute__((always_inline)) {
+    const int cum = s_cum[d], tc = d < D0 ? 1 : fs_cost;
+    t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0;
+    t1 = (hi - cum + tc - 1) / tc;
+    t0 = __builtin_amdgcn_readfirstlane(t0 < tiles ? t0 : tiles), t1 = __builtin_amdgcn_readfirstlane(t1 < tiles ? t1 : tiles);
+  };
+  // items dA .. dB - 1, of one weight format, their rows in the slots from 0
+  auto run = [&](auto fmt, const int dA, const int dB, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
+    using Fm = decltype(fmt);
+    constexpr int DEPTH = Fm::perm ? 8 / TL : MODE == 0 ? 3 : 2;
+    const int pos = s_off[dA], nrows = s_off[dB - 1] + s_num[dB - 1] - pos, k8 = L.Kp / 8;
+    if (tid == 0) s_ticket = 0;
+    for (int q = tid; q < nrows * k8; q += MR_NT) {
+      const int slot = q / k8, k = (q - slot * k8) * 8, pr = s_list[pos + slot];
+      float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < TL; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) red[par][wave][i][r][lane] = o[i][r];
-        lds_barrier();
-        const int tile = t * RG + rg, nr = tile < tiles && rg < RG ? cnt : 0;
-        // register r of lane l: row 4 (l / 16) + r of x, column l % 16; the KS waves share the registers
-        auto part = [&](auto ks) __attribute__((always_inline)) {
-          constexpr int KK = decltype(ks)::value;
-          const int base = rg * KS;
-          auto total = [&](int i, int r) {
-            float v = 0.f;
-#pragma unroll
-            for (int k = 0; k < KK; ++k) {
-              const float q = red[par][base + (k < KS ? k : 0)][i][r][lane];
-              v += k < KS ? q : 0.f;
-            }
-            return v;
-          };
-          for (int q = MODE == 0 && KS == 8 ? wk ^ (4 * par) : wk; q < (MODE == 0 ? 4 : 4 * TL); q += KS) {
-            const int r = q & 3, row = 4 * (lane >> 4) + r;
-            if (r >= nr) continue;
-            const bool live = row < nr;
-            const int pr = s_list[off + (live ? row : 0)];
-            if constexpr (MODE == 0) {
-              const float g = total(0, r), v = total(1, r);
-              if (live) {
-                const float act = g / (1.f + expf(-g)) * v;
-                uint16_t* dst = a.act + (size_t)pr * a.i + 16 * tile + (lane & 15);
-                const float hi8 = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi8;
-                const float mi8 = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi8;
-                dst[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
-                dst[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
-                dst[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
-              }
-            } else {
-              const float v = total(q >> 2, r);
-              if (live) a.yp[(size_t)pr * a.h + 32 * tile + 16 * (q >> 2) + (lane & 15)] = v;
-            }
-          }
-        };
-        if (KS > 4) part(std::integral_constant<int, 8>{});
-        else if (KS > 2) part(std::integral_constant<int, 4>{});
-        else if (KS == 2) part(std::integral_constant<int, 2>{});
-        else part(std::integral_constant<int, 1>{});
-        par ^= 1;
-      };
-      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-      f32x4 o[TL];
-      if (cpw == 1) {  // x stays
-#pragma unroll
-        for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t0, 0);
-        fetch_x(0);
-#pragma unroll
-        for (int i = 0; i < TL; ++i) load_w(w[1][i], i, t0 + 1, 0);
-        const float xs = order_x<Fm, NP>(x);
-        auto body = [&](Fm (&f)[TL], int t) __attribute__((always_inline)) {
-#pragma unroll
-          for (int i = 0; i < TL; ++i) o[i] = z, f[i].template mac<NP>(x, xs, half_of(wk), o[i]), load_w(f[i], i, t + 2, 0);
-          finish(o, t);
-        };
-        for (int t = t0;;) {
-          body(w[0], t);
-          if (++t >= t1) break;
-          body(w[1], t);
-          if (++t >= t1) break;
+      for (int p = NP - 1; p >= 0; --p) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (k < K) v = ld16(MODE == 0 ? a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K + k : a.act + p * plane + (size_t)pr * K + k);
+        if constexpr (Fm::perm) {
+          sum += ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) + ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
+          v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                         __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
         }
-      } else {
-        // step and chunk, and those of the one ahead (x) and the two ahead (weights)
-        int t = t0, ci = 0, tx = t0, cx = 0, tw = t0, cw = 0;
-        auto next = [&](int& t, int& ci) {
-          if (++ci == cpw) ci = 0, ++t;
-        };
+        *reinterpret_cast<uint4*>(xb + slot * L.RB + (p * L.Kp + k) * 2) = v;
+      }
+      if constexpr (Fm::perm) {
+        // the 8 pieces of a group are 8 consecutive threads (k8 is a multiple of 8), all in or all past the rows
+        sum = xsum_step<4>(xsum_step<2>(xsum_step<1>(sum)));
+        if ((q & 7) == 0) sums[slot * L.GS + k / 64] = sum;
+      }
+    }
+    lds_barrier();
+    // the position to load next: chunk lc of tile lt of item ld, whose tiles here are the counter's lbase .. lbase + ln - 1
+    int ld = dA, lbase = 0, lt = 0, lt0, lt1, lc = nch;
+    bool over = false;
+    range(ld, lt0, lt1);
+    Rsrc Q, S;
+    auto open = [&]() __attribute__((always_inline)) {
+      const size_t m = sh ? 0 : __builtin_amdgcn_readfirstlane(s_e[ld]);
+      Q = rsrc(Wq + m * Fm::q_bytes(N, K), (uint32_t)Fm::q_bytes(N, K));
+      S = rsrc(reinterpret_cast<const char*>(Ws) + m * Fm::s_bytes(N, K), (uint32_t)Fm::s_bytes(N, K));
+    };
+    open();
+    int td[DEPTH], tt[DEPTH], tc[DEPTH];  // item (-1: none), tile and chunk of the ring's places
+    Fm w[DEPTH][TL];
+    auto advance = [&](Fm (&f)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {
+      if (++lc >= nch && !over) {
+        int k = 0;
+        if (lane == 0) k = atomicAdd(&s_ticket, 1);
+        k = __builtin_amdgcn_readfirstlane(k);
+        if (k >= lbase + lt1 - lt0) {
+          do {
+            lbase += lt1 - lt0;
+            if (++ld >= dB) {
+              over = true;
+              break;
+            }
+            range(ld, lt0, lt1);
+          } while (k >= lbase + lt1 - lt0);
+          if (!over) open();
+        }
+        lt = lt0 + k - lbase, lc = 0;
+      }
+      d = over ? -1 : ld, t = lt, c = lc;
+      const bool none = over | (lc * 256 + 128 >= K);
 #pragma unroll
-        for (int i = 0; i < TL; ++i) load_w(w[0][i], i, t0, 0);
-        fetch_x(0);
-        next(tw, cw), next(tx, cx);
+      for (int i = 0; i < TL; ++i) f[i].load(Q, S, MODE == 0 ? 16 * lt + i * a.i : 64 * lt + 16 * i, K, lc, none, over);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { advance(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
+    f32x4 o[TL];
+    const char* xr = xb;
+    const float* sr = sums;
+    // one chunk; false: there is none
+    auto body = [&](Fm (&f)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {
+      if (d < 0) return false;
+      if (c == 0) {
+        const int cnt = s_num[d], slot = s_off[d] - pos + (c16 < cnt ? c16 : cnt - 1);
+        xr = xb + slot * L.RB + 2 * Fm::xoff(g);
+        sr = sums + slot * L.GS + g;
 #pragma unroll
-        for (int i = 0; i < TL; ++i) load_w(w[1][i], i, tw, cw);
-        auto body = [&](Fm (&f)[TL]) __attribute__((always_inline)) {
-          const float xs = order_x<Fm, NP>(x);
-          if (ci == 0)
+        for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      const bool half = c * 256 + 128 >= K;
+      const float xs = Fm::perm ? sr[4 * c] : 0.f;
 #pragma unroll
-            for (int i = 0; i < TL; ++i) o[i] = z;
+      for (int i = 0; i < TL; ++i) f[i].prep(half), f[i].rest(xs, o[i]);
 #pragma unroll
-          for (int i = 0; i < TL; ++i) f[i].template mac<NP>(x, xs, half_of(wk + KS * ci), o[i]);
-          fetch_x(cx);
-          next(tx, cx), next(tw, cw);
+      for (int p = 0; p < 2; ++p) {
+        f32x4 acc[TL];
 #pragma unroll
-          for (int i = 0; i < TL; ++i) load_w(f[i], i, tw, cw);
-          if (ci == cpw - 1) finish(o, t);
-          next(t, ci);
-        };
-        for (;;) {
-          body(w[0]);
-          if (t >= t1) break;
-          body(w[1]);
-          if (t >= t1) break;
+        for (int h = 0; h < 2; ++h) {
+          uint4 x[NP][2];
+#pragma unroll
+          for (int q = 0; q < NP; ++q) {
+            const uint4* src = reinterpret_cast<const uint4*>(xr + q * L.Kp * 2 + (c * 256 + 128 * p + 64 * h) * 2);
+            x[q][0] = src[0], x[q][1] = src[1];
+          }
+#pragma unroll
+          for (int i = 0; i < TL; ++i) f[i].template group<NP>(p, h, x, acc[i], o[i]);
         }
       }
+      if (c == nch - 1) {
+        // register r of lane l: row 4 (l / 16) + r of x, column l % 16
+        const int off = s_off[d], cnt = s_num[d];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r >= cnt) break;
+          const int row = 4 * g + r;
+          if (row >= cnt) continue;
+          const int pr = s_list[off + row];
+          if constexpr (MODE == 0) {
+            const float act = o[0][r] / (1.f + expf(-o[0][r])) * o[1][r];
+            uint16_t* dst = a.act + (size_t)pr * a.i + 16 * t + c16;
+            const float hi8 = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi8;
+            const float mi8 = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi8;
+            dst[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
+            dst[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
+            dst[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
+          } else {
+#pragma unroll
+            for (int i = 0; i < TL; ++i) a.yp[(size_t)pr * a.h + 64 * t + 16 * i + c16] = o[i][r];
+          }
+        }
+      }
+      advance(f, d, t, c);
+      return true;
     };
-    if (sh) segment(FS{}, MODE == 0 ? a.sgu_q : a.sd_q, MODE == 0 ? a.sgu_s : a.sd_s);
-    else
-      segment(F{}, (MODE == 0 ? a.gu_q : a.d_q) + e * F::q_bytes(N, K),
-              reinterpret_cast<const char*>(MODE == 0 ? a.gu_s : a.d_s) + e * F::s_bytes(N, K));
+    bool more = true;
+    do {
+      static_for<DEPTH>([&](auto k) __attribute__((always_inline)) {
+        if (more) more = body(w[k.value], td[k.value], tt[k.value], tc[k.value]);
+      });
+    } while (more);
+    lds_barrier();  // the rows may be replaced
+  };
+  int d1 = s_first;
+  while (d1 < D && s_cum[d1] < hi) ++d1;  // items s_first .. d1 - 1 are this block's
+  for (int d = s_first; d < d1;) {
+    int e = d + 1;
+    const bool sh = d >= D0;
+    while (e < d1 && (e >= D0) == sh && s_off[e] + s_num[e] - s_off[d] <= L.R) ++e;
+    if (sh) run(FS{}, d, e, true, reinterpret_cast<const uint8_t*>(MODE == 0 ? a.sgu_q : a.sd_q), MODE == 0 ? a.sgu_s : a.sd_s);
+    else run(F{}, d, e, false, MODE == 0 ? a.gu_q : a.d_q, MODE == 0 ? a.gu_s : a.d_s);
+    d = e;
   }
 }
 
@@ -553,16 +566,6 @@ struct WsLayout {
   }
 };
 
-// The waves that share a tile's K inputs and the chunks each takes: a wave per chunk up to all eight.
-struct Split {
-  int ks, cpw;
-  Split(int K) {
-    const int nch = (K + 255) / 256;
-    cpw = (nch + MR_NW - 1) / MR_NW;
-    ks = (nch + cpw - 1) / cpw;
-  }
-};
-
 template <class F, class SH, bool BYTES>
 int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   if (!rows_shape_ok(a.rows, a.e, a.h, a.i, a.topk)) return -1;
@@ -584,9 +587,8 @@ int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   else if (a.rows <= 8) hipLaunchKernelGGL(k_moe_rows_router<2>, dim3(nb, (a.rows + 1) / 2), dim3(MR_NT), 0, st, a);
   else if (a.rows <= 32) hipLaunchKernelGGL(k_moe_rows_router<4>, dim3(nb, (a.rows + 3) / 4), dim3(MR_NT), 0, st, a);
   else hipLaunchKernelGGL(k_moe_rows_router<8>, dim3(nb, (a.rows + 7) / 8), dim3(MR_NT), 0, st, a);
-  const Split g(a.h), d(a.i);
-  hipLaunchKernelGGL((k_moe_rows_experts<0, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, g.ks, g.cpw, BYTES ? 1 : 2);
-  hipLaunchKernelGGL((k_moe_rows_experts<1, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), 0, st, a, d.ks, d.cpw, BYTES ? 1 : 2);
+  hipLaunchKernelGGL((k_moe_rows_experts<0, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), MR_X, st, a, BYTES ? 1 : 2);
+  hipLaunchKernelGGL((k_moe_rows_experts<1, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), MR_X, st, a, BYTES ? 1 : 2);
   hipLaunchKernelGGL(k_moe_rows_combine, dim3(a.rows, (a.h + 1023) / 1024), dim3(256), 0, st, a);
   return 0;
 }
