@@ -67,7 +67,8 @@ DEV Rsrc rsrc(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
 }
 constexpr uint32_t NOWHERE = 0x80000000u;  // past every matrix
-DEV uint4 buf16(const Rsrc& r, uint32_t off) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); }
+DEV gu32x4 buf16(const Rsrc& r, uint32_t off) { return __builtin_bit_cast(gu32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); }
+DEV uint4 words(const gu32x4& v) { return make_uint4(v.x, v.y, v.z, v.w); }
 
 // Where lane l's piece of a row pair's loads lies: row l % 8 (+ 8 in the second load), bytes 16 (4 (l / 8 % 2) + l / 16) of the 128
 DEV int pair_row() { return lane_id() & 7; }
@@ -86,17 +87,21 @@ DEV void pair_up(uint4& a, uint4& b) {
 template <class SC>
 struct RowsQ4 {
   static constexpr bool perm = true;  // fragment order 0 4 1 5 2 6 3 7
+  // as loaded, each a register quadruple that stays one (split into words, the ring's loop would copy them, and wait for them)
+  struct Raw {
+    gu32x4 w[2], s;
+  };
   uint4 w[2], s;
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K / 2; }
   static DEV size_t s_bytes(int N, int K) { return (size_t)N * K / 16; }
   static DEV int xoff(int g) { return 32 * (g & 1) + 16 * (g >> 1); }
   // n: the tile's first row
-  DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
+  static DEV void load(Raw& f, const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
     const bool none = off || (half && (lane_id() & 8));
     const uint32_t p = (n + pair_row()) * (K / 2) + c * 128 + pair_byte();
-    w[0] = buf16(Q, none ? NOWHERE : p);
-    w[1] = buf16(Q, none ? NOWHERE : p + 4 * K);
-    s = buf16(S, off ? NOWHERE : ((n + (lane_id() & 15)) * (K / 64) + c * 4) * 4);
+    f.w[0] = buf16(Q, none ? NOWHERE : p);
+    f.w[1] = buf16(Q, none ? NOWHERE : p + 4 * K);
+    f.s = buf16(S, off ? NOWHERE : ((n + (lane_id() & 15)) * (K / 64) + c * 4) * 4);
   }
   // nibbles of a word as 16 + q in bf16: the nibble is the top four mantissa bits of a number in [16, 32)
   // (the two constants in registers, so that each pair of nibbles is a shift and one v_and_or_b32)
@@ -107,9 +112,10 @@ struct RowsQ4 {
     return make_uint4(((v << 3) & m) | b, ((v >> 1) & m) | b, ((v >> 5) & m) | b, ((v >> 9) & m) | b);
   }
   // The tile's words in the order of the products: w[p].x, .y the fragments of group 2 p, .z, .w of group 2 p + 1
-  DEV void prep(bool half) {
+  DEV void prep(const Raw& f, bool half) {
+    w[0] = words(f.w[0]), w[1] = words(f.w[1]);
     pair_up(w[0], w[1]);
-    if (half) s.z = s.w = 0;
+    s = make_uint4(f.s.x, f.s.y, pick(half, 0, f.s.z), pick(half, 0, f.s.w));
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       // lanes g = 0, 1 hold group 2 p, g = 2, 3 group 2 p + 1: two words of each change places
@@ -144,18 +150,27 @@ struct RowsQ4 {
 template <class D>
 struct Rows8 {
   static constexpr bool perm = false;
+  struct Raw {
+    gu32x4 w[4];
+    uint32_t s[2];
+  };
   uint4 w[4];
   uint32_t s[2];
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K; }
   static DEV int xoff(int g) { return 16 * g; }
-  DEV void load(const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
+  static DEV void load(Raw& f, const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
     const uint32_t p = (n + pair_row()) * K + c * 256 + pair_byte();
-    w[0] = buf16(Q, off ? NOWHERE : p), w[1] = buf16(Q, off ? NOWHERE : p + 8 * K);
-    w[2] = buf16(Q, half ? NOWHERE : p + 128), w[3] = buf16(Q, half ? NOWHERE : p + 128 + 8 * K);
-    s[0] = D::scale_raw(S, n + (lane_id() & 15), 2 * c, K, off);
-    s[1] = D::scale_raw(S, n + (lane_id() & 15), 2 * c + 1, K, half);
+    f.w[0] = buf16(Q, off ? NOWHERE : p), f.w[1] = buf16(Q, off ? NOWHERE : p + 8 * K);
+    f.w[2] = buf16(Q, half ? NOWHERE : p + 128), f.w[3] = buf16(Q, half ? NOWHERE : p + 128 + 8 * K);
+    f.s[0] = D::scale_raw(S, n + (lane_id() & 15), 2 * c, K, off);
+    f.s[1] = D::scale_raw(S, n + (lane_id() & 15), 2 * c + 1, K, half);
   }
-  DEV void prep(bool) { pair_up(w[0], w[1]), pair_up(w[2], w[3]); }
+  DEV void prep(const Raw& f, bool) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = words(f.w[q]);
+    pair_up(w[0], w[1]), pair_up(w[2], w[3]);
+    s[0] = f.s[0], s[1] = f.s[1];
+  }
   DEV void rest(float, f32x4&) const {}
   template <int NP>
   DEV void group(int p, int h, const uint4 (&x)[NP][2], f32x4& a, f32x4& out) const {
@@ -422,8 +437,8 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
     };
     open();
     int td[DEPTH], tt[DEPTH], tc[DEPTH];  // item (-1: none), tile and chunk of the ring's places
-    Fm w[DEPTH][TL];
-    auto advance = [&](Fm (&f)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {
+    typename Fm::Raw w[DEPTH][TL];
+    auto advance = [&](typename Fm::Raw (&f)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {
       if (++lc >= nch && !over) {
         int k = 0;
         if (lane == 0) k = atomicAdd(&s_ticket, 1);
@@ -444,17 +459,15 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
       d = over ? -1 : ld, t = lt, c = lc;
       const bool none = over | (lc * 256 + 128 >= K);
 #pragma unroll
-      for (int i = 0; i < TL; ++i) f[i].load(Q, S, MODE == 0 ? 16 * lt + i * a.i : 64 * lt + 16 * i, K, lc, none, over);
+      for (int i = 0; i < TL; ++i) Fm::load(f[i], Q, S, MODE == 0 ? 16 * lt + i * a.i : 64 * lt + 16 * i, K, lc, none, over);
       __builtin_amdgcn_sched_barrier(0);
     };
     static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { advance(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
     f32x4 o[TL];
     const char* xr = xb;
     const float* sr = sums;
-    // one chunk; false: there is none
-    auto body = [&](Fm (&f)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {
-      if (d < 0) return false;
-      if (c == 0) {
+    auto body = [&](typename Fm::Raw (&raw)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {  // one chunk
+      if (c == 0 && d >= 0) {
         const int cnt = s_num[d], slot = s_off[d] - pos + (c16 < cnt ? c16 : cnt - 1);
         xr = xb + slot * L.RB + 2 * Fm::xoff(g);
         sr = sums + slot * L.GS + g;
@@ -462,9 +475,10 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
         for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
       const bool half = c * 256 + 128 >= K;
+      Fm f[TL];
       const float xs = Fm::perm ? sr[4 * c] : 0.f;
 #pragma unroll
-      for (int i = 0; i < TL; ++i) f[i].prep(half), f[i].rest(xs, o[i]);
+      for (int i = 0; i < TL; ++i) f[i].prep(raw[i], half), f[i].rest(xs, o[i]);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         f32x4 acc[TL];
@@ -480,7 +494,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
           for (int i = 0; i < TL; ++i) f[i].template group<NP>(p, h, x, acc[i], o[i]);
         }
       }
-      if (c == nch - 1) {
+      if (c == nch - 1 && d >= 0) {
         // register r of lane l: row 4 (l / 16) + r of x, column l % 16
         const int off = s_off[d], cnt = s_num[d];
 #pragma unroll
@@ -503,15 +517,11 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
           }
         }
       }
-      advance(f, d, t, c);
-      return true;
+      advance(raw, d, t, c);
     };
-    bool more = true;
-    do {
-      static_for<DEPTH>([&](auto k) __attribute__((always_inline)) {
-        if (more) more = body(w[k.value], td[k.value], tt[k.value], tc[k.value]);
-      });
-    } while (more);
+    // One exit, at the head: places of the ring without a tile are computed too (zeros, not stored), since paths that
+    // skip loads and join the loop again would make every wait in it a wait for all loads.
+    while (td[0] >= 0) static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { body(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
     lds_barrier();  // the rows may be replaced
   };
   int d1 = s_first;
