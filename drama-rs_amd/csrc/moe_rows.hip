@@ -284,6 +284,17 @@ __global__ void __launch_bounds__(MR_NT) k_moe_rows_router(MoeRows a) {
 }
 
 // ---- experts ----------------------------------------------------------------------------------
+// inclusive sum over the lanes
+DEV int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 64 t, K = i).
 //
 // Items are passes of up to P rows of an expert, ascending, then of the shared expert (whose rows are all); their
@@ -314,9 +325,8 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
   extern __shared__ uint4 xlds[];
   __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert, then the shared expert's rows
   __shared__ uint16_t s_e[MR_ITEMS], s_off[MR_ITEMS], s_num[MR_ITEMS];  // items: expert, first place in s_list, rows
-  __shared__ int s_cum[MR_ITEMS + 1];              // cost of the items before
-  __shared__ uint32_t s_rows[256][2];
-  __shared__ int s_start[256], s_tot[8][3], s_first, s_ticket;
+  __shared__ uint2 s_rows[256];
+  __shared__ int s_start[256], s_d0, s_ticket;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x, c16 = lane & 15, g = lane >> 4;
   const int pairs = a.rows * a.topk;
   const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 64, N = MODE == 0 ? 2 * a.i : a.h;
@@ -328,103 +338,74 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
   int pe[PPT];
 #pragma unroll
   for (int q = 0; q < PPT; ++q) pe[q] = tid + MR_NT * q < pairs ? a.idx[tid + MR_NT * q] & 255 : -1;
-  if (tid < 256) s_rows[tid][0] = s_rows[tid][1] = 0;
+  if (tid < 256) s_rows[tid] = make_uint2(0, 0);
   lds_barrier();
 #pragma unroll
   for (int q = 0; q < PPT; ++q)
     if (pe[q] >= 0) {
       const int r = (tid + MR_NT * q) / a.topk;
-      atomicOr(&s_rows[pe[q]][r >> 5], 1u << (r & 31));
+      atomicOr(r < 32 ? &s_rows[pe[q]].x : &s_rows[pe[q]].y, 1u << (r & 31));
     }
   lds_barrier();
-  // sums over the experts (thread e) of their rows, their passes and their cost
-  {
-    int v[3] = {0, 0, 0}, own[3];
-    const bool sh = tid == 256;
-    const int cost = tiles * (sh ? fs_cost : 1);
-    if (tid <= 256) {
-      v[0] = sh ? (a.shared ? a.rows : 0) : __builtin_popcount(s_rows[tid][0]) + __builtin_popcount(s_rows[tid][1]);
-      v[1] = (v[0] + P - 1) / P;
-      v[2] = v[1] * cost;
-    }
+  if (wave == 0) {
+    // lane l: experts 4 l .. 4 l + 3; rows and passes summed over the experts before, in the halves of a word
+    int n[4], v = 0;
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
-      own[q] = v[q];
-      for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(v[q], o);
-        if (lane >= o) v[q] += up;
-      }
-      if (lane == 63) s_tot[wave][q] = v[q];
+    for (int j = 0; j < 4; ++j) {
+      const uint2 m = s_rows[4 * lane + j];
+      n[j] = __builtin_popcount(m.x) + __builtin_popcount(m.y);
+      v += n[j] | (n[j] + P - 1) / P << 16;
     }
-    lds_barrier();
-    int base[3] = {0, 0, 0};
-    for (int w = 0; w < wave; ++w)
+    int at = wave_scan(v) - v;
 #pragma unroll
-      for (int q = 0; q < 3; ++q) base[q] += s_tot[w][q];
-    lds_barrier();
-    if (tid <= 256) {
-      const int off = base[0] + v[0] - own[0], cum = base[2] + v[2] - own[2], d0 = base[1] + v[1] - own[1];
-      for (int p = 0; p < own[1]; ++p) {
-        s_e[d0 + p] = tid, s_off[d0 + p] = off + P * p, s_num[d0 + p] = own[0] - P * p < P ? own[0] - P * p : P;
-        s_cum[d0 + p] = cum + cost * p;
-      }
-      if (!sh) s_start[tid] = off;
-      else s_cum[d0 + own[1]] = base[2] + v[2], s_tot[0][0] = d0 + own[1], s_tot[1][0] = d0;
+    for (int j = 0; j < 4; ++j) {
+      int off = at & 0xffff, d = at >> 16;
+      s_start[4 * lane + j] = off;
+      at += n[j] | (n[j] + P - 1) / P << 16;
+      for (int left = n[j]; left > 0; left -= P, off += P, ++d) s_e[d] = 4 * lane + j, s_off[d] = off, s_num[d] = left < P ? left : P;
     }
-    lds_barrier();
+    if (lane == 63) {
+      int d = at >> 16;
+      s_d0 = d, s_ticket = 0;
+      if (a.shared)
+        for (int r = 0; r < a.rows; r += P, ++d) s_e[d] = 256, s_off[d] = pairs + r, s_num[d] = a.rows - r < P ? a.rows - r : P;
+    }
   }
-  const int D = s_tot[0][0], D0 = s_tot[1][0];  // items, those of the routed experts
-  const int lo = (int)((long long)s_cum[D] * blockIdx.x / gridDim.x), hi = (int)((long long)s_cum[D] * (blockIdx.x + 1) / gridDim.x);
-  for (int d = tid; d < D; d += MR_NT)
-    if (s_cum[d] <= lo && lo < s_cum[d + 1]) s_first = d;
+  lds_barrier();
 #pragma unroll
   for (int q = 0; q < PPT; ++q)
     if (pe[q] >= 0) {
       const int r = (tid + MR_NT * q) / a.topk;
-      const uint32_t lo32 = s_rows[pe[q]][0], hi32 = s_rows[pe[q]][1], below = (1u << (r & 31)) - 1;
-      s_list[s_start[pe[q]] + (r < 32 ? __builtin_popcount(lo32 & below) : __builtin_popcount(lo32) + __builtin_popcount(hi32 & below))] =
+      const uint2 m = s_rows[pe[q]];
+      const uint32_t below = (1u << (r & 31)) - 1;
+      s_list[s_start[pe[q]] + (r < 32 ? __builtin_popcount(m.x & below) : __builtin_popcount(m.x) + __builtin_popcount(m.y & below))] =
           tid + MR_NT * q;
     }
   if (a.shared && tid < a.rows) s_list[pairs + tid] = pairs + tid;
   lds_barrier();
+  // items of the routed experts, of all; cost of the items before d: 1 a tile, fs_cost a tile of the shared expert
+  const int D0 = __builtin_amdgcn_readfirstlane(s_d0), D = D0 + (a.shared ? (a.rows + P - 1) / P : 0);
+  auto cost_before = [&](int d) { return d <= D0 ? d * tiles : D0 * tiles + (d - D0) * tiles * fs_cost; };
+  const long long all = cost_before(D);
+  const int lo = (int)(all * blockIdx.x / gridDim.x), hi = (int)(all * (blockIdx.x + 1) / gridDim.x);
   if (lo >= hi) return;
+  auto item_at = [&](int c) { return c < D0 * tiles ? c / tiles : D0 + (c - D0 * tiles) / (tiles * fs_cost); };
+  const int dfirst = item_at(lo), dend = item_at(hi - 1) + 1;  // this block's items
   const size_t plane = (size_t)(pairs + a.rows) * a.i;
   char* xb = reinterpret_cast<char*>(xlds);
   float* sums = reinterpret_cast<float*>(xb + (size_t)L.R * L.RB);
   // the block's tiles [t0, t1) of item d
   auto range = [&](int d, int& t0, int& t1) __attribute__((always_inline)) {
-    const int cum = s_cum[d], tc = d < D0 ? 1 : fs_cost;
+    const int cum = cost_before(d), tc = d < D0 ? 1 : fs_cost;
     t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0;
     t1 = (hi - cum + tc - 1) / tc;
-    t0 = __builtin_amdgcn_readfirstlane(t0 < tiles ? t0 : tiles), t1 = __builtin_amdgcn_readfirstlane(t1 < tiles ? t1 : tiles);
+    t0 = t0 < tiles ? t0 : tiles, t1 = t1 < tiles ? t1 : tiles;
   };
   // items dA .. dB - 1, of one weight format, their rows in the slots from 0
   auto run = [&](auto fmt, const int dA, const int dB, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
     using Fm = decltype(fmt);
     constexpr int DEPTH = Fm::perm ? 8 / TL : MODE == 0 ? 3 : 2;
     const int pos = s_off[dA], nrows = s_off[dB - 1] + s_num[dB - 1] - pos, k8 = L.Kp / 8;
-    if (tid == 0) s_ticket = 0;
-    for (int q = tid; q < nrows * k8; q += MR_NT) {
-      const int slot = q / k8, k = (q - slot * k8) * 8, pr = s_list[pos + slot];
-      float sum = 0.f;
-#pragma unroll
-      for (int p = NP - 1; p >= 0; --p) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (k < K) v = ld16(MODE == 0 ? a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K + k : a.act + p * plane + (size_t)pr * K + k);
-        if constexpr (Fm::perm) {
-          sum += ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) + ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
-          v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                         __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
-        }
-        *reinterpret_cast<uint4*>(xb + slot * L.RB + (p * L.Kp + k) * 2) = v;
-      }
-      if constexpr (Fm::perm) {
-        // the 8 pieces of a group are 8 consecutive threads (k8 is a multiple of 8), all in or all past the rows
-        sum = xsum_step<4>(xsum_step<2>(xsum_step<1>(sum)));
-        if ((q & 7) == 0) sums[slot * L.GS + k / 64] = sum;
-      }
-    }
-    lds_barrier();
     // the position to load next: chunk lc of tile lt of item ld, whose tiles here are the counter's lbase .. lbase + ln - 1
     int ld = dA, lbase = 0, lt = 0, lt0, lt1, lc = nch;
     bool over = false;
@@ -463,6 +444,28 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
       __builtin_amdgcn_sched_barrier(0);
     };
     static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { advance(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
+    // the rows, requested behind the first weights: the two waits are one
+    for (int q = tid; q < nrows * k8; q += MR_NT) {
+      const int slot = q / k8, k = (q - slot * k8) * 8, pr = s_list[pos + slot];
+      float sum = 0.f;
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (k < K) v = ld16(MODE == 0 ? a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K + k : a.act + p * plane + (size_t)pr * K + k);
+        if constexpr (Fm::perm) {
+          sum += ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) + ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
+          v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                         __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
+        }
+        *reinterpret_cast<uint4*>(xb + slot * L.RB + (p * L.Kp + k) * 2) = v;
+      }
+      if constexpr (Fm::perm) {
+        // the 8 pieces of a group are 8 consecutive threads (k8 is a multiple of 8), all in or all past the rows
+        sum = xsum_step<4>(xsum_step<2>(xsum_step<1>(sum)));
+        if ((q & 7) == 0) sums[slot * L.GS + k / 64] = sum;
+      }
+    }
+    lds_barrier();
     f32x4 o[TL];
     const char* xr = xb;
     const float* sr = sums;
@@ -522,14 +525,14 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
     // One exit, at the head: places of the ring without a tile are computed too (zeros, not stored), since paths that
     // skip loads and join the loop again would make every wait in it a wait for all loads.
     while (td[0] >= 0) static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { body(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
-    lds_barrier();  // the rows may be replaced
+    lds_barrier();  // the rows may be replaced, the counter starts again
+    if (tid == 0) s_ticket = 0;
+    lds_barrier();
   };
-  int d1 = s_first;
-  while (d1 < D && s_cum[d1] < hi) ++d1;  // items s_first .. d1 - 1 are this block's
-  for (int d = s_first; d < d1;) {
+  for (int d = dfirst; d < dend;) {
     int e = d + 1;
     const bool sh = d >= D0;
-    while (e < d1 && (e >= D0) == sh && s_off[e] + s_num[e] - s_off[d] <= L.R) ++e;
+    while (e < dend && (e >= D0) == sh && s_off[e] + s_num[e] - s_off[d] <= L.R) ++e;
     if (sh) run(FS{}, d, e, true, reinterpret_cast<const uint8_t*>(MODE == 0 ? a.sgu_q : a.sd_q), MODE == 0 ? a.sgu_s : a.sd_s);
     else run(F{}, d, e, false, MODE == 0 ? a.gu_q : a.d_q, MODE == 0 ? a.gu_s : a.d_s);
     d = e;
