@@ -235,24 +235,36 @@ __global__ void __launch_bounds__(MR_NT) k_moe_rows_router(MoeRows a) {
 #pragma unroll
     for (int t = 0; t < TS; ++t) acc[t] = 0.f;
     const uint16_t* wr = a.router + (size_t)n * a.h;
-    const uint16_t* xr[TS];
+    // 2048 inputs at a time: the row of the router, then the rows of x one after the other with the next one in flight;
+    // chunks past h are neither loaded nor added
+    for (int c0 = lane * 8; c0 - lane * 8 < a.h; c0 += 2048) {
+      uint4 w[4], v[2][4];
+      auto load = [&](const uint16_t* p, uint4 (&d)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < TS; ++t) xr[t] = a.x + (size_t)(r0 + t < a.rows ? r0 + t : a.rows - 1) * a.h;
-#pragma unroll 4
-    for (int c = lane * 8; c < a.h; c += WAVE * 8) {
-      const uint4 w = ld16(wr + c);
+        for (int j = 0; j < 4; ++j) d[j] = ld16(p + (c0 + 512 * j < a.h ? c0 + 512 * j : 0));
+      };
+      auto row = [&](int t) { return a.x + (size_t)(r0 + t < a.rows ? r0 + t : a.rows - 1) * a.h; };
+      load(wr, w);
+      load(row(0), v[0]);
+      static_for<TS>([&](auto tt) __attribute__((always_inline)) {
+        constexpr int t = decltype(tt)::value;
+        if constexpr (t + 1 < TS) load(row(t + 1), v[(t + 1) & 1]);
+        issue_fence();
 #pragma unroll
-      for (int t = 0; t < TS; ++t) {
-        const uint4 v = ld16(xr[t] + c);
-        acc[t] = __builtin_fmaf(bf16_lo(w.x), bf16_lo(v.x), acc[t]);
-        acc[t] = __builtin_fmaf(bf16_hi(w.x), bf16_hi(v.x), acc[t]);
-        acc[t] = __builtin_fmaf(bf16_lo(w.y), bf16_lo(v.y), acc[t]);
-        acc[t] = __builtin_fmaf(bf16_hi(w.y), bf16_hi(v.y), acc[t]);
-        acc[t] = __builtin_fmaf(bf16_lo(w.z), bf16_lo(v.z), acc[t]);
-        acc[t] = __builtin_fmaf(bf16_hi(w.z), bf16_hi(v.z), acc[t]);
-        acc[t] = __builtin_fmaf(bf16_lo(w.w), bf16_lo(v.w), acc[t]);
-        acc[t] = __builtin_fmaf(bf16_hi(w.w), bf16_hi(v.w), acc[t]);
-      }
+        for (int j = 0; j < 4; ++j) {
+          const uint4 q = w[j], u = v[t & 1][j];
+          float s = acc[t];
+          s = __builtin_fmaf(bf16_lo(q.x), bf16_lo(u.x), s);
+          s = __builtin_fmaf(bf16_hi(q.x), bf16_hi(u.x), s);
+          s = __builtin_fmaf(bf16_lo(q.y), bf16_lo(u.y), s);
+          s = __builtin_fmaf(bf16_hi(q.y), bf16_hi(u.y), s);
+          s = __builtin_fmaf(bf16_lo(q.z), bf16_lo(u.z), s);
+          s = __builtin_fmaf(bf16_hi(q.z), bf16_hi(u.z), s);
+          s = __builtin_fmaf(bf16_lo(q.w), bf16_lo(u.w), s);
+          s = __builtin_fmaf(bf16_hi(q.w), bf16_hi(u.w), s);
+          acc[t] = c0 + 512 * j < a.h ? s : acc[t];
+        }
+      });
     }
 #pragma unroll
     for (int t = 0; t < TS; ++t) {
@@ -270,8 +282,21 @@ __global__ void __launch_bounds__(MR_NT) k_moe_rows_router(MoeRows a) {
   if (!s_last) return;
   if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const int nr = a.rows - r0 < TS ? a.rows - r0 : TS;
-  for (int q = threadIdx.x; q < nr * E1; q += MR_NT)
-    lg[q / E1][q % E1] = __hip_atomic_load(a.logits + (size_t)r0 * E1 + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  {
+    // every row's logits requested at once
+    constexpr int NL = (TS * 257 + MR_NT - 1) / MR_NT;
+    float v[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int q = threadIdx.x + MR_NT * i;
+      v[i] = q < nr * E1 ? __hip_atomic_load(a.logits + (size_t)r0 * E1 + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int q = threadIdx.x + MR_NT * i;
+      if (q < nr * E1) lg[q / E1][q % E1] = v[i];
+    }
+  }
   __syncthreads();
   if (wave < nr) {
     int id;
