@@ -17,6 +17,7 @@ constexpr int MR_NW = 8, MR_NT = MR_NW * 64, MR_ROWS = 64, MR_TOPK = 32, MR_PAIR
 constexpr int MR_GRID = 256;             // a block per CU
 constexpr int MR_X = 120 * 1024;         // LDS bytes for rows of x
 constexpr int MR_ITEMS = MR_PAIRS + MR_ROWS;  // passes, the experts' and the shared expert's, of one row each at worst
+constexpr int FEW_RING = 2;              // chunks a wave of few rows has under way
 constexpr int MR_SETS = 8;               // row sets of the router
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -87,6 +88,7 @@ DEV void pair_up(uint4& a, uint4& b) {
 template <class SC>
 struct RowsQ4 {
   static constexpr bool perm = true;  // fragment order 0 4 1 5 2 6 3 7
+  static constexpr bool sums = true;  // needs the sums of x's groups
   // as loaded, each a register quadruple that stays one (split into words, the ring's loop would copy them, and wait for them)
   struct Raw {
     gu32x4 w[2], s;
@@ -147,9 +149,9 @@ struct RowsQ4 {
 
 // One byte per weight: 64 inputs of a row per 16-byte load of four lanes, scales per 128 inputs.  D: the
 // format's conversions
-template <class D>
+template <class D, bool PERM>
 struct Rows8 {
-  static constexpr bool perm = false;
+  static constexpr bool perm = PERM, sums = false;
   struct Raw {
     gu32x4 w[4];
     uint32_t s[2];
@@ -188,7 +190,7 @@ struct Rows8 {
 DEV uint32_t buf_half(const Rsrc& S, uint32_t off) { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(S, off, 0, 0); }
 
 template <int SF>
-struct RowsFP8 : Rows8<RowsFP8<SF>> {
+struct RowsFP8 : Rows8<RowsFP8<SF>, false> {
   static DEV size_t s_bytes(int N, int K) { return (size_t)(N / 128) * (K / 128) * (SF ? 2 : 4); }
   static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
     const uint32_t i = (n >> 7) * (K / 128) + b;
@@ -204,18 +206,22 @@ struct RowsFP8 : Rows8<RowsFP8<SF>> {
   }
 };
 
-template <class SH>
-struct RowsQ8 : Rows8<RowsQ8<SH>> {
+// PERM: the fragment order of int4, beside whose experts it stands
+template <class SH, bool PERM>
+struct RowsQ8 : Rows8<RowsQ8<SH, PERM>, PERM> {
   static DEV size_t s_bytes(int N, int K) { return (size_t)N * (SH::per_row ? 1 : K / 128) * 2; }
   static DEV uint32_t scale_raw(const Rsrc& S, int n, int b, int K, bool off) {
     return buf_half(S, off ? NOWHERE : 2 * (SH::per_row ? n : n * (K / 128) + b));
   }
   static DEV float scale_cvt(uint32_t r) { return SH::cvt(r); }
-  static DEV uint32_t pk(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
-    const float a = (float)(int8_t)(v >> (8 * i)), b = (float)(int8_t)(v >> (8 * i + 8));
+  static DEV uint32_t pk(uint32_t u, int i, uint32_t v, int j) {  // byte i of u and byte j of v as bf16 (exact)
+    const float a = (float)(int8_t)(u >> (8 * i)), b = (float)(int8_t)(v >> (8 * j));
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
   }
-  static DEV uint4 frag(uint32_t a, uint32_t b) { return make_uint4(pk(a, 0), pk(a, 2), pk(b, 0), pk(b, 2)); }
+  static DEV uint4 frag(uint32_t a, uint32_t b) {
+    if constexpr (PERM) return make_uint4(pk(a, 0, b, 0), pk(a, 1, b, 1), pk(a, 2, b, 2), pk(a, 3, b, 3));
+    else return make_uint4(pk(a, 0, a, 1), pk(a, 2, a, 3), pk(b, 0, b, 1), pk(b, 2, b, 3));
+  }
 };
 
 // ---- router -----------------------------------------------------------------------------------
@@ -323,8 +329,10 @@ DEV int wave_scan(int v) {
 // MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 64 t, K = i).
 //
 // Items are passes of up to P rows of an expert, ascending, then of the shared expert (whose rows are all); their
-// tiles are dealt to the blocks in contiguous runs of even cost, the shared expert's counting twice where its bytes are
-// twice the others'.  A block stages the rows of its items in LDS (as many items at a time as R rows hold, most
+// tiles are dealt to the blocks in contiguous runs of even length.  The shared expert has blocks of its own (a block with
+// tiles of both formats would stage and wait twice: gate_up of 4 rows, 256 experts, h 2048, i 512, 25 us instead of 19), twice as
+// many for its tiles as the others: its passes are the fullest and its format the widest (fp8 beside it, 8 rows: 32.0 us with
+// equal numbers, 28.6 with twice, 28.4 with three times as many).  A block stages the rows of its items in LDS (as many items at a time as R rows hold, most
 // often all), then each of its waves takes one tile after the other from a counter and multiplies all of its inputs, in chunks
 // of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights come in a ring of DEPTH chunks that
 // runs on across tiles and items.
@@ -344,9 +352,73 @@ struct XLayout {
   }
 };
 
+// nrows rows (row_of(slot): of x, or of act) into the slots from 0; all threads
+template <int MODE, bool PERM, bool SUMS, class RowOf>
+DEV void stage_rows(const MoeRows& a, const XLayout<MODE>& L, int K, int nrows, char* xb, float* sums, size_t plane, RowOf row_of) {
+  constexpr int NP = XLayout<MODE>::NP;
+  const int k8 = L.Kp / 8;
+  for (int q = threadIdx.x; q < nrows * k8; q += MR_NT) {
+    const int slot = q / k8, k = (q - slot * k8) * 8;
+    const uint16_t* src = (MODE == 0 ? a.x : a.act) + (size_t)row_of(slot) * K + k;
+    float sum = 0.f;
+#pragma unroll
+    for (int p = NP - 1; p >= 0; --p) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (k < K) v = ld16(src + p * plane);
+      if constexpr (SUMS)
+        sum += ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) + ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
+      if constexpr (PERM)
+        v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
+      *reinterpret_cast<uint4*>(xb + slot * L.RB + (p * L.Kp + k) * 2) = v;
+    }
+    if constexpr (SUMS) {
+      // the 8 pieces of a group are 8 consecutive threads (k8 is a multiple of 8), all in or all past the rows
+      sum = xsum_step<4>(xsum_step<2>(xsum_step<1>(sum)));
+      if ((q & 7) == 0) sums[slot * L.GS + k / 64] = sum;
+    }
+  }
+}
+
+// o += the products of chunk c of a lane's row of x (at xr, its sums at sr) with TL tiles of weights
+template <int MODE, class Fm, int TL>
+DEV void chunk_mac(const typename Fm::Raw (&raw)[TL], const char* xr, const float* sr, int Kp, int c, bool half, f32x4 (&o)[TL]) {
+  constexpr int NP = XLayout<MODE>::NP;
+  Fm f[TL];
+  const float xs = Fm::sums ? sr[4 * c] : 0.f;
+#pragma unroll
+  for (int i = 0; i < TL; ++i) f[i].prep(raw[i], half), f[i].rest(xs, o[i]);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    f32x4 acc[TL];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint4 x[NP][2];
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        const uint4* src = reinterpret_cast<const uint4*>(xr + q * Kp * 2 + (c * 256 + 128 * p + 64 * h) * 2);
+        x[q][0] = src[0], x[q][1] = src[1];
+      }
+#pragma unroll
+      for (int i = 0; i < TL; ++i) f[i].template group<NP>(p, h, x, acc[i], o[i]);
+    }
+  }
+}
+
+// silu(g) u as three bf16 planes: 8 mantissa bits each, the last exact
+DEV void store_act(const MoeRows& a, size_t plane, int pair, int col, float g, float u) {
+  const float act = g / (1.f + expf(-g)) * u;
+  uint16_t* dst = a.act + (size_t)pair * a.i + col;
+  const float hi = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi;
+  const float mi = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi;
+  dst[0] = (uint16_t)(__float_as_uint(hi) >> 16);
+  dst[plane] = (uint16_t)(__float_as_uint(mi) >> 16);
+  dst[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
+}
+
 template <int MODE, class F, class FS>
-__global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs_cost) {
-  constexpr int NP = MODE == 0 ? 1 : 3, TL = MODE == 0 ? 2 : 4;
+__global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
+  constexpr int TL = MODE == 0 ? 2 : 4;
   extern __shared__ uint4 xlds[];
   __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert, then the shared expert's rows
   __shared__ uint16_t s_e[MR_ITEMS], s_off[MR_ITEMS], s_num[MR_ITEMS];  // items: expert, first place in s_list, rows
@@ -408,29 +480,27 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
     }
   if (a.shared && tid < a.rows) s_list[pairs + tid] = pairs + tid;
   lds_barrier();
-  // items of the routed experts, of all; cost of the items before d: 1 a tile, fs_cost a tile of the shared expert
-  const int D0 = __builtin_amdgcn_readfirstlane(s_d0), D = D0 + (a.shared ? (a.rows + P - 1) / P : 0);
-  auto cost_before = [&](int d) { return d <= D0 ? d * tiles : D0 * tiles + (d - D0) * tiles * fs_cost; };
-  const long long all = cost_before(D);
-  const int lo = (int)(all * blockIdx.x / gridDim.x), hi = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  // the shared expert's blocks, in the measure of its cost, and this block's items: from dbase, to dtop
+  const int D0 = __builtin_amdgcn_readfirstlane(s_d0), DS = a.shared ? (a.rows + P - 1) / P : 0;
+  const int grid = gridDim.x, cost = 2 * DS, nS = DS == 0 ? 0 : max(1, min(grid - 1, (2 * grid * cost + D0 + cost) / (2 * (D0 + cost))));
+  const bool sh = (int)blockIdx.x < nS;
+  const int b = sh ? blockIdx.x : blockIdx.x - nS, nb = sh ? nS : grid - nS, all = (sh ? DS : D0) * tiles, dbase = sh ? D0 : 0;
+  const int lo = (int)((long long)all * b / nb), hi = (int)((long long)all * (b + 1) / nb);
   if (lo >= hi) return;
-  auto item_at = [&](int c) { return c < D0 * tiles ? c / tiles : D0 + (c - D0 * tiles) / (tiles * fs_cost); };
-  const int dfirst = item_at(lo), dend = item_at(hi - 1) + 1;  // this block's items
+  const int dfirst = dbase + lo / tiles, dend = dbase + (hi - 1) / tiles + 1;
   const size_t plane = (size_t)(pairs + a.rows) * a.i;
   char* xb = reinterpret_cast<char*>(xlds);
   float* sums = reinterpret_cast<float*>(xb + (size_t)L.R * L.RB);
   // the block's tiles [t0, t1) of item d
   auto range = [&](int d, int& t0, int& t1) __attribute__((always_inline)) {
-    const int cum = cost_before(d), tc = d < D0 ? 1 : fs_cost;
-    t0 = lo > cum ? (lo - cum + tc - 1) / tc : 0;
-    t1 = (hi - cum + tc - 1) / tc;
-    t0 = t0 < tiles ? t0 : tiles, t1 = t1 < tiles ? t1 : tiles;
+    const int cum = (d - dbase) * tiles;
+    t0 = lo > cum ? lo - cum : 0, t1 = hi - cum < tiles ? hi - cum : tiles;
   };
-  // items dA .. dB - 1, of one weight format, their rows in the slots from 0
+  // items dA .. dB - 1, their rows in the slots from 0
   auto run = [&](auto fmt, const int dA, const int dB, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
     using Fm = decltype(fmt);
-    constexpr int DEPTH = Fm::perm ? 8 / TL : MODE == 0 ? 3 : 2;
-    const int pos = s_off[dA], nrows = s_off[dB - 1] + s_num[dB - 1] - pos, k8 = L.Kp / 8;
+    constexpr int DEPTH = Fm::sums ? 8 / TL : MODE == 0 ? 3 : 2;
+    const int pos = s_off[dA], nrows = s_off[dB - 1] + s_num[dB - 1] - pos;
     // the position to load next: chunk lc of tile lt of item ld, whose tiles here are the counter's lbase .. lbase + ln - 1
     int ld = dA, lbase = 0, lt = 0, lt0, lt1, lc = nch;
     bool over = false;
@@ -470,26 +540,10 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
     };
     static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { advance(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
     // the rows, requested behind the first weights: the two waits are one
-    for (int q = tid; q < nrows * k8; q += MR_NT) {
-      const int slot = q / k8, k = (q - slot * k8) * 8, pr = s_list[pos + slot];
-      float sum = 0.f;
-#pragma unroll
-      for (int p = NP - 1; p >= 0; --p) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (k < K) v = ld16(MODE == 0 ? a.x + (size_t)(sh ? pr - pairs : pr / a.topk) * K + k : a.act + p * plane + (size_t)pr * K + k);
-        if constexpr (Fm::perm) {
-          sum += ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) + ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
-          v = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                         __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
-        }
-        *reinterpret_cast<uint4*>(xb + slot * L.RB + (p * L.Kp + k) * 2) = v;
-      }
-      if constexpr (Fm::perm) {
-        // the 8 pieces of a group are 8 consecutive threads (k8 is a multiple of 8), all in or all past the rows
-        sum = xsum_step<4>(xsum_step<2>(xsum_step<1>(sum)));
-        if ((q & 7) == 0) sums[slot * L.GS + k / 64] = sum;
-      }
-    }
+    stage_rows<MODE, Fm::perm, Fm::sums>(a, L, K, nrows, xb, sums, plane, [&](int slot) {
+      const int pr = s_list[pos + slot];
+      return MODE == 0 ? (sh ? pr - pairs : pr / a.topk) : pr;
+    });
     lds_barrier();
     f32x4 o[TL];
     const char* xr = xb;
@@ -502,26 +556,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
 #pragma unroll
         for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      const bool half = c * 256 + 128 >= K;
-      Fm f[TL];
-      const float xs = Fm::perm ? sr[4 * c] : 0.f;
-#pragma unroll
-      for (int i = 0; i < TL; ++i) f[i].prep(raw[i], half), f[i].rest(xs, o[i]);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        f32x4 acc[TL];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint4 x[NP][2];
-#pragma unroll
-          for (int q = 0; q < NP; ++q) {
-            const uint4* src = reinterpret_cast<const uint4*>(xr + q * L.Kp * 2 + (c * 256 + 128 * p + 64 * h) * 2);
-            x[q][0] = src[0], x[q][1] = src[1];
-          }
-#pragma unroll
-          for (int i = 0; i < TL; ++i) f[i].template group<NP>(p, h, x, acc[i], o[i]);
-        }
-      }
+      chunk_mac<MODE, Fm, TL>(raw, xr, sr, L.Kp, c, c * 256 + 128 >= K, o);
       if (c == nch - 1 && d >= 0) {
         // register r of lane l: row 4 (l / 16) + r of x, column l % 16
         const int off = s_off[d], cnt = s_num[d];
@@ -532,13 +567,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
           if (row >= cnt) continue;
           const int pr = s_list[off + row];
           if constexpr (MODE == 0) {
-            const float act = o[0][r] / (1.f + expf(-o[0][r])) * o[1][r];
-            uint16_t* dst = a.act + (size_t)pr * a.i + 16 * t + c16;
-            const float hi8 = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi8;
-            const float mi8 = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi8;
-            dst[0] = (uint16_t)(__float_as_uint(hi8) >> 16);
-            dst[plane] = (uint16_t)(__float_as_uint(mi8) >> 16);
-            dst[2 * plane] = (uint16_t)(__float_as_uint(r2) >> 16);
+            store_act(a, plane, pr, 16 * t + c16, o[0][r], o[1][r]);
           } else {
 #pragma unroll
             for (int i = 0; i < TL; ++i) a.yp[(size_t)pr * a.h + 64 * t + 16 * i + c16] = o[i][r];
@@ -556,11 +585,180 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a, int fs
   };
   for (int d = dfirst; d < dend;) {
     int e = d + 1;
-    const bool sh = d >= D0;
-    while (e < dend && (e >= D0) == sh && s_off[e] + s_num[e] - s_off[d] <= L.R) ++e;
+    while (e < dend && s_off[e] + s_num[e] - s_off[d] <= L.R) ++e;
     if (sh) run(FS{}, d, e, true, reinterpret_cast<const uint8_t*>(MODE == 0 ? a.sgu_q : a.sd_q), MODE == 0 ? a.sgu_s : a.sd_s);
     else run(F{}, d, e, false, MODE == 0 ? a.gu_q : a.d_q, MODE == 0 ? a.gu_s : a.d_s);
     d = e;
+  }
+}
+
+// ---- experts of very few rows ----------------------------------------------------------------
+// One row or two: with so few tiles the kernels above wait for one wave's walk through all inputs of a tile, and their last
+// launch (the combine) costs little but its start.  gate_up: the eight waves of a block share the inputs of a tile (16 gate and 16 up
+// rows), their sums meet in LDS.  down: a block owns 16 outputs of all rows; its waves share out (expert, chunk), add
+// the weighted products into their own sums, and the block joins those with res: y is complete.  Each wave finds the experts'
+// rows itself, one pick a lane.  With 256 experts, h 2048, i 512, 8 picks and the shared expert, experts above / here in us:
+// 1 row 14.7 + 11.1 + 4.1 / 9.7 + 10.3, 2 rows 16.1 + 11.8 + 4.0 / 12.5 + 16.2, 4 rows 19.2 + 14.2 + 4.1 / 17.7 + 28.6.
+// Two chunks under way per wave in down; four or eight cost 13.8 and 22.8 us at 1 row (places without work are multiplied too).
+template <int MODE, class F, class FS>
+__global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_few(MoeRows a) {
+  constexpr int TL = MODE == 0 ? 2 : 1;
+  extern __shared__ uint4 xlds[];
+  __shared__ float red[MODE == 0 ? 2 * MR_NW * TL * 4 * 64 : MR_NW * 16 * 16];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
+  const int pairs = a.rows * a.topk;
+  const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 16, N = MODE == 0 ? 2 * a.i : a.h;
+  const int nch = (K + 255) / 256, S = a.shared ? 1 : 0;
+  const XLayout<MODE> L(K);
+  const int slots = MODE == 0 ? a.rows : pairs + S * a.rows;
+  const size_t plane = (size_t)(pairs + a.rows) * a.i;
+  char* xb = reinterpret_cast<char*>(xlds);
+  float* sums = reinterpret_cast<float*>(xb + (size_t)slots * L.RB);
+  // lane p < pairs: the expert of pick p, and whether no pick before it has that expert; items are experts in that order
+  const int mine = lane < pairs ? a.idx[lane] & 255 : -1;
+  bool first = lane < pairs;
+  for (int q = 0; q < pairs - 1; ++q) first = first && !(q < lane && __builtin_amdgcn_readlane(mine, q) == mine);
+  const uint64_t firsts = __ballot(first);
+  const int D0 = __builtin_popcountll(firsts);
+  auto expert_at = [&](int d) __attribute__((always_inline)) {
+    uint64_t m = firsts;
+    for (; d > 0; --d) m &= m - 1;
+    return __builtin_amdgcn_readlane(mine, __builtin_ctzll(m));
+  };
+  // picks of an expert as a mask; the c16-th of them (the last where there are fewer)
+  auto nth = [&](uint64_t m, int n) __attribute__((always_inline)) {
+    const int cnt = __builtin_popcountll(m);
+    for (int j = 0; j < cnt - 1; ++j) m = j < n ? m & (m - 1) : m;
+    return __builtin_ctzll(m);
+  };
+  bool staged = false;
+  auto stage = [&]() __attribute__((always_inline)) {
+    if (staged) return;
+    stage_rows<MODE, F::perm, F::sums>(a, L, K, slots, xb, sums, plane, [](int slot) { return slot; });
+    lds_barrier();
+    staged = true;
+  };
+  const int grid = gridDim.x, blk = blockIdx.x;
+  if constexpr (MODE == 0) {
+    int par = 0;
+    // tiles u0, u0 + grid, .. of the items of one format (sh: the shared expert's, of all rows)
+    auto run = [&](auto fmt, int u0, int units, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
+      using Fm = decltype(fmt);
+      if (u0 >= units) return;
+      typename Fm::Raw raw[TL];
+      auto load = [&](int u, int c) __attribute__((always_inline)) {
+        const bool none = u >= units || c >= nch;
+        const int d = u / tiles, tile = u - d * tiles;
+        const size_t m = sh || none ? 0 : expert_at(d);
+        const Rsrc Q = rsrc(Wq + m * Fm::q_bytes(N, K), (uint32_t)Fm::q_bytes(N, K));
+        const Rsrc Z = rsrc(reinterpret_cast<const char*>(Ws) + m * Fm::s_bytes(N, K), (uint32_t)Fm::s_bytes(N, K));
+#pragma unroll
+        for (int i = 0; i < TL; ++i) Fm::load(raw[i], Q, Z, 16 * tile + i * a.i, K, c, none || c * 256 + 128 >= K, none);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      load(u0, wave);
+      stage();
+      for (int u = u0; u < units; u += grid) {
+        const int d = u / tiles, tile = u - d * tiles;
+        // the item's picks (for the shared expert: one bit a row)
+        uint64_t m = (1ull << a.rows) - 1;
+        if (!sh) {
+          const int e = expert_at(d);
+          m = __ballot(mine == e);
+        }
+        const int cnt = __builtin_popcountll(m), pick_ = nth(m, c16), slot = sh ? pick_ : pick_ / a.topk;
+        const char* xr = xb + slot * L.RB + 2 * Fm::xoff(g);
+        const float* sr = sums + slot * L.GS + g;
+        f32x4 o[TL];
+#pragma unroll
+        for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = wave; c < nch; c += MR_NW) {
+          if (c != wave) load(u, c);
+          chunk_mac<MODE, Fm, TL>(raw, xr, sr, L.Kp, c, c * 256 + 128 >= K, o);
+        }
+        load(u + grid, wave);
+        float* rd = red + par * (MR_NW * TL * 4 * 64);
+#pragma unroll
+        for (int i = 0; i < TL; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) rd[((wave * TL + i) * 4 + r) * 64 + lane] = o[i][r];
+        lds_barrier();
+        // register r of lane l: row 4 (l / 16) + r, column l % 16; four of the eight waves by turns
+        const int r = wave ^ (4 * par);
+        if (r < 4 && r < cnt) {
+          float v[2] = {0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < MR_NW; ++k)
+#pragma unroll
+            for (int i = 0; i < TL; ++i) v[i] += rd[((k * TL + i) * 4 + r) * 64 + lane];
+          const int row = 4 * g + r, pr = nth(m, row) + (sh ? pairs : 0);
+          if (row < cnt) store_act(a, plane, pr, 16 * tile + c16, v[0], v[1]);
+        }
+        par ^= 1;
+      }
+    };
+    const int us = S * tiles, ur = D0 * tiles;
+    if (S) run(FS{}, blk, us, true, reinterpret_cast<const uint8_t*>(a.sgu_q), a.sgu_s);
+    run(F{}, (blk + grid - us % grid) % grid, ur, false, a.gu_q, a.gu_s);
+  } else {
+    float* mysum = red + wave * 256;
+    for (int tile = blk; tile < tiles; tile += grid) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) mysum[64 * q + lane] = 0.f;
+      // (item, chunk) q0, q0 + 8, .. of one format
+      auto run = [&](auto fmt, int q0, int units, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
+        using Fm = decltype(fmt);
+        typename Fm::Raw raw[FEW_RING][TL];
+        auto load = [&](typename Fm::Raw (&f)[TL], int q) __attribute__((always_inline)) {
+          const bool none = q >= units;
+          const int d = q / nch, c = q - d * nch;
+          const size_t m = sh || none ? 0 : expert_at(d);
+          const Rsrc Q = rsrc(Wq + m * Fm::q_bytes(N, K), (uint32_t)Fm::q_bytes(N, K));
+          const Rsrc Z = rsrc(reinterpret_cast<const char*>(Ws) + m * Fm::s_bytes(N, K), (uint32_t)Fm::s_bytes(N, K));
+          Fm::load(f[0], Q, Z, 16 * tile, K, c, none || c * 256 + 128 >= K, none);
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        auto body = [&](typename Fm::Raw (&f)[TL], int q) __attribute__((always_inline)) {
+          const int d = q / nch, c = q - d * nch;
+          uint64_t m = (1ull << a.rows) - 1;
+          if (!sh) {
+            const int e = expert_at(q < units ? d : 0);
+            m = __ballot(mine == e);
+          }
+          const int cnt = __builtin_popcountll(m), slot = nth(m, c16) + (sh ? pairs : 0);
+          f32x4 o[TL] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+          chunk_mac<MODE, Fm, TL>(f, xb + slot * L.RB + 2 * Fm::xoff(g), sums + slot * L.GS + g, L.Kp, c, c * 256 + 128 >= K, o);
+          load(f, q + FEW_RING * MR_NW);
+          if (q < units)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = 4 * g + r;
+              if (r >= cnt) break;
+              if (row >= cnt) continue;
+              const int p = nth(m, row), t = sh ? p : p / a.topk;
+              const float w = sh ? 1.f / (1.f + expf(-a.sgate[t])) : a.wts[p];
+              mysum[16 * t + c16] += w * o[0][r];
+            }
+        };
+        static_for<FEW_RING>([&](auto j) __attribute__((always_inline)) { load(raw[j], q0 + j * MR_NW); });
+        stage();
+        for (int q = q0; q < units; q += FEW_RING * MR_NW)
+          static_for<FEW_RING>([&](auto j) __attribute__((always_inline)) { body(raw[j], q + j * MR_NW); });
+      };
+      const int ur = D0 * nch;
+      run(F{}, wave, ur, false, a.d_q, a.d_s);
+      if (S) run(FS{}, (wave + MR_NW - ur % MR_NW) % MR_NW, nch, true, reinterpret_cast<const uint8_t*>(a.sd_q), a.sd_s);
+      lds_barrier();
+      const int t = threadIdx.x >> 4;
+      if (t < a.rows) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < MR_NW; ++k) v += red[256 * k + 16 * t + (threadIdx.x & 15)];
+        const size_t o = (size_t)t * a.h + 16 * tile + (threadIdx.x & 15);
+        a.y[o] = a.res ? a.res[o] + v : v;
+      }
+      lds_barrier();
+    }
   }
 }
 
@@ -604,7 +802,7 @@ struct WsLayout {
   }
 };
 
-template <class F, class SH, bool BYTES>
+template <class F, class SH>
 int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   if (!rows_shape_ok(a.rows, a.e, a.h, a.i, a.topk)) return -1;
   const int given = (a.sgu_q != nullptr) + (a.sgu_s != nullptr) + (a.sd_q != nullptr) + (a.sd_s != nullptr);
@@ -625,8 +823,17 @@ int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   else if (a.rows <= 8) hipLaunchKernelGGL(k_moe_rows_router<2>, dim3(nb, (a.rows + 1) / 2), dim3(MR_NT), 0, st, a);
   else if (a.rows <= 32) hipLaunchKernelGGL(k_moe_rows_router<4>, dim3(nb, (a.rows + 3) / 4), dim3(MR_NT), 0, st, a);
   else hipLaunchKernelGGL(k_moe_rows_router<8>, dim3(nb, (a.rows + 7) / 8), dim3(MR_NT), 0, st, a);
-  hipLaunchKernelGGL((k_moe_rows_experts<0, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), MR_X, st, a, BYTES ? 1 : 2);
-  hipLaunchKernelGGL((k_moe_rows_experts<1, F, RowsQ8<SH>>), dim3(MR_GRID), dim3(MR_NT), MR_X, st, a, BYTES ? 1 : 2);
+  const XLayout<0> gl(a.h);
+  const XLayout<1> dl(a.i);
+  const int slots = a.rows * (a.topk + a.shared);
+  if (a.rows <= 2 && slots <= 64 && a.rows <= gl.R && slots <= dl.R) {
+    const int ug = a.i / 16 * slots, ud = a.h / 16;
+    hipLaunchKernelGGL((k_moe_rows_few<0, F, RowsQ8<SH, F::perm>>), dim3(ug < 512 ? ug : 512), dim3(MR_NT), a.rows * (gl.RB + 4 * gl.GS), st, a);
+    hipLaunchKernelGGL((k_moe_rows_few<1, F, RowsQ8<SH, F::perm>>), dim3(ud < 256 ? ud : 256), dim3(MR_NT), slots * (dl.RB + 4 * dl.GS), st, a);
+    return 0;
+  }
+  hipLaunchKernelGGL((k_moe_rows_experts<0, F, RowsQ8<SH, F::perm>>), dim3(MR_GRID), dim3(MR_NT), MR_X, st, a);
+  hipLaunchKernelGGL((k_moe_rows_experts<1, F, RowsQ8<SH, F::perm>>), dim3(MR_GRID), dim3(MR_NT), MR_X, st, a);
   hipLaunchKernelGGL(k_moe_rows_combine, dim3(a.rows, (a.h + 1023) / 1024), dim3(256), 0, st, a);
   return 0;
 }
@@ -637,16 +844,16 @@ API size_t dr_moe_layer_rows_ws(int rows, int e, int h, int i, int topk) {
   return rows_shape_ok(rows, e, h, i, topk) ? WsLayout(rows, e, h, i, topk).bytes : 0;
 }
 
-#define MOE_ROWS_ENTRY(NAME, S, F, SH, BYTES)                                                                             \
+#define MOE_ROWS_ENTRY(NAME, S, F, SH)                                                                             \
   API int NAME(const uint16_t* router, const uint8_t* gu_q, const S* gu_s, const uint8_t* d_q, const S* d_s,              \
                const int8_t* sgu_q, const uint16_t* sgu_s, const int8_t* sd_q, const uint16_t* sd_s, const uint16_t* x,   \
                const float* res, int* idx, float* wts, float* sgate, void* ws, float* y, int rows, int e, int h, int i,   \
                int topk, hipStream_t st) {                                                                                \
     const MoeRows a{router, gu_q, d_q, gu_s, d_s, sgu_q, sd_q, sgu_s, sd_s, x, res, idx, wts, sgate, y, nullptr, nullptr, \
                     nullptr, nullptr, rows, e, h, i, topk, 0};                                                            \
-    return moe_rows<F, SH, BYTES>(a, ws, st);                                                                             \
+    return moe_rows<F, SH>(a, ws, st);                                                                             \
   }
-MOE_ROWS_ENTRY(dr_moe_layer_rows, uint16_t, RowsQ4<ScaleF16>, Q8G128F16, false)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_bf16s, uint16_t, RowsQ4<ScaleBF16>, Q8RowBF16, false)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8, float, RowsFP8<0>, Q8G128F16, true)
-MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8_bf16s, uint16_t, RowsFP8<1>, Q8RowBF16, true)
+MOE_ROWS_ENTRY(dr_moe_layer_rows, uint16_t, RowsQ4<ScaleF16>, Q8G128F16)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_bf16s, uint16_t, RowsQ4<ScaleBF16>, Q8RowBF16)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8, float, RowsFP8<0>, Q8G128F16)
+MOE_ROWS_ENTRY(dr_moe_layer_rows_fp8_bf16s, uint16_t, RowsFP8<1>, Q8RowBF16)

@@ -158,7 +158,8 @@ CASES = [
     ("fp8", "ref", 33, 24, 1024, 256, 6, False), ("q4", "ref", 64, 64, 512, 256, 8, True), ("q4", "cfg", 64, 3, 256, 384, 1, True),
     ("fp8", "cfg", 61, 4, 256, 128, 4, True), ("q4", "ref", 5, 64, 128, 128, 32, True), ("q4", "cfg", 2, 4, 8192, 128, 2, True),
     ("fp8", "ref", 3, 4, 4224, 128, 2, True), ("q4", "ref", 4, 4, 256, 2688, 2, True), ("fp8", "cfg", 64, 256, 256, 128, 8, True),
-    ("q4", "cfg", 31, 256, 256, 128, 3, False),
+    ("q4", "cfg", 31, 256, 256, 128, 3, False), ("q4", "ref", 1, 64, 256, 128, 32, True), ("fp8", "cfg", 2, 64, 256, 128, 32, True),
+    ("q4", "cfg", 1, 4, 128, 8192, 3, False), ("fp8", "ref", 2, 32, 2176, 640, 6, False), ("q4", "ref", 2, 3, 1152, 1024, 3, True),
 ]
 
 
