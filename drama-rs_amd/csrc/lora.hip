@@ -34,6 +34,8 @@ struct Lora {
   int rp;            // rmax rounded up to the 32 of an MFMA
 };
 
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+
 constexpr int LR_NW = 8, LR_NT = LR_NW * 64;
 
 // adapter of row r, -1 for none (an id outside 0 .. adapters - 1, an adapter without rank)
@@ -54,6 +56,11 @@ __global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
   const int r0 = blockIdx.x * 16, j0 = blockIdx.z * 16 * RT;
   const uint16_t* xr = a.x + (size_t)(r0 + c16 < a.rows ? r0 + c16 : a.rows - 1) * a.ldx + 8 * g;
+  // the first turn's x is requested ahead of the ids (12 adapters in any order over 4096 rows: 104 -> 89 us)
+  uint4 x0[4];
+#pragma unroll
+  for (int f = 0; f < 4; ++f) x0[f] = ld16(xr + (wave * 128 < a.k ? wave * 128 : 0) + 32 * f);
+  __builtin_amdgcn_sched_barrier(0);
   const int mine = adapter_of(a, r0 + c16);
   // row c16 is the first of its adapter: no earlier row of the 16 has it
   bool first = mine >= 0;
@@ -80,7 +87,7 @@ __global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
       for (int c = wave * 128; c < a.k; c += LR_NW * 128) {
         uint4 xv[4], av[RT][4];
 #pragma unroll
-        for (int f = 0; f < 4; ++f) xv[f] = ld16(xr + c + 32 * f);
+        for (int f = 0; f < 4; ++f) xv[f] = c == wave * 128 ? x0[f] : ld16(xr + c + 32 * f);
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -128,7 +135,8 @@ DEV uint32_t pk8(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
 DEV uint4 frag8(uint32_t a, uint32_t b) { return make_uint4(pk8(a, 0), pk8(a, 2), pk8(b, 0), pk8(b, 2)); }
 
 // Few rows: a block owns 16 columns and MT 16-row tiles; its eight waves take 128 inputs each in turn and
-// add their sums through LDS.  Column l % 16 of the weights in lane l, 16 inputs (16 (l / 16)) of each 64.
+// add their sums through LDS.  48 rows, n 4096, k 2048, 40 adapters of 32 ranks: 12.5 us behind 7.6 of k_lora_down, 18 MB
+// in all (3.8 at the copy rate); an empty launch takes 4 of each, the rest are the chains of dependent loads.  Column l % 16 of the weights in lane l, 16 inputs (16 (l / 16)) of each 64.
 template <class SH, int MT>
 __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
   __shared__ float red[LR_NW][MT][4][64];
@@ -212,6 +220,62 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
   }
 }
 
+// One row whose adapters have at most 16 ranks: every block computes t itself, beside its columns and from the same x, so no
+// launch goes before it (n = k = 2048: 6.4 us; A x and the product apart 5.0 + 3.8 and the second launch.  Each further 16
+// ranks or row cost 3 to 4 us here, as all blocks ask for the same lines: 2 rows 9.3 against 5.2 + 3.9).
+template <class SH>
+__global__ void __launch_bounds__(LR_NT) k_lora_gemm_one(Lora a) {
+  __shared__ float red[LR_NW][2][16];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
+  const int col = blockIdx.x * 16 + c16;
+  const size_t n = col < a.n ? col : a.n - 1;
+  const uint16_t* xr = a.x + 16 * g;
+  const uint8_t* wr = reinterpret_cast<const uint8_t*>(a.w) + n * a.k + 16 * g;
+  const bool mine = threadIdx.x < 16 && col < a.n;
+  const float base = mine && a.res ? a.res[col] : 0.f;
+  const int ad = __builtin_amdgcn_readfirstlane(adapter_of(a, 0)), rk = ad < 0 ? 0 : __builtin_amdgcn_readfirstlane(rank_of(a, ad));
+  const uint16_t* ar = a.la + ((size_t)(ad < 0 ? 0 : ad) * a.rmax + (c16 < rk ? c16 : rk > 0 ? rk - 1 : 0)) * a.k + 16 * g;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f}, at = acc;
+  for (int c = wave * 128; c < a.k; c += LR_NW * 128) {
+    const uint4 w0 = ld16(wr + c), w1 = ld16(wr + c + 64);
+    const float sc = SH::scale(a.s, n, c, a.k);
+    uint4 x[4], av[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) x[f] = ld16(xr + c + 64 * (f >> 1) + 8 * (f & 1));
+#pragma unroll
+    for (int f = 0; f < 4; ++f) av[f] = ld16(ar + c + 64 * (f >> 1) + 8 * (f & 1));
+    f32x4 p = {0.f, 0.f, 0.f, 0.f};
+    p = mfma(x[0], frag8(w0.x, w0.y), p), p = mfma(x[1], frag8(w0.z, w0.w), p), p = mfma(x[2], frag8(w1.x, w1.y), p), p = mfma(x[3], frag8(w1.z, w1.w), p);
+    acc[0] = __builtin_fmaf(sc, p[0], acc[0]);
+#pragma unroll
+    for (int f = 0; f < 4; ++f) at = mfma(x[f], av[f], at);
+  }
+  // all 16 rows of the products are the one row
+  if (g == 0) red[wave][0][c16] = acc[0], red[wave][1][c16] = at[0];
+  uint4 b[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (mine)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (8 * i < rk) b[i] = ld16(a.lb + ((size_t)ad * a.n + col) * a.rmax + 8 * i);
+  __syncthreads();
+  if (wave != 0) return;
+  float v = 0.f, t = 0.f, d = 0.f;
+#pragma unroll
+  for (int w = 0; w < LR_NW; ++w) v += red[w][0][c16], t += red[w][1][c16];
+  t *= ad < 0 ? 0.f : a.lscale[ad];
+  // ranks in order; those past the rank, where A's and B's padding must not count, are left out
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t q[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float tj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(t), 8 * i + j));
+      if (8 * i + j < rk) d = __builtin_fmaf(j & 1 ? bf16_hi(q[j >> 1]) : bf16_lo(q[j >> 1]), tj, d);
+    }
+  }
+  if (mine) a.y[col] = base + (v + d);
+}
+
 // Many rows: a block of 2 x 2 waves owns 32 MT rows x 32 NT columns, a wave 16 MT x 16 NT of them.  Slices of 64 inputs
 // go through two LDS buffers, a slice's global loads in flight for the whole of the slice before; the barrier between slices
 // leaves them in flight.  The LDS reads set the pace (a wave tile of 64 x 64 in bf16 asks for 64 KB a slice, at ~64 bytes a
@@ -220,7 +284,14 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
 // x: row r's 16-byte piece j lies at j ^ (r % 8), so the fragment reads meet no bank twice; W: four pieces a row in order, a
 // fragment pair being 1 KB in a row.  Lane (l % 16, g = l / 16) has the inputs 16 g .. 16 g + 15 of a slice, 8 a product.
 // 8 XCDs take the tiles in 8 contiguous runs, down columns of 8 row tiles, so that an XCD's blocks share x and W in its L2.
+// 4096 rows, n 4096, k 2048, runs of 12 adapters of up to 64 ranks, one scale a row: 114 us, of which the product 79 (870
+// TFLOP/s; LDS reads), the residual and the store 24 (128 MB, the card's copy rate; nothing is left to overlap them with when
+// every CU has its two tiles at once) and the adapters the rest.
 constexpr int LG_K = 64;
+// 16 bytes of each lane to dst + 16 lane
+DEV void to_lds(const void* src, uint4* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
 template <class SH, int MT, int NT>
 __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int tn) {
   constexpr int BM = 32 * MT, BN = 32 * NT, PX = BM * 8 / 256, PW = BN * 4 / 256;
@@ -339,50 +410,81 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
       }
     }
   }
-  // B t: the distinct adapters of the wave's rows, the t of other rows zero; B's fragments serve all row tiles
+  // B t, 64 ranks at a time: t of the block's rows goes to LDS (plane p in place of the x and W slices, laid out as a slice of x), then each wave
+  // multiplies the distinct adapters of its rows, the t of other rows zero; B's fragments serve all row tiles.
   if (a.adapter) {
+    static_assert(sizeof(lw) >= sizeof(lx[0]), "plane 2 of t");
     const size_t plane = (size_t)a.rows * a.rp;
-    uint32_t left[MT];
+    uint32_t rows_of[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) left[m] = (uint32_t)__ballot(mine[m] >= 0) & 0xffffu;
+    for (int m = 0; m < MT; ++m) rows_of[m] = (uint32_t)__ballot(mine[m] >= 0) & 0xffffu;
+    uint4 b[2][NT];
+    auto load_b = [&](int h, int ad, int rk, int j0) __attribute__((always_inline)) {  // ranks j0 + 32 h ..
+      const int last = n0 + BN < a.n ? BN : a.n - n0, j = j0 + 32 * h + 8 * g;
+      const Rsrc B = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.lb + ((size_t)ad * a.n + n0) * a.rmax), 0, (uint32_t)(last * a.rmax * 2), 0x00020000);
 #pragma unroll
-    for (int f = 0; f < MT; ++f)
-      while (left[f]) {
-        const int ad = __builtin_amdgcn_readlane(mine[f], __builtin_ctz(left[f]));
-        bool has[MT];
+      for (int n = 0; n < NT; ++n) {
+        const uint32_t off = ((wn + 16 * n + c16) * a.rmax + j) * 2;
+        b[h][n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(B, j < rk ? off : 0x80000000u, 0, 0));
+      }
+    };
+    for (int j0 = 0; j0 < a.rp; j0 += 64) {
+      uint32_t left[MT];
 #pragma unroll
-        for (int m = f; m < MT; ++m) {
-          const uint32_t b = (uint32_t)__ballot(mine[m] == ad) & 0xffffu;
-          has[m] = b != 0, left[m] &= ~b;
+      for (int m = 0; m < MT; ++m) left[m] = rows_of[m];
+      // the next adapter, -1 for none: its rows leave `left` and are those of `has`
+      uint32_t has[MT];
+      auto next = [&]() __attribute__((always_inline)) {
+        int ad = -1;
+#pragma unroll
+        for (int m = MT - 1; m >= 0; --m)
+          if (left[m]) ad = __builtin_amdgcn_readlane(mine[m], __builtin_ctz(left[m]));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          has[m] = ad < 0 ? 0u : (uint32_t)__ballot(mine[m] == ad) & 0xffffu;
+          left[m] &= ~has[m];
         }
-        const int rk = rank_of(a, ad);
-        for (int j = 0; j < rk; j += 32) {
-          uint4 tf[MT][3], b[NT];
-          const int on = rk - j - 8 * g;  // of this lane's 8 ranks, those below rk
+        return ad;
+      };
+      int ad = next(), rk = ad < 0 ? 0 : rank_of(a, ad);
+      if (ad >= 0) load_b(0, ad, rk, j0), load_b(1, ad, rk, j0);
+      if (j0) lds_barrier();
+      // straight to LDS, 64 pieces a wave in order: no registers beside the sums and B's fragments
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            b[n] = make_uint4(0, 0, 0, 0);
-            if (on > 0) b[n] = ld16(a.lb + ((size_t)ad * a.n + col[n]) * a.rmax + j + 8 * g);
-          }
+      for (int i = 0; i < PX; ++i) {
+        const int at = 256 * i + 64 * wave, rl = (at + lane) >> 3, r = m0 + rl, j = j0 + 8 * ((lane & 7) ^ (rl & 7));
+        const uint16_t* src = a.planes + (size_t)(r < a.rows ? r : a.rows - 1) * a.rp + (j < a.rp ? j : 0);
+        to_lds(src, &lx[0][at]), to_lds(src + plane, &lx[1][at]), to_lds(src + 2 * plane, &lw[0][0] + at);
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      lds_barrier();
+      while (ad >= 0) {
 #pragma unroll
-          for (int m = f; m < MT; ++m) {
-            const uint16_t* tp = a.planes + (size_t)(mine[m] == ad ? m0 + wm + 16 * m + c16 : 0) * a.rp + 8 * g + j;
-#pragma unroll
-            for (int p = 0; p < 3; ++p) tf[m][p] = has[m] && mine[m] == ad ? ld16(tp + p * plane) : make_uint4(0, 0, 0, 0);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int on = rk - j0 - 32 * h - 8 * g;  // of this lane's 8 ranks, those below rk
+          if (rk <= j0 + 32 * h) continue;
           const uint32_t k0 = on >= 2 ? 0xffffffffu : on == 1 ? 0xffffu : 0u, k1 = on >= 4 ? 0xffffffffu : on == 3 ? 0xffffu : 0u;
           const uint32_t k2 = on >= 6 ? 0xffffffffu : on == 5 ? 0xffffu : 0u, k3 = on >= 8 ? 0xffffffffu : on == 7 ? 0xffffu : 0u;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) b[n] = make_uint4(b[n].x & k0, b[n].y & k1, b[n].z & k2, b[n].w & k3);
+          for (int n = 0; n < NT; ++n) b[h][n] = make_uint4(b[h][n].x & k0, b[h][n].y & k1, b[h][n].z & k2, b[h][n].w & k3);
 #pragma unroll
-          for (int m = f; m < MT; ++m)
-            if (has[m])
+          for (int m = 0; m < MT; ++m) {
+            if (!has[m]) continue;
+            const int r = wm + 16 * m + c16, at = r * 8 + ((4 * h + g) ^ (r & 7));
+            const bool on_row = has[m] >> c16 & 1;
+            uint4 tf[3] = {lx[0][at], lx[1][at], (&lw[0][0])[at]};
 #pragma unroll
-              for (int p = 0; p < 3; ++p)
+            for (int q3 = 0; q3 < 3; ++q3) {
+              const uint4 v = on_row ? tf[q3] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) acc[m][n] = mfma(tf[m][p], b[n], acc[m][n]);
+              for (int n = 0; n < NT; ++n) acc[m][n] = mfma(v, b[h][n], acc[m][n]);
+            }
+          }
         }
+        ad = next();
+        if (ad >= 0) rk = rank_of(a, ad), load_b(0, ad, rk, j0), load_b(1, ad, rk, j0);
       }
+    }
   }
   // the residual of 16 rows in flight at a time (y may be res: its loads could not pass the stores)
 #pragma unroll
@@ -422,6 +524,10 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
   const bool few = a.rows <= 64;
   a.rp = (a.rmax + 31) & ~31;
   a.planes = few || !a.adapter ? nullptr : reinterpret_cast<uint16_t*>(a.t);
+  if (a.adapter && a.rows == 1 && a.rmax <= 16) {
+    hipLaunchKernelGGL((k_lora_gemm_one<SH>), dim3((a.n + 15) / 16), dim3(LR_NT), 0, st, a);
+    return 0;
+  }
   if (a.adapter && few) hipLaunchKernelGGL(k_lora_down<1>, dim3(tiles, 16, (a.rmax + 15) / 16), dim3(LR_NT), 0, st, a);
   else if (a.adapter) hipLaunchKernelGGL(k_lora_down<2>, dim3(tiles, 2, a.rp / 32), dim3(LR_NT), 0, st, a);
   if (few) {
@@ -440,8 +546,10 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
   constexpr std::integral_constant<int, 2> i2{};
   constexpr std::integral_constant<int, 4> i4{};
   constexpr std::integral_constant<int, SH::per_row ? 8 : 4> wide{};
+  // the wide tile once there are two for each CU, the middle one once there is one (4096 x 4096 x 2048, ranks to 64, W with one
+  // scale a row: wide 114 us, middle 128; 2048 rows: 74 and 67)
   const long long m128 = (a.rows + 127) / 128;
-  if (m128 * ((a.n + 32 * wide.value - 1) / (32 * wide.value)) >= 256) go(i4, wide);
+  if (m128 * ((a.n + 32 * wide.value - 1) / (32 * wide.value)) >= 512) go(i4, wide);
   else if (m128 * ((a.n + 127) / 128) >= 256) go(i4, i4);
   else go(i2, i2);
   return 0;

@@ -107,6 +107,8 @@ SIZES = [
     (64, 33, 1152, 64, 128, "each", 0, 0), (65, 130, 256, 5, 16, "each", 0, 2), (100, 1000, 512, 3, 16, "runs", 8, 0),
     (129, 257, 384, 12, 48, "each", 0, 7), (300, 2048, 512, 6, 16, "runs", 0, 0), (513, 96, 128, 30, 8, "each", 0, 0),
     (700, 1031, 1024, 5, 16, "runs", 0, 0), (3, 8, 16384, 2, 16, [0, 1, 1], 0, 0), (1025, 384, 256, 20, 112, "runs", 0, 0),
+    (4, 40, 384, 3, 16, [2, 2, -1, 0], 0, 0), (3, 300, 1152, 4, 16, [1, 0, 3], 8, 0), (2, 100, 512, 5, 32, [4, 1], 0, 1), (1, 333, 2048, 2, 64, [1], 0, 0),
+    (2, 64, 128, 3, 8, [0, 0], 0, 0), (2000, 8200, 128, 9, 24, "each", 0, 0), (1025, 4100, 256, 7, 72, "runs", 0, 3),
 ]
 
 
