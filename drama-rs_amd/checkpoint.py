@@ -235,6 +235,7 @@ class MoeStack:
                 self.packed.append(pk)
             torch.cuda.synchronize()
         self._gemm = {}  # stream handle -> GEMM handle (one per stream for the stack's lifetime)
+        self._rows_ws = {}  # stream handle -> workspace of the layers for a few rows
 
     def _gemm_handle(self, st) -> int:
         import ctypes
@@ -269,7 +270,8 @@ class MoeStack:
         if int(self.sync[1].item()) != 0:
             raise dramamoe.DramaMoeError("dr_moe_decode_step timed out waiting for its workgroups")
 
-    def prefill(self, l: int, x, hn, chunk: int = 1024, stream=None, keep: dict | None = None) -> None:
+    def prefill(self, l: int, x, hn, chunk: int = 1024, stream=None, keep: dict | None = None, nw_next=None,
+                hn_next=None) -> None:
         """Prefill of loaded layer l for rows token rows (the engine's moe_prefill,
         src/engine.rs:544-604): x f32 [rows, H] residual stream updated in place, hn bf16
         [rows, H] its RMSNorm.  Rows go in chunks of at most `chunk` (grouping handles up to
@@ -277,7 +279,8 @@ class MoeStack:
         grouped expert GEMMs and the weighted combine, with the shared expert on a second stream
         beside them; no host round trip.  With ``keep`` (a dict), the last chunk's routing
         (idx, wts, sgate), grouping (slot_of) and bf16 activations (act in grouped-slot order,
-        sact per row) are left in it for inspection."""
+        sact per row) are left in it for inspection.  With ``nw_next`` (f32 [H]) the combine also
+        leaves the RMSNorm of the new x by that weight, bf16, in ``hn_next`` [rows, H], which may be hn."""
         import torch
 
         P = dramamoe.ptr
@@ -287,6 +290,8 @@ class MoeStack:
         H, E, I, k = self.H, self.E, self.I, self.topk
         if chunk * k > 8192:
             raise ValueError("chunk * topk must be <= 8192 (the pairs dr_moe_topk_group sorts in one call)")
+        if (nw_next is None) != (hn_next is None):
+            raise ValueError("nw_next and hn_next belong together")
         c = min(chunk, rows)
         dev = x.device
         # temporaries come from the caching allocator of the stream the kernels run on, so they
@@ -334,10 +339,60 @@ class MoeStack:
                P(act), P(yp), E, H, I, st)
             if overlap:
                 main.wait_event(join)
-            lib.dr_moe_combine(P(xr), P(yp), P(slot_of), P(wts), P(sg), P(sh), n, k, H, st)
+            if nw_next is None:
+                lib.dr_moe_combine(P(xr), P(yp), P(slot_of), P(wts), P(sg), P(sh), n, k, H, st)
+            else:
+                lib.dr_moe_combine_norm(P(yp), P(slot_of), P(wts), P(sg), P(sh), k, P(xr), H, None, None, 0, 0, None, 1.0,
+                                        1.0, P(nw_next), self.eps, P(xr), H, P(hn_next[r0:r0 + n]), H, n, H, st)
         if keep is not None:
             keep.update({"idx": idx[:n * k], "wts": wts[:n * k], "sgate": sg[:n], "slot_of": slot_of[:n * k],
                          "act": act[:n * k * I], "sact": sact[:n * I]})
+
+    def rows(self, l: int, x, hn, stream=None, keep: dict | None = None) -> None:
+        """Loaded layer l for 1 .. 64 token rows (one decode step of that many sequences): x f32 [rows, H] residual
+        stream updated in place, hn bf16 [rows, H] its RMSNorm.  Each expert is read once for all rows that
+        picked it.  With ``keep`` (a dict), the routing (idx, wts, sgate) is left in it."""
+        import torch
+
+        P, L, lib = dramamoe.ptr, self.layers[l], self.lib
+        st = stream if stream is not None else dramamoe.stream_ptr()
+        n = x.shape[0]
+        need = lib.dr_moe_layer_rows_ws(n, self.E, self.H, self.I, self.topk)
+        if need == 0:
+            raise ValueError(f"no layer kernel for {n} rows of this shape")
+        main = torch.cuda.ExternalStream(st) if int(st) != 0 else torch.cuda.current_stream(x.device)
+        with torch.cuda.stream(main):
+            ws = self._rows_ws.get(int(st or 0))
+            if ws is None or ws.numel() < need:
+                ws = self._rows_ws[int(st or 0)] = torch.zeros(need, dtype=torch.uint8, device=x.device)
+            idx = torch.empty(n * self.topk, dtype=torch.int32, device=x.device)
+            wts, sg = torch.empty(n * self.topk, device=x.device), torch.empty(n, device=x.device)
+        f = lib.dr_moe_layer_rows_fp8 if self.fp8 else lib.dr_moe_layer_rows
+        f(P(L["router"]), P(L["gu_q"]), P(L["gu_s"]), P(L["d_q"]), P(L["d_s"]), P(L["sgu_q"]), P(L["sgu_s"]), P(L["sd_q"]),
+          P(L["sd_s"]), P(hn), P(x), P(idx), P(wts), P(sg), P(ws), P(x), n, self.E, self.H, self.I, self.topk, st)
+        if keep is not None:
+            keep.update({"idx": idx, "wts": wts, "sgate": sg})
+
+    def forward(self, x, stream=None, chunk: int = 1024) -> None:
+        """x (f32 [rows, H], device) through every loaded layer in place, each behind its own RMSNorm: up to 64 rows
+        through ``rows``, more through ``prefill``, whose combine carries the next layer's norm."""
+        import torch
+
+        P = dramamoe.ptr
+        st = stream if stream is not None else dramamoe.stream_ptr()
+        n, few = x.shape[0], x.shape[0] <= 64
+        main = torch.cuda.ExternalStream(st) if int(st) != 0 else torch.cuda.current_stream(x.device)
+        with torch.cuda.stream(main):
+            hn = torch.empty((n, self.H), dtype=torch.bfloat16, device=x.device)
+        for l, L in enumerate(self.layers):
+            if few or l == 0:
+                self.lib.dr_block_norm(None, 0, P(x), self.H, None, None, 0, 0, None, 0.0, 1.0, P(L["nw"]), self.eps, None, 0,
+                                       P(hn), self.H, n, self.H, st)
+            if few:
+                self.rows(l, x, hn, stream=st)
+            else:
+                nw = self.layers[l + 1]["nw"] if l + 1 < len(self.layers) else None
+                self.prefill(l, x, hn, chunk=chunk, stream=st, nw_next=nw, hn_next=None if nw is None else hn)
 
     def chain(self, x, stream=None) -> None:
         """The same layers through the engine's per-layer launches (router, then decode)."""
