@@ -17,7 +17,6 @@ constexpr int MR_NW = 8, MR_NT = MR_NW * 64, MR_ROWS = 64, MR_TOPK = 32, MR_PAIR
 constexpr int MR_GRID = 256;             // a block per CU
 constexpr int MR_X = 120 * 1024;         // LDS bytes for rows of x
 constexpr int MR_ITEMS = MR_PAIRS + MR_ROWS;  // passes, the experts' and the shared expert's, of one row each at worst
-constexpr int FEW_RING = 2;              // chunks a wave of few rows has under way
 constexpr int MR_SETS = 8;               // row sets of the router
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -134,16 +133,17 @@ struct RowsQ4 {
     const float2 o = SC::pair(pick(g & 2, hi, lo));
     out = __builtin_amdgcn_mfma_f32_16x16x4f32(xsum, o.y - 16.f * o.x, out, 0, 0, 0);
   }
-  // group 2 p + h of the chunk
-  template <int NP>
-  DEV void group(int p, int h, const uint4 (&x)[NP][2], f32x4&, f32x4& out) const {
+  // group 2 p + h of the chunk, the x fragments x[q] into out[q][i]
+  template <int NQ, int MQ, int TL>
+  DEV void group(int p, int h, const uint4 (&x)[NQ][2], f32x4 (&)[NQ][TL], f32x4 (&out)[MQ][TL], int i) const {
     const uint4 b0 = frag(pick(h, w[p].z, w[p].x)), b1 = frag(pick(h, w[p].w, w[p].y));
-    f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int q = 0; q < NP; ++q) a = mfma(x[q][0], b0, a), a = mfma(x[q][1], b1, a);
     const float sc = SC::pair(p ? pick(h, s.w, s.z) : pick(h, s.y, s.x)).x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
+    for (int q = 0; q < NQ; ++q) {
+      const f32x4 a = mfma(x[q][1], b1, mfma(x[q][0], b0, f32x4{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) out[q][i][r] = __builtin_fmaf(sc, a[r], out[q][i][r]);
+    }
   }
 };
 
@@ -174,17 +174,20 @@ struct Rows8 {
     s[0] = f.s[0], s[1] = f.s[1];
   }
   DEV void rest(float, f32x4&) const {}
-  template <int NP>
-  DEV void group(int p, int h, const uint4 (&x)[NP][2], f32x4& a, f32x4& out) const {
+  template <int NQ, int MQ, int TL>
+  DEV void group(int p, int h, const uint4 (&x)[NQ][2], f32x4 (&acc)[NQ][TL], f32x4 (&out)[MQ][TL], int i) const {
     const uint4& v = w[2 * p + h];
     const uint4 b0 = D::frag(v.x, v.y), b1 = D::frag(v.z, v.w);
-    if (h == 0) a = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int q = 0; q < NP; ++q) a = mfma(x[q][0], b0, a), a = mfma(x[q][1], b1, a);
-    if (h == 0) return;
     const float sc = D::scale_cvt(s[p]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) out[r] = __builtin_fmaf(sc, a[r], out[r]);
+    for (int q = 0; q < NQ; ++q) {
+      f32x4& a = acc[q][i];
+      if (h == 0) a = f32x4{0.f, 0.f, 0.f, 0.f};
+      a = mfma(x[q][1], b1, mfma(x[q][0], b0, a));
+      if (h == 0) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) out[q][i][r] = __builtin_fmaf(sc, a[r], out[q][i][r]);
+    }
   }
 };
 DEV uint32_t buf_half(const Rsrc& S, uint32_t off) { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(S, off, 0, 0); }
@@ -326,16 +329,23 @@ DEV int wave_scan(int v) {
   return v;
 }
 
-// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 64 t, K = i).
+// MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 32 t, K = i).
 //
-// Items are passes of up to P rows of an expert, ascending, then of the shared expert (whose rows are all); their
+// Items are passes of up to P rows (16; down: 8, two fragments of four rows and their planes) of an expert, ascending, then of the
+// shared expert (whose rows are all); their
 // tiles are dealt to the blocks in contiguous runs of even length.  The shared expert has blocks of its own (a block with
 // tiles of both formats would stage and wait twice: gate_up of 4 rows, 256 experts, h 2048, i 512, 25 us instead of 19), twice as
 // many for its tiles as the others: its passes are the fullest and its format the widest (fp8 beside it, 8 rows: 32.0 us with
-// equal numbers, 28.6 with twice, 28.4 with three times as many).  A block stages the rows of its items in LDS (as many items at a time as R rows hold, most
-// often all), then each of its waves takes one tile after the other from a counter and multiplies all of its inputs, in chunks
-// of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights come in a ring of DEPTH chunks that
-// runs on across tiles and items.
+// equal numbers, 28.6 with twice, 28.4 with three times as many).  A block stages the rows of its items in LDS (as many
+// items at a time as R rows hold, most often all), then each of its waves takes one tile after the other from a counter and
+// multiplies all of its inputs, in chunks of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights
+// come in a ring of DEPTH chunks that runs on across tiles and items.
+//
+// 64 rows, 256 experts, h 2048, i 512, 8 picks and the shared expert: gate_up 68 us, down 39, for 266 and 133 MB, of which 62 and
+// 32 are left without the products and 6 pass before the first load (launch, plan).  The down planes as rows of one fragment:
+// 41 -> 38 us, 16 rows 25 -> 20.  Rings of 2 / 3 / 4 chunks: down 39.2 / 40.4 / 43.6, gate_up 69.0 / 70.8 / 69.8 (19 rows, h 1280, i
+// 896, 48 experts: 18.6 / 21.4 / 22.4).  16 waves a block: gate_up 67 and 20 us, level; two blocks a CU with half the rows each: 68
+// and 22.
 //
 // LDS: row slot s at s * RB, its planes Kp * 2 bytes apart (Kp: K rounded up to a chunk, zeros past K), pieces of 8 inputs
 // reordered for int4; RB is 16 bytes more than the planes, so that the 16 rows of a fragment meet different banks.
@@ -380,30 +390,44 @@ DEV void stage_rows(const MoeRows& a, const XLayout<MODE>& L, int K, int nrows, 
   }
 }
 
-// o += the products of chunk c of a lane's row of x (at xr, its sums at sr) with TL tiles of weights
-template <int MODE, class Fm, int TL>
-DEV void chunk_mac(const typename Fm::Raw (&raw)[TL], const char* xr, const float* sr, int Kp, int c, bool half, f32x4 (&o)[TL]) {
-  constexpr int NP = XLayout<MODE>::NP;
+// o[q] += the products of chunk c of x fragments 0 .. NQ - 1 (a lane's row of each at xr[q], its group sums at sr[q], counted if
+// lead) with TL tiles of weights, converted once for all of them
+template <int NQ, class Fm, int TL, int MQ>
+DEV void chunk_mac(const typename Fm::Raw (&raw)[TL], const char* const (&xr)[MQ], const float* const (&sr)[MQ], bool lead, int c, bool half,
+                   f32x4 (&o)[MQ][TL]) {
   Fm f[TL];
-  const float xs = Fm::sums ? sr[4 * c] : 0.f;
 #pragma unroll
-  for (int i = 0; i < TL; ++i) f[i].prep(raw[i], half), f[i].rest(xs, o[i]);
+  for (int i = 0; i < TL; ++i) f[i].prep(raw[i], half);
+  if constexpr (Fm::sums)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const float xs = lead ? sr[q][4 * c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < TL; ++i) f[i].rest(xs, o[q][i]);
+    }
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    f32x4 acc[TL];
+    f32x4 acc[NQ][TL];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint4 x[NP][2];
+      uint4 x[NQ][2];
 #pragma unroll
-      for (int q = 0; q < NP; ++q) {
-        const uint4* src = reinterpret_cast<const uint4*>(xr + q * Kp * 2 + (c * 256 + 128 * p + 64 * h) * 2);
+      for (int q = 0; q < NQ; ++q) {
+        const uint4* src = reinterpret_cast<const uint4*>(xr[q] + (c * 256 + 128 * p + 64 * h) * 2);
         x[q][0] = src[0], x[q][1] = src[1];
       }
 #pragma unroll
-      for (int i = 0; i < TL; ++i) f[i].template group<NP>(p, h, x, acc[i], o[i]);
+      for (int i = 0; i < TL; ++i) f[i].template group<NQ>(p, h, x, acc, o, i);
     }
   }
 }
+
+// down: the planes of four rows share a fragment, plane p of row s in its row 4 s + p (the last of each four unused): lane l has the
+// outputs of row l / 16, its planes' in registers 0 .. 2
+DEV int quad_row() { return (lane_id() & 15) >> 2; }
+DEV int quad_plane() { return min(lane_id() & 3, 2); }
+DEV bool quad_lead() { return (lane_id() & 3) == 0; }
+DEV float quad_sum(const f32x4& o) { return o[0] + o[1] + o[2]; }
 
 // silu(g) u as three bf16 planes: 8 mantissa bits each, the last exact
 DEV void store_act(const MoeRows& a, size_t plane, int pair, int col, float g, float u) {
@@ -418,7 +442,7 @@ DEV void store_act(const MoeRows& a, size_t plane, int pair, int col, float g, f
 
 template <int MODE, class F, class FS>
 __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
-  constexpr int TL = MODE == 0 ? 2 : 4;
+  constexpr int TL = 2, MQ = MODE == 0 ? 1 : 2;  // tiles of 16 weight rows, x fragments
   extern __shared__ uint4 xlds[];
   __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert, then the shared expert's rows
   __shared__ uint16_t s_e[MR_ITEMS], s_off[MR_ITEMS], s_num[MR_ITEMS];  // items: expert, first place in s_list, rows
@@ -426,10 +450,11 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
   __shared__ int s_start[256], s_d0, s_ticket;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x, c16 = lane & 15, g = lane >> 4;
   const int pairs = a.rows * a.topk;
-  const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 64, N = MODE == 0 ? 2 * a.i : a.h;
+  const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 32, N = MODE == 0 ? 2 * a.i : a.h;
   const int nch = (K + 255) / 256;
   const XLayout<MODE> L(K);
-  const int P = L.R < 16 ? L.R : 16;
+  constexpr int PM = MODE == 0 ? 16 : 4 * MQ;
+  const int P = L.R < PM ? L.R : PM;
   // rows of each expert as a 64-bit mask (a row picks an expert once), so that every block has the same passes
   constexpr int PPT = MR_PAIRS / MR_NT;
   int pe[PPT];
@@ -499,7 +524,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
   // items dA .. dB - 1, their rows in the slots from 0
   auto run = [&](auto fmt, const int dA, const int dB, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
     using Fm = decltype(fmt);
-    constexpr int DEPTH = Fm::sums ? 8 / TL : MODE == 0 ? 3 : 2;
+    constexpr int DEPTH = 2;
     const int pos = s_off[dA], nrows = s_off[dB - 1] + s_num[dB - 1] - pos;
     // the position to load next: chunk lc of tile lt of item ld, whose tiles here are the counter's lbase .. lbase + ln - 1
     int ld = dA, lbase = 0, lt = 0, lt0, lt1, lc = nch;
@@ -535,7 +560,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
       d = over ? -1 : ld, t = lt, c = lc;
       const bool none = over | (lc * 256 + 128 >= K);
 #pragma unroll
-      for (int i = 0; i < TL; ++i) Fm::load(f[i], Q, S, MODE == 0 ? 16 * lt + i * a.i : 64 * lt + 16 * i, K, lc, none, over);
+      for (int i = 0; i < TL; ++i) Fm::load(f[i], Q, S, MODE == 0 ? 16 * lt + i * a.i : 32 * lt + 16 * i, K, lc, none, over);
       __builtin_amdgcn_sched_barrier(0);
     };
     static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { advance(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
@@ -545,32 +570,46 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
       return MODE == 0 ? (sh ? pr - pairs : pr / a.topk) : pr;
     });
     lds_barrier();
-    f32x4 o[TL];
-    const char* xr = xb;
-    const float* sr = sums;
+    f32x4 o[MQ][TL];
+    const char* xr[MQ];
+    const float* sr[MQ];
+    int cnt = 0;
+#pragma unroll
+    for (int q = 0; q < MQ; ++q) xr[q] = xb, sr[q] = sums;
     auto body = [&](typename Fm::Raw (&raw)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {  // one chunk
       if (c == 0 && d >= 0) {
-        const int cnt = s_num[d], slot = s_off[d] - pos + (c16 < cnt ? c16 : cnt - 1);
-        xr = xb + slot * L.RB + 2 * Fm::xoff(g);
-        sr = sums + slot * L.GS + g;
+        cnt = s_num[d];
 #pragma unroll
-        for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < MQ; ++q) {
+          const int row = MODE == 0 ? c16 : 4 * q + quad_row(), slot = s_off[d] - pos + (row < cnt ? row : cnt - 1);
+          xr[q] = xb + slot * L.RB + 2 * Fm::xoff(g) + (MODE == 0 ? 0 : quad_plane() * L.Kp * 2);
+          sr[q] = sums + slot * L.GS + g;
+#pragma unroll
+          for (int i = 0; i < TL; ++i) o[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
       }
-      chunk_mac<MODE, Fm, TL>(raw, xr, sr, L.Kp, c, c * 256 + 128 >= K, o);
+      const bool half = c * 256 + 128 >= K, lead = MODE == 0 || quad_lead();
+      if (MODE == 0 || cnt <= 4) chunk_mac<1, Fm>(raw, xr, sr, lead, c, half, o);
+      else chunk_mac<MQ, Fm>(raw, xr, sr, lead, c, half, o);
       if (c == nch - 1 && d >= 0) {
-        // register r of lane l: row 4 (l / 16) + r of x, column l % 16
-        const int off = s_off[d], cnt = s_num[d];
+        const int off = s_off[d];
+        if constexpr (MODE == 0) {
+          // register r of lane l: row 4 (l / 16) + r of x, column l % 16
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (r >= cnt) break;
-          const int row = 4 * g + r;
-          if (row >= cnt) continue;
-          const int pr = s_list[off + row];
-          if constexpr (MODE == 0) {
-            store_act(a, plane, pr, 16 * t + c16, o[0][r], o[1][r]);
-          } else {
+          for (int r = 0; r < 4; ++r) {
+            if (r >= cnt) break;
+            const int row = 4 * g + r;
+            if (row < cnt) store_act(a, plane, s_list[off + row], 16 * t + c16, o[0][0][r], o[0][1][r]);
+          }
+        } else {
 #pragma unroll
-            for (int i = 0; i < TL; ++i) a.yp[(size_t)pr * a.h + 64 * t + 16 * i + c16] = o[i][r];
+          for (int q = 0; q < MQ; ++q) {
+            if (4 * q >= cnt) break;
+            const int row = 4 * q + g;
+            if (row >= cnt) continue;
+            float* dst = a.yp + (size_t)s_list[off + row] * a.h + 32 * t + c16;
+#pragma unroll
+            for (int i = 0; i < TL; ++i) dst[16 * i] = quad_sum(o[q][i]);
           }
         }
       }
@@ -592,172 +631,129 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
   }
 }
 
-// ---- experts of very few rows ----------------------------------------------------------------
-// One row or two: with so few tiles the kernels above wait for one wave's walk through all inputs of a tile, and their last
-// launch (the combine) costs little but its start.  gate_up: the eight waves of a block share the inputs of a tile (16 gate and 16 up
-// rows), their sums meet in LDS.  down: a block owns 16 outputs of all rows; its waves share out (expert, chunk), add
-// the weighted products into their own sums, and the block joins those with res: y is complete.  Each wave finds the experts'
-// rows itself, one pick a lane.  With 256 experts, h 2048, i 512, 8 picks and the shared expert, experts above / here in us:
-// 1 row 14.7 + 11.1 + 4.1 / 9.7 + 10.3, 2 rows 16.1 + 11.8 + 4.0 / 12.5 + 16.2, 4 rows 19.2 + 14.2 + 4.1 / 17.7 + 28.6.
-// Two chunks under way per wave in down; four or eight cost 13.8 and 22.8 us at 1 row (places without work are multiplied too).
+// ---- experts of one row -----------------------------------------------------------------------
+// With so few tiles the kernels above wait for one wave's walk through all inputs of a tile, and their last launch (the
+// combine) costs little but its start.  gate_up: the eight waves of a block share the inputs of a tile (16 gate and 16 up rows),
+// their sums meet in LDS.  down: a block owns 16 outputs; its waves share out (pick, chunk), weight and add the
+// products, and the block joins those with res: y is complete.  The row stands in all rows of the fragments.
+// 256 experts, h 2048, i 512, 8 picks and the shared expert: 8.7 + 8.4 us, the kernels above 12.8 + 8.2 + 4.1 and one launch
+// more (two rows, in kernels like these: 12.6 + 14.3 against 13.8 + 9.2 + 4.0).
+// Two chunks under way per wave in down; four cost 4 us more (places without work are multiplied too).
 template <int MODE, class F, class FS>
-__global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_few(MoeRows a) {
-  constexpr int TL = MODE == 0 ? 2 : 1;
+__global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_one(MoeRows a) {
+  constexpr int TL = MODE == 0 ? 2 : 1, RING = 2;
   extern __shared__ uint4 xlds[];
-  __shared__ float red[MODE == 0 ? 2 * MR_NW * TL * 4 * 64 : MR_NW * 16 * 16];
+  __shared__ float red[2][MR_NW][TL][16];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
-  const int pairs = a.rows * a.topk;
   const int K = MODE == 0 ? a.h : a.i, tiles = MODE == 0 ? a.i / 16 : a.h / 16, N = MODE == 0 ? 2 * a.i : a.h;
-  const int nch = (K + 255) / 256, S = a.shared ? 1 : 0;
+  const int nch = (K + 255) / 256, S = a.shared ? 1 : 0, grid = gridDim.x, blk = blockIdx.x;
   const XLayout<MODE> L(K);
-  const int slots = MODE == 0 ? a.rows : pairs + S * a.rows;
-  const size_t plane = (size_t)(pairs + a.rows) * a.i;
+  const int slots = MODE == 0 ? 1 : a.topk + S;
+  const size_t plane = (size_t)(a.topk + 1) * a.i;
   char* xb = reinterpret_cast<char*>(xlds);
   float* sums = reinterpret_cast<float*>(xb + (size_t)slots * L.RB);
-  // lane p < pairs: the expert of pick p, and whether no pick before it has that expert; items are experts in that order
-  const int mine = lane < pairs ? a.idx[lane] & 255 : -1;
-  bool first = lane < pairs;
-  for (int q = 0; q < pairs - 1; ++q) first = first && !(q < lane && __builtin_amdgcn_readlane(mine, q) == mine);
-  const uint64_t firsts = __ballot(first);
-  const int D0 = __builtin_popcountll(firsts);
-  auto expert_at = [&](int d) __attribute__((always_inline)) {
-    uint64_t m = firsts;
-    for (; d > 0; --d) m &= m - 1;
-    return __builtin_amdgcn_readlane(mine, __builtin_ctzll(m));
-  };
-  // picks of an expert as a mask; the c16-th of them (the last where there are fewer)
-  auto nth = [&](uint64_t m, int n) __attribute__((always_inline)) {
-    const int cnt = __builtin_popcountll(m);
-    for (int j = 0; j < cnt - 1; ++j) m = j < n ? m & (m - 1) : m;
-    return __builtin_ctzll(m);
+  // pick p in lane p, with its weight in y (the shared expert's the last)
+  const int mine = lane < a.topk ? a.idx[lane] & 255 : 0;
+  float wt = 0.f;
+  if constexpr (MODE == 1) {
+    wt = lane < a.topk ? a.wts[lane] : 0.f;
+    if (S && lane == a.topk) wt = 1.f / (1.f + expf(-a.sgate[0]));
+  }
+  // chunk c of tile `tile` of pick d (none: nothing is fetched)
+  auto load = [&](auto fmt, auto& raw, const bool sh, const uint8_t* Wq, const void* Ws, int d, int tile, int c, bool none) __attribute__((always_inline)) {
+    using Fm = decltype(fmt);
+    const size_t m = sh || none ? 0 : __builtin_amdgcn_readlane(mine, d);
+    const Rsrc Q = rsrc(Wq + m * Fm::q_bytes(N, K), (uint32_t)Fm::q_bytes(N, K));
+    const Rsrc Z = rsrc(reinterpret_cast<const char*>(Ws) + m * Fm::s_bytes(N, K), (uint32_t)Fm::s_bytes(N, K));
+#pragma unroll
+    for (int i = 0; i < TL; ++i) Fm::load(raw[i], Q, Z, 16 * tile + i * a.i, K, c, none || c * 256 + 128 >= K, none);
+    __builtin_amdgcn_sched_barrier(0);
   };
   bool staged = false;
-  auto stage = [&]() __attribute__((always_inline)) {
+  auto stage = [&]() __attribute__((always_inline)) {  // behind the first weights
     if (staged) return;
     stage_rows<MODE, F::perm, F::sums>(a, L, K, slots, xb, sums, plane, [](int slot) { return slot; });
     lds_barrier();
     staged = true;
   };
-  const int grid = gridDim.x, blk = blockIdx.x;
   if constexpr (MODE == 0) {
+    const float* const sr[1] = {sums + g};
     int par = 0;
-    // tiles u0, u0 + grid, .. of the items of one format (sh: the shared expert's, of all rows)
+    // tiles u0, u0 + grid, .. of the picks or of the shared expert
     auto run = [&](auto fmt, int u0, int units, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
       using Fm = decltype(fmt);
       if (u0 >= units) return;
+      const char* const xr[1] = {xb + 2 * Fm::xoff(g)};
       typename Fm::Raw raw[TL];
-      auto load = [&](int u, int c) __attribute__((always_inline)) {
-        const bool none = u >= units || c >= nch;
-        const int d = u / tiles, tile = u - d * tiles;
-        const size_t m = sh || none ? 0 : expert_at(d);
-        const Rsrc Q = rsrc(Wq + m * Fm::q_bytes(N, K), (uint32_t)Fm::q_bytes(N, K));
-        const Rsrc Z = rsrc(reinterpret_cast<const char*>(Ws) + m * Fm::s_bytes(N, K), (uint32_t)Fm::s_bytes(N, K));
-#pragma unroll
-        for (int i = 0; i < TL; ++i) Fm::load(raw[i], Q, Z, 16 * tile + i * a.i, K, c, none || c * 256 + 128 >= K, none);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      load(u0, wave);
+      load(fmt, raw, sh, Wq, Ws, u0 / tiles, u0 % tiles, wave, wave >= nch);
       stage();
       for (int u = u0; u < units; u += grid) {
-        const int d = u / tiles, tile = u - d * tiles;
-        // the item's picks (for the shared expert: one bit a row)
-        uint64_t m = (1ull << a.rows) - 1;
-        if (!sh) {
-          const int e = expert_at(d);
-          m = __ballot(mine == e);
-        }
-        const int cnt = __builtin_popcountll(m), pick_ = nth(m, c16), slot = sh ? pick_ : pick_ / a.topk;
-        const char* xr = xb + slot * L.RB + 2 * Fm::xoff(g);
-        const float* sr = sums + slot * L.GS + g;
-        f32x4 o[TL];
+        const int d = u / tiles, tile = u - d * tiles, v = u + grid;
+        f32x4 o[1][TL];
 #pragma unroll
-        for (int i = 0; i < TL; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < TL; ++i) o[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int c = wave; c < nch; c += MR_NW) {
-          if (c != wave) load(u, c);
-          chunk_mac<MODE, Fm, TL>(raw, xr, sr, L.Kp, c, c * 256 + 128 >= K, o);
+          if (c != wave) load(fmt, raw, sh, Wq, Ws, d, tile, c, false);
+          chunk_mac<1, Fm>(raw, xr, sr, true, c, c * 256 + 128 >= K, o);
         }
-        load(u + grid, wave);
-        float* rd = red + par * (MR_NW * TL * 4 * 64);
+        load(fmt, raw, sh, Wq, Ws, v / tiles, v % tiles, wave, v >= units || wave >= nch);
+        if (g == 0)
 #pragma unroll
-        for (int i = 0; i < TL; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) rd[((wave * TL + i) * 4 + r) * 64 + lane] = o[i][r];
+          for (int i = 0; i < TL; ++i) red[par][wave][i][c16] = o[0][i][0];
         lds_barrier();
-        // register r of lane l: row 4 (l / 16) + r, column l % 16; four of the eight waves by turns
-        const int r = wave ^ (4 * par);
-        if (r < 4 && r < cnt) {
-          float v[2] = {0.f, 0.f};
+        if (wave == 4 * par) {
+          float s[TL] = {0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < MR_NW; ++k)
 #pragma unroll
-            for (int i = 0; i < TL; ++i) v[i] += rd[((k * TL + i) * 4 + r) * 64 + lane];
-          const int row = 4 * g + r, pr = nth(m, row) + (sh ? pairs : 0);
-          if (row < cnt) store_act(a, plane, pr, 16 * tile + c16, v[0], v[1]);
+            for (int i = 0; i < TL; ++i) s[i] += red[par][k][i][c16];
+          if (g == 0) store_act(a, plane, sh ? a.topk : d, 16 * tile + c16, s[0], s[1]);
         }
         par ^= 1;
       }
     };
-    const int us = S * tiles, ur = D0 * tiles;
+    const int us = S * tiles;
     if (S) run(FS{}, blk, us, true, reinterpret_cast<const uint8_t*>(a.sgu_q), a.sgu_s);
-    run(F{}, (blk + grid - us % grid) % grid, ur, false, a.gu_q, a.gu_s);
+    run(F{}, (blk + grid - us % grid) % grid, a.topk * tiles, false, a.gu_q, a.gu_s);
   } else {
-    float* mysum = red + wave * 256;
+    int par = 0;
     for (int tile = blk; tile < tiles; tile += grid) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) mysum[64 * q + lane] = 0.f;
-      // (item, chunk) q0, q0 + 8, .. of one format
+      float sum = 0.f;
+      // (pick, chunk) q0, q0 + 8, .. of one format
       auto run = [&](auto fmt, int q0, int units, const bool sh, const uint8_t* Wq, const void* Ws) __attribute__((always_inline)) {
         using Fm = decltype(fmt);
-        typename Fm::Raw raw[FEW_RING][TL];
-        auto load = [&](typename Fm::Raw (&f)[TL], int q) __attribute__((always_inline)) {
-          const bool none = q >= units;
-          const int d = q / nch, c = q - d * nch;
-          const size_t m = sh || none ? 0 : expert_at(d);
-          const Rsrc Q = rsrc(Wq + m * Fm::q_bytes(N, K), (uint32_t)Fm::q_bytes(N, K));
-          const Rsrc Z = rsrc(reinterpret_cast<const char*>(Ws) + m * Fm::s_bytes(N, K), (uint32_t)Fm::s_bytes(N, K));
-          Fm::load(f[0], Q, Z, 16 * tile, K, c, none || c * 256 + 128 >= K, none);
-          __builtin_amdgcn_sched_barrier(0);
+        typename Fm::Raw raw[RING][TL];
+        auto ask = [&](typename Fm::Raw (&f)[TL], int q) __attribute__((always_inline)) {
+          load(fmt, f, sh, Wq, Ws, q / nch, tile, q % nch, q >= units);
         };
         auto body = [&](typename Fm::Raw (&f)[TL], int q) __attribute__((always_inline)) {
-          const int d = q / nch, c = q - d * nch;
-          uint64_t m = (1ull << a.rows) - 1;
-          if (!sh) {
-            const int e = expert_at(q < units ? d : 0);
-            m = __ballot(mine == e);
-          }
-          const int cnt = __builtin_popcountll(m), slot = nth(m, c16) + (sh ? pairs : 0);
-          f32x4 o[TL] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-          chunk_mac<MODE, Fm, TL>(f, xb + slot * L.RB + 2 * Fm::xoff(g), sums + slot * L.GS + g, L.Kp, c, c * 256 + 128 >= K, o);
-          load(f, q + FEW_RING * MR_NW);
-          if (q < units)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int row = 4 * g + r;
-              if (r >= cnt) break;
-              if (row >= cnt) continue;
-              const int p = nth(m, row), t = sh ? p : p / a.topk;
-              const float w = sh ? 1.f / (1.f + expf(-a.sgate[t])) : a.wts[p];
-              mysum[16 * t + c16] += w * o[0][r];
-            }
+          const int d = q < units ? q / nch : 0, c = q % nch, slot = sh ? a.topk : d;
+          const char* const xr[1] = {xb + slot * L.RB + 2 * Fm::xoff(g) + quad_plane() * L.Kp * 2};
+          const float* const sr[1] = {sums + slot * L.GS + g};
+          f32x4 o[1][TL] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
+          chunk_mac<1, Fm>(f, xr, sr, quad_lead(), c, c * 256 + 128 >= K, o);
+          ask(f, q + RING * MR_NW);
+          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), slot));
+          if (q < units) sum += w * quad_sum(o[0][0]);
         };
-        static_for<FEW_RING>([&](auto j) __attribute__((always_inline)) { load(raw[j], q0 + j * MR_NW); });
+        static_for<RING>([&](auto j) __attribute__((always_inline)) { ask(raw[j], q0 + j * MR_NW); });
         stage();
-        for (int q = q0; q < units; q += FEW_RING * MR_NW)
-          static_for<FEW_RING>([&](auto j) __attribute__((always_inline)) { body(raw[j], q + j * MR_NW); });
+        for (int q = q0; q < units; q += RING * MR_NW)
+          static_for<RING>([&](auto j) __attribute__((always_inline)) { body(raw[j], q + j * MR_NW); });
       };
-      const int ur = D0 * nch;
+      const int ur = a.topk * nch;
       run(F{}, wave, ur, false, a.d_q, a.d_s);
       if (S) run(FS{}, (wave + MR_NW - ur % MR_NW) % MR_NW, nch, true, reinterpret_cast<const uint8_t*>(a.sd_q), a.sd_s);
+      if (g == 0) red[par][wave][0][c16] = sum;
       lds_barrier();
-      const int t = threadIdx.x >> 4;
-      if (t < a.rows) {
+      if (threadIdx.x < 16) {
         float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < MR_NW; ++k) v += red[256 * k + 16 * t + (threadIdx.x & 15)];
-        const size_t o = (size_t)t * a.h + 16 * tile + (threadIdx.x & 15);
+        for (int k = 0; k < MR_NW; ++k) v += red[par][k][0][c16];
+        const int o = 16 * tile + c16;
         a.y[o] = a.res ? a.res[o] + v : v;
       }
-      lds_barrier();
+      par ^= 1;
     }
   }
 }
@@ -825,11 +821,11 @@ int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   else hipLaunchKernelGGL(k_moe_rows_router<8>, dim3(nb, (a.rows + 7) / 8), dim3(MR_NT), 0, st, a);
   const XLayout<0> gl(a.h);
   const XLayout<1> dl(a.i);
-  const int slots = a.rows * (a.topk + a.shared);
-  if (a.rows <= 2 && slots <= 64 && a.rows <= gl.R && slots <= dl.R) {
+  const int slots = a.topk + a.shared;
+  if (a.rows == 1 && slots <= dl.R) {
     const int ug = a.i / 16 * slots, ud = a.h / 16;
-    hipLaunchKernelGGL((k_moe_rows_few<0, F, RowsQ8<SH, F::perm>>), dim3(ug < 512 ? ug : 512), dim3(MR_NT), a.rows * (gl.RB + 4 * gl.GS), st, a);
-    hipLaunchKernelGGL((k_moe_rows_few<1, F, RowsQ8<SH, F::perm>>), dim3(ud < 256 ? ud : 256), dim3(MR_NT), slots * (dl.RB + 4 * dl.GS), st, a);
+    hipLaunchKernelGGL((k_moe_rows_one<0, F, RowsQ8<SH, F::perm>>), dim3(ug < 512 ? ug : 512), dim3(MR_NT), gl.RB + 4 * gl.GS, st, a);
+    hipLaunchKernelGGL((k_moe_rows_one<1, F, RowsQ8<SH, F::perm>>), dim3(ud < 256 ? ud : 256), dim3(MR_NT), slots * (dl.RB + 4 * dl.GS), st, a);
     return 0;
   }
   hipLaunchKernelGGL((k_moe_rows_experts<0, F, RowsQ8<SH, F::perm>>), dim3(MR_GRID), dim3(MR_NT), MR_X, st, a);
