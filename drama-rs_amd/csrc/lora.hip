@@ -284,6 +284,8 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_one(Lora a) {
 // x: row r's 16-byte piece j lies at j ^ (r % 8), so the fragment reads meet no bank twice; W: four pieces a row in order, a
 // fragment pair being 1 KB in a row.  Lane (l % 16, g = l / 16) has the inputs 16 g .. 16 g + 15 of a slice, 8 a product.
 // 8 XCDs take the tiles in 8 contiguous runs, down columns of 8 row tiles, so that an XCD's blocks share x and W in its L2.
+// KS = 2 (the small tile): two groups of 2 x 2 waves take half of the inputs each and join their sums through LDS, since
+// small products wait for a tile's slices in turn (700 rows, n 1031, k 1024: 14.9 -> 11.2 us; 300 x 2048 x 2048: 19.3 -> 15.2).
 // 4096 rows, n 4096, k 2048, runs of 12 adapters of up to 64 ranks, one scale a row: 114 us, of which the product 79 (870
 // TFLOP/s; LDS reads), the residual and the store 24 (128 MB, the card's copy rate; nothing is left to overlap them with when
 // every CU has its two tiles at once) and the adapters the rest.
@@ -292,33 +294,39 @@ constexpr int LG_K = 64;
 DEV void to_lds(const void* src, uint4* dst) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
-template <class SH, int MT, int NT>
-__global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int tn) {
+template <class SH, int MT, int NT, int KS>
+__global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, int tm, int tn) {
   constexpr int BM = 32 * MT, BN = 32 * NT, PX = BM * 8 / 256, PW = BN * 4 / 256;
-  static_assert(PX * 256 == BM * 8 && PW * 256 == BN * 4, "pieces per thread");
-  __shared__ uint4 lx[2][BM * 8], lw[2][BN * 4];
-  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
+  constexpr int ME = MT / KS;  // row tiles of a wave once the parts of K are joined
+  static_assert(PX * 256 == BM * 8 && PW * 256 == BN * 4 && PX % KS == 0, "pieces per thread");
+  __shared__ uint4 lds_x[KS][2][BM * 8], lds_w[KS][2][BN * 4];
+  const int part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  auto& lx = lds_x[part];
+  auto& lw = lds_w[part];
+  const int tid = threadIdx.x & 255, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()) & 3, c16 = lane & 15, g = lane >> 4;
   // tile of this block
   const int total = tm * tn, per = (total + 7) / 8, q = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || q >= total) return;
   const int band = q / (8 * tn), bh = tm - 8 * band < 8 ? tm - 8 * band : 8, in = q - band * 8 * tn;
   const int m0 = (8 * band + in % bh) * BM, n0 = in / bh * BN;
-  const int wm = (wave >> 1) * 16 * MT, wn = (wave & 1) * 16 * NT;
+  const int wm = (wave >> 1) * 16 * MT, wn = (wave & 1) * 16 * NT, we = wm + 16 * ME * part;
   // adapters of the wave's rows, known before the product ends
-  int mine[MT];
+  int mine[ME];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) mine[m] = adapter_of(a, m0 + wm + 16 * m + c16);
+  for (int m = 0; m < ME; ++m) mine[m] = adapter_of(a, m0 + we + 16 * m + c16);
+  // this part's inputs, whole pairs of slices
+  const int pairs = a.k / 128, k0 = part * ((pairs + KS - 1) / KS) * 128, k1 = KS == 1 || part ? a.k : (pairs + KS - 1) / KS * 128;
   const uint16_t* xp[PX];
   const uint8_t* wp[PW];
 #pragma unroll
   for (int i = 0; i < PX; ++i) {
     const int r = m0 + (tid + 256 * i) / 8;
-    xp[i] = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + 8 * (tid & 7);
+    xp[i] = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + 8 * (tid & 7) + (k0 < a.k ? k0 : 0);
   }
 #pragma unroll
   for (int i = 0; i < PW; ++i) {
     const int n = n0 + (tid + 256 * i) / 4;
-    wp[i] = reinterpret_cast<const uint8_t*>(a.w) + (size_t)(n < a.n ? n : a.n - 1) * a.k + 16 * (tid & 3);
+    wp[i] = reinterpret_cast<const uint8_t*>(a.w) + (size_t)(n < a.n ? n : a.n - 1) * a.k + 16 * (tid & 3) + (k0 < a.k ? k0 : 0);
   }
   uint4 xv[PX], wv[PW];
   auto load = [&](int k) __attribute__((always_inline)) {
@@ -352,13 +360,17 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
     const int c = n0 + wn + 16 * n + c16;
     col[n] = c < a.n ? c : a.n - 1;
   }
-  const int steps = a.k / LG_K;  // even: k is a multiple of 128
+  const int steps = (k1 - k0) / LG_K, most = KS == 1 ? steps : (pairs + KS - 1) / KS * 2;  // even
   load(0);
   store(0);
-  load(LG_K);
+  load(steps > 0 ? LG_K : 0);
   lds_barrier();
   auto step = [&](auto odd, int s) __attribute__((always_inline)) {
     constexpr int B = decltype(odd)::value;
+    if (KS > 1 && s >= steps) {  // the longer part's barriers
+      lds_barrier();
+      return;
+    }
     if (s + 1 < steps) {
       store(B ^ 1);
       load(s + 2 < steps ? (s + 2) * LG_K : (s + 1) * LG_K);
@@ -366,7 +378,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
     float sc[NT];
     if constexpr (B == 1 && !SH::per_row) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) sc[n] = SH::scale(a.s, col[n], s * LG_K, a.k);
+      for (int n = 0; n < NT; ++n) sc[n] = SH::scale(a.s, col[n], k0 + s * LG_K, a.k);
     }
     uint4 xf[2][MT];
 #pragma unroll
@@ -393,7 +405,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
     }
     lds_barrier();
   };
-  for (int s = 0; s < steps; s += 2) {
+  for (int s = 0; s < most; s += 2) {
     step(std::integral_constant<int, 0>{}, s);
     step(std::integral_constant<int, 1>{}, s + 1);
   }
@@ -410,14 +422,36 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
       }
     }
   }
+  f32x4 out[ME][NT];
+  if constexpr (KS == 1) {
+#pragma unroll
+    for (int m = 0; m < ME; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) out[m][n] = acc[m][n];
+  } else {
+    // each wave joins its share of the row tiles with the other part's sums
+    static_assert(KS == 1 || (KS == 2 && sizeof(lds_x) >= 8 * ME * NT * 64 * 16), "sums on their way");
+    f32x4* ex = reinterpret_cast<f32x4*>(&lds_x[0][0][0]);
+#pragma unroll
+    for (int m = 0; m < ME; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) ex[(((part ^ 1) * 4 + wave) * ME * NT + m * NT + n) * 64 + lane] = part ? acc[m][n] : acc[ME + m][n];
+    lds_barrier();
+#pragma unroll
+    for (int m = 0; m < ME; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) out[m][n] = (part ? acc[ME + m][n] : acc[m][n]) + ex[((part * 4 + wave) * ME * NT + m * NT + n) * 64 + lane];
+    lds_barrier();
+  }
   // B t, 64 ranks at a time: t of the block's rows goes to LDS (plane p in place of the x and W slices, laid out as a slice of x), then each wave
   // multiplies the distinct adapters of its rows, the t of other rows zero; B's fragments serve all row tiles.
   if (a.adapter) {
-    static_assert(sizeof(lw) >= sizeof(lx[0]), "plane 2 of t");
+    static_assert(sizeof(lds_w[0]) >= sizeof(lds_x[0][0]), "plane 2 of t");
+    uint4 *l0 = lds_x[0][0], *l1 = lds_x[0][1], *l2 = lds_w[0][0];
     const size_t plane = (size_t)a.rows * a.rp;
-    uint32_t rows_of[MT];
+    uint32_t rows_of[ME];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) rows_of[m] = (uint32_t)__ballot(mine[m] >= 0) & 0xffffu;
+    for (int m = 0; m < ME; ++m) rows_of[m] = (uint32_t)__ballot(mine[m] >= 0) & 0xffffu;
     uint4 b[2][NT];
     auto load_b = [&](int h, int ad, int rk, int j0) __attribute__((always_inline)) {  // ranks j0 + 32 h ..
       const int last = n0 + BN < a.n ? BN : a.n - n0, j = j0 + 32 * h + 8 * g;
@@ -429,18 +463,18 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
       }
     };
     for (int j0 = 0; j0 < a.rp; j0 += 64) {
-      uint32_t left[MT];
+      uint32_t left[ME];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) left[m] = rows_of[m];
+      for (int m = 0; m < ME; ++m) left[m] = rows_of[m];
       // the next adapter, -1 for none: its rows leave `left` and are those of `has`
-      uint32_t has[MT];
+      uint32_t has[ME];
       auto next = [&]() __attribute__((always_inline)) {
         int ad = -1;
 #pragma unroll
-        for (int m = MT - 1; m >= 0; --m)
+        for (int m = ME - 1; m >= 0; --m)
           if (left[m]) ad = __builtin_amdgcn_readlane(mine[m], __builtin_ctz(left[m]));
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < ME; ++m) {
           has[m] = ad < 0 ? 0u : (uint32_t)__ballot(mine[m] == ad) & 0xffffu;
           left[m] &= ~has[m];
         }
@@ -451,10 +485,10 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
       if (j0) lds_barrier();
       // straight to LDS, 64 pieces a wave in order: no registers beside the sums and B's fragments
 #pragma unroll
-      for (int i = 0; i < PX; ++i) {
+      for (int i = part; i < PX; i += KS) {
         const int at = 256 * i + 64 * wave, rl = (at + lane) >> 3, r = m0 + rl, j = j0 + 8 * ((lane & 7) ^ (rl & 7));
         const uint16_t* src = a.planes + (size_t)(r < a.rows ? r : a.rows - 1) * a.rp + (j < a.rp ? j : 0);
-        to_lds(src, &lx[0][at]), to_lds(src + plane, &lx[1][at]), to_lds(src + 2 * plane, &lw[0][0] + at);
+        to_lds(src, l0 + at), to_lds(src + plane, l1 + at), to_lds(src + 2 * plane, l2 + at);
       }
       __builtin_amdgcn_s_waitcnt(0);
       lds_barrier();
@@ -468,16 +502,16 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
 #pragma unroll
           for (int n = 0; n < NT; ++n) b[h][n] = make_uint4(b[h][n].x & k0, b[h][n].y & k1, b[h][n].z & k2, b[h][n].w & k3);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
+          for (int m = 0; m < ME; ++m) {
             if (!has[m]) continue;
-            const int r = wm + 16 * m + c16, at = r * 8 + ((4 * h + g) ^ (r & 7));
+            const int r = we + 16 * m + c16, at = r * 8 + ((4 * h + g) ^ (r & 7));
             const bool on_row = has[m] >> c16 & 1;
-            uint4 tf[3] = {lx[0][at], lx[1][at], (&lw[0][0])[at]};
+            const uint4 tf[3] = {l0[at], l1[at], l2[at]};
 #pragma unroll
             for (int q3 = 0; q3 < 3; ++q3) {
               const uint4 v = on_row ? tf[q3] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) acc[m][n] = mfma(v, b[h][n], acc[m][n]);
+              for (int n = 0; n < NT; ++n) out[m][n] = mfma(v, b[h][n], out[m][n]);
             }
           }
         }
@@ -488,20 +522,20 @@ __global__ void __launch_bounds__(256, 2) k_lora_gemm_tiles(Lora a, int tm, int 
   }
   // the residual of 16 rows in flight at a time (y may be res: its loads could not pass the stores)
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int m = 0; m < ME; ++m) {
     float rv[4][NT];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = m0 + wm + 16 * m + 4 * g + r;
+      const int row = m0 + we + 16 * m + 4 * g + r;
 #pragma unroll
       for (int n = 0; n < NT; ++n) rv[r][n] = a.res ? gld<float>(a.res + (size_t)(row < a.rows ? row : a.rows - 1) * a.ldy + col[n]) : 0.f;
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = m0 + wm + 16 * m + 4 * g + r;
+      const int row = m0 + we + 16 * m + 4 * g + r;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        if (row < a.rows && n0 + wn + 16 * n + c16 < a.n) a.y[row * a.ldy + col[n]] = rv[r][n] + acc[m][n][r];
+        if (row < a.rows && n0 + wn + 16 * n + c16 < a.n) a.y[row * a.ldy + col[n]] = rv[r][n] + out[m][n][r];
     }
   }
 }
@@ -538,20 +572,21 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
     else hipLaunchKernelGGL((k_lora_gemm_rows<SH, 4>), g, b, 0, st, a);
     return 0;
   }
-  auto go = [&](auto mt, auto nt) {
-    constexpr int M = decltype(mt)::value, N = decltype(nt)::value;
+  auto go = [&](auto mt, auto nt, auto ks) {
+    constexpr int M = decltype(mt)::value, N = decltype(nt)::value, KS = decltype(ks)::value;
     const long long tm = (a.rows + 32ll * M - 1) / (32 * M), tn = (a.n + 32ll * N - 1) / (32 * N), per = (tm * tn + 7) / 8;
-    hipLaunchKernelGGL((k_lora_gemm_tiles<SH, M, N>), dim3((unsigned)(8 * per)), dim3(256), 0, st, a, (int)tm, (int)tn);
+    hipLaunchKernelGGL((k_lora_gemm_tiles<SH, M, N, KS>), dim3((unsigned)(8 * per)), dim3(256 * KS), 0, st, a, (int)tm, (int)tn);
   };
+  constexpr std::integral_constant<int, 1> i1{};
   constexpr std::integral_constant<int, 2> i2{};
   constexpr std::integral_constant<int, 4> i4{};
   constexpr std::integral_constant<int, SH::per_row ? 8 : 4> wide{};
   // the wide tile once there are two for each CU, the middle one once there is one (4096 x 4096 x 2048, ranks to 64, W with one
-  // scale a row: wide 114 us, middle 128; 2048 rows: 74 and 67)
+  // scale a row: wide 114 us, middle 128; 2048 rows: 74 and 67), else the small one with two parts of K a block
   const long long m128 = (a.rows + 127) / 128;
-  if (m128 * ((a.n + 32 * wide.value - 1) / (32 * wide.value)) >= 512) go(i4, wide);
-  else if (m128 * ((a.n + 127) / 128) >= 256) go(i4, i4);
-  else go(i2, i2);
+  if (m128 * ((a.n + 32 * wide.value - 1) / (32 * wide.value)) >= 512) go(i4, wide, i1);
+  else if (m128 * ((a.n + 127) / 128) >= 256) go(i4, i4, i1);
+  else go(i2, i2, i2);
   return 0;
 }
 
