@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, in
     lds_barrier();
   }
   // B t, 64 ranks at a time: t of the block's rows goes to LDS (plane p in place of the x and W slices, laid out as a slice of x), then each wave
-  // multiplies the distinct adapters of its rows, the t of other rows zero; B's fragments serve all row tiles.
+  // multiplies the distinct adapters of its rows and adds what belongs to each row; B's fragments serve all row tiles.
   if (a.adapter) {
     static_assert(sizeof(lds_w[0]) >= sizeof(lds_x[0][0]), "plane 2 of t");
     uint4 *l0 = lds_x[0][0], *l1 = lds_x[0][1], *l2 = lds_w[0][0];
@@ -496,23 +496,29 @@ __global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, in
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int on = rk - j0 - 32 * h - 8 * g;  // of this lane's 8 ranks, those below rk
-          if (rk <= j0 + 32 * h) continue;
           const uint32_t k0 = on >= 2 ? 0xffffffffu : on == 1 ? 0xffffu : 0u, k1 = on >= 4 ? 0xffffffffu : on == 3 ? 0xffffu : 0u;
           const uint32_t k2 = on >= 6 ? 0xffffffffu : on == 5 ? 0xffffu : 0u, k3 = on >= 8 ? 0xffffffffu : on == 7 ? 0xffffu : 0u;
 #pragma unroll
           for (int n = 0; n < NT; ++n) b[h][n] = make_uint4(b[h][n].x & k0, b[h][n].y & k1, b[h][n].z & k2, b[h][n].w & k3);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (rk <= j0 + 32 * h) continue;
 #pragma unroll
           for (int m = 0; m < ME; ++m) {
             if (!has[m]) continue;
             const int r = we + 16 * m + c16, at = r * 8 + ((4 * h + g) ^ (r & 7));
-            const bool on_row = has[m] >> c16 & 1;
             const uint4 tf[3] = {l0[at], l1[at], l2[at]};
 #pragma unroll
-            for (int q3 = 0; q3 < 3; ++q3) {
-              const uint4 v = on_row ? tf[q3] : make_uint4(0, 0, 0, 0);
+            for (int n = 0; n < NT; ++n) {
+              f32x4 s = z;
 #pragma unroll
-              for (int n = 0; n < NT; ++n) out[m][n] = mfma(v, b[h][n], out[m][n]);
+              for (int q3 = 0; q3 < 3; ++q3) s = mfma(tf[q3], b[h][n], s);
+              // (chosen, not multiplied by zero: another row's adapter may hold infinities)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) out[m][n][i] += has[m] >> (4 * g + i) & 1 ? s[i] : 0.f;
             }
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
         ad = next();

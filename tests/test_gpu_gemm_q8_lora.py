@@ -190,6 +190,11 @@ def test_rows_keep_to_themselves(rows):
     keep = [r for r in range(rows) if r not in (3, 9, rows - 1)]
     assert torch.equal(y[keep], z[keep])
     assert torch.isnan(z[3, :200]).all() and torch.isnan(z[rows - 1, :200]).all()
+    # the same of B: a product with another row's zero would be NaN
+    c.tlb[5, :, 0], c.tlb[5, :, 1] = float("inf"), float("nan")
+    z = c.call()
+    torch.cuda.synchronize()
+    assert torch.equal(y[keep], z[keep])
 
 
 @pytest.mark.parametrize("rows,n", [(40, 512), (333, 640)])
