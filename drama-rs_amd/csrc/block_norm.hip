@@ -6,9 +6,11 @@
 //   b = sigmoid(sgate) shared + sum_k wts[k] y[slot_of[k]]  (k ascending, as dr_moe_combine).
 //
 // Every element of a row is read once and stays in the registers of the L lanes that share the row
-// (8 elements a lane, 16 beyond 8192 columns), so b's sum of squares, xo and xo's sum of squares
-// need no second read and xo may be x or b.  Bound by HBM; with few rows by the chain load, two row
-// sums, store.
+// (8 elements a lane, 16 beyond 4096 columns), so b's sum of squares, xo and xo's sum of squares
+// need no second read and xo may be x or b.  Bound by HBM: 4096 rows of 4096, 235 MB, 53 us = 4.4 TB/s where a large copy
+// reaches 4.7 (single elements where something is not aligned: 58); with few rows by the chain load, two row sums, store: 3.2 us for one
+// row of 2048.  The combine form reads topk rows of y besides: 300 rows of 2048, top 8, 28 MB in 9.8 us, a third of it
+// the chain slot, load, two sums.
 #include "common.hpp"
 
 using namespace drm;
@@ -204,7 +206,9 @@ void launch(const BlockNorm& a, hipStream_t st) {
   hipLaunchKernelGGL((k_block_norm<BK, V, L, PER>), dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(NT), 0, st, a);
 }
 
-// the fewest lanes that hold the row in 8 elements each (16 beyond 8192 columns)
+// The fewest lanes that hold the row in 8 elements each, 16 beyond 4096 columns: more in a lane hide less of the next load (4096 rows:
+// h 2048 20.6 us, 29.0 with 16; h 4096 54.0 and 55.3), but blocks of 1024 threads leave a CU idle while a row ends (2000
+// rows of 8192: 56.5 us with 512 lanes of 16, 67.9 with 1024 of 8; above 8192 512 lanes of 32 spill: 66 and 73).
 template <int BK, int V>
 void launch_l(const BlockNorm& a, hipStream_t st) {
   constexpr int P = 8 / V;
@@ -212,7 +216,7 @@ void launch_l(const BlockNorm& a, hipStream_t st) {
   else if (a.h <= 1024) launch<BK, V, 256, P / 2>(a, st);
   else if (a.h <= 2048) launch<BK, V, 256, P>(a, st);
   else if (a.h <= 4096) launch<BK, V, 512, P>(a, st);
-  else if (a.h <= 8192) launch<BK, V, 1024, P>(a, st);
+  else if (a.h <= 8192) launch<BK, V, 512, 2 * P>(a, st);
   else launch<BK, V, 1024, 2 * P>(a, st);
 }
 
