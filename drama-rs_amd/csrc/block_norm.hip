@@ -9,8 +9,7 @@
 // (8 elements a lane, 16 beyond 4096 columns), so b's sum of squares, xo and xo's sum of squares
 // need no second read and xo may be x or b.  Bound by HBM: 4096 rows of 4096, 235 MB, 53 us = 4.4 TB/s where a large copy
 // reaches 4.7 (single elements where something is not aligned: 58); with few rows by the chain load, two row sums, store: 3.2 us for one
-// row of 2048.  The combine form reads topk rows of y besides: 300 rows of 2048, top 8, 28 MB in 9.8 us, a third of it
-// the chain slot, load, two sums.
+// row of 2048.  The combine form reads topk rows of y besides: 300 rows of 2048, top 8, 28 MB in 9.8 us.
 #include "common.hpp"
 
 using namespace drm;

@@ -568,8 +568,12 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
     hipLaunchKernelGGL((k_lora_gemm_one<SH>), dim3((a.n + 15) / 16), dim3(LR_NT), 0, st, a);
     return 0;
   }
-  if (a.adapter && few) hipLaunchKernelGGL(k_lora_down<1>, dim3(tiles, 16, (a.rmax + 15) / 16), dim3(LR_NT), 0, st, a);
-  else if (a.adapter) hipLaunchKernelGGL(k_lora_down<2>, dim3(tiles, 2, a.rp / 32), dim3(LR_NT), 0, st, a);
+  // Blocks along the distinct adapters: 16 rows may have 16, but runs of rows have one or two, and blocks without one cost
+  // their start (4096 rows in runs: 21 us with 2, 54 with 16; in any order 300 rows of 40 adapters: 38 and 14, 48 rows: 26 and 7.5).
+  // 32 ranks a block take x half as often as 16 and have fewer blocks: from 65 rows on (4096 rows: 21 and 25 us; 48: 8.9 and 7.5).
+  const unsigned ny = 256 / tiles < 2 ? 2 : 256 / tiles > 16 ? 16 : 256 / tiles;
+  if (a.adapter && few) hipLaunchKernelGGL(k_lora_down<1>, dim3(tiles, ny, (a.rmax + 15) / 16), dim3(LR_NT), 0, st, a);
+  else if (a.adapter) hipLaunchKernelGGL(k_lora_down<2>, dim3(tiles, ny, a.rp / 32), dim3(LR_NT), 0, st, a);
   if (few) {
     const dim3 g((a.n + 15) / 16), b(LR_NT);
     if (tiles == 1) hipLaunchKernelGGL((k_lora_gemm_rows<SH, 1>), g, b, 0, st, a);

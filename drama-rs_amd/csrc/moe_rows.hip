@@ -815,8 +815,10 @@ int moe_rows(MoeRows a, void* ws, hipStream_t st) {
   a.act = reinterpret_cast<uint16_t*>(w + l.act);
   a.yp = reinterpret_cast<float*>(w + l.yp);
   const int nb = (a.e + a.shared + MR_NW - 1) / MR_NW;
-  if (a.rows <= 2) hipLaunchKernelGGL(k_moe_rows_router<1>, dim3(nb, a.rows), dim3(MR_NT), 0, st, a);
-  else if (a.rows <= 8) hipLaunchKernelGGL(k_moe_rows_router<2>, dim3(nb, (a.rows + 1) / 2), dim3(MR_NT), 0, st, a);
+  // the smallest sets that MR_SETS counters allow: shorter chains for the last block (1 / 2 / 4 / 8 rows a set in us: 1 row 6.0 / 6.5 /
+  // 7.0 / 8.2, 8 rows 6.7 / 6.6 / 7.3 / 8.9, 16 rows - / 7.8 / 7.9 / 9.3, 32 rows - / - / 9.7 / 10.0; 64 rows 12.9)
+  if (a.rows <= 4) hipLaunchKernelGGL(k_moe_rows_router<1>, dim3(nb, a.rows), dim3(MR_NT), 0, st, a);
+  else if (a.rows <= 16) hipLaunchKernelGGL(k_moe_rows_router<2>, dim3(nb, (a.rows + 1) / 2), dim3(MR_NT), 0, st, a);
   else if (a.rows <= 32) hipLaunchKernelGGL(k_moe_rows_router<4>, dim3(nb, (a.rows + 3) / 4), dim3(MR_NT), 0, st, a);
   else hipLaunchKernelGGL(k_moe_rows_router<8>, dim3(nb, (a.rows + 7) / 8), dim3(MR_NT), 0, st, a);
   const XLayout<0> gl(a.h);
