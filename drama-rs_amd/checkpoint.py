@@ -235,7 +235,7 @@ class MoeStack:
                 self.packed.append(pk)
             torch.cuda.synchronize()
         self._gemm = {}  # stream handle -> GEMM handle (one per stream for the stack's lifetime)
-        self._rows_ws = {}  # stream handle -> workspace of the layers for a few rows
+        self._rows_buf = {}  # stream handle -> buffers of the layers for a few rows (_rows_buffers)
 
     def _gemm_handle(self, st) -> int:
         import ctypes
@@ -348,42 +348,62 @@ class MoeStack:
             keep.update({"idx": idx[:n * k], "wts": wts[:n * k], "sgate": sg[:n], "slot_of": slot_of[:n * k],
                          "act": act[:n * k * I], "sact": sact[:n * I]})
 
+    def _rows_buffers(self, st, device) -> dict:
+        """The layer workspace, routing and norm buffers of ``rows`` and ``forward`` for 64 rows, one set a stream for the
+        stack's lifetime, so that a captured call finds them where they were.  Made by the first call on the stream,
+        which cannot be a captured one."""
+        import torch
+
+        key = int(st or 0)
+        if key not in self._rows_buf:
+            main = torch.cuda.ExternalStream(key) if key != 0 else torch.cuda.current_stream(device)
+            with torch.cuda.stream(main):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("call rows or forward once on this stream before capturing it")
+                n = self.lib.dr_moe_layer_rows_ws(64, self.E, self.H, self.I, self.topk)
+                if n == 0:
+                    raise ValueError("no layer kernel for few rows of this shape")
+                e = lambda *s, dt=torch.float32: torch.empty(s, dtype=dt, device=device)
+                self._rows_buf[key] = {"ws": torch.zeros(n, dtype=torch.uint8, device=device),
+                                       "idx": e(64 * self.topk, dt=torch.int32), "wts": e(64 * self.topk), "sgate": e(64),
+                                       "hn": e(64, self.H, dt=torch.bfloat16)}
+        return self._rows_buf[key]
+
     def rows(self, l: int, x, hn, stream=None, keep: dict | None = None) -> None:
         """Loaded layer l for 1 .. 64 token rows (one decode step of that many sequences): x f32 [rows, H] residual
         stream updated in place, hn bf16 [rows, H] its RMSNorm.  Each expert is read once for all rows that
-        picked it.  With ``keep`` (a dict), the routing (idx, wts, sgate) is left in it."""
-        import torch
-
-        P, L, lib = dramamoe.ptr, self.layers[l], self.lib
-        st = stream if stream is not None else dramamoe.stream_ptr()
+        picked it.  With ``keep`` (a dict), the routing (idx, wts, sgate) is left in it, in buffers that the next call on
+        the stream overwrites."""
         n = x.shape[0]
-        need = lib.dr_moe_layer_rows_ws(n, self.E, self.H, self.I, self.topk)
-        if need == 0:
-            raise ValueError(f"no layer kernel for {n} rows of this shape")
-        main = torch.cuda.ExternalStream(st) if int(st) != 0 else torch.cuda.current_stream(x.device)
-        with torch.cuda.stream(main):
-            ws = self._rows_ws.get(int(st or 0))
-            if ws is None or ws.numel() < need:
-                ws = self._rows_ws[int(st or 0)] = torch.zeros(need, dtype=torch.uint8, device=x.device)
-            idx = torch.empty(n * self.topk, dtype=torch.int32, device=x.device)
-            wts, sg = torch.empty(n * self.topk, device=x.device), torch.empty(n, device=x.device)
-        f = lib.dr_moe_layer_rows_fp8 if self.fp8 else lib.dr_moe_layer_rows
+        if not 1 <= n <= 64:
+            raise ValueError(f"{n} rows: 1 .. 64")
+        P, L = dramamoe.ptr, self.layers[l]
+        st = stream if stream is not None else dramamoe.stream_ptr()
+        b = self._rows_buffers(st, x.device)
+        f = self.lib.dr_moe_layer_rows_fp8 if self.fp8 else self.lib.dr_moe_layer_rows
         f(P(L["router"]), P(L["gu_q"]), P(L["gu_s"]), P(L["d_q"]), P(L["d_s"]), P(L["sgu_q"]), P(L["sgu_s"]), P(L["sd_q"]),
-          P(L["sd_s"]), P(hn), P(x), P(idx), P(wts), P(sg), P(ws), P(x), n, self.E, self.H, self.I, self.topk, st)
+          P(L["sd_s"]), P(hn), P(x), P(b["idx"]), P(b["wts"]), P(b["sgate"]), P(b["ws"]), P(x), n, self.E, self.H, self.I,
+          self.topk, st)
         if keep is not None:
-            keep.update({"idx": idx, "wts": wts, "sgate": sg})
+            keep.update({"idx": b["idx"][:n * self.topk], "wts": b["wts"][:n * self.topk], "sgate": b["sgate"][:n]})
 
     def forward(self, x, stream=None, chunk: int = 1024) -> None:
         """x (f32 [rows, H], device) through every loaded layer in place, each behind its own RMSNorm: up to 64 rows
-        through ``rows``, more through ``prefill``, whose combine carries the next layer's norm."""
+        through ``rows`` (capturable after a first call on the stream; two graphs that may run at once need a stack each),
+        more through ``prefill``, whose combine carries the next layer's norm."""
         import torch
 
         P = dramamoe.ptr
         st = stream if stream is not None else dramamoe.stream_ptr()
         n, few = x.shape[0], x.shape[0] <= 64
-        main = torch.cuda.ExternalStream(st) if int(st) != 0 else torch.cuda.current_stream(x.device)
-        with torch.cuda.stream(main):
-            hn = torch.empty((n, self.H), dtype=torch.bfloat16, device=x.device)
+        if n == 0:
+            return
+        if few:
+            hn = self._rows_buffers(st, x.device)["hn"]
+        else:
+            main = torch.cuda.ExternalStream(st) if int(st) != 0 else torch.cuda.current_stream(x.device)
+            with torch.cuda.stream(main):
+                hn = torch.empty((n, self.H), dtype=torch.bfloat16, device=x.device)
         for l, L in enumerate(self.layers):
             if few or l == 0:
                 self.lib.dr_block_norm(None, 0, P(x), self.H, None, None, 0, 0, None, 0.0, 1.0, P(L["nw"]), self.eps, None, 0,

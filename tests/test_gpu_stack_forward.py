@@ -112,3 +112,44 @@ def test_forward_of_a_prefill(tmp_path):
         st.prefill(0, x, hn, nw_next=st.layers[1]["nw"])
     with pytest.raises(ValueError, match="65 rows"):
         st.rows(0, torch.zeros(65, H, device="cuda"), hn)
+
+
+def test_forward_captured(tmp_path):
+    """forward captured for 3 rows and replayed on new rows, with eager calls of 1 and 40 rows on the same stream in between; a
+    first call under capture is refused."""
+    import ctypes
+
+    import torch
+
+    st, _ = make(tmp_path, "q4", 2)
+    s, g = torch.cuda.Stream(), ctypes.c_void_p()
+    x, z = torch.randn(3, H, device="cuda"), torch.randn(40, H, device="cuda")
+    torch.cuda.synchronize()
+    st.lib.dr_graph_begin(s.cuda_stream)
+    try:
+        with pytest.raises(RuntimeError, match="before capturing"):
+            st.forward(x, stream=s.cuda_stream)
+    finally:
+        assert st.lib.dr_graph_end(s.cuda_stream, ctypes.byref(g)) == 0
+    st.lib.dr_graph_destroy(g)
+    one = x.clone()
+    torch.cuda.synchronize()
+    st.forward(one, stream=s.cuda_stream)
+    s.synchronize()
+    g = ctypes.c_void_p()
+    st.lib.dr_graph_begin(s.cuda_stream)
+    st.forward(x, stream=s.cuda_stream)
+    assert st.lib.dr_graph_end(s.cuda_stream, ctypes.byref(g)) == 0
+    try:
+        for _ in range(4):
+            x.copy_(torch.randn(3, H, device="cuda"))
+            want, one, many = x.clone(), z[:1].clone(), z.clone()
+            torch.cuda.synchronize()
+            st.forward(want, stream=s.cuda_stream)
+            st.forward(one, stream=s.cuda_stream)
+            st.forward(many, stream=s.cuda_stream)
+            st.lib.dr_graph_launch(g, s.cuda_stream)
+            s.synchronize()
+            assert torch.equal(x, want)
+    finally:
+        st.lib.dr_graph_destroy(g)
