@@ -96,13 +96,27 @@ struct RowsQ4 {
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K / 2; }
   static DEV size_t s_bytes(int N, int K) { return (size_t)N * K / 16; }
   static DEV int xoff(int g) { return 32 * (g & 1) + 16 * (g >> 1); }
-  // n: the tile's first row
+  // n: the tile's first row.  WIN: the chunks of a tile come in order, so the scales of four (16 bytes a row each, of as many
+  // lines) come with the first, chunk c + l / 16 in lane l; `scales` hands them out (gate_up of 64 rows, 256 experts, h 2048, i
+  // 512: 64 -> 57 us; down, of two chunks there, 36.4 -> 36.8, asks for each chunk's).
+  template <bool WIN>
   static DEV void load(Raw& f, const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
     const bool none = off || (half && (lane_id() & 8));
     const uint32_t p = (n + pair_row()) * (K / 2) + c * 128 + pair_byte();
     f.w[0] = buf16(Q, none ? NOWHERE : p);
     f.w[1] = buf16(Q, none ? NOWHERE : p + 4 * K);
-    f.s = buf16(S, off ? NOWHERE : ((n + (lane_id() & 15)) * (K / 64) + c * 4) * 4);
+    f.s = buf16(S, off || (WIN && (c & 3)) ? NOWHERE : ((n + (lane_id() & 15)) * (K / 64) + (WIN ? c + (lane_id() >> 4) : c) * 4) * 4);
+  }
+  struct Win {
+    gu32x4 s;
+  };
+  template <bool WIN>
+  static DEV uint4 scales(Win& win, const Raw& f, int c) {
+    if constexpr (!WIN) return words(f.s);
+    if ((c & 3) == 0) win.s = f.s;
+    const int from = ((c & 3) * 16 + (lane_id() & 15)) * 4;
+    auto of = [&](uint32_t v) __attribute__((always_inline)) { return (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)v); };
+    return make_uint4(of(win.s.x), of(win.s.y), of(win.s.z), of(win.s.w));
   }
   // nibbles of a word as 16 + q in bf16: the nibble is the top four mantissa bits of a number in [16, 32)
   // (the two constants in registers, so that each pair of nibbles is a shift and one v_and_or_b32)
@@ -113,10 +127,10 @@ struct RowsQ4 {
     return make_uint4(((v << 3) & m) | b, ((v >> 1) & m) | b, ((v >> 5) & m) | b, ((v >> 9) & m) | b);
   }
   // The tile's words in the order of the products: w[p].x, .y the fragments of group 2 p, .z, .w of group 2 p + 1
-  DEV void prep(const Raw& f, bool half) {
+  DEV void prep(const Raw& f, bool half, const uint4& sc) {
     w[0] = words(f.w[0]), w[1] = words(f.w[1]);
     pair_up(w[0], w[1]);
-    s = make_uint4(f.s.x, f.s.y, pick(half, 0, f.s.z), pick(half, 0, f.s.w));
+    s = make_uint4(sc.x, sc.y, pick(half, 0, sc.z), pick(half, 0, sc.w));
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       // lanes g = 0, 1 hold group 2 p, g = 2, 3 group 2 p + 1: two words of each change places
@@ -160,6 +174,7 @@ struct Rows8 {
   uint32_t s[2];
   static DEV size_t q_bytes(int N, int K) { return (size_t)N * K; }
   static DEV int xoff(int g) { return 16 * g; }
+  template <bool>
   static DEV void load(Raw& f, const Rsrc& Q, const Rsrc& S, int n, int K, int c, bool half, bool off) {
     const uint32_t p = (n + pair_row()) * K + c * 256 + pair_byte();
     f.w[0] = buf16(Q, off ? NOWHERE : p), f.w[1] = buf16(Q, off ? NOWHERE : p + 8 * K);
@@ -167,7 +182,10 @@ struct Rows8 {
     f.s[0] = D::scale_raw(S, n + (lane_id() & 15), 2 * c, K, off);
     f.s[1] = D::scale_raw(S, n + (lane_id() & 15), 2 * c + 1, K, half);
   }
-  DEV void prep(const Raw& f, bool) {
+  struct Win {};
+  template <bool>
+  static DEV uint4 scales(Win&, const Raw&, int) { return make_uint4(0, 0, 0, 0); }
+  DEV void prep(const Raw& f, bool, const uint4&) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) w[q] = words(f.w[q]);
     pair_up(w[0], w[1]), pair_up(w[2], w[3]);
@@ -334,18 +352,18 @@ DEV int wave_scan(int v) {
 // Items are passes of up to P rows (16; down: 8, two fragments of four rows and their planes) of an expert, ascending, then of the
 // shared expert (whose rows are all); their
 // tiles are dealt to the blocks in contiguous runs of even length.  The shared expert has blocks of its own (a block with
-// tiles of both formats would stage and wait twice: gate_up of 4 rows, 256 experts, h 2048, i 512, 25 us instead of 19), twice as
-// many for its tiles as the others: its passes are the fullest and its format the widest (fp8 beside it, 8 rows: 32.0 us with
-// equal numbers, 28.6 with twice, 28.4 with three times as many).  A block stages the rows of its items in LDS (as many
+// tiles of both formats would stage and wait twice: gate_up of 4 rows, 256 experts, h 2048, i 512, 25 us instead of 19), three
+// times as many for its tiles as the others: its passes are the fullest and its format the widest (2 / 3 / 4 times: 64 rows 66.5 /
+// 63.6 / 64.8 us, 8 rows of fp8 experts 26.8 / 25.4 / 25.4, 24 rows of 16 experts of 4096 x 2048 71 / 71 / 76).  A block stages the rows of its items in LDS (as many
 // items at a time as R rows hold, most often all), then each of its waves takes one tile after the other from a counter and
 // multiplies all of its inputs, in chunks of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights
 // come in a ring of DEPTH chunks that runs on across tiles and items.
 //
-// 64 rows, 256 experts, h 2048, i 512, 8 picks and the shared expert: gate_up 68 us, down 39, for 266 and 133 MB, of which 62 and
-// 32 are left without the products and 6 pass before the first load (launch, plan).  The down planes as rows of one fragment:
-// 41 -> 38 us, 16 rows 25 -> 20.  Rings of 2 / 3 / 4 chunks: down 39.2 / 40.4 / 43.6, gate_up 69.0 / 70.8 / 69.8 (19 rows, h 1280, i
-// 896, 48 experts: 18.6 / 21.4 / 22.4).  16 waves a block: gate_up 67 and 20 us, level; two blocks a CU with half the rows each: 68
-// and 22.
+// 64 rows, 256 experts, h 2048, i 512, 8 picks and the shared expert: gate_up 64 us, down 39, for 266 and 133 MB; without the
+// products the loads alone take 52 (no shared expert; 58 with them) and 32, 4 of each the launch.  The down planes as rows of one
+// fragment: 41 -> 38 us, 16 rows 25 -> 20.  Rings of 2 / 3 / 4 chunks: down 39.2 / 40.4 / 43.6, gate_up (19 rows, h 1280, i 896, 48
+// experts) 18.6 / 21.4 / 22.4.  16 waves a block: gate_up level, down twice as long (spills); two blocks a CU with half the rows
+// each: level to slower.
 //
 // LDS: row slot s at s * RB, its planes Kp * 2 bytes apart (Kp: K rounded up to a chunk, zeros past K), pieces of 8 inputs
 // reordered for int4; RB is 16 bytes more than the planes, so that the 16 rows of a fragment meet different banks.
@@ -393,11 +411,11 @@ DEV void stage_rows(const MoeRows& a, const XLayout<MODE>& L, int K, int nrows, 
 // o[q] += the products of chunk c of x fragments 0 .. NQ - 1 (a lane's row of each at xr[q], its group sums at sr[q], counted if
 // lead) with TL tiles of weights, converted once for all of them
 template <int NQ, class Fm, int TL, int MQ>
-DEV void chunk_mac(const typename Fm::Raw (&raw)[TL], const char* const (&xr)[MQ], const float* const (&sr)[MQ], bool lead, int c, bool half,
+DEV void chunk_mac(const typename Fm::Raw (&raw)[TL], const uint4 (&sc)[TL], const char* const (&xr)[MQ], const float* const (&sr)[MQ], bool lead, int c, bool half,
                    f32x4 (&o)[MQ][TL]) {
   Fm f[TL];
 #pragma unroll
-  for (int i = 0; i < TL; ++i) f[i].prep(raw[i], half);
+  for (int i = 0; i < TL; ++i) f[i].prep(raw[i], half, sc[i]);
   if constexpr (Fm::sums)
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
@@ -443,6 +461,7 @@ DEV void store_act(const MoeRows& a, size_t plane, int pair, int col, float g, f
 template <int MODE, class F, class FS>
 __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
   constexpr int TL = 2, MQ = MODE == 0 ? 1 : 2;  // tiles of 16 weight rows, x fragments
+  constexpr bool WIN = MODE == 0;
   extern __shared__ uint4 xlds[];
   __shared__ uint16_t s_list[MR_PAIRS + MR_ROWS];  // pairs by expert, then the shared expert's rows
   __shared__ uint16_t s_e[MR_ITEMS], s_off[MR_ITEMS], s_num[MR_ITEMS];  // items: expert, first place in s_list, rows
@@ -507,7 +526,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
   lds_barrier();
   // the shared expert's blocks, in the measure of its cost, and this block's items: from dbase, to dtop
   const int D0 = __builtin_amdgcn_readfirstlane(s_d0), DS = a.shared ? (a.rows + P - 1) / P : 0;
-  const int grid = gridDim.x, cost = 2 * DS, nS = DS == 0 ? 0 : max(1, min(grid - 1, (2 * grid * cost + D0 + cost) / (2 * (D0 + cost))));
+  const int grid = gridDim.x, cost = 3 * DS, nS = DS == 0 ? 0 : max(1, min(grid - 1, (2 * grid * cost + D0 + cost) / (2 * (D0 + cost))));
   const bool sh = (int)blockIdx.x < nS;
   const int b = sh ? blockIdx.x : blockIdx.x - nS, nb = sh ? nS : grid - nS, all = (sh ? DS : D0) * tiles, dbase = sh ? D0 : 0;
   const int lo = (int)((long long)all * b / nb), hi = (int)((long long)all * (b + 1) / nb);
@@ -560,7 +579,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
       d = over ? -1 : ld, t = lt, c = lc;
       const bool none = over | (lc * 256 + 128 >= K);
 #pragma unroll
-      for (int i = 0; i < TL; ++i) Fm::load(f[i], Q, S, MODE == 0 ? 16 * lt + i * a.i : 32 * lt + 16 * i, K, lc, none, over);
+      for (int i = 0; i < TL; ++i) Fm::template load<WIN>(f[i], Q, S, MODE == 0 ? 16 * lt + i * a.i : 32 * lt + 16 * i, K, lc, none, over);
       __builtin_amdgcn_sched_barrier(0);
     };
     static_for<DEPTH>([&](auto k) __attribute__((always_inline)) { advance(w[k.value], td[k.value], tt[k.value], tc[k.value]); });
@@ -574,6 +593,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
     const char* xr[MQ];
     const float* sr[MQ];
     int cnt = 0;
+    typename Fm::Win win[TL] = {};
 #pragma unroll
     for (int q = 0; q < MQ; ++q) xr[q] = xb, sr[q] = sums;
     auto body = [&](typename Fm::Raw (&raw)[TL], int& d, int& t, int& c) __attribute__((always_inline)) {  // one chunk
@@ -589,8 +609,11 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
         }
       }
       const bool half = c * 256 + 128 >= K, lead = MODE == 0 || quad_lead();
-      if (MODE == 0 || cnt <= 4) chunk_mac<1, Fm>(raw, xr, sr, lead, c, half, o);
-      else chunk_mac<MQ, Fm>(raw, xr, sr, lead, c, half, o);
+      uint4 sc[TL];
+#pragma unroll
+      for (int i = 0; i < TL; ++i) sc[i] = Fm::template scales<WIN>(win[i], raw[i], c);
+      if (MODE == 0 || cnt <= 4) chunk_mac<1, Fm>(raw, sc, xr, sr, lead, c, half, o);
+      else chunk_mac<MQ, Fm>(raw, sc, xr, sr, lead, c, half, o);
       if (c == nch - 1 && d >= 0) {
         const int off = s_off[d];
         if constexpr (MODE == 0) {
@@ -666,7 +689,7 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_one(MoeRo
     const Rsrc Q = rsrc(Wq + m * Fm::q_bytes(N, K), (uint32_t)Fm::q_bytes(N, K));
     const Rsrc Z = rsrc(reinterpret_cast<const char*>(Ws) + m * Fm::s_bytes(N, K), (uint32_t)Fm::s_bytes(N, K));
 #pragma unroll
-    for (int i = 0; i < TL; ++i) Fm::load(raw[i], Q, Z, 16 * tile + i * a.i, K, c, none || c * 256 + 128 >= K, none);
+    for (int i = 0; i < TL; ++i) Fm::template load<false>(raw[i], Q, Z, 16 * tile + i * a.i, K, c, none || c * 256 + 128 >= K, none);
     __builtin_amdgcn_sched_barrier(0);
   };
   bool staged = false;
@@ -694,7 +717,11 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_one(MoeRo
         for (int i = 0; i < TL; ++i) o[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int c = wave; c < nch; c += MR_NW) {
           if (c != wave) load(fmt, raw, sh, Wq, Ws, d, tile, c, false);
-          chunk_mac<1, Fm>(raw, xr, sr, true, c, c * 256 + 128 >= K, o);
+          typename Fm::Win win;
+          uint4 sc[TL];
+#pragma unroll
+          for (int i = 0; i < TL; ++i) sc[i] = Fm::template scales<false>(win, raw[i], c);
+          chunk_mac<1, Fm>(raw, sc, xr, sr, true, c, c * 256 + 128 >= K, o);
         }
         load(fmt, raw, sh, Wq, Ws, v / tiles, v % tiles, wave, v >= units || wave >= nch);
         if (g == 0)
@@ -731,7 +758,9 @@ __global__ void __launch_bounds__(MR_NT, MODE == 0 ? 4 : 2) k_moe_rows_one(MoeRo
           const char* const xr[1] = {xb + slot * L.RB + 2 * Fm::xoff(g) + quad_plane() * L.Kp * 2};
           const float* const sr[1] = {sums + slot * L.GS + g};
           f32x4 o[1][TL] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
-          chunk_mac<1, Fm>(f, xr, sr, quad_lead(), c, c * 256 + 128 >= K, o);
+          typename Fm::Win win;
+          const uint4 sc[TL] = {Fm::template scales<false>(win, f[0], c)};
+          chunk_mac<1, Fm>(f, sc, xr, sr, quad_lead(), c, c * 256 + 128 >= K, o);
           ask(f, q + RING * MR_NW);
           const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), slot));
           if (q < units) sum += w * quad_sum(o[0][0]);
