@@ -559,7 +559,6 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
   if (a.adapter && (!a.la || !a.lb || !a.rank || !a.lscale || !a.t || ((uintptr_t)a.la & 15) || ((uintptr_t)a.lb & 15) || ((uintptr_t)a.t & 15)))
     return -1;
   a.ldx = ldx, a.ldy = ldy;
-  if (a.t) a.t += 64;  // the first 256 bytes of the workspace hold counters
   const int tiles = (a.rows + 15) / 16;
   const bool few = a.rows <= 64;
   a.rp = (a.rmax + 31) & ~31;
@@ -603,8 +602,8 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
 }  // namespace
 
 API size_t dr_gemm_q8_lora_ws(int rows, int n, int k, int rmax) {
-  // counters, then t: fp32 of rmax ranks or three bf16 planes of rmax rounded up to 32
-  return lora_shape_ok(rows, n, k, rmax) ? 256 + (((size_t)rows * ((rmax + 31) & ~31) * 6 + 255) & ~(size_t)255) : 0;
+  // t: fp32 of rmax ranks or three bf16 planes of rmax rounded up to 32
+  return lora_shape_ok(rows, n, k, rmax) ? ((size_t)(rows ? rows : 1) * ((rmax + 31) & ~31) * 6 + 255) & ~(size_t)255 : 0;
 }
 
 API int dr_gemm_q8_lora(const int8_t* w, const uint16_t* s, const uint16_t* x, int ldx, const int* adapter, const uint16_t* la,

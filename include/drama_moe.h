@@ -405,8 +405,7 @@ int dr_moe_combine_norm(const float* y, const int* slot_of, const float* wts, co
  * adapter has rank[a] < 1 has none; NULL: no row has one.  la bf16 [adapters, rmax, k] (A_a), lb bf16
  * [adapters, n, rmax] (B_a), rank i32 [adapters] (above rmax: rmax), lscale f32 [adapters]; ranks past rank[a] are
  * not read.  x, A, B and W enter exactly, A_a x and all sums are fp32.
- * ws: dr_gemm_q8_lora_ws(rows, n, k, rmax) bytes of scratch, its first 256 zero before the first call and then owned by
- * the library.  Calls that share ws must not overlap (two graphs that may run at once need one each).
+ * ws: dr_gemm_q8_lora_ws(rows, n, k, rmax) bytes of scratch, holding anything.  Calls that share ws must not overlap (two graphs that may run at once need one each).
  * w, x, la, lb and ws are multiples of 16 bytes.  rows == 0 does nothing.
  * Unsupported: rows < 0 or > 1048576, n < 1, k < 128, > 16384 or no multiple of 128, ldx < k or no multiple of 8,
  * ldy < n, rmax < 8, > 128 or no multiple of 8 (without adapters too), adapters < 0, a missing or misaligned buffer -> -1 (ws size: 0). */

@@ -49,7 +49,6 @@ class Case:
         self.trank, self.tscale = dev(self.rank), dev(self.scale)
         nb = D.lib().dr_gemm_q8_lora_ws(rows, n, k, rmax)
         self.ws = torch.full((nb + 256,), 0xFF, dtype=torch.uint8, device="cuda")  # NaN where nothing is written
-        self.ws[:256] = 0
 
     def call(self, y=None, stream=None):
         import torch
@@ -89,7 +88,7 @@ class Case:
         assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:3], got[bad][:3], want[bad][:3], bound[bad][:3])
         assert np.abs(got - want).max() <= 1e-3 * np.abs(want).max()  # the bound stays tight enough to mean something
         assert (y[:self.rows, self.n:] == 5).all() and (y[self.rows:] == 5).all()
-        assert (self.ws[-256:] == 0xFF).all() and (self.ws[:256] == 0).all()
+        assert (self.ws[-256:] == 0xFF).all()
 
 
 def ids_each(rows, adapters, seed=1):
