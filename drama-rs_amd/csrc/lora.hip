@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_one(Lora a) {
 // 8 XCDs take the tiles in 8 contiguous runs, down columns of 8 row tiles, so that an XCD's blocks share x and W in its L2.
 // KS = 2 (the small tile): two groups of 2 x 2 waves take half of the inputs each and join their sums through LDS, since
 // small products wait for a tile's slices in turn (700 rows, n 1031, k 1024: 14.9 -> 11.2 us; 300 x 2048 x 2048: 19.3 -> 15.2).
-// 4096 rows, n 4096, k 2048, runs of 12 adapters of up to 64 ranks, one scale a row: 114 us, of which the product 79 (870
+// 4096 rows, n 4096, k 2048, runs of 12 adapters of up to 64 ranks, one scale a row: 112 us, of which the product 79 (870
 // TFLOP/s; LDS reads), the residual and the store 24 (128 MB, the card's copy rate; nothing is left to overlap them with when
 // every CU has its two tiles at once) and the adapters the rest.
 constexpr int LG_K = 64;
