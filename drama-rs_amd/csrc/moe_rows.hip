@@ -6,7 +6,8 @@
 // v_mfma_f32_16x16x32_bf16 with A = up to 16 rows of x and B = 16 weight rows, converted exactly to bf16
 // in registers (int4: 16 + q, with the rest of q scale + min in one fp32 MFMA of the group sums of x), so x
 // enters exactly.  The activations are fp32; they travel as three bf16 planes of 8 mantissa
-// bits each (their sum is the fp32 value), three MFMAs per weight fragment, so nothing is rounded but the fp32 sums.
+// bits each (their sum is the fp32 value), so nothing is rounded but the fp32 sums.
+// Four launches: router, gate_up, down, combine; for one row three, the last of which completes y.
 #include "canon.hpp"
 
 using namespace drm;
@@ -349,15 +350,15 @@ DEV int wave_scan(int v) {
 
 // MODE 0: gate_up (tile t: gate rows 16 t and up rows i + 16 t, K = h), MODE 1: down (tile t: rows 32 t, K = i).
 //
-// Items are passes of up to P rows (16; down: 8, two fragments of four rows and their planes) of an expert, ascending, then of the
-// shared expert (whose rows are all); their
-// tiles are dealt to the blocks in contiguous runs of even length.  The shared expert has blocks of its own (a block with
-// tiles of both formats would stage and wait twice: gate_up of 4 rows, 256 experts, h 2048, i 512, 25 us instead of 19), three
-// times as many for its tiles as the others: its passes are the fullest and its format the widest (2 / 3 / 4 times: 64 rows 66.5 /
-// 63.6 / 64.8 us, 8 rows of fp8 experts 26.8 / 25.4 / 25.4, 24 rows of 16 experts of 4096 x 2048 71 / 71 / 76).  A block stages the rows of its items in LDS (as many
-// items at a time as R rows hold, most often all), then each of its waves takes one tile after the other from a counter and
-// multiplies all of its inputs, in chunks of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights
-// come in a ring of DEPTH chunks that runs on across tiles and items.
+// Items are passes of up to P rows (16; down: 8, two fragments of four rows and their planes) of an expert, ascending, then of
+// the shared expert (whose rows are all); their tiles are dealt to the blocks in contiguous runs of even length.  The
+// shared expert has blocks of its own (a block with tiles of both formats would stage and wait twice: gate_up of 4 rows, 256
+// experts, h 2048, i 512, 25 us instead of 19), three times as many for its tiles as the others: its passes are the fullest and
+// its format the widest (2 / 3 / 4 times: 64 rows 66.5 / 63.6 / 64.8 us, 8 rows of fp8 experts 26.8 / 25.4 / 25.4, 24 rows of 16
+// experts of 4096 x 2048 71 / 71 / 76).  A block stages the rows of its items in LDS (as many items at a time as R rows
+// hold, most often all), then each of its waves takes one tile after the other from a counter and multiplies all of its
+// inputs, in chunks of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights come in a ring of
+// DEPTH chunks that runs on across tiles and items.
 //
 // 64 rows, 256 experts, h 2048, i 512, 8 picks and the shared expert: gate_up 64 us, down 39, for 266 and 133 MB; without the
 // products the loads alone take 52 (no shared expert; 58 with them) and 32, 4 of each the launch.  The down planes as rows of one
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
     }
   if (a.shared && tid < a.rows) s_list[pairs + tid] = pairs + tid;
   lds_barrier();
-  // the shared expert's blocks, in the measure of its cost, and this block's items: from dbase, to dtop
+  // the shared expert's blocks, in the measure of its cost, and this block's tiles lo .. hi - 1 of the items from dbase on
   const int D0 = __builtin_amdgcn_readfirstlane(s_d0), DS = a.shared ? (a.rows + P - 1) / P : 0;
   const int grid = gridDim.x, cost = 3 * DS, nS = DS == 0 ? 0 : max(1, min(grid - 1, (2 * grid * cost + D0 + cost) / (2 * (D0 + cost))));
   const bool sh = (int)blockIdx.x < nS;
