@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(LR_NT) k_lora_down(Lora a) {
         if (j < a.rmax) a.t[(size_t)row * a.rmax + j] = v;
       } else if (j < a.rp) {
         // 8 mantissa bits each, the last exact: hi + mid + lo = v
-        const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u), r1 = v - hi;
+        const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u), r1 = v == hi ? 0.f : v - hi;  // (an infinity stays one)
         const float mi = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi;
         uint16_t* p = a.planes + (size_t)row * a.rp + j;
         const size_t plane = (size_t)a.rows * a.rp;

@@ -452,7 +452,7 @@ DEV float quad_sum(const f32x4& o) { return o[0] + o[1] + o[2]; }
 DEV void store_act(const MoeRows& a, size_t plane, int pair, int col, float g, float u) {
   const float act = g / (1.f + expf(-g)) * u;
   uint16_t* dst = a.act + (size_t)pair * a.i + col;
-  const float hi = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act - hi;
+  const float hi = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act == hi ? 0.f : act - hi;  // (an infinity stays one)
   const float mi = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), r2 = r1 - mi;
   dst[0] = (uint16_t)(__float_as_uint(hi) >> 16);
   dst[plane] = (uint16_t)(__float_as_uint(mi) >> 16);

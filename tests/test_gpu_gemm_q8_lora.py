@@ -196,6 +196,22 @@ def test_rows_keep_to_themselves(rows):
     assert torch.equal(y[keep], z[keep])
 
 
+@pytest.mark.parametrize("rows", [1, 24, 150])
+def test_overflow_stays_infinite(rows):
+    """A_a x past the range of fp32 in one rank: the outputs are infinities with that rank's signs, not NaN."""
+    import torch
+
+    c = Case("cfg", rows, 200, 512, 2, 16, [0] * rows)
+    c.tx[0, :512] = 1.0
+    c.tla[0, 0], c.tla[0, 1:] = 3e38, 0.0
+    c.tlb[0] = torch.where(torch.arange(200, device="cuda") % 3 == 0, -1.0, 1.0)[:, None].to(torch.bfloat16)
+    c.tscale[0] = 1.0
+    c.trank[0] = 16
+    y = c.call()[0, :200]
+    torch.cuda.synchronize()
+    assert torch.isinf(y).all() and torch.equal(y < 0, torch.arange(200, device="cuda") % 3 == 0)
+
+
 @pytest.mark.parametrize("rows,n", [(40, 512), (333, 640)])
 def test_graph_replays(rows, n):
     """Captured once, replayed with new rows and new adapter ids, eager calls on the same workspace in between."""
