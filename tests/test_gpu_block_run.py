@@ -87,3 +87,22 @@ def test_block_run(rows):
             assert all(torch.equal(a, b) for a, b in zip(got, blk.outputs()))
     finally:
         lib.dr_graph_destroy(g)
+
+
+def test_two_streams_at_once():
+    """Two runs of different sizes, each with its workspaces, on two streams beside each other: the bits of each alone."""
+    import torch
+
+    blocks = [Block(3, 512, 16, 256, 4), Block(40, 1024, 24, 384, 6)]
+    want = []
+    for b in blocks:
+        b.run()
+        torch.cuda.synchronize()
+        want.append(b.outputs())
+    streams = [torch.cuda.Stream() for _ in blocks]
+    for _ in range(10):
+        for b, s in zip(blocks, streams):
+            b.run(stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for b, w in zip(blocks, want):
+        assert all(torch.equal(p, q) for p, q in zip(b.outputs(), w))
