@@ -310,10 +310,10 @@ __global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, in
   const int band = q / (8 * tn), bh = tm - 8 * band < 8 ? tm - 8 * band : 8, in = q - band * 8 * tn;
   const int m0 = (8 * band + in % bh) * BM, n0 = in / bh * BN;
   const int wm = (wave >> 1) * 16 * MT, wn = (wave & 1) * 16 * NT, we = wm + 16 * ME * part;
-  // adapters of the wave's rows, known before the product ends
-  int mine[ME];
+  // adapters of the wave's rows and their ranks, known before the product ends
+  int mine[ME], ranks[ME];
 #pragma unroll
-  for (int m = 0; m < ME; ++m) mine[m] = adapter_of(a, m0 + we + 16 * m + c16);
+  for (int m = 0; m < ME; ++m) mine[m] = adapter_of(a, m0 + we + 16 * m + c16), ranks[m] = mine[m] < 0 ? 0 : rank_of(a, mine[m]);
   // this part's inputs, whole pairs of slices
   const int pairs = a.k / 128, k0 = part * ((pairs + KS - 1) / KS) * 128, k1 = KS == 1 || part ? a.k : (pairs + KS - 1) / KS * 128;
   const uint16_t* xp[PX];
@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, in
   }
   // B t, 64 ranks at a time: t of the block's rows goes to LDS (plane p in place of the x and W slices, laid out as a slice of x), then each wave
   // multiplies the distinct adapters of its rows and adds what belongs to each row; B's fragments serve all row tiles.
+  // (B of two or four adapters asked for at once: level, 700 rows of 40 adapters 59 -> 64 and 71 us.)
   if (a.adapter) {
     static_assert(sizeof(lds_w[0]) >= sizeof(lds_x[0][0]), "plane 2 of t");
     uint4 *l0 = lds_x[0][0], *l1 = lds_x[0][1], *l2 = lds_w[0][0];
@@ -466,13 +467,17 @@ __global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, in
       uint32_t left[ME];
 #pragma unroll
       for (int m = 0; m < ME; ++m) left[m] = rows_of[m];
-      // the next adapter, -1 for none: its rows leave `left` and are those of `has`
+      // the next adapter and its rank, -1 for none: its rows leave `left` and are those of `has`
       uint32_t has[ME];
+      int rk = 0;
       auto next = [&]() __attribute__((always_inline)) {
         int ad = -1;
 #pragma unroll
         for (int m = ME - 1; m >= 0; --m)
-          if (left[m]) ad = __builtin_amdgcn_readlane(mine[m], __builtin_ctz(left[m]));
+          if (left[m]) {
+            const int at = __builtin_ctz(left[m]);
+            ad = __builtin_amdgcn_readlane(mine[m], at), rk = __builtin_amdgcn_readlane(ranks[m], at);
+          }
 #pragma unroll
         for (int m = 0; m < ME; ++m) {
           has[m] = ad < 0 ? 0u : (uint32_t)__ballot(mine[m] == ad) & 0xffffu;
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, in
         }
         return ad;
       };
-      int ad = next(), rk = ad < 0 ? 0 : rank_of(a, ad);
+      int ad = next();
       if (ad >= 0) load_b(0, ad, rk, j0), load_b(1, ad, rk, j0);
       if (j0) lds_barrier();
       // straight to LDS, 64 pieces a wave in order: no registers beside the sums and B's fragments
@@ -522,7 +527,7 @@ __global__ void __launch_bounds__(256 * KS, 2 * KS) k_lora_gemm_tiles(Lora a, in
           }
         }
         ad = next();
-        if (ad >= 0) rk = rank_of(a, ad), load_b(0, ad, rk, j0), load_b(1, ad, rk, j0);
+        if (ad >= 0) load_b(0, ad, rk, j0), load_b(1, ad, rk, j0);
       }
     }
   }
