@@ -596,7 +596,7 @@ int gemm_lora(Lora a, int ldx, int ldy, hipStream_t st) {
   constexpr std::integral_constant<int, 4> i4{};
   constexpr std::integral_constant<int, SH::per_row ? 8 : 4> wide{};
   // the wide tile once there are two for each CU, the middle one once there is one (4096 x 4096 x 2048, ranks to 64, W with one
-  // scale a row: wide 114 us, middle 128; 2048 rows: 74 and 67), else the small one with two parts of K a block
+  // scale a row: wide 113 us, middle 128; 2048 rows: 74 and 67), else the small one with two parts of K a block
   const long long m128 = (a.rows + 127) / 128;
   if (m128 * ((a.n + 32 * wide.value - 1) / (32 * wide.value)) >= 512) go(i4, wide, i1);
   else if (m128 * ((a.n + 127) / 128) >= 256) go(i4, i4, i1);
