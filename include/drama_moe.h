@@ -427,7 +427,8 @@ int dr_gemm_q8_lora_bf16s(const int8_t* w, const dr_bf16* s, const dr_bf16* x, i
  * dr_moe_decode, dr_moe_decode_bf16s, dr_moe_decode_fp8 and dr_moe_decode_fp8_bf16s; the four shared
  * pointers all NULL: no shared expert (sgate is then not written and may be NULL).  Each expert is
  * fetched once for all rows that picked it (8 at a time).  x enters exactly, activations,
- * sums and the combine are fp32; the same call gives the same bits, and in calls of two rows or more a
+ * sums and the combine are fp32; an activation beyond fp32 is an infinity and gives what the formula gives (an infinity of its
+ * weight's sign, NaN for a weight of zero); the same call gives the same bits, and in calls of two rows or more a
  * row's y has the same bits whichever rows stand beside it (one row alone: sums in another order).  res f32 [rows, h] may be NULL; y f32 [rows, h] may be res, and overlaps nothing else.
  * ws: dr_moe_layer_rows_ws(rows, e, h, i, topk) bytes, its first 1024 zero before the first call and
  * then owned by the library; it serves calls of any size it is large enough for.  Calls that share ws must
