@@ -27,7 +27,7 @@ struct BlockNorm {
   int gate_mode, rows, h;
   // combine form
   const int* slot_of;
-  const float *wts, *sgate, *shared;
+  const float *wts, *sgate, *shared;  // sgate null without shared: the kernel reads what it is given
   int topk;
 };
 
@@ -270,6 +270,6 @@ API int dr_moe_combine_norm(const float* y, const int* slot_of, const float* wts
                             uint16_t* hn, int ldh, int rows, int h, hipStream_t st) {
   if (topk < 1 || topk > 32 || (rows > 0 && (!y || !slot_of || !wts || (shared && !sgate)))) return -1;
   BlockNorm a = norm_args(y, h, x, ldx, pw, gate, gate_mode, ldg, cs, bscale, xscale, nw, eps, xo, ldo, hn, ldh, rows, h);
-  a.slot_of = slot_of, a.wts = wts, a.sgate = sgate, a.shared = shared, a.topk = topk;
+  a.slot_of = slot_of, a.wts = wts, a.sgate = shared ? sgate : nullptr, a.shared = shared, a.topk = topk;
   return block_norm<B_COMBINE>(a, st);
 }
