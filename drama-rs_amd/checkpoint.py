@@ -237,6 +237,14 @@ class MoeStack:
         self._gemm = {}  # stream handle -> GEMM handle (one per stream for the stack's lifetime)
         self._rows_buf = {}  # stream handle -> buffers of the layers for a few rows (_rows_buffers)
 
+    @staticmethod
+    def _torch_stream(st, device):
+        """torch's name for the stream of handle st, which the kernels of a call run on and its buffers are made on: 0 is the null
+        stream, whatever stream is torch's current one."""
+        import torch
+
+        return torch.cuda.ExternalStream(st) if int(st or 0) != 0 else torch.cuda.default_stream(device)
+
     def _gemm_handle(self, st) -> int:
         import ctypes
 
@@ -297,7 +305,7 @@ class MoeStack:
         # temporaries come from the caching allocator of the stream the kernels run on, so they
         # are not handed out again while this call's kernels are pending on it; the side stream
         # waits for `main` before it touches them and `main` waits for it before the combine
-        main = torch.cuda.ExternalStream(st) if int(st) != 0 else torch.cuda.current_stream(dev)
+        main = self._torch_stream(st, dev)
         with torch.cuda.stream(main):
             z = lambda n, dt=torch.float32: torch.empty(n, dtype=dt, device=dev)
             logits, idx, wts, sg = z(c * (E + 1)), z(c * k, torch.int32), z(c * k), z(c)
@@ -356,8 +364,7 @@ class MoeStack:
 
         key = int(st or 0)
         if key not in self._rows_buf:
-            main = torch.cuda.ExternalStream(key) if key != 0 else torch.cuda.current_stream(device)
-            with torch.cuda.stream(main):
+            with torch.cuda.stream(self._torch_stream(key, device)):
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("call rows or forward once on this stream before capturing it")
                 n = self.lib.dr_moe_layer_rows_ws(64, self.E, self.H, self.I, self.topk)
@@ -401,8 +408,7 @@ class MoeStack:
         if few:
             hn = self._rows_buffers(st, x.device)["hn"]
         else:
-            main = torch.cuda.ExternalStream(st) if int(st) != 0 else torch.cuda.current_stream(x.device)
-            with torch.cuda.stream(main):
+            with torch.cuda.stream(self._torch_stream(st, x.device)):
                 hn = torch.empty((n, self.H), dtype=torch.bfloat16, device=x.device)
         for l, L in enumerate(self.layers):
             if few or l == 0:
