@@ -471,7 +471,9 @@ DEV bool quad_lead() { return (lane_id() & 3) == 0; }
 DEV float quad_sum(const f32x4& o) { return o[0] + o[1] + o[2]; }
 
 // silu(g) u as three bf16 planes: 8 mantissa bits each, the last exact; returns it
+// (no contraction: act - hi of the product before its rounding would leave planes that are not act, nor their group sums for int4)
 DEV float store_act(const MoeRows& a, size_t plane, int pair, int col, float g, float u) {
+#pragma clang fp contract(off)
   const float act = g / (1.f + expf(-g)) * u;
   uint16_t* dst = a.act + (size_t)pair * a.i + col;
   const float hi = __uint_as_float(__float_as_uint(act) & 0xffff0000u), r1 = act == hi ? 0.f : act - hi;  // (an infinity stays one)
