@@ -106,3 +106,42 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for b, w in zip(blocks, want):
         assert all(torch.equal(p, q) for p, q in zip(b.outputs(), w))
+
+
+def test_two_streams_every_run_counts():
+    """As above with every run's outputs seen: each run starts on outputs filled with other values and on inputs of its own, and
+    its outputs are kept on its stream before the next one."""
+    import torch
+
+    blocks, runs = [Block(3, 512, 16, 256, 4), Block(40, 1024, 24, 384, 6)], 10
+    inputs = [[torch.randn_like(b.x) for _ in range(runs)] for b in blocks]
+
+    def start(b, x):
+        b.x.copy_(x)
+        for t in (*b.hn, b.p, b.x1, b.o["y"]):
+            t.fill_(5.0)
+        for k in ("idx", "wts", "sgate"):
+            b.o[k].fill_(-3)
+
+    want = []
+    for b, xs in zip(blocks, inputs):
+        b.run()  # makes its outputs
+        want.append([])
+        for x in xs:
+            start(b, x)
+            b.run()
+            torch.cuda.synchronize()
+            want[-1].append(b.outputs())
+    streams, got = [torch.cuda.Stream() for _ in blocks], [[] for _ in blocks]
+    torch.cuda.synchronize()
+    for k in range(runs):
+        for b, s, xs, g in zip(blocks, streams, inputs, got):
+            with torch.cuda.stream(s):
+                start(b, xs[k])
+                b.run(stream=s.cuda_stream)
+                g.append(b.outputs())
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for k in range(runs):
+            assert all(torch.equal(p, q) for p, q in zip(g[k], w[k])), k
+        assert not any(torch.equal(g[k][-4], g[k + 1][-4]) for k in range(runs - 1))
