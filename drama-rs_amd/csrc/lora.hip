@@ -134,14 +134,14 @@ DEV uint32_t pk8(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
 }
 DEV uint4 frag8(uint32_t a, uint32_t b) { return make_uint4(pk8(a, 0), pk8(a, 2), pk8(b, 0), pk8(b, 2)); }
 
-// Few rows: a block owns 16 columns and MT 16-row tiles; its eight waves take 128 inputs each in turn and
+// Few rows: a block owns 16 columns and all rows, MT tiles of 16; its eight waves take 128 inputs each in turn and
 // add their sums through LDS.  48 rows, n 4096, k 2048, 40 adapters of 32 ranks: 12.5 us behind 7.6 of k_lora_down, 18 MB
 // in all (3.8 at the copy rate); an empty launch takes 4 of each, the rest are the chains of dependent loads.  Column l % 16 of the weights in lane l, 16 inputs (16 (l / 16)) of each 64.
 template <class SH, int MT>
 __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
   __shared__ float red[LR_NW][MT][4][64];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, r0 = blockIdx.y * 16 * MT;
+  const int n0 = blockIdx.x * 16;
   const size_t n = n0 + c16 < a.n ? n0 + c16 : a.n - 1;
   // the rows and columns of this thread's outputs: output o = tid + 512 i is row 16 (o / 256) + 4 (o / 16 % 4) + o / 64 % 4 of
   // the block; what the epilogue needs of them is requested ahead of the product
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
 #pragma unroll
   for (int i = 0; i < OPT; ++i) {
     const int o = threadIdx.x + LR_NT * i;
-    row[i] = r0 + 16 * (o >> 8) + 4 * (o >> 4 & 3) + (o >> 6 & 3);
+    row[i] = 16 * (o >> 8) + 4 * (o >> 4 & 3) + (o >> 6 & 3);
     const bool live = o < 256 * MT && row[i] < a.rows && col < a.n;
     if (!live) row[i] = -1;
     base[i] = live && a.res ? a.res[row[i] * a.ldy + col] : 0.f;
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
   const uint16_t* xr[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int r = r0 + 16 * m + c16;
+    const int r = 16 * m + c16;
     xr[m] = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + 16 * g;
   }
   for (int c = wave * 128; c < a.k; c += LR_NW * 128) {
