@@ -207,7 +207,8 @@ void launch(const BlockNorm& a, hipStream_t st) {
 
 // The fewest lanes that hold the row in 8 elements each, 16 beyond 4096 columns: more in a lane hide less of the next load (4096 rows:
 // h 2048 20.6 us, 29.0 with 16; h 4096 54.0 and 55.3), but blocks of 1024 threads leave a CU idle while a row ends (2000
-// rows of 8192: 56.5 us with 512 lanes of 16, 67.9 with 1024 of 8; above 8192 512 lanes of 32 spill: 66 and 73).
+// rows of 8192: 56.5 us with 512 lanes of 16, 67.9 with 1024 of 8; above 8192 512 lanes of 32 spill: 66 and 73).  Of the
+// kernels here those for unaligned rows past 8192 columns keep 44 to 56 registers in memory.
 template <int BK, int V>
 void launch_l(const BlockNorm& a, hipStream_t st) {
   constexpr int P = 8 / V;

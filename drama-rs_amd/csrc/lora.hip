@@ -135,7 +135,7 @@ DEV uint32_t pk8(uint32_t v, int i) {  // bytes i, i + 1 as bf16 (exact)
 DEV uint4 frag8(uint32_t a, uint32_t b) { return make_uint4(pk8(a, 0), pk8(a, 2), pk8(b, 0), pk8(b, 2)); }
 
 // Few rows: a block owns 16 columns and all rows, MT tiles of 16; its eight waves take 128 inputs each in turn and
-// add their sums through LDS.  48 rows, n 4096, k 2048, 40 adapters of 32 ranks: 12.5 us behind 7.6 of k_lora_down, 18 MB
+// add their sums through LDS.  48 rows, n 4096, k 2048, 40 adapters of 32 ranks: 12.6 us behind 8 to 9 of k_lora_down, 18 MB
 // in all (3.8 at the copy rate); an empty launch takes 4 of each, the rest are the chains of dependent loads.  Column l % 16 of the weights in lane l, 16 inputs (16 (l / 16)) of each 64.
 template <class SH, int MT>
 __global__ void __launch_bounds__(LR_NT) k_lora_gemm_rows(Lora a) {
@@ -278,16 +278,18 @@ __global__ void __launch_bounds__(LR_NT) k_lora_gemm_one(Lora a) {
 
 // Many rows: a block of 2 x 2 waves owns 32 MT rows x 32 NT columns, a wave 16 MT x 16 NT of them.  Slices of 64 inputs
 // go through two LDS buffers, a slice's global loads in flight for the whole of the slice before; the barrier between slices
-// leaves them in flight.  The LDS reads set the pace (a wave tile of 64 x 64 in bf16 asks for 64 KB a slice, at ~64 bytes a
-// clock twice the time of its products), so W stays int8 there and is converted in the registers of the wave that
-// multiplies it, and the tile is as wide as the registers allow.
-// x: row r's 16-byte piece j lies at j ^ (r % 8), so the fragment reads meet no bank twice; W: four pieces a row in order, a
-// fragment pair being 1 KB in a row.  Lane (l % 16, g = l / 16) has the inputs 16 g .. 16 g + 15 of a slice, 8 a product.
+// leaves them in flight.  W stays int8 in LDS and is converted in the registers of the wave that multiplies it (in bf16 a wave tile
+// of 64 x 64 would read 64 KB a slice, at ~64 bytes a clock twice the time of its products), and the tile is as wide as the
+// registers allow; the widest keeps 22 of them in memory.
+// x: row r's 16-byte piece j lies at j ^ (r % 8), so its fragment reads meet no bank twice; W: four pieces a row in order, a
+// fragment pair being 1 KB in a row, but 64 bytes from lane to lane: its reads do meet (4.2 M conflict cycles for 1.6 M LDS
+// instructions in the case below).  Lane (l % 16, g = l / 16) has the inputs 16 g .. 16 g + 15 of a slice, 8 a product.
 // 8 XCDs take the tiles in 8 contiguous runs, down columns of 8 row tiles, so that an XCD's blocks share x and W in its L2.
 // KS = 2 (the small tile): two groups of 2 x 2 waves take half of the inputs each and join their sums through LDS, since
 // small products wait for a tile's slices in turn (700 rows, n 1031, k 1024: 14.9 -> 11.2 us; 300 x 2048 x 2048: 19.3 -> 15.2).
-// 4096 rows, n 4096, k 2048, runs of 12 adapters of up to 64 ranks, one scale a row: 112 us, of which the product 79 (870
-// TFLOP/s; LDS reads), the residual and the store 24 (128 MB, the card's copy rate; nothing is left to overlap them with when
+// 4096 rows, n 4096, k 2048, runs of 12 adapters of up to 64 ranks, one scale a row: 113 us, of which the product 79 (870
+// TFLOP/s; no one pipe fills them, they wait for each other: LDS reads 27, its writes 14, matrix unit 29, the conversions of W, done by two waves
+// each, and the rest of the VALU 35), the residual and the store 24 (128 MB, the card's copy rate; nothing is left to overlap them with when
 // every CU has its two tiles at once) and the adapters the rest.
 constexpr int LG_K = 64;
 // 16 bytes of each lane to dst + 16 lane

@@ -2,7 +2,7 @@
 //   l = R x, picks by (l desc, index asc), w = softmax(l) renormalised over the picks,
 //   y = res + sigmoid(l_E) D_s (silu(G_s x) * (U_s x)) + sum_k w_k D_k (silu(G_k x) * (U_k x)).
 //
-// An expert is fetched once for all the rows that picked it.  Matrix products run on
+// An expert is fetched once for each pass of rows that picked it (gate_up: 16 rows, down: 8, fewer of large sizes).  Matrix products run on
 // v_mfma_f32_16x16x32_bf16 with A = up to 16 rows of x and B = 16 weight rows, converted exactly to bf16
 // in registers (int4: 16 + q, with the rest of q scale + min in one fp32 MFMA of the group sums of x), so x
 // enters exactly.  The activations are fp32; they travel as three bf16 planes of 8 mantissa
@@ -382,14 +382,16 @@ DEV int wave_scan(int v) {
 // inputs, in chunks of 256: no sum crosses waves and no barrier stands between tiles.  A wave's weights come in a ring of
 // DEPTH chunks that runs on across tiles and items.
 //
-// 64 rows, 256 experts, h 2048, i 512, 8 picks and the shared expert: gate_up 64 us, down 39, for 266 and 133 MB; without the
+// 64 rows, 256 experts, h 2048, i 512, 8 picks and the shared expert: gate_up 64 us, down 40, for 266 and 133 MB; without the
 // products the loads alone take 52 (no shared expert; 58 with them) and 32, 4 of each the launch.  The down planes as rows of one
 // fragment: 41 -> 38 us, 16 rows 25 -> 20.  Rings of 2 / 3 / 4 chunks: down 39.2 / 40.4 / 43.6, gate_up (19 rows, h 1280, i 896, 48
 // experts) 18.6 / 21.4 / 22.4.  16 waves a block: gate_up level, down twice as long (spills); two blocks a CU with half the rows
 // each: level to slower.
 //
 // LDS: row slot s at s * RB, its planes Kp * 2 bytes apart (Kp: K rounded up to a chunk, zeros past K), pieces of 8 inputs
-// reordered for int4; RB is 16 bytes more than the planes, so that the 16 rows of a fragment meet different banks.
+// reordered for int4; RB is 16 bytes more than the planes, so that the rows of a fragment meet different banks.  In down a
+// row's three planes share a fragment and meet the same ones, as Kp * 2 is a multiple of 512: 2.3 M conflict cycles for 0.41 M LDS
+// instructions (gate_up 0.16 M for 1.07 M) in the case above.
 // Then, for int4, the fp32 sums of each 64 inputs.
 template <int MODE>
 struct XLayout {
@@ -755,7 +757,7 @@ __global__ void __launch_bounds__(MR_NT, 2) k_moe_rows_experts(MoeRows a) {
 // combine) costs little but its start.  gate_up: the eight waves of a block share the inputs of a tile (16 gate and 16 up rows),
 // their sums meet in LDS.  down: a block owns 16 outputs; its waves share out (pick, chunk), weight and add the
 // products, and the block joins those with res: y is complete.  The row stands in all rows of the fragments.
-// 256 experts, h 2048, i 512, 8 picks and the shared expert: 8.7 + 8.4 us, the kernels above 12.8 + 8.2 + 4.1 and one launch
+// 256 experts, h 2048, i 512, 8 picks and the shared expert: 9.6 + 8.4 us, the kernels above 12.8 + 8.2 + 4.1 and one launch
 // more (two rows, in kernels like these: 12.6 + 14.3 against 13.8 + 9.2 + 4.0).
 // Two chunks under way per wave in down; four cost 4 us more (places without work are multiplied too).
 template <int MODE, class F, class FS>

@@ -425,8 +425,10 @@ int dr_gemm_q8_lora_bf16s(const int8_t* w, const dr_bf16* s, const dr_bf16* x, i
  *   y[r] = res[r] + sigmoid(sgate[r]) * SD (silu(SG x) * (SU x)) + sum_k wts[r, k] * D_k (silu(G_k x) * (U_k x)).
  * router bf16 [e + 1, h] (row e: the shared expert's gate; [e, h] without a shared expert); experts as
  * dr_moe_decode, dr_moe_decode_bf16s, dr_moe_decode_fp8 and dr_moe_decode_fp8_bf16s; the four shared
- * pointers all NULL: no shared expert (sgate is then not written and may be NULL).  Each expert is
- * fetched once for all rows that picked it (8 at a time).  x enters exactly, activations,
+ * pointers all NULL: no shared expert (sgate is then not written and may be NULL).  An expert's rows go in passes, each of
+ * which reads its matrix once: of 16 rows for gate and up (14 at h 4096, 7 at h 8192) and of 8 for down (up to i 2304; 4 at i
+ * 4096, 2 at i 8192); the shared expert's likewise.  So 64 rows read the shared down 8 times at i 512 and 32 times at i 8192 (over PCIe
+ * where experts lie in host memory, but for what the caches hold).  x enters exactly, activations,
  * sums and the combine are fp32; an activation beyond fp32 is an infinity and gives what the formula gives (an infinity of its
  * weight's sign, NaN for a weight of zero); the same call gives the same bits, and in calls of two rows or more a
  * row's y has the same bits whichever rows stand beside it (one row alone: sums in another order).  res f32 [rows, h] may be NULL; y f32 [rows, h] may be res, and overlaps nothing else.
