@@ -379,9 +379,10 @@ class MoeStack:
     def rows(self, l: int, x, hn, stream=None, keep: dict | None = None) -> None:
         """Loaded layer l for 1 .. 64 token rows (one decode step of that many sequences): x f32 [rows, H] residual
         stream updated in place, hn bf16 [rows, H] its RMSNorm.  Each expert is read once for a pass of rows that
-        picked it (16 rows for gate and up, 8 for down, fewer of large sizes).  Up to four rows of H 2048, I 512, topk 8 the calls
-        dr_router_topk_rows and dr_moe_decode_rows of the library are faster (1 row 17 against 23 us, 4 rows 32 against 41).  With ``keep`` (a dict), the routing (idx, wts, sgate) is left in it, in buffers that the next call on
-        the stream overwrites."""
+        picked it (16 rows for gate and up, 8 for down, fewer of large sizes).  Up to four rows of H 2048, I 512, topk 8 the
+        library's dr_router_topk_rows and dr_moe_decode_rows are faster (1 row 17 against 23 us, 4 rows 32 against 41).  With
+        ``keep`` (a dict), the routing (idx, wts, sgate) is left in it, in buffers that the next call on the stream
+        overwrites."""
         n = x.shape[0]
         if not 1 <= n <= 64:
             raise ValueError(f"{n} rows: 1 .. 64")

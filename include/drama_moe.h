@@ -430,7 +430,8 @@ int dr_gemm_q8_lora_bf16s(const int8_t* w, const dr_bf16* s, const dr_bf16* x, i
  * 4096, 2 at i 8192); the shared expert's likewise.  So 64 rows read the shared down 8 times at i 512 and 32 times at i 8192 (over PCIe
  * where experts lie in host memory, but for what the caches hold).  x enters exactly, activations,
  * sums and the combine are fp32; an activation beyond fp32 is an infinity and gives what the formula gives (an infinity of its
- * weight's sign, NaN for a weight of zero); the same call gives the same bits, and in calls of two rows or more a
+ * weight's sign, NaN for a weight of zero).  fp8 and int8 products are summed over 128 inputs before their scale: where that
+ * sum passes fp32 (inputs or activations beyond 5e33) the output can be no finite number.  The same call gives the same bits, and in calls of two rows or more a
  * row's y has the same bits whichever rows stand beside it (one row alone: sums in another order).  res f32 [rows, h] may be NULL; y f32 [rows, h] may be res, and overlaps nothing else.
  * ws: dr_moe_layer_rows_ws(rows, e, h, i, topk) bytes, its first 1024 zero before the first call and
  * then owned by the library; it serves calls of any size it is large enough for.  Calls that share ws must
