@@ -1,0 +1,199 @@
+// The norm of each head and its rotary positions:
+//   n = x rsqrt(mean(x^2) + eps) nw          over a head's d elements (nw null: n = x)
+//   th = pos freq[j], c = mscale cos th, s = mscale sin th,  j < rot / 2
+//   (a, b) = (n[j], n[j + rot/2]) or, in pairs, (n[2 j], n[2 j + 1]) -> (a c - b s, b c + a s); elements from rot on stay n.
+//
+// A block takes a row, or as many rows as give its lanes work: it requests its elements, works out the rows' cosines and
+// sines once for all heads (LDS), and turns.  The lanes of a head (a power of two within a wave) hold both partners of
+// each pair, so the norm is a butterfly and nothing else crosses lanes, and y may be x.  Angles: the product of a position
+// and a frequency in 64 bits, its whole turns taken off there (at position 10^6 fp32 would be 0.06 rad off), the
+// sine and cosine of the rest in fp32.
+#include "common.hpp"
+
+using namespace drm;
+
+namespace {
+
+constexpr int NT = 256;
+
+struct Rope {
+  const void* x;
+  const float* nw;
+  const int* pos;
+  const float* freq;
+  float* y;
+  uint16_t* yb;
+  size_t ldx, hsx, ldn, ldy, ldb;
+  float eps, mscale;
+  int rows, heads, d, rot, pairs;
+};
+
+// V elements of a row from `at` on
+template <bool B16, int V>
+DEV void ld_x(const void* x, size_t at, float (&o)[V]) {
+  if constexpr (B16) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + at;
+    if constexpr (V == 4) {
+      const uint2 w = ld8(p);
+      o[0] = bf16_lo(w.x), o[1] = bf16_hi(w.x), o[2] = bf16_lo(w.y), o[3] = bf16_hi(w.y);
+    } else {
+      o[0] = bf16f(ld2(p));
+    }
+  } else {
+    const float* p = reinterpret_cast<const float*>(x) + at;
+    if constexpr (V == 4) {
+      const float4 v = ldf4(p);
+      o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+    } else {
+      o[0] = gld<float>(p);
+    }
+  }
+}
+
+template <int V>
+DEV void st_y(const Rope& a, size_t row, int at, const float (&o)[V]) {
+  if (a.y) {
+    float* p = a.y + row * a.ldy + at;
+    if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+    else *p = o[0];
+  }
+  if (a.yb) {
+    uint16_t* p = a.yb + row * a.ldb + at;
+    uint32_t q[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) q[v] = to_bf16(o[v]);
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+    else *p = (uint16_t)q[0];
+  }
+}
+
+// Sum over the L lanes of a head; all lanes of the wave take part.
+DEV float head_sum(float v, int L) {
+  if (L > 1) v = xsum_step<1>(v);
+  if (L > 2) v = xsum_step<2>(v);
+  if (L > 4) v = xsum_step<4>(v);
+  if (L > 8) v = xsum_step<8>(v);
+  if (L > 16) v = xsum_step<16>(v);
+  if (L > 32) v = xsum_step<32>(v);
+  return v;
+}
+
+// V elements a load (4, or 1 where sizes, strides or addresses allow no more); a unit is two vectors: partners of V pairs, or
+// elements behind rot.  L lanes a head, up to PER units a lane; RB rows a block.
+template <bool B16, int V, int PER>
+__global__ void __launch_bounds__(NT) k_rope(Rope a, int L, int RB) {
+  extern __shared__ float2 cs[];  // [RB][rot / 2]
+  const int half = a.rot >> 1, turned = half / V, units = turned + (a.d - a.rot + 2 * V - 1) / (2 * V);
+  const long long r0 = (long long)blockIdx.x * RB;
+  const int nr = a.rows - r0 < RB ? (int)(a.rows - r0) : RB, items = nr * a.heads * L;
+  bool ready = false;
+  for (int w0 = 0; w0 < items; w0 += NT) {
+    const int w = w0 + threadIdx.x, l = w & (L - 1), hr = w / L, rl = hr / a.heads, h = hr - rl * a.heads;
+    const bool on = w < items;
+    const size_t r = (size_t)r0 + rl, xb = r * a.ldx + (size_t)h * a.hsx;
+    float p[PER][2][V], nw[PER][2][V];
+    int e0[PER], e1[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int k = l + L * u;
+      // the two vectors' first elements
+      if (k >= turned) e0[u] = a.rot + 2 * V * (k - turned), e1[u] = e0[u] + V;
+      else if (a.pairs) e0[u] = 2 * V * k, e1[u] = e0[u] + V;
+      else e0[u] = V * k, e1[u] = e0[u] + half;
+      if (!on || k >= units) e0[u] = e1[u] = a.d;
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[u][0][v] = p[u][1][v] = 0.f, nw[u][0][v] = nw[u][1][v] = 1.f;
+      if (e0[u] < a.d) ld_x<B16, V>(a.x, xb + e0[u], p[u][0]);
+      if (e1[u] < a.d) ld_x<B16, V>(a.x, xb + e1[u], p[u][1]);
+      if (a.nw) {
+        if (e0[u] < a.d) ld_x<false, V>(a.nw, h * a.ldn + e0[u], nw[u][0]);
+        if (e1[u] < a.d) ld_x<false, V>(a.nw, h * a.ldn + e1[u], nw[u][1]);
+      }
+    }
+    if (!ready) {
+      // behind the first loads, which are on their way meanwhile
+      for (int t = threadIdx.x; t < nr * half; t += NT) {
+        const int tr = t / half;
+        double turns = (double)a.pos[r0 + tr] * (double)a.freq[t - tr * half] * 0.15915494309189533577;
+        turns -= rint(turns);
+        float sn, cn;
+        sincospif(2.f * (float)turns, &sn, &cn);
+        cs[t] = make_float2(a.mscale * cn, a.mscale * sn);
+      }
+      __syncthreads();
+      ready = true;
+    }
+    if (a.nw) {
+      float ss = 0.f;
+#pragma unroll
+      for (int u = 0; u < PER; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) ss += p[u][0][v] * p[u][0][v] + p[u][1][v] * p[u][1][v];
+      const float inv = rsqrtf(head_sum(ss, L) / (float)a.d + a.eps);
+#pragma unroll
+      for (int u = 0; u < PER; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[u][0][v] *= inv * nw[u][0][v], p[u][1][v] *= inv * nw[u][1][v];
+    }
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int k = l + L * u;
+      if (e0[u] >= a.d) continue;
+      if (k < turned) {
+        const float2* c = cs + rl * half + V * k;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          // in pairs the 2 V elements are a, b, a, b, ..
+          float& x0 = a.pairs && V > 1 ? (v < V / 2 ? p[u][0][(2 * v) % V] : p[u][1][(2 * v) % V]) : p[u][0][v];
+          float& x1 = a.pairs && V > 1 ? (v < V / 2 ? p[u][0][(2 * v + 1) % V] : p[u][1][(2 * v + 1) % V]) : p[u][1][v];
+          const float2 t = c[v];
+          const float x = x0 * t.x - x1 * t.y, y = x1 * t.x + x0 * t.y;
+          x0 = x, x1 = y;
+        }
+      }
+      st_y<V>(a, r, h * a.d + e0[u], p[u][0]);
+      if (e1[u] < a.d) st_y<V>(a, r, h * a.d + e1[u], p[u][1]);
+    }
+  }
+}
+
+template <bool B16>
+int rope(const Rope& a, int ldx, int hsx, int ldn, int ldy, int ldb, hipStream_t st) {
+  const long long n = (long long)a.heads * a.d;
+  if (a.rows < 0 || a.heads < 1 || a.heads > 4096 || a.d < 1 || a.d > 512 || a.rot < 0 || a.rot > a.d || a.rot % 2 || a.pairs < 0 || a.pairs > 1) return -1;
+  if (hsx < a.d || ldx < (long long)(a.heads - 1) * hsx + a.d || (a.nw && ldn != 0 && ldn < a.d) || (!a.y && !a.yb) || (a.y && ldy < n) ||
+      (a.yb && ldb < n) || (a.rot && (!a.pos || !a.freq)) || !a.x)
+    return -1;
+  if (a.rows == 0) return 0;
+  auto al = [](const void* p, uintptr_t m) { return ((uintptr_t)p & (m - 1)) == 0; };
+  const bool vec = a.d % 4 == 0 && a.rot % 8 == 0 && al(a.x, B16 ? 8 : 16) && ldx % 4 == 0 && hsx % 4 == 0 && al(a.nw, 16) && ldn % 4 == 0 &&
+                   (!a.y || (al(a.y, 16) && ldy % 4 == 0)) && (!a.yb || (al(a.yb, 8) && ldb % 4 == 0));
+  const int V = vec ? 4 : 1, units = (a.rot >> 1) / V + (a.d - a.rot + 2 * V - 1) / (2 * V);
+  int L = 1;
+  while (L < units && L < WAVE) L <<= 1;
+  const int per_row = a.heads * L, RB = per_row >= NT ? 1 : NT / per_row;
+  const dim3 g((unsigned)(((long long)a.rows + RB - 1) / RB)), b(NT);
+  const size_t lds = (size_t)RB * (a.rot >> 1) * sizeof(float2);
+  if (vec) hipLaunchKernelGGL((k_rope<B16, 4, 1>), g, b, lds, st, a, L, RB);
+  else if (units <= L) hipLaunchKernelGGL((k_rope<B16, 1, 1>), g, b, lds, st, a, L, RB);
+  else hipLaunchKernelGGL((k_rope<B16, 1, 4>), g, b, lds, st, a, L, RB);
+  return 0;
+}
+
+Rope rope_args(const void* x, int ldx, int hsx, const float* nw, int ldn, float eps, const int* pos, const float* freq, float mscale, int pairs,
+               float* y, int ldy, uint16_t* yb, int ldb, int rows, int heads, int d, int rot) {
+  auto ld = [](int v) { return v < 0 ? (size_t)0 : (size_t)v; };
+  return Rope{x, nw, pos, freq, y, yb, ld(ldx), ld(hsx), ld(ldn), ld(ldy), ld(ldb), eps, mscale, rows, heads, d, rot, pairs};
+}
+
+}  // namespace
+
+API int dr_rope(const float* x, int ldx, int hsx, const float* nw, int ldn, float eps, const int* pos, const float* freq, float mscale, int layout,
+                float* y, int ldy, uint16_t* yb, int ldb, int rows, int heads, int d, int rot, hipStream_t st) {
+  return rope<false>(rope_args(x, ldx, hsx, nw, ldn, eps, pos, freq, mscale, layout, y, ldy, yb, ldb, rows, heads, d, rot), ldx, hsx, ldn, ldy, ldb, st);
+}
+
+API int dr_rope_bf16(const uint16_t* x, int ldx, int hsx, const float* nw, int ldn, float eps, const int* pos, const float* freq, float mscale, int layout,
+                     float* y, int ldy, uint16_t* yb, int ldb, int rows, int heads, int d, int rot, hipStream_t st) {
+  return rope<true>(rope_args(x, ldx, hsx, nw, ldn, eps, pos, freq, mscale, layout, y, ldy, yb, ldb, rows, heads, d, rot), ldx, hsx, ldn, ldy, ldb, st);
+}

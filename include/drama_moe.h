@@ -461,6 +461,79 @@ int dr_moe_layer_rows_fp8_bf16s(const dr_bf16* router, const uint8_t* gu_w, cons
                                 dr_stream_t st);
 
 /* ===================================================================================== */
+/* Between an attention block's projections, for one sequence or many -- no reference     */
+/* counterpart of this form (the reference keeps a bf16 cache of one sequence)            */
+/* ===================================================================================== */
+
+/* layout of the rotated pairs */
+#define DR_ROPE_HALF 0  /* element j with element j + rot / 2 */
+#define DR_ROPE_PAIRS 1 /* element 2 j with element 2 j + 1 */
+
+/* The norm of each head and its rotary positions, per row and head:
+ *   n = x * rsqrt(mean(x^2) + eps) * nw            (over the head's d elements; nw NULL: n = x)
+ *   th = pos[row] * freq[j], c = mscale * cos(th), s = mscale * sin(th), j < rot / 2
+ *   the pair (a, b) of n -> (a c - b s, b c + a s); elements from rot on stay n.
+ * x f32 (dr_rope) or bf16 (dr_rope_bf16): head h of row r starts r * ldx + h * hsx elements in (hsx = 2 d where each head's gate
+ * lies beside it).  nw f32, head h at h * ldn (ldn 0: one for all heads; heads of q and k in one call have a row each).
+ * pos i32 [rows]; freq f32 [rot / 2], radians per position, scaled for long contexts as the model asks (rope_freq of
+ * drama-rs_amd/kvcache.py); both may be NULL where rot is 0.  y f32 and yb bf16: either may be NULL; head h of row r at r * ldy (ldb) + h * d.
+ * y may be an f32 x, and yb a bf16 x, at the same strides with hsx = d.  Angles are formed in 64 bits, all else in fp32.  16-byte addresses
+ * and strides of whole 16 bytes (8 for bf16) with d a multiple of 4 and rot of 8 take the wide path; any others work.
+ * Unsupported: rows < 0, heads < 1 or > 4096, d < 1 or > 512, rot odd, < 0 or > d, an unknown layout, a missing x, neither y nor
+ * yb, rot without pos or freq, hsx < d, rows that overlap (ldx < (heads - 1) hsx + d; ldy, ldb < heads d), ldn between 1 and d - 1 or
+ * negative -> -1.  rows == 0 does nothing. */
+int dr_rope(const float* x, int ldx, int hsx, const float* nw, int ldn, float eps, const int* pos, const float* freq, float mscale,
+            int layout, float* y, int ldy, dr_bf16* yb, int ldb, int rows, int heads, int d, int rot, dr_stream_t st);
+int dr_rope_bf16(const dr_bf16* x, int ldx, int hsx, const float* nw, int ldn, float eps, const int* pos, const float* freq,
+                 float mscale, int layout, float* y, int ldy, dr_bf16* yb, int ldb, int rows, int heads, int d, int rot, dr_stream_t st);
+
+/* tokens of a cached block */
+#define DR_KV8_BLOCK 64
+
+/* A cache of k and v in 8 bits: blocks of 64 tokens of one sequence, one f32 scale for each block, head and k or v, any page of the cache
+ * for any block.  Buffers of one layer, all the caller's:
+ *   kq u8 [pages, hkv, d / 16, 64, 16]: element 16 c + e of the block's token t at [.., c, t, e];
+ *   vq u8 [pages, hkv, d, 64]: token 16 a + 4 b + c of element x at [.., x, 16 b + 4 a + c];  both hold q + 128, -127 <= q <= 127;
+ *   ks, vs f32 [pages, hkv]: an element is q * scale.
+ * table i32 [seqs, maxp] names the page of each block of a sequence: block b holds tokens 64 b .. 64 b + 63.  An entry outside 0 .. pages - 1
+ * (or a token past 64 maxp): that block is not there.  The same page may stand for several sequences as long as no call appends to it.
+ * start i32 [seqs + 1], ascending: rows start[i] .. start[i + 1] - 1 of a call belong to sequence i.  len i32 [seqs]: its tokens with
+ * those rows, so that its first row has position len[i] - (start[i + 1] - start[i]); a row of negative position is no token.  Rows before start[0] and
+ * from start[seqs] on belong to none: nothing of theirs is read or written.  All of these are read on the device.  kq and vq are multiples of 16 bytes.
+ *
+ * dr_kv8_append: the rows' k and v (f32, or bf16 for _bf16; head h of row r at r * ldk + h * d) become their tokens.  A block whose first
+ * token is in the call gets the scale fl(A / 127), A the largest magnitude of the call's tokens in it; one that holds tokens
+ * already keeps its scale, doubled as often as A > 127 scale asks, its integers then rounded to the new step (together less
+ * than one step off, however often that happens).  Integers are round(x / scale), half to even, from the exact quotient.  An infinity or NaN gives the block, all its
+ * tokens, the scale NaN.  Appending the same rows again changes nothing.  Places of a block behind its last token hold nothing of use.
+ * dr_kv8_read: the reverse, k and v f32 of the rows' tokens (0 for a row that is none or whose block is not there).
+ * Unsupported: rows or seqs < 0 or > 1048576, hkv < 1 or > 1024, d < 16, > 256 or no multiple of 16, maxp < 1 or >= 33554432, pages < 1, ldk or ldv below hkv d or
+ * no multiple of 16 bytes, a missing buffer, one of k, v, kq, vq that is no multiple of 16 bytes -> -1.  No rows or no sequences: does nothing. */
+int dr_kv8_append(const float* k, int ldk, const float* v, int ldv, const int* start, const int* len, const int* table, int maxp,
+                  uint8_t* kq, float* ks, uint8_t* vq, float* vs, int pages, int rows, int seqs, int hkv, int d, dr_stream_t st);
+int dr_kv8_append_bf16(const dr_bf16* k, int ldk, const dr_bf16* v, int ldv, const int* start, const int* len, const int* table, int maxp,
+                       uint8_t* kq, float* ks, uint8_t* vq, float* vs, int pages, int rows, int seqs, int hkv, int d, dr_stream_t st);
+int dr_kv8_read(const int* start, const int* len, const int* table, int maxp, const uint8_t* kq, const float* ks, const uint8_t* vq,
+                const float* vs, int pages, float* k, int ldk, float* v, int ldv, int rows, int seqs, int hkv, int d, dr_stream_t st);
+
+/* Attention over that cache: a row at position p of its sequence sees tokens 0 .. p (its own among them: append first),
+ *   y = bf16(sigmoid(gate) * sum_t softmax_t(scale * q . k_t) v_t), queries h (hq / hkv) .. of cached head h.
+ * q bf16 and y bf16: query h of row r at r * ldq (ldy) + h * d; gate f32, NULL for none: at r * ldg + h * hsg.  y may be q at the same stride.  A row that
+ * sees no token (a negative position, blocks that are not there) gets zeros; rows of no sequence are left as they were.  A query
+ * with an infinity or NaN, or a block of scale NaN among what it sees, gives NaN to that row's query alone.
+ * max_rows: no sequence has more rows (rows past it are not computed); max_len: the longest sequence, as far as the host knows it (a longer one
+ * is computed as well).  The cut into blocks goes by these, so a graph that is replayed for growing sequences takes their final values.
+ * Scores, softmax and sums are fp32; weights enter the product with v in fp16 (2^-11 of each).
+ * ws: dr_attn_kv8_ws(same sizes) bytes of scratch, holding anything, a multiple of 16 bytes.  Calls that share ws must not overlap (two graphs that may run at once need one each).
+ * Unsupported: as above, and hq > 1024 or no multiple of hkv, max_rows or max_len < 0, ldq < hq d or no multiple of 8, ldy < hq d or
+ * no multiple of 4, hsg < d, ldg < (hq - 1) hsg + d, either no multiple of 4, a missing q, y or ws, q, gate or ws no multiple of 16 bytes, y none of 8 -> -1 (ws size: 0). */
+size_t dr_attn_kv8_ws(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d);
+int dr_attn_kv8(const dr_bf16* q, int ldq, const int* start, const int* len, const int* table, int maxp, const uint8_t* kq,
+                const float* ks, const uint8_t* vq, const float* vs, int pages, float scale, const float* gate, int ldg, int hsg,
+                void* ws, dr_bf16* y, int ldy, int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d,
+                dr_stream_t st);
+
+/* ===================================================================================== */
 /* Fused multi-layer decode step (persistent kernel) -- no single reference symbol: it    */
 /* replaces the per-layer chain dr_router_topk + dr_moe_decode that src/engine.rs:1001-   */
 /* 1007 records for every MoE layer of a decode step (src/ffi.rs:41-46).                  */
