@@ -11,9 +11,9 @@
 // are fp32; a block's k scale multiplies its scores, its v scale joins the exponent, relative to a
 // power of two that no scale so far exceeds (a row's bits then do not turn on the scale of a block that it does not see).
 //
-// A wave walks over cached blocks by itself: no barrier, k of the next block requested as soon as this one's is used, v likewise.  Few columns:
-// the four waves of a block of threads take every fourth cached block, their sums meet in LDS.  Where that leaves CUs idle the
-// cached blocks are split over `splits` blocks of threads, whose sums (fp32) a second launch joins.
+// Two kernels.  Few columns (a decode step): a wave walks over cached blocks by itself with no barrier, the next block's bytes requested as soon
+// as this one's are used.  Many (prompts): a block's bytes are converted once for all waves, in LDS.  Where the columns alone leave CUs
+// idle the cached blocks are split over blocks of threads, whose sums (fp32) a second launch joins.
 #include "kv8.hpp"
 
 using namespace drm;
@@ -35,7 +35,7 @@ struct Attn {
   float *part, *ml;  // [splits, rows, hq, d] and [splits, rows, hq, 2]
   size_t ldq, ldg, hsg, ldy;
   float scale;
-  int hq, g, splits, scan;
+  int hq, g, splits, chunk, scan;
 };
 
 DEV half8 to_half8(uint32_t a, uint32_t b) {
@@ -79,54 +79,35 @@ DEV void emit(const Attn& a, int split, size_t row, int head, int e, const f32x4
   *reinterpret_cast<uint2*>(a.y + row * a.ldy + (size_t)head * d + e) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
 }
 
-// DC: 64-element chunks of a head (the last may be part of one: what lies past d is loaded from inside the head, times zero queries, and
-// not stored).  MT: tiles of 16 columns a wave.  WQ: waves along the columns, the other W / WQ along the cached blocks.
-template <int DC, int MT, int WQ, int OCC>
-__global__ void __launch_bounds__(NT, OCC) k_attn_kv8(Attn a) {
-  constexpr int WK = W / WQ, TP = 16 * MT * WQ, LD = 64 * DC + 4;
-  __shared__ __align__(16) float sm[WK > 1 ? W * 16 * LD : 4];
-  __shared__ float sml[WK > 1 ? W * 32 : 2];
-  const int l = lane_id(), j = l >> 4, wv = wave_id(), wq = WQ > 1 ? wv : 0, wk = WQ > 1 ? 0 : wv;
-  const int h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
-  int at = blockIdx.x, i = at;
-  if (a.scan) i = find_item(a.c, at, [g](const Seq& s) { return (s.n * g + TP - 1) / TP; });
-  else at = 0;
-  if (i < 0) return;
-  const Seq s = seq_of(a.c, i);
-  const int np = s.n * g, c0 = at * TP + wq * 16 * MT;
-  if (c0 >= np) return;  // no rows; with waves along the columns there is no barrier behind this
-  const int c1 = c0 + 16 * MT < np ? c0 + 16 * MT : np;
-  const long long cap = (long long)a.c.maxp * KB - 1;
-  const int p_lo = s.first + c0 / g, p_end = s.first + (c1 - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
-  // cached blocks of this wave: b0 + wk, b0 + wk + WK .. below b1
-  const int nb = p_hi < 0 ? 0 : (p_hi >> 6) + 1, each = (nb + a.splits - 1) / a.splits, chunk = each < WK ? WK : each;
-  const int b0 = sp * chunk < nb ? sp * chunk : nb, b1 = b0 + chunk < nb ? b0 + chunk : nb;
-  if (a.splits > 1 && b0 == b1 && sp > 0) {
-    for (int p = c0 + (WQ > 1 ? l : (int)threadIdx.x); p < c1; p += WQ > 1 ? WAVE : NT) {
-      const size_t r = ((size_t)sp * a.c.rows + s.r0 + p / g) * a.hq + h * g + p % g;
-      a.ml[2 * r] = -kInf, a.ml[2 * r + 1] = 0.f;
-    }
-    return;
-  }
+// A wave's columns: MT tiles of 16, lane l holds column l & 15 of each.  DC: 64-element chunks of a head.
+template <int DC, int MT>
+struct Cols {
+  half8 q[MT][DC][2];      // elements 64 c + 16 (l >> 4) + 8 x + (0 .. 7), times a power of two
+  f32x4 o[MT][4 * DC];     // O^T, elements 16 u + 4 (l >> 4) + (0 .. 3), over 2^(unit - 15)
+  float m[MT], sum[MT], qm[MT];  // maximum of the log2 scores, the lane's share of the sum, log2 score of a unit of S and of k's scale
+  int pos[MT];             // the columns' positions, -1 where there is none
+  int unit;                // 2^unit: a power of two not below any v scale so far
+};
 
-  // the columns' queries in fp16 (see above), their positions, the running maximum and sum
-  half8 q[MT][DC][2];
-  f32x4 o[MT][4 * DC];
-  float m[MT], sum[MT], qm[MT];
-  int pos[MT], unit = -200;  // o holds the sums over 2^unit, a power of two not below any v scale so far
+// Columns c0 .. of the np pairs (row, query) of sequence s and cached head h.
+template <int DC, int MT>
+DEV void begin(Cols<DC, MT>& w, const Attn& a, const Seq& s, int h, int c0, int np) {
+  const int l = lane_id(), j = l >> 4, d = a.c.d, g = a.g;
+  const long long cap = (long long)a.c.maxp * KB - 1;
+  w.unit = -200;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int p = c0 + 16 * t + (l & 15), row = p / g;
     const bool on = p < np;
     const uint16_t* src = a.q + (size_t)(s.r0 + row) * a.ldq + (size_t)(h * g + p - row * g) * d;
-    uint4 w[DC][2];
+    uint4 r[DC][2];
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int e = 64 * c + 16 * j + 8 * x;
-        w[c][x] = make_uint4(0, 0, 0, 0);
-        if (on && e < d) w[c][x] = ld16(src + e);
+        r[c][x] = make_uint4(0, 0, 0, 0);
+        if (on && e < d) r[c][x] = ld16(src + e);
       }
     float top = 0.f;
     bool num = true;
@@ -134,7 +115,7 @@ __global__ void __launch_bounds__(NT, OCC) k_attn_kv8(Attn a) {
     for (int c = 0; c < DC; ++c)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t v[4] = {w[c][x].x, w[c][x].y, w[c][x].z, w[c][x].w};
+        const uint32_t v[4] = {r[c][x].x, r[c][x].y, r[c][x].z, r[c][x].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float lo = fabsf(bf16_lo(v[k])), hi = fabsf(bf16_hi(v[k]));
@@ -151,20 +132,117 @@ __global__ void __launch_bounds__(NT, OCC) k_attn_kv8(Attn a) {
     for (int c = 0; c < DC; ++c)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t v[4] = {w[c][x].x, w[c][x].y, w[c][x].z, w[c][x].w};
+        const uint32_t v[4] = {r[c][x].x, r[c][x].y, r[c][x].z, r[c][x].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          q[t][c][x][2 * k] = (_Float16)(sign * __builtin_ldexpf(bf16_lo(v[k]), e));
-          q[t][c][x][2 * k + 1] = (_Float16)(sign * __builtin_ldexpf(bf16_hi(v[k]), e));
+          w.q[t][c][x][2 * k] = (_Float16)(sign * __builtin_ldexpf(bf16_lo(v[k]), e));
+          w.q[t][c][x][2 * k + 1] = (_Float16)(sign * __builtin_ldexpf(bf16_hi(v[k]), e));
         }
       }
-    qm[t] = __builtin_ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
+    w.qm[t] = __builtin_ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
     const int ps = s.first + row;
-    pos[t] = on ? (ps < cap ? ps : (int)cap) : -1;
-    m[t] = -kInf, sum[t] = 0.f;
+    w.pos[t] = on ? (ps < cap ? ps : (int)cap) : -1;
+    w.m[t] = -kInf, w.sum[t] = 0.f;
 #pragma unroll
-    for (int u = 0; u < 4 * DC; ++u) o[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < 4 * DC; ++u) w.o[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+}
+
+// One step of the softmax: the scores sc of a block (k scale ks, v scale vs, its first place at position b0) become fp16 weights.
+// EDGE: not every column sees every place; `there`: the block is in the cache.
+template <bool EDGE, int DC, int MT>
+DEV void soften(Cols<DC, MT>& w, const f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], float ks, float vs, int b0, bool there) {
+  const int j = lane_id() >> 4;
+  // v's scale enters relative to 2^unit; a block whose scale is no number leaves none to the columns that see it
+  const bool vnum = vs >= 0.f && vs < kInf;
+  const int ve = vnum && vs > 0.f ? __builtin_amdgcn_frexp_expf(vs) : -200, unew = w.unit > ve ? w.unit : ve;
+  const float ratio = vnum ? fmaxf(__builtin_ldexpf(vs, -unew), 0x1p-40f) : 0x1p-40f, shrink = __builtin_ldexpf(1.f, w.unit - unew);
+  const float lw = 15.f + __builtin_amdgcn_logf(ratio), iw = 1.f / ratio;
+#pragma unroll
+  for (int x = 0; x < MT; ++x) {
+    const int lim = there ? w.pos[x] - b0 : -1;  // places up to here are seen
+    const float f = w.qm[x] * ks;
+    float mx = -kInf;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, EDGE && 16 * t + 4 * j + e > lim ? -kInf : sc[x][t][e]);
+    mx = quad_max(mx);
+    const float mnew = fmaxf(w.m[x], mx * f), ms = mnew == -kInf ? 0.f : mnew;
+    if (__any(mnew > w.m[x]) || unew > w.unit) {
+      const float al = __builtin_amdgcn_exp2f(w.m[x] - ms), ao = al * shrink;
+      w.sum[x] *= al;
+#pragma unroll
+      for (int u = 0; u < 4 * DC; ++u) w.o[x][u] *= ao;
+      w.m[x] = mnew;
+    }
+    if (!vnum && lim >= 0) w.sum[x] = __builtin_nanf("");
+    const float base = lw - ms;
+    float add = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][t][e], f, base));
+        if (EDGE && 16 * t + 4 * j + e > lim) v = 0.f;
+        add += v;
+        pf[x][t >> 1][4 * (t & 1) + e] = (_Float16)v;
+      }
+    w.sum[x] += add * iw;
+  }
+  w.unit = unew;
+}
+
+// Pages and scales of up to 64 blocks of a sequence, a lane each.
+struct Pages {
+  int page;
+  float ks, vs;
+  unsigned long long have;
+  DEV void fetch(const Attn& a, int seq, int h, int block, bool on) {
+    const int p = on ? page_of(a.c, seq, block) : -1;
+    have = __ballot(p >= 0);
+    page = p >= 0 ? p : 0;
+    ks = vs = 0.f;
+    if (on) ks = a.c.ks[(size_t)page * a.c.hkv + h], vs = a.c.vs[(size_t)page * a.c.hkv + h];
+  }
+  DEV int at(int k) const { return __builtin_amdgcn_readlane(page, k); }
+  DEV float k_scale(int k) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), k)); }
+  DEV float v_scale(int k) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), k)); }
+};
+
+// The blocks [b0, b1) of a sequence that split sp takes of the nb blocks that its columns see.
+DEV void share(const Attn& a, int nb, int sp, int& b0, int& b1) {
+  const int each = (nb + a.splits - 1) / a.splits, n = each > a.chunk ? each : a.chunk;
+  b0 = sp * n < nb ? sp * n : nb, b1 = b0 + n < nb ? b0 + n : nb;
+}
+
+// A split without blocks leaves word of that for its columns [c0, c1).
+DEV void emit_none(const Attn& a, const Seq& s, int h, int sp, int c0, int c1, int t, int nt) {
+  for (int p = c0 + t; p < c1; p += nt) {
+    const size_t r = ((size_t)sp * a.c.rows + s.r0 + p / a.g) * a.hq + h * a.g + p % a.g;
+    a.ml[2 * r] = -kInf, a.ml[2 * r + 1] = 0.f;
+  }
+}
+
+// Few columns: the four waves of a block of threads hold the same MT tiles of them and take every fourth cached block.  The last chunk of a
+// head may be part of one: what lies past d is loaded from inside the head, times zero queries, and not stored.
+template <int DC, int MT>
+__global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
+  constexpr int TP = 16 * MT, LD = 64 * DC + 4;
+  __shared__ __align__(16) float sm[W * 16 * LD];
+  __shared__ float sml[W * 32];
+  const int l = lane_id(), j = l >> 4, wv = wave_id();
+  const int i = blockIdx.x, h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
+  const Seq s = seq_of(a.c, i);
+  const int np = s.n * g < TP ? s.n * g : TP;
+  if (np == 0) return;
+  const long long cap = (long long)a.c.maxp * KB - 1;
+  const int p_lo = s.first, p_end = s.first + (np - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
+  const int nb = p_hi < 0 ? 0 : (p_hi >> 6) + 1;
+  int b0, b1;
+  share(a, nb, sp, b0, b1);
+  if (b0 == b1 && sp > 0) return emit_none(a, s, h, sp, 0, np, threadIdx.x, NT);
+  const int cnt = (b1 - b0 - wv + W - 1) / W;  // the wave's blocks b0 + wv, b0 + wv + W ..
 
   int koff[DC];
 #pragma unroll
@@ -184,27 +262,20 @@ __global__ void __launch_bounds__(NT, OCC) k_attn_kv8(Attn a) {
     for (int u = 0; u < 4 * DC; ++u) vr[u] = ld16(p + voff + 16 * KB * (u < d16 ? u : d16 - 1));
   };
 
-  const int cnt = (b1 - b0 - wk + WK - 1) / WK;  // 0 where b0 + wk >= b1
+  Pages pg;
+  Cols<DC, MT> w;
+  // the first block's bytes are on their way while the queries arrive
+  pg.fetch(a, i, h, b0 + wv + W * l, l < cnt);
+  if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
+  begin(w, a, s, h, 0, np);
   for (int k0 = 0; k0 < cnt; k0 += WAVE) {
-    // pages and scales of the next 64 of the wave's blocks, a lane each
     const int n = cnt - k0 < WAVE ? cnt - k0 : WAVE;
-    int pg = 0;
-    float sk = 0.f, sv = 0.f;
-    bool there = false;
-    if (l < n) {
-      const int t = page_of(a.c, i, b0 + wk + WK * (k0 + l));
-      there = t >= 0;
-      pg = there ? t : 0;
-      sk = a.c.ks[(size_t)pg * a.c.hkv + h], sv = a.c.vs[(size_t)pg * a.c.hkv + h];
+    if (k0) {
+      pg.fetch(a, i, h, b0 + wv + W * (k0 + l), l < n);
+      load_k(pg.at(0)), load_v(pg.at(0));
     }
-    const unsigned long long have = __ballot(there);
-    load_k(__builtin_amdgcn_readlane(pg, 0));
-    load_v(__builtin_amdgcn_readlane(pg, 0));
     for (int k = 0; k < n; ++k) {
-      const int b = b0 + wk + WK * (k0 + k), nx = __builtin_amdgcn_readlane(pg, k + 1 < n ? k + 1 : k);
-      const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sk), k));
-      const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sv), k));
-      const bool exists = (have >> k) & 1;
+      const int b = b0 + wv + W * (k0 + k), nx = pg.at(k + 1 < n ? k + 1 : k);
       f32x4 sc[MT][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -212,163 +283,242 @@ __global__ void __launch_bounds__(NT, OCC) k_attn_kv8(Attn a) {
         for (int x = 0; x < MT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
-          const half8 k8a = to_half8(kr[c][t].x, kr[c][t].y), k8b = to_half8(kr[c][t].z, kr[c][t].w);
+          const half8 ka = to_half8(kr[c][t].x, kr[c][t].y), kb = to_half8(kr[c][t].z, kr[c][t].w);
 #pragma unroll
-          for (int x = 0; x < MT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8a, q[x][c][0], sc[x][t], 0, 0, 0);
+          for (int x = 0; x < MT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, w.q[x][c][0], sc[x][t], 0, 0, 0);
 #pragma unroll
-          for (int x = 0; x < MT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8b, q[x][c][1], sc[x][t], 0, 0, 0);
+          for (int x = 0; x < MT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, w.q[x][c][1], sc[x][t], 0, 0, 0);
         }
       }
       if (k + 1 < n) load_k(nx);
-
-      // v's scale enters relative to `unit`; a block whose scale is no number leaves none to the rows that see it
-      const bool vnum = vs >= 0.f && vs < kInf;
-      const int ve = vnum && vs > 0.f ? __builtin_amdgcn_frexp_expf(vs) : -200, unew = unit > ve ? unit : ve;
-      const float ratio = vnum ? fmaxf(__builtin_ldexpf(vs, -unew), 0x1p-40f) : 0x1p-40f, ushrink = __builtin_ldexpf(1.f, unit - unew);
-      const float lw = 15.f + __builtin_amdgcn_logf(ratio), iw = 1.f / ratio;
-      const bool edge = !exists || b * KB + KB - 1 > p_lo;
+      const bool there = (pg.have >> k) & 1;
       half8 pf[MT][2];
-#pragma unroll
-      for (int x = 0; x < MT; ++x) {
-        // places t <= lim of the block are seen by the lane's column
-        const int lim = exists ? pos[x] - b * KB : -1;
-        const float f = qm[x] * ks;
-        float mx = -kInf;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float z = edge && 16 * t + 4 * j + e > lim ? -kInf : sc[x][t][e];
-            mx = fmaxf(mx, z);
-          }
-        mx = quad_max(mx);
-        const float mnew = fmaxf(m[x], mx * f), ms = mnew == -kInf ? 0.f : mnew;
-        if (__any(mnew > m[x]) || unew > unit) {
-          const float al = __builtin_amdgcn_exp2f(m[x] - ms), ao = al * ushrink;
-          sum[x] *= al;
-#pragma unroll
-          for (int u = 0; u < 4 * DC; ++u) o[x][u] *= ao;
-          m[x] = mnew;
-        }
-        if (!vnum && lim >= 0) sum[x] = __builtin_nanf("");
-        float add = 0.f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][t][e], f, lw - ms));
-            if (edge && 16 * t + 4 * j + e > lim) w = 0.f;
-            add += w;
-            pf[x][t >> 1][4 * (t & 1) + e] = (_Float16)w;
-          }
-        sum[x] += add * iw;
-      }
-      unit = unew;
+      if (!there || b * KB + KB - 1 > p_lo) soften<true>(w, sc, pf, pg.k_scale(k), pg.v_scale(k), b * KB, there);
+      else soften<false>(w, sc, pf, pg.k_scale(k), pg.v_scale(k), b * KB, true);
 #pragma unroll
       for (int u = 0; u < 4 * DC; ++u) {
-        const half8 v8a = to_half8(vr[u].x, vr[u].y), v8b = to_half8(vr[u].z, vr[u].w);
+        const half8 va = to_half8(vr[u].x, vr[u].y), vb = to_half8(vr[u].z, vr[u].w);
 #pragma unroll
-        for (int x = 0; x < MT; ++x) o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8a, pf[x][0], o[x][u], 0, 0, 0);
+        for (int x = 0; x < MT; ++x) w.o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[x][0], w.o[x][u], 0, 0, 0);
 #pragma unroll
-        for (int x = 0; x < MT; ++x) o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8b, pf[x][1], o[x][u], 0, 0, 0);
+        for (int x = 0; x < MT; ++x) w.o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, pf[x][1], w.o[x][u], 0, 0, 0);
       }
       if (k + 1 < n) load_v(nx);
     }
   }
 
+  // the waves' sums joined in LDS, both less 2^16 so that a v scale next to fp32's largest does not leave it
+  const float us = __builtin_ldexpf(1.f, w.unit - 16);
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
-    // both sums less 2^16, so that a v scale next to fp32's largest does not leave it
-    const float us = __builtin_ldexpf(1.f, unit - 16);
-    sum[x] = quad_sum(sum[x]) * 0x1p-16f;
-    if constexpr (WK == 1) {
-      const int p = c0 + 16 * x + (l & 15), row = p / g;
-      if (p < np)
+    w.sum[x] = quad_sum(w.sum[x]) * 0x1p-16f;
+    if (x) __syncthreads();
+    if (j == 0) sml[wv * 32 + 2 * l] = w.m[x], sml[wv * 32 + 2 * l + 1] = w.sum[x];
 #pragma unroll
-        for (int u = 0; u < 4 * DC; ++u)
-          if (u < d16) emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, 16 * u + 4 * j, o[x][u] * us, sum[x], m[x]);
-    } else {
-      if (x) __syncthreads();
-      if (j == 0) sml[wv * 32 + 2 * l] = m[x], sml[wv * 32 + 2 * l + 1] = sum[x];
+    for (int u = 0; u < 4 * DC; ++u) *reinterpret_cast<f32x4*>(sm + (wv * 16 + (l & 15)) * LD + 16 * u + 4 * j) = w.o[x][u] * us;
+    __syncthreads();
+    const int col = threadIdx.x >> 4, p = 16 * x + col, row = p / g;
+    float wt[W], mm = -kInf, ll = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4 * DC; ++u) *reinterpret_cast<f32x4*>(sm + (wv * 16 + (l & 15)) * LD + 16 * u + 4 * j) = o[x][u] * us;
-      __syncthreads();
-      const int col = threadIdx.x >> 4, p = c0 + 16 * x + col, row = p / g;
-      float wt[W], mm = -kInf, ll = 0.f;
+    for (int v = 0; v < W; ++v) mm = fmaxf(mm, sml[v * 32 + 2 * col]);
 #pragma unroll
-      for (int w = 0; w < W; ++w) mm = fmaxf(mm, sml[w * 32 + 2 * col]);
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        wt[w] = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(sml[w * 32 + 2 * col] - mm);
-        ll += wt[w] * sml[w * 32 + 2 * col + 1];
-      }
-      if (p < np)
-        for (int e = 4 * (threadIdx.x & 15); e < d; e += 64) {
-          f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < W; ++w) v += wt[w] * *reinterpret_cast<const f32x4*>(sm + (w * 16 + col) * LD + e);
-          emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, e, v, ll, mm);
-        }
+    for (int v = 0; v < W; ++v) {
+      wt[v] = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(sml[v * 32 + 2 * col] - mm);
+      ll += wt[v] * sml[v * 32 + 2 * col + 1];
     }
+    if (p < np)
+      for (int e = 4 * (threadIdx.x & 15); e < d; e += 64) {
+        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int z = 0; z < W; ++z) v += wt[z] * *reinterpret_cast<const f32x4*>(sm + (z * 16 + col) * LD + e);
+        emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, e, v, ll, mm);
+      }
   }
 }
 
-// Joins the parts of a row's query: a block of threads each, groups of LE lanes (LE 4 >= d) take every NT / LE'th part.
-__global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
-  __shared__ __align__(16) float sm[NT * 4];
-  __shared__ float red[2 * W];
-  const int head = blockIdx.x % a.hq, row = blockIdx.x / a.hq, s0 = a.c.start[0], s1 = a.c.start[a.c.seqs];
-  if (row < s0 || row >= s1) return;
-  const int l = threadIdx.x & (LE - 1), grp = threadIdx.x / LE, n = NT / LE, d = a.c.d;
+// Many columns: each of the NW waves holds MT tiles of its own, and all go through the cached blocks together.  A block is loaded once for
+// all of them (a 1 / NW of it a wave, two blocks ahead), becomes fp16 once, and lies in LDS as the operands are read: 1 KB a fragment, lane by
+// lane, so neither the writes nor the reads of 16 bytes meet in a bank.  Two buffers, one barrier a block.
+template <int DC, int MT, int NW>
+__global__ void __launch_bounds__(64 * NW, NW / 4) k_attn_tiles(Attn a) {
+  constexpr int TP = 16 * MT * NW, F = 4 * DC, PER = (F + NW - 1) / NW;  // F: 16-byte loads a lane of k, and of v, for one block
+  __shared__ __align__(16) half8 lds[2 * 4 * F * WAVE];                  // [2][k, v][F][2][64]
+  const int l = lane_id(), j = l >> 4, wv = wave_id();
+  const int h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
+  int at = gridDim.x - 1 - blockIdx.x, i = at;  // the last rows, which see most, first
+  if (a.scan) i = find_item(a.c, at, [g](const Seq& s) { return (s.n * g + TP - 1) / TP; });
+  else at = 0;
+  if (i < 0) return;
+  const Seq s = seq_of(a.c, i);
+  const int np = a.scan || s.n * g < TP ? s.n * g : TP, c0 = at * TP, c1 = c0 + TP < np ? c0 + TP : np;
+  if (c0 >= np) return;
+  const long long cap = (long long)a.c.maxp * KB - 1;
+  const int p_end = s.first + (c1 - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
+  int b0, b1;
+  share(a, p_hi < 0 ? 0 : (p_hi >> 6) + 1, sp, b0, b1);
+  if (b0 == b1 && sp > 0) return emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);
+  // the wave's columns and the blocks that they see
+  const int w0 = c0 + 16 * MT * wv, w1 = w0 + 16 * MT < c1 ? w0 + 16 * MT : c1;
+  const int w_lo = s.first + w0 / g, w_end = s.first + (w1 - 1) / g, w_nb = w0 < c1 && w_end >= 0 ? (w_end >> 6) + 1 : 0;
+
+  int off[PER];  // of the wave's loads; v's differ by what follows
+#pragma unroll
+  for (int f = 0; f < PER; ++f) {
+    const int c = (wv * PER + f) >> 2, t = (wv * PER + f) & 3;
+    off[f] = ((4 * c + j < d16 ? 4 * c + j : d16 - 1) * KB + 16 * t + (l & 15)) * 16;
+  }
+  uint4 kr[PER], vr[PER];
+  auto load = [&](int page) {
+    const size_t base = ((size_t)page * a.c.hkv + h) * KB * d;
+#pragma unroll
+    for (int f = 0; f < PER; ++f) {
+      const int u = wv * PER + f;
+      if (F % NW && u >= F) break;
+      kr[f] = ld16(a.c.kq + base + off[f]);
+      vr[f] = ld16(a.c.vq + base + (16 * (u < d16 ? u : d16 - 1) + (l & 15)) * KB + 16 * j);
+    }
+  };
+  auto store = [&](int buf) {
+    half8* k = lds + buf * 4 * F * WAVE;
+#pragma unroll
+    for (int f = 0; f < PER; ++f) {
+      const int u = wv * PER + f;
+      if (F % NW && u >= F) break;
+      k[(2 * u) * WAVE + l] = to_half8(kr[f].x, kr[f].y), k[(2 * u + 1) * WAVE + l] = to_half8(kr[f].z, kr[f].w);
+      half8* v = k + 2 * F * WAVE;
+      v[(2 * u) * WAVE + l] = to_half8(vr[f].x, vr[f].y), v[(2 * u + 1) * WAVE + l] = to_half8(vr[f].z, vr[f].w);
+    }
+  };
+
+  Pages pg, px;  // of 64 blocks, and of the 64 behind them
+  Cols<DC, MT> w;
+  const int cnt = b1 - b0;
+  pg.fetch(a, i, h, b0 + l, l < cnt);
+  if (cnt > 0) load(pg.at(0));
+  px.fetch(a, i, h, b0 + WAVE + l, WAVE + l < cnt);
+  begin(w, a, s, h, w0, c1);
+  if (cnt > 0) store(0);
+  if (cnt > 1) load(pg.at(1));
+  for (int k = 0; k < cnt; ++k) {
+    const int kk = k & (WAVE - 1);
+    if (k && kk == 0) {
+      pg = px;
+      px.fetch(a, i, h, b0 + k + WAVE + l, k + WAVE + l < cnt);
+    }
+    __syncthreads();
+    if (k + 1 < cnt) store((k + 1) & 1);
+    if (k + 2 < cnt) load(kk + 2 < WAVE ? pg.at(kk + 2) : px.at(kk + 2 - WAVE));
+    const int b = b0 + k;
+    if (b >= w_nb) continue;  // later than all of the wave's columns
+    const half8* kf = lds + (k & 1) * 4 * F * WAVE + l;
+    const half8* vf = kf + 2 * F * WAVE;
+    f32x4 sc[MT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int x = 0; x < MT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const half8 ka = kf[(2 * (4 * c + t) + y) * WAVE];
+#pragma unroll
+          for (int x = 0; x < MT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, w.q[x][c][y], sc[x][t], 0, 0, 0);
+        }
+    const bool there = (pg.have >> kk) & 1;
+    half8 pf[MT][2];
+    if (!there || b * KB + KB - 1 > w_lo) soften<true>(w, sc, pf, pg.k_scale(kk), pg.v_scale(kk), b * KB, there);
+    else soften<false>(w, sc, pf, pg.k_scale(kk), pg.v_scale(kk), b * KB, true);
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int u = 0; u < 4 * DC; ++u) {
+        const half8 va = vf[(2 * u + y) * WAVE];
+#pragma unroll
+        for (int x = 0; x < MT; ++x) w.o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[x][y], w.o[x][u], 0, 0, 0);
+      }
+  }
+  const float us = __builtin_ldexpf(1.f, w.unit - 16);
+#pragma unroll
+  for (int x = 0; x < MT; ++x) {
+    const float sum = quad_sum(w.sum[x]) * 0x1p-16f;
+    const int p = w0 + 16 * x + (l & 15), row = p / g;
+    if (p < c1)
+#pragma unroll
+      for (int u = 0; u < 4 * DC; ++u)
+        if (u < d16) emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, 16 * u + 4 * j, w.o[x][u] * us, sum, w.m[x]);
+  }
+}
+
+// Joins the parts of 64 elements of a row's query: 16 groups of 16 lanes take every 16th part, all their loads together.
+constexpr int kSplits = 128;  // at most
+__global__ void __launch_bounds__(NT) k_attn_join(Attn a) {
+  __shared__ __align__(16) f32x4 sm[NT];
+  __shared__ float wt[kSplits], red[2 * W];
+  const int head = blockIdx.x % a.hq, row = blockIdx.x / a.hq;
+  if (row < a.c.start[0] || row >= a.c.start[a.c.seqs]) return;
+  const int t = threadIdx.x, grp = t >> 4, e = 64 * blockIdx.y + 4 * (t & 15), d = a.c.d;
   const size_t at = (size_t)row * a.hq + head, step = (size_t)a.c.rows * a.hq;
-  float m = -kInf;
-  if ((int)threadIdx.x < a.splits) m = a.ml[2 * (at + threadIdx.x * step)];
+  float m = -kInf, s = 0.f;
+  if (t < a.splits) m = a.ml[2 * (at + t * step)], s = a.ml[2 * (at + t * step) + 1];
   float mm = wave_max(m);
   if (lane_id() == 0) red[wave_id()] = mm;
   __syncthreads();
   mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float ms = mm == -kInf ? 0.f : mm;
-  float ls = 0.f;
-  if ((int)threadIdx.x < a.splits) ls = a.ml[2 * (at + threadIdx.x * step) + 1] * __builtin_amdgcn_exp2f(m == -kInf && mm == -kInf ? 0.f : m - ms);
-  ls = wave_sum(ls);
-  if (lane_id() == 0) red[W + wave_id()] = ls;
-  f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int sp = grp; sp < a.splits; sp += n) {
-    const size_t r = at + sp * step;
-    const float pm = a.ml[2 * r], pl = a.ml[2 * r + 1];
-    if (pl == 0.f || 4 * l >= d) continue;  // a part that saw no token has no sums
-    v += __builtin_amdgcn_exp2f(pm - ms) * *reinterpret_cast<const f32x4*>(a.part + r * d + 4 * l);
-  }
-  *reinterpret_cast<f32x4*>(sm + 4 * threadIdx.x) = v;
+  const float p = m == -kInf && mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - mm);
+  if (t < a.splits) wt[t] = s == 0.f ? 0.f : p;  // a part that saw no token has no sums
+  s = wave_sum(s * p);
+  if (lane_id() == 0) red[W + wave_id()] = s;
   __syncthreads();
-  if (grp == 0 && 4 * l < d) {
-    for (int t = 1; t < n; ++t) v += *reinterpret_cast<const f32x4*>(sm + 4 * (t * LE + l));
+  f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f}, r[kSplits / 16];
+#pragma unroll
+  for (int k = 0; k < kSplits / 16; ++k) {
+    const int sp = grp + 16 * k;
+    r[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (sp < a.splits && wt[sp] != 0.f && e < d) r[k] = *reinterpret_cast<const f32x4*>(a.part + (at + sp * step) * d + e);
+  }
+#pragma unroll
+  for (int k = 0; k < kSplits / 16; ++k)
+    if (grp + 16 * k < a.splits) v += wt[grp + 16 * k] * r[k];
+  sm[t] = v;
+  __syncthreads();
+  if (t < 16 && e < d) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) v += sm[16 * k + t];
     Attn o = a;
     o.splits = 1;
-    emit(o, 0, row, head, 4 * l, v, red[W] + red[W + 1] + red[W + 2] + red[W + 3], 0.f);
+    emit(o, 0, row, head, e, v, red[W] + red[W + 1] + red[W + 2] + red[W + 3], 0.f);
   }
 }
 
-// How a call is cut: from sizes alone, so that the workspace is known before.
+// How a call is cut: by its sizes alone, so that the workspace is known before.
 struct Plan {
-  int mt, wq, splits, scan;
+  bool few, scan;
+  int mt, nw, splits, chunk;
   long long tiles;
 };
 Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d) {
   Plan p;
-  const long long pairs = (long long)(max_rows < rows ? max_rows : rows) * (hq / hkv);
-  p.mt = pairs <= 16 || d > 128 ? 1 : 2;
-  p.wq = pairs <= 16 * p.mt ? 1 : W;
-  const long long tp = 16ll * p.mt * p.wq, per = (pairs + tp - 1) / tp;
-  p.scan = per > 1;
-  p.tiles = per > 1 ? (long long)rows * (hq / hkv) / tp + seqs : seqs;
-  if (per > 1 && p.tiles > per * seqs) p.tiles = per * seqs;
-  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv;
-  long long s = (1024 + units - 1) / units;
+  const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g;
+  p.few = pairs <= 16 || (d <= 128 && pairs <= 32);
+  p.mt = p.few ? (pairs <= 16 ? 1 : 2) : d <= 64 ? 3 : d <= 128 ? 2 : 1;
+  auto cut = [&](long long tp) {
+    const long long per = (pairs + tp - 1) / tp, all = rows * g / tp + seqs;
+    p.scan = per > 1, p.tiles = per > 1 && all < per * seqs ? all : per * seqs;
+  };
+  p.nw = p.few ? W : 8;
+  cut(p.few ? 16 * p.mt : 16 * p.mt * p.nw);
+  if (!p.few && p.tiles * hkv < 256) p.nw = 4, cut(16 * p.mt * p.nw);
+  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = p.few ? 2048 : 512;
+  long long s = units >= want / 2 && !p.few ? 1 : (want + units - 1) / units;
   const long long most = (blocks + W - 1) / W;
-  if (s > most) s = most;
-  if (s > 128) s = 128;
+  s = s > most ? most : s;
+  s = s > kSplits ? kSplits : s;
   p.splits = s < 1 || blocks <= 16 ? 1 : (int)s;
+  p.chunk = (int)((blocks + p.splits - 1) / p.splits);
+  if (p.chunk < W) p.chunk = W;
   return p;
 }
 
@@ -381,7 +531,7 @@ bool attn_shape_ok(int rows, int seqs, int max_rows, int max_len, int hq, int hk
 
 API size_t dr_attn_kv8_ws(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d) {
   if (!attn_shape_ok(rows, seqs, max_rows, max_len, hq, hkv, d)) return 0;
-  if (rows == 0 || seqs == 0) return 256;
+  if (rows == 0 || seqs == 0 || max_rows == 0) return 256;
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
   return p.splits > 1 ? ((size_t)p.splits * rows * hq * (d + 2) * sizeof(float) + 255) & ~(size_t)255 : 256;
 }
@@ -396,31 +546,31 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   if (rows == 0 || seqs == 0 || max_rows == 0) return 0;
   if (!kv8_buffers_ok(c) || !q || !y || !ws || ((uintptr_t)q & 15) || ((uintptr_t)y & 7) || ((uintptr_t)ws & 15)) return -1;
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
-  const size_t n = (size_t)p.splits * rows * hq;
   float* part = reinterpret_cast<float*>(ws);
-  const Attn a{c, q, gate, y, part, part + n * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0), (size_t)ldy, scale, hq, hq / hkv,
-               p.splits, p.scan};
+  const Attn a{c, q, gate, y, part, part + (size_t)p.splits * rows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
+               (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan};
   const dim3 grid((unsigned)p.tiles, hkv, p.splits);
-  auto go = [&](auto dc, auto mt, auto wq, auto occ) {
-    hipLaunchKernelGGL((k_attn_kv8<decltype(dc)::value, decltype(mt)::value, decltype(wq)::value, decltype(occ)::value>), grid, dim3(NT), 0, st, a);
+  auto few = [&](auto dc, auto mt) {
+    hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), grid, dim3(NT), 0, st, a);
+  };
+  auto tiles = [&](auto dc, auto mt) {
+    constexpr int DC = decltype(dc)::value, MT = decltype(mt)::value;
+    if (p.nw == 8) hipLaunchKernelGGL((k_attn_tiles<DC, MT, 8>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_tiles<DC, MT, 4>), grid, dim3(256), 0, st, a);
   };
   constexpr std::integral_constant<int, 1> i1{};
   constexpr std::integral_constant<int, 2> i2{};
   constexpr std::integral_constant<int, 3> i3{};
   constexpr std::integral_constant<int, 4> i4{};
-  auto one = [&](auto dc) { p.wq == 1 ? go(dc, i1, i1, i1) : go(dc, i1, i4, i1); };
-  auto two = [&](auto dc) {
-    if (p.mt == 1) go(dc, i1, i1, i1);
-    else p.wq == 1 ? go(dc, i2, i1, i1) : go(dc, i2, i4, i1);
-  };
-  if (d <= 64) two(i1);
-  else if (d <= 128) two(i2);
-  else if (d <= 192) one(i3);
-  else one(i4);
-  if (p.splits > 1) {
-    int le = 4;
-    while (4 * le < d) le <<= 1;
-    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(rows * hq)), dim3(NT), 0, st, a, le);
+  if (p.few) {
+    if (d <= 64) p.mt == 1 ? few(i1, i1) : few(i1, i2);
+    else if (d <= 128) p.mt == 1 ? few(i2, i1) : few(i2, i2);
+    else d <= 192 ? few(i3, i1) : few(i4, i1);
+  } else {
+    if (d <= 64) tiles(i1, i3);
+    else if (d <= 128) tiles(i2, i2);
+    else d <= 192 ? tiles(i3, i1) : tiles(i4, i1);
   }
+  if (p.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(rows * hq), (d + 63) / 64), dim3(NT), 0, st, a);
   return 0;
 }

@@ -107,6 +107,7 @@ class Lib:
                 raise DramaMoeError(f"{name} returned {rc}: {msg}")
             return rc
 
+        self.__dict__[name] = call  # the next access finds it without this function
         return call
 
 
