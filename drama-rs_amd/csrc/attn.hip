@@ -148,67 +148,96 @@ DEV void begin(Cols<DC, MT>& w, const Attn& a, const Seq& s, int h, int c0, int 
   }
 }
 
-// One step of the softmax: the scores sc of a block (k scale ks, v scale vs, its first place at position b0) become fp16 weights.
-// EDGE: not every column sees every place; `there`: the block is in the cache.
-template <bool EDGE, int DC, int MT>
-DEV void soften(Cols<DC, MT>& w, const f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], float ks, float vs, int b0, bool there) {
+// Pages and scales of up to 64 blocks of a sequence, a lane each.
+struct Pages {
+  int page, ve;          // v's scale is a fraction in [1/2, 1) times 2^ve,
+  float ks, lv, rv;      // the fraction's log2 and reciprocal
+  unsigned long long have, num;  // blocks in the cache; those whose scales are numbers
+  DEV void fetch(const Attn& a, int seq, int h, int block, bool on) {
+    const int p = on ? page_of(a.c, seq, block) : -1;
+    have = __ballot(p >= 0);
+    page = p >= 0 ? p : 0;
+    ks = 0.f;
+    float vs = 0.f;
+    if (on) ks = a.c.ks[(size_t)page * a.c.hkv + h], vs = a.c.vs[(size_t)page * a.c.hkv + h];
+    const bool ok = vs >= 0.f && vs < kInf && ks >= 0.f && ks < kInf;
+    num = __ballot(ok);
+    if (!ok) ks = 0.f;
+    // a scale of 0 weighs nothing, by an exponent far below any
+    const bool pos = ok && vs > 0.f;
+    ve = pos ? __builtin_amdgcn_frexp_expf(vs) : -200;
+    const float fr = pos ? __builtin_amdgcn_frexp_mantf(vs) : 0.5f;
+    lv = __builtin_amdgcn_logf(fr), rv = 1.f / fr;
+  }
+  DEV static float lane(float v, int k) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k)); }
+  DEV int at(int k) const { return __builtin_amdgcn_readlane(page, k); }
+};
+
+// One step of the softmax: the scores sc of block k of pg, its first place at position b0, become fp16 weights.
+// lo: every column sees the places up to lo.
+template <int DC, int MT>
+DEV void soften(Cols<DC, MT>& w, f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], const Pages& pg, int k, int b0, int lo) {
   const int j = lane_id() >> 4;
-  // v's scale enters relative to 2^unit; a block whose scale is no number leaves none to the columns that see it
-  const bool vnum = vs >= 0.f && vs < kInf;
-  const int ve = vnum && vs > 0.f ? __builtin_amdgcn_frexp_expf(vs) : -200, unew = w.unit > ve ? w.unit : ve;
-  const float ratio = vnum ? fmaxf(__builtin_ldexpf(vs, -unew), 0x1p-40f) : 0x1p-40f, shrink = __builtin_ldexpf(1.f, w.unit - unew);
-  const float lw = 15.f + __builtin_amdgcn_logf(ratio), iw = 1.f / ratio;
+  const bool there = pg.have >> k & 1;
+  if (!there || b0 + KB - 1 > lo) {
+#pragma unroll
+    for (int x = 0; x < MT; ++x) {
+      const int lim = there ? w.pos[x] - b0 - 4 * j : -1000;  // of the lane's places 16 t + 4 j + e those with 16 t + e <= lim are seen
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[x][t][e] = 16 * t + e > lim ? -kInf : sc[x][t][e];
+    }
+  }
+  // v's scale enters relative to 2^unit.  f > 0, so that what is hidden (-infinity) stays it with a k scale of 0
+  const float ks = Pages::lane(pg.ks, k);
+  const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
+  const float lw = 15.f + Pages::lane(pg.lv, k) + (float)dv, iw = __builtin_ldexpf(Pages::lane(pg.rv, k), -dv);
+  float f[MT], mnew[MT];
+  bool up = unew > w.unit;
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
-    const int lim = there ? w.pos[x] - b0 : -1;  // places up to here are seen
-    const float f = w.qm[x] * ks;
+    f[x] = fmaxf(w.qm[x] * ks, 0x1p-126f);
     float mx = -kInf;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, EDGE && 16 * t + 4 * j + e > lim ? -kInf : sc[x][t][e]);
-    mx = quad_max(mx);
-    const float mnew = fmaxf(w.m[x], mx * f), ms = mnew == -kInf ? 0.f : mnew;
-    if (__any(mnew > w.m[x]) || unew > w.unit) {
-      const float al = __builtin_amdgcn_exp2f(w.m[x] - ms), ao = al * shrink;
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[x][t][e]);
+    mnew[x] = fmaxf(w.m[x], quad_max(mx) * f[x]);
+    up = up || mnew[x] > w.m[x];
+  }
+  if (__any(up)) {
+#pragma unroll
+    for (int x = 0; x < MT; ++x) {
+      const float al = mnew[x] == -kInf ? 0.f : __builtin_amdgcn_exp2f(w.m[x] - mnew[x]), ao = __builtin_ldexpf(al, w.unit - unew);
       w.sum[x] *= al;
 #pragma unroll
       for (int u = 0; u < 4 * DC; ++u) w.o[x][u] *= ao;
-      w.m[x] = mnew;
+      w.m[x] = mnew[x];
     }
-    if (!vnum && lim >= 0) w.sum[x] = __builtin_nanf("");
-    const float base = lw - ms;
+    w.unit = unew;
+  }
+  if (!(pg.num >> k & 1)) {
+    // a block whose scales are no numbers leaves none to the columns that see it
+#pragma unroll
+    for (int x = 0; x < MT; ++x)
+      if (there && w.pos[x] >= b0) w.sum[x] = __builtin_nanf("");
+  }
+#pragma unroll
+  for (int x = 0; x < MT; ++x) {
+    const float base = lw - (w.m[x] == -kInf ? 0.f : w.m[x]);
     float add = 0.f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][t][e], f, base));
-        if (EDGE && 16 * t + 4 * j + e > lim) v = 0.f;
+        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][t][e], f[x], base));
         add += v;
         pf[x][t >> 1][4 * (t & 1) + e] = (_Float16)v;
       }
     w.sum[x] += add * iw;
   }
-  w.unit = unew;
 }
-
-// Pages and scales of up to 64 blocks of a sequence, a lane each.
-struct Pages {
-  int page;
-  float ks, vs;
-  unsigned long long have;
-  DEV void fetch(const Attn& a, int seq, int h, int block, bool on) {
-    const int p = on ? page_of(a.c, seq, block) : -1;
-    have = __ballot(p >= 0);
-    page = p >= 0 ? p : 0;
-    ks = vs = 0.f;
-    if (on) ks = a.c.ks[(size_t)page * a.c.hkv + h], vs = a.c.vs[(size_t)page * a.c.hkv + h];
-  }
-  DEV int at(int k) const { return __builtin_amdgcn_readlane(page, k); }
-  DEV float k_scale(int k) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), k)); }
-  DEV float v_scale(int k) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), k)); }
-};
 
 // The blocks [b0, b1) of a sequence that split sp takes of the nb blocks that its columns see.
 DEV void share(const Attn& a, int nb, int sp, int& b0, int& b1) {
@@ -231,7 +260,7 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
   constexpr int TP = 16 * MT, LD = 64 * DC + 4;
   __shared__ __align__(16) float sm[W * 16 * LD];
   __shared__ float sml[W * 32];
-  const int l = lane_id(), j = l >> 4, wv = wave_id();
+  const int l = lane_id(), j = l >> 4, wv = __builtin_amdgcn_readfirstlane(wave_id());
   const int i = blockIdx.x, h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
   const Seq s = seq_of(a.c, i);
   const int np = s.n * g < TP ? s.n * g : TP;
@@ -291,10 +320,8 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
         }
       }
       if (k + 1 < n) load_k(nx);
-      const bool there = (pg.have >> k) & 1;
       half8 pf[MT][2];
-      if (!there || b * KB + KB - 1 > p_lo) soften<true>(w, sc, pf, pg.k_scale(k), pg.v_scale(k), b * KB, there);
-      else soften<false>(w, sc, pf, pg.k_scale(k), pg.v_scale(k), b * KB, true);
+      soften(w, sc, pf, pg, k, b * KB, p_lo);
 #pragma unroll
       for (int u = 0; u < 4 * DC; ++u) {
         const half8 va = to_half8(vr[u].x, vr[u].y), vb = to_half8(vr[u].z, vr[u].w);
@@ -336,14 +363,31 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
   }
 }
 
+// Order of N reads of fragments from LDS and their MT products each: six reads ahead, more than an LDS read's latency (left to itself the compiler
+// waits for every read before it issues the next).
+template <int N, int MT>
+DEV void reads_ahead() {
+  constexpr int A = N < 6 ? N : 6;
+  __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, MT, 0);
+    if (i + A < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+}
+
 // Many columns: each of the NW waves holds MT tiles of its own, and all go through the cached blocks together.  A block is loaded once for
-// all of them (a 1 / NW of it a wave, two blocks ahead), becomes fp16 once, and lies in LDS as the operands are read: 1 KB a fragment, lane by
-// lane, so neither the writes nor the reads of 16 bytes meet in a bank.  Two buffers, one barrier a block.
-template <int DC, int MT, int NW>
-__global__ void __launch_bounds__(64 * NW, NW / 4) k_attn_tiles(Attn a) {
+// all of them (a 1 / NW of it a wave), becomes fp16 once, and lies in LDS as the operands are read: 1 KB a fragment, lane by lane, so neither
+// the writes nor the reads of 16 bytes meet in a bank.  A step has two halves, each ended by a barrier: products (O += V P of the
+// block before, S = K Q of this one) and softmax.  With eight waves the second four are half a step behind, so that on every SIMD one wave
+// multiplies while the other's softmax has the vector unit.  k of block n + 1 and v of block n are written during block n's two
+// half steps of the first waves, into buffers whose last readers ended before them.
+template <int DC, int MT, int NW, int OCC>
+__global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   constexpr int TP = 16 * MT * NW, F = 4 * DC, PER = (F + NW - 1) / NW;  // F: 16-byte loads a lane of k, and of v, for one block
-  __shared__ __align__(16) half8 lds[2 * 4 * F * WAVE];                  // [2][k, v][F][2][64]
-  const int l = lane_id(), j = l >> 4, wv = wave_id();
+  __shared__ __align__(16) half8 kb[2 * 2 * F * WAVE], vb[2 * 2 * F * WAVE];  // [2][F][2][64]
+  const int l = lane_id(), j = l >> 4, wv = __builtin_amdgcn_readfirstlane(wave_id());
+  const bool late = NW == 8 && wv >= 4;
   const int h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
   int at = gridDim.x - 1 - blockIdx.x, i = at;  // the last rows, which see most, first
   if (a.scan) i = find_item(a.c, at, [g](const Seq& s) { return (s.n * g + TP - 1) / TP; });
@@ -357,62 +401,69 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) k_attn_tiles(Attn a) {
   int b0, b1;
   share(a, p_hi < 0 ? 0 : (p_hi >> 6) + 1, sp, b0, b1);
   if (b0 == b1 && sp > 0) return emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);
-  // the wave's columns and the blocks that they see
+  const int cnt = b1 - b0;
+  // the wave's columns and how many of the blocks they see
   const int w0 = c0 + 16 * MT * wv, w1 = w0 + 16 * MT < c1 ? w0 + 16 * MT : c1;
-  const int w_lo = s.first + w0 / g, w_end = s.first + (w1 - 1) / g, w_nb = w0 < c1 && w_end >= 0 ? (w_end >> 6) + 1 : 0;
+  const int w_lo = s.first + w0 / g, w_end = s.first + (w1 - 1) / g, w_cnt = w0 < c1 && w_end >= 0 ? (w_end >> 6) + 1 - b0 : 0;
 
-  int off[PER];  // of the wave's loads; v's differ by what follows
+  int koff[PER], voff[PER];
 #pragma unroll
   for (int f = 0; f < PER; ++f) {
-    const int c = (wv * PER + f) >> 2, t = (wv * PER + f) & 3;
-    off[f] = ((4 * c + j < d16 ? 4 * c + j : d16 - 1) * KB + 16 * t + (l & 15)) * 16;
+    const int u = wv * PER + f, c = u >> 2, t = u & 3;
+    koff[f] = ((4 * c + j < d16 ? 4 * c + j : d16 - 1) * KB + 16 * t + (l & 15)) * 16;
+    voff[f] = (16 * (u < d16 ? u : d16 - 1) + (l & 15)) * KB + 16 * j;
   }
   uint4 kr[PER], vr[PER];
-  auto load = [&](int page) {
-    const size_t base = ((size_t)page * a.c.hkv + h) * KB * d;
+  auto mine = [&](int f) { return F % NW == 0 || wv * PER + f < F; };
+  auto load_k = [&](int page) {
+    const uint8_t* p = a.c.kq + ((size_t)page * a.c.hkv + h) * KB * d;
 #pragma unroll
-    for (int f = 0; f < PER; ++f) {
-      const int u = wv * PER + f;
-      if (F % NW && u >= F) break;
-      kr[f] = ld16(a.c.kq + base + off[f]);
-      vr[f] = ld16(a.c.vq + base + (16 * (u < d16 ? u : d16 - 1) + (l & 15)) * KB + 16 * j);
-    }
+    for (int f = 0; f < PER; ++f)
+      if (mine(f)) kr[f] = ld16(p + koff[f]);
   };
-  auto store = [&](int buf) {
-    half8* k = lds + buf * 4 * F * WAVE;
+  auto load_v = [&](int page) {
+    const uint8_t* p = a.c.vq + ((size_t)page * a.c.hkv + h) * KB * d;
 #pragma unroll
-    for (int f = 0; f < PER; ++f) {
-      const int u = wv * PER + f;
-      if (F % NW && u >= F) break;
-      k[(2 * u) * WAVE + l] = to_half8(kr[f].x, kr[f].y), k[(2 * u + 1) * WAVE + l] = to_half8(kr[f].z, kr[f].w);
-      half8* v = k + 2 * F * WAVE;
-      v[(2 * u) * WAVE + l] = to_half8(vr[f].x, vr[f].y), v[(2 * u + 1) * WAVE + l] = to_half8(vr[f].z, vr[f].w);
-    }
+    for (int f = 0; f < PER; ++f)
+      if (mine(f)) vr[f] = ld16(p + voff[f]);
+  };
+  auto store = [&](half8* b, const uint4 (&r)[PER], int n) {
+    b += (n & 1) * 2 * F * WAVE + l;
+#pragma unroll
+    for (int f = 0; f < PER; ++f)
+      if (mine(f)) {
+        const int u = wv * PER + f;
+        b[(2 * u) * WAVE] = to_half8(r[f].x, r[f].y), b[(2 * u + 1) * WAVE] = to_half8(r[f].z, r[f].w);
+      }
   };
 
   Pages pg, px;  // of 64 blocks, and of the 64 behind them
-  Cols<DC, MT> w;
-  const int cnt = b1 - b0;
   pg.fetch(a, i, h, b0 + l, l < cnt);
-  if (cnt > 0) load(pg.at(0));
+  if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
   px.fetch(a, i, h, b0 + WAVE + l, WAVE + l < cnt);
+  int base = 0;
+  auto page = [&](int n) { return n - base < WAVE ? pg.at(n - base) : px.at(n - base - WAVE); };
+  // k of block n + 1 and v of block n into LDS, the wave's share; the loads of the blocks behind them.  A load stands where its registers' last
+  // contents have been stored on every path, or it would wait for the loads in flight.
+  auto put = [&](int n) {
+    if (n >= cnt) return;
+    store(vb, vr, n);
+    if (n + 1 >= cnt) return;
+    store(kb, kr, n + 1);
+    load_v(page(n + 1));
+    if (n + 2 < cnt) load_k(page(n + 2));
+  };
+  Cols<DC, MT> w;
   begin(w, a, s, h, w0, c1);
-  if (cnt > 0) store(0);
-  if (cnt > 1) load(pg.at(1));
-  for (int k = 0; k < cnt; ++k) {
-    const int kk = k & (WAVE - 1);
-    if (k && kk == 0) {
-      pg = px;
-      px.fetch(a, i, h, b0 + k + WAVE + l, k + WAVE + l < cnt);
-    }
-    __syncthreads();
-    if (k + 1 < cnt) store((k + 1) & 1);
-    if (k + 2 < cnt) load(kk + 2 < WAVE ? pg.at(kk + 2) : px.at(kk + 2 - WAVE));
-    const int b = b0 + k;
-    if (b >= w_nb) continue;  // later than all of the wave's columns
-    const half8* kf = lds + (k & 1) * 4 * F * WAVE + l;
-    const half8* vf = kf + 2 * F * WAVE;
-    f32x4 sc[MT][4];
+  if (cnt > 0) {
+    store(kb, kr, 0);
+    if (cnt > 1) load_k(page(1));
+  }
+  lds_barrier();
+  if (late) put(0), lds_barrier();
+  f32x4 sc[MT][4];
+  auto scores = [&](int k) {
+    const half8* kf = kb + (k & 1) * 2 * F * WAVE + l;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -427,28 +478,47 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) k_attn_tiles(Attn a) {
 #pragma unroll
           for (int x = 0; x < MT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, w.q[x][c][y], sc[x][t], 0, 0, 0);
         }
-    const bool there = (pg.have >> kk) & 1;
+    reads_ahead<8 * DC, MT>();
+  };
+  // blocks later than all of the wave's columns are left out
+  const int mine_cnt = cnt < w_cnt ? cnt : w_cnt;
+  if (mine_cnt > 0) scores(0);
+  for (int k = 0; k < cnt; ++k) {
+    lds_barrier();
+    if (k - base == WAVE) {
+      pg = px, base = k;
+      px.fetch(a, i, h, b0 + k + WAVE + l, k + WAVE + l < cnt);
+    }
+    put(late ? k + 1 : k);
     half8 pf[MT][2];
-    if (!there || b * KB + KB - 1 > w_lo) soften<true>(w, sc, pf, pg.k_scale(kk), pg.v_scale(kk), b * KB, there);
-    else soften<false>(w, sc, pf, pg.k_scale(kk), pg.v_scale(kk), b * KB, true);
+    if (k < mine_cnt) soften(w, sc, pf, pg, k - base, (b0 + k) * KB, w_lo);
+    lds_barrier();
+    if (k < mine_cnt) {
+      const half8* vf = vb + (k & 1) * 2 * F * WAVE + l;
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int u = 0; u < 4 * DC; ++u) {
-        const half8 va = vf[(2 * u + y) * WAVE];
+        for (int u = 0; u < 4 * DC; ++u) {
+          const half8 va = vf[(2 * u + y) * WAVE];
 #pragma unroll
-        for (int x = 0; x < MT; ++x) w.o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[x][y], w.o[x][u], 0, 0, 0);
-      }
+          for (int x = 0; x < MT; ++x) w.o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[x][y], w.o[x][u], 0, 0, 0);
+        }
+      reads_ahead<8 * DC, MT>();
+    }
+    if (k + 1 < mine_cnt) scores(k + 1);
   }
+  if (NW == 8 && !late) lds_barrier();
   const float us = __builtin_ldexpf(1.f, w.unit - 16);
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
     const float sum = quad_sum(w.sum[x]) * 0x1p-16f;
-    const int p = w0 + 16 * x + (l & 15), row = p / g;
+    int z = threadIdx.x & 63;  // worked out again: values kept from begin() would cost registers through the loop
+    asm volatile("" : "+v"(z));
+    const int p = w0 + 16 * x + (z & 15), row = p / g;
     if (p < c1)
 #pragma unroll
       for (int u = 0; u < 4 * DC; ++u)
-        if (u < d16) emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, 16 * u + 4 * j, w.o[x][u] * us, sum, w.m[x]);
+        if (u < d16) emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, 16 * u + 4 * (z >> 4), w.o[x][u] * us, sum, w.m[x]);
   }
 }
 
@@ -503,7 +573,7 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   Plan p;
   const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g;
   p.few = pairs <= 16 || (d <= 128 && pairs <= 32);
-  p.mt = p.few ? (pairs <= 16 ? 1 : 2) : d <= 64 ? 3 : d <= 128 ? 2 : 1;
+  p.mt = p.few ? (pairs <= 16 ? 1 : 2) : d <= 128 ? 2 : 1;
   auto cut = [&](long long tp) {
     const long long per = (pairs + tp - 1) / tp, all = rows * g / tp + seqs;
     p.scan = per > 1, p.tiles = per > 1 && all < per * seqs ? all : per * seqs;
@@ -543,6 +613,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
               pages, rows, seqs, hkv, d};
   if (!attn_shape_ok(rows, seqs, max_rows, max_len, hq, hkv, d) || !kv8_ok(c) || ldq < hq * d || ldq % 8 || ldy < hq * d || ldy % 4) return -1;
   if (gate && (hsg < d || hsg % 4 || ldg % 4 || ldg < (long long)(hq - 1) * hsg + d || ((uintptr_t)gate & 15))) return -1;
+  if (!(fabsf(scale) < kInf)) return -1;
   if (rows == 0 || seqs == 0 || max_rows == 0) return 0;
   if (!kv8_buffers_ok(c) || !q || !y || !ws || ((uintptr_t)q & 15) || ((uintptr_t)y & 7) || ((uintptr_t)ws & 15)) return -1;
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
@@ -555,8 +626,8 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   };
   auto tiles = [&](auto dc, auto mt) {
     constexpr int DC = decltype(dc)::value, MT = decltype(mt)::value;
-    if (p.nw == 8) hipLaunchKernelGGL((k_attn_tiles<DC, MT, 8>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_tiles<DC, MT, 4>), grid, dim3(256), 0, st, a);
+    if (p.nw == 8) hipLaunchKernelGGL((k_attn_tiles<DC, MT, 8, 2>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_tiles<DC, MT, 4, DC <= 2 ? 2 : 1>), grid, dim3(256), 0, st, a);
   };
   constexpr std::integral_constant<int, 1> i1{};
   constexpr std::integral_constant<int, 2> i2{};
@@ -567,7 +638,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
     else if (d <= 128) p.mt == 1 ? few(i2, i1) : few(i2, i2);
     else d <= 192 ? few(i3, i1) : few(i4, i1);
   } else {
-    if (d <= 64) tiles(i1, i3);
+    if (d <= 64) tiles(i1, i2);
     else if (d <= 128) tiles(i2, i2);
     else d <= 192 ? tiles(i3, i1) : tiles(i4, i1);
   }
