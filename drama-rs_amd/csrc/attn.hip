@@ -23,6 +23,7 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int W = 4, NT = W * WAVE;
 constexpr float kInf = __builtin_inff();
@@ -363,30 +364,140 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
   }
 }
 
-// Order of N reads of fragments from LDS and their MT products each: six reads ahead, more than an LDS read's latency (left to itself the compiler
-// waits for every read before it issues the next).
-template <int N, int MT>
-DEV void reads_ahead() {
-  constexpr int A = N < 6 ? N : 6;
-  __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, MT, 0);
-    if (i + A < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-  }
-}
-
-// Many columns: each of the NW waves holds MT tiles of its own, and all go through the cached blocks together.  A block is loaded once for
+// Many columns: each of the NW waves holds 32 of its own, and all go through the cached blocks together.  A block is loaded once for
 // all of them (a 1 / NW of it a wave), becomes fp16 once, and lies in LDS as the operands are read: 1 KB a fragment, lane by lane, so neither
 // the writes nor the reads of 16 bytes meet in a bank.  A step has two halves, each ended by a barrier: products (O += V P of the
 // block before, S = K Q of this one) and softmax.  With eight waves the second four are half a step behind, so that on every SIMD one wave
-// multiplies while the other's softmax has the vector unit.  k of block n + 1 and v of block n are written during block n's two
-// half steps of the first waves, into buffers whose last readers ended before them.
-template <int DC, int MT, int NW, int OCC>
+// multiplies while the other's softmax has the vector unit.  k of block n + 1 and v of block n are written beside the products of S of block
+// n, into buffers whose last readers ended before them.
+// What bounds it is the vector unit, which a product keeps for 10 to 12 cycles whatever its size: hence 32 x 32 x 16 products, and a
+// softmax without a maximum where it can be: a column's reference is the maximum of an earlier block, and only where a lane's sum says that a
+// weight may have passed fp16 (or the column has no reference yet) is the block's maximum taken, O rescaled and the weights formed again.
+template <int DC>
+struct Cols32 {
+  half8 q[2 * DC];   // 32-element chunk i, half y: elements 32 i + 16 (l >> 5) + 8 y + (0 .. 7), times a power of two
+  f32x16 o[DC];      // O^T: elements 32 u + 8 (r >> 2) + 4 (l >> 5) + (r & 3), over 2^(unit - kBase)
+  float m, sum, qm;  // reference of the log2 scores, the lane's share of the sum, log2 score of a unit of S and of k's scale
+  int pos, unit;
+};
+constexpr float kBase = 4.f;      // a weight is 2^kBase times its ratio to the reference's: 2^11 above it before fp16 ends,
+constexpr float kMost = 40000.f;  // which a lane's sum of weights up to kMost rules out
+
+template <int DC>
+DEV void begin32(Cols32<DC>& w, const Attn& a, const Seq& s, int h, int c0, int np) {
+  const int l = lane_id(), hh = l >> 5, d = a.c.d, g = a.g;
+  const long long cap = (long long)a.c.maxp * KB - 1;
+  const int p = c0 + (l & 31), row = p / g;
+  const bool on = p < np;
+  const uint16_t* src = a.q + (size_t)(s.r0 + row) * a.ldq + (size_t)(h * g + p - row * g) * d;
+  uint4 r[2 * DC];
+#pragma unroll
+  for (int i = 0; i < 2 * DC; ++i) {
+    const int e = 32 * (i >> 1) + 16 * hh + 8 * (i & 1);
+    r[i] = make_uint4(0, 0, 0, 0);
+    if (on && e < d) r[i] = ld16(src + e);
+  }
+  float top = 0.f;
+  bool num = true;
+#pragma unroll
+  for (int i = 0; i < 2 * DC; ++i) {
+    const uint32_t v[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float lo = fabsf(bf16_lo(v[k])), hi = fabsf(bf16_hi(v[k]));
+      top = fmaxf(top, fmaxf(lo, hi));
+      num = num && lo < kInf && hi < kInf;
+    }
+  }
+  top = xmax_step<32>(num ? top : kInf);
+  const bool bad = !(top < kInf);  // as in begin()
+  const int e = bad || top == 0.f ? 0 : 13 - __builtin_amdgcn_frexp_expf(top);
+  const float sign = bad ? __builtin_nanf("") : a.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+  for (int i = 0; i < 2 * DC; ++i) {
+    const uint32_t v[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w.q[i][2 * k] = (_Float16)(sign * __builtin_ldexpf(bf16_lo(v[k]), e));
+      w.q[i][2 * k + 1] = (_Float16)(sign * __builtin_ldexpf(bf16_hi(v[k]), e));
+    }
+  }
+  w.qm = __builtin_ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
+  const int ps = s.first + row;
+  w.pos = on ? (ps < cap ? ps : (int)cap) : -1;
+  w.m = -kInf, w.sum = 0.f, w.unit = -200;
+#pragma unroll
+  for (int u = 0; u < DC; ++u)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) w.o[u][k] = 0.f;
+}
+
+// The scores sc of block k of pg (first place at position b0, every column sees the places up to lo) become fp16 weights.
+template <int DC>
+DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages& pg, int k, int b0, int lo) {
+  const int hh = lane_id() >> 5;
+  const bool there = pg.have >> k & 1;
+  const int lim = there ? w.pos - b0 : -1000;
+  if (!there || b0 + KB - 1 > lo) {
+    const int mine = lim - 4 * hh;  // of the lane's places 32 t + 8 (r >> 2) + 4 hh + (r & 3)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) > mine ? -kInf : sc[t][r];
+  }
+  const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
+  const float f = fmaxf(w.qm * Pages::lane(pg.ks, k), 0x1p-126f), iw = __builtin_ldexpf(Pages::lane(pg.rv, k), -dv);  // as in soften()
+  float at = kBase + Pages::lane(pg.lv, k) + (float)dv - (w.m == -kInf ? 0.f : w.m);
+  if (unew > w.unit) {
+    const int sh = w.unit - unew;
+#pragma unroll
+    for (int u = 0; u < DC; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w.o[u][r] = __builtin_ldexpf(w.o[u][r], sh);
+    w.unit = unew;
+  }
+  if (!(pg.num >> k & 1) && lim >= 0) w.sum = __builtin_nanf("");  // scales that are no numbers
+  float add = 0.f;
+  auto form = [&]() {
+    add = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], f, at));
+        add += v;
+        pf[t][r >> 2 & 1][4 * (r >> 3) + (r & 3)] = (_Float16)v;
+      }
+  };
+  form();
+  if (__any(!(add <= kMost) || (w.m == -kInf && lim >= 0))) {
+    float mx = -kInf;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
+    const float top = xmax_step<32>(mx) * f;
+    if (top > w.m) {
+      // less than the reference stays as it is; without one (m -infinity) there are no sums to scale
+      const float al = w.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(w.m - top);
+      at -= top - (w.m == -kInf ? 0.f : w.m);
+      w.m = top;
+      w.sum *= al;
+#pragma unroll
+      for (int u = 0; u < DC; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w.o[u][r] *= al;
+    }
+    form();
+  }
+  w.sum += add * iw;
+}
+
+template <int DC, int NW, int OCC>
 __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
-  constexpr int TP = 16 * MT * NW, F = 4 * DC, PER = (F + NW - 1) / NW;  // F: 16-byte loads a lane of k, and of v, for one block
+  constexpr int TP = 32 * NW, F = 2 * DC, PER = (F + NW - 1) / NW;  // F: 16-byte loads a lane of k, and of v, for one block
   __shared__ __align__(16) half8 kb[2 * 2 * F * WAVE], vb[2 * 2 * F * WAVE];  // [2][F][2][64]
-  const int l = lane_id(), j = l >> 4, wv = __builtin_amdgcn_readfirstlane(wave_id());
+  const int l = lane_id(), hh = l >> 5, wv = __builtin_amdgcn_readfirstlane(wave_id());
   const bool late = NW == 8 && wv >= 4;
   const int h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
   int at = gridDim.x - 1 - blockIdx.x, i = at;  // the last rows, which see most, first
@@ -403,15 +514,17 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   if (b0 == b1 && sp > 0) return emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);
   const int cnt = b1 - b0;
   // the wave's columns and how many of the blocks they see
-  const int w0 = c0 + 16 * MT * wv, w1 = w0 + 16 * MT < c1 ? w0 + 16 * MT : c1;
+  const int w0 = c0 + 32 * wv, w1 = w0 + 32 < c1 ? w0 + 32 : c1;
   const int w_lo = s.first + w0 / g, w_end = s.first + (w1 - 1) / g, w_cnt = w0 < c1 && w_end >= 0 ? (w_end >> 6) + 1 - b0 : 0;
 
+  // load f of the wave: k of 32 tokens (tile t) and of 32 elements (chunk c), 16 of them a lane; v of 32 elements (tile) and of the tokens
+  // 16 .. + 8 jj + 4 hh + .. (see kv8.hpp)
   int koff[PER], voff[PER];
 #pragma unroll
   for (int f = 0; f < PER; ++f) {
-    const int u = wv * PER + f, c = u >> 2, t = u & 3;
-    koff[f] = ((4 * c + j < d16 ? 4 * c + j : d16 - 1) * KB + 16 * t + (l & 15)) * 16;
-    voff[f] = (16 * (u < d16 ? u : d16 - 1) + (l & 15)) * KB + 16 * j;
+    const int u = wv * PER + f, c = u >> 1, b = u & 1, e = 32 * c + (l & 31);
+    koff[f] = ((2 * c + hh < d16 ? 2 * c + hh : d16 - 1) * KB + 32 * b + (l & 31)) * 16;
+    voff[f] = (e < d ? e : d - 1) * KB + 16 * (2 * b + hh);
   }
   uint4 kr[PER], vr[PER];
   auto mine = [&](int f) { return F % NW == 0 || wv * PER + f < F; };
@@ -427,99 +540,126 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
     for (int f = 0; f < PER; ++f)
       if (mine(f)) vr[f] = ld16(p + voff[f]);
   };
-  auto store = [&](half8* b, const uint4 (&r)[PER], int n) {
-    b += (n & 1) * 2 * F * WAVE + l;
-#pragma unroll
-    for (int f = 0; f < PER; ++f)
-      if (mine(f)) {
-        const int u = wv * PER + f;
-        b[(2 * u) * WAVE] = to_half8(r[f].x, r[f].y), b[(2 * u + 1) * WAVE] = to_half8(r[f].z, r[f].w);
-      }
-  };
 
   Pages pg, px;  // of 64 blocks, and of the 64 behind them
   pg.fetch(a, i, h, b0 + l, l < cnt);
   if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
   px.fetch(a, i, h, b0 + WAVE + l, WAVE + l < cnt);
   int base = 0;
-  auto page = [&](int n) { return n - base < WAVE ? pg.at(n - base) : px.at(n - base - WAVE); };
-  // k of block n + 1 and v of block n into LDS, the wave's share; the loads of the blocks behind them.  A load stands where its registers' last
-  // contents have been stored on every path, or it would wait for the loads in flight.
-  auto put = [&](int n) {
-    if (n >= cnt) return;
-    store(vb, vr, n);
-    if (n + 1 >= cnt) return;
-    store(kb, kr, n + 1);
-    load_v(page(n + 1));
-    if (n + 2 < cnt) load_k(page(n + 2));
+  auto page = [&](int n) {
+    const int p = pg.at((n - base) & (WAVE - 1)), x = px.at((n - base) & (WAVE - 1));  // no branch
+    return n - base < WAVE ? p : x;
   };
-  Cols<DC, MT> w;
-  begin(w, a, s, h, w0, c1);
+  // k of block n + 1 and v of block n into LDS, the wave's share in 4 PER parts; the loads of the blocks behind them (past the last one again
+  // that one, into a buffer that nobody reads any more): no branch, so that it goes between the products.
+  auto put_part = [&](int n, int f) {
+    const bool isk = f >= 2 * PER;
+    const int i = (f % (2 * PER)) >> 1, y = f & 1, u = wv * PER + i;
+    const uint4 r = isk ? kr[i] : vr[i];
+    half8* b = (isk ? kb : vb) + ((n + isk) & 1) * 2 * F * WAVE + l;
+    if (mine(i)) b[(2 * u + y) * WAVE] = y ? to_half8(r.z, r.w) : to_half8(r.x, r.y);
+  };
+  auto put_loads = [&](int n) {
+    load_v(page(n + 1 < cnt ? n + 1 : cnt - 1));
+    load_k(page(n + 2 < cnt ? n + 2 : cnt - 1));
+  };
+  auto put = [&](int n) {
+#pragma unroll
+    for (int f = 0; f < 4 * PER; ++f) put_part(n, f);
+    put_loads(n);
+  };
+  Cols32<DC> w;
+  begin32(w, a, s, h, w0, c1);
   if (cnt > 0) {
-    store(kb, kr, 0);
-    if (cnt > 1) load_k(page(1));
+#pragma unroll
+    for (int f = 2 * PER; f < 4 * PER; ++f) put_part(-1, f);
+    load_k(page(cnt > 1 ? 1 : 0));
   }
   lds_barrier();
-  if (late) put(0), lds_barrier();
-  f32x4 sc[MT][4];
-  auto scores = [&](int k) {
-    const half8* kf = kb + (k & 1) * 2 * F * WAVE + l;
+  if (late) lds_barrier();
+  f32x16 sc[2], zero;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+  for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+  half8 pf[2][2];
+  // Products in turns of four, with the next turn's operands on their way from LDS and a share of put(n) between: left to itself the compiler
+  // waits for every read before it issues the next, and a product that waits for the one before it on the same sum takes twice its time, so
+  // those of O += V P of block k and of S = K Q of block k + 1 alternate.
+  enum { WEIGH = 1, SCORE = 2 };
+  auto products = [&](auto what, int k, int n) {
+    constexpr int M = decltype(what)::value, N = M == 3 ? 8 * DC : 4 * DC, T = N / 4, PT = T > 2 ? T - 2 : 1;
+    const half8* vf = vb + (k & 1) * 2 * F * WAVE + l;
+    const half8* kf = kb + ((k + 1) & 1) * 2 * F * WAVE + l;
+    auto is_score = [](int x) { return M == SCORE || (M == 3 && (x & 1)); };
+    auto operand = [&](int x) {
+      const int y = M == 3 ? x >> 1 : x;
+      if (is_score(x)) return kf[(2 * (2 * (y >> 2) + (y & 1)) + (y >> 1 & 1)) * WAVE];
+      return vf[(2 * (2 * (y % DC) + (y / DC >> 1)) + (y / DC & 1)) * WAVE];
+    };
+    half8 fr[2][4];
 #pragma unroll
-      for (int x = 0; x < MT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < 4; ++x) fr[0][x] = operand(x);
 #pragma unroll
-    for (int c = 0; c < DC; ++c)
+    for (int c = 0; c < T; ++c) {
+      if (c + 1 < T)
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+        for (int x = 0; x < 4; ++x) fr[(c + 1) & 1][x] = operand(4 * c + 4 + x);
+      if (n >= 0 && M == 3) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const half8 ka = kf[(2 * (4 * c + t) + y) * WAVE];
+        for (int f = 0; f < 4 * PER; ++f)
+          if (f * PT / (4 * PER) == c) put_part(n, f);
+        if (c == T - 1) put_loads(n);
+      }
 #pragma unroll
-          for (int x = 0; x < MT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, w.q[x][c][y], sc[x][t], 0, 0, 0);
-        }
-    reads_ahead<8 * DC, MT>();
+      for (int x = 0; x < 4; ++x) {
+        const int z = 4 * c + x, y = M == 3 ? z >> 1 : z;
+        if (is_score(z))
+          sc[y & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[c & 1][x], w.q[y >> 1], y < 2 ? zero : sc[y & 1], 0, 0, 0);
+        else
+          w.o[y % DC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[c & 1][x], pf[y / DC & 1][y / DC >> 1], w.o[y % DC], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
+  constexpr std::integral_constant<int, WEIGH> weigh{};
+  constexpr std::integral_constant<int, SCORE> score{};
+  constexpr std::integral_constant<int, WEIGH + SCORE> both{};
   // blocks later than all of the wave's columns are left out
   const int mine_cnt = cnt < w_cnt ? cnt : w_cnt;
-  if (mine_cnt > 0) scores(0);
-  for (int k = 0; k < cnt; ++k) {
+  if (mine_cnt > 0) products(score, -1, -1);
+  if (cnt > 0) put(0);
+  auto soft = [&](int k) {
     lds_barrier();
     if (k - base == WAVE) {
       pg = px, base = k;
       px.fetch(a, i, h, b0 + k + WAVE + l, k + WAVE + l < cnt);
     }
-    put(late ? k + 1 : k);
-    half8 pf[MT][2];
-    if (k < mine_cnt) soften(w, sc, pf, pg, k - base, (b0 + k) * KB, w_lo);
+    if (k < mine_cnt) soften32(w, sc, pf, pg, k - base, (b0 + k) * KB, w_lo);
     lds_barrier();
-    if (k < mine_cnt) {
-      const half8* vf = vb + (k & 1) * 2 * F * WAVE + l;
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int u = 0; u < 4 * DC; ++u) {
-          const half8 va = vf[(2 * u + y) * WAVE];
-#pragma unroll
-          for (int x = 0; x < MT; ++x) w.o[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[x][y], w.o[x][u], 0, 0, 0);
-        }
-      reads_ahead<8 * DC, MT>();
-    }
-    if (k + 1 < mine_cnt) scores(k + 1);
+  };
+  int k = 0;
+  for (; k + 1 < mine_cnt; ++k) {
+    soft(k);
+    products(both, k, k + 1);
+  }
+  for (; k < cnt; ++k) {
+    soft(k);
+    if (k < mine_cnt) products(weigh, k, -1);
+    if (k + 1 < cnt) put(k + 1);
   }
   if (NW == 8 && !late) lds_barrier();
-  const float us = __builtin_ldexpf(1.f, w.unit - 16);
+  const float us = __builtin_ldexpf(1.f, w.unit - 16), sum = xsum_step<32>(w.sum) * 0x1p-16f;
+  int z = threadIdx.x & 63;  // worked out again: values kept from begin32() would cost registers through the loop
+  asm volatile("" : "+v"(z));
+  const int p = w0 + (z & 31), row = p / g;
+  if (p < c1)
 #pragma unroll
-  for (int x = 0; x < MT; ++x) {
-    const float sum = quad_sum(w.sum[x]) * 0x1p-16f;
-    int z = threadIdx.x & 63;  // worked out again: values kept from begin() would cost registers through the loop
-    asm volatile("" : "+v"(z));
-    const int p = w0 + 16 * x + (z & 15), row = p / g;
-    if (p < c1)
+    for (int u = 0; u < DC; ++u)
 #pragma unroll
-      for (int u = 0; u < 4 * DC; ++u)
-        if (u < d16) emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, 16 * u + 4 * (z >> 4), w.o[x][u] * us, sum, w.m[x]);
-  }
+      for (int r = 0; r < 16; r += 4) {
+        const int e = 32 * u + 2 * r + 4 * (z >> 5);
+        if (e < d)
+          emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, e, f32x4{w.o[u][r] * us, w.o[u][r + 1] * us, w.o[u][r + 2] * us, w.o[u][r + 3] * us}, sum, w.m);
+      }
 }
 
 // Joins the parts of 64 elements of a row's query: 16 groups of 16 lanes take every 16th part, all their loads together.
@@ -573,14 +713,14 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   Plan p;
   const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g;
   p.few = pairs <= 16 || (d <= 128 && pairs <= 32);
-  p.mt = p.few ? (pairs <= 16 ? 1 : 2) : d <= 128 ? 2 : 1;
+  p.mt = pairs <= 16 ? 1 : 2;
   auto cut = [&](long long tp) {
     const long long per = (pairs + tp - 1) / tp, all = rows * g / tp + seqs;
     p.scan = per > 1, p.tiles = per > 1 && all < per * seqs ? all : per * seqs;
   };
-  p.nw = p.few ? W : 8;
-  cut(p.few ? 16 * p.mt : 16 * p.mt * p.nw);
-  if (!p.few && p.tiles * hkv < 256) p.nw = 4, cut(16 * p.mt * p.nw);
+  p.nw = p.few || d > 128 ? 4 : 8;
+  cut(p.few ? 16 * p.mt : 32 * p.nw);
+  if (p.nw == 8 && p.tiles * hkv < 256) p.nw = 4, cut(32 * p.nw);
   const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = p.few ? 2048 : 512;
   long long s = units >= want / 2 && !p.few ? 1 : (want + units - 1) / units;
   const long long most = (blocks + W - 1) / W;
@@ -624,23 +764,29 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   auto few = [&](auto dc, auto mt) {
     hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), grid, dim3(NT), 0, st, a);
   };
-  auto tiles = [&](auto dc, auto mt) {
-    constexpr int DC = decltype(dc)::value, MT = decltype(mt)::value;
-    if (p.nw == 8) hipLaunchKernelGGL((k_attn_tiles<DC, MT, 8, 2>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_tiles<DC, MT, 4, DC <= 2 ? 2 : 1>), grid, dim3(256), 0, st, a);
+  auto tiles = [&](auto dc) {
+    constexpr int DC = decltype(dc)::value;
+    if constexpr (DC <= 4) {
+      if (p.nw == 8) hipLaunchKernelGGL((k_attn_tiles<DC, 8, 2>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((k_attn_tiles<DC, 4, 2>), grid, dim3(256), 0, st, a);
+    } else {
+      hipLaunchKernelGGL((k_attn_tiles<DC, 4, 1>), grid, dim3(256), 0, st, a);
+    }
   };
   constexpr std::integral_constant<int, 1> i1{};
   constexpr std::integral_constant<int, 2> i2{};
   constexpr std::integral_constant<int, 3> i3{};
   constexpr std::integral_constant<int, 4> i4{};
+  constexpr std::integral_constant<int, 6> i6{};
+  constexpr std::integral_constant<int, 8> i8{};
   if (p.few) {
     if (d <= 64) p.mt == 1 ? few(i1, i1) : few(i1, i2);
     else if (d <= 128) p.mt == 1 ? few(i2, i1) : few(i2, i2);
     else d <= 192 ? few(i3, i1) : few(i4, i1);
   } else {
-    if (d <= 64) tiles(i1, i2);
-    else if (d <= 128) tiles(i2, i2);
-    else d <= 192 ? tiles(i3, i1) : tiles(i4, i1);
+    if (d <= 64) tiles(i2);
+    else if (d <= 128) tiles(i4);
+    else d <= 192 ? tiles(i6) : tiles(i8);
   }
   if (p.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(rows * hq), (d + 63) / 64), dim3(NT), 0, st, a);
   return 0;

@@ -124,8 +124,9 @@ def attention(c, q, start, lens, scale, gate):
 
     Bound, U an fp32 rounding: a score is a sum of d exact products, in fp32 with a rounding (up to 2 U) a term, and two factors: (2 d + 4) U
     of the sum of the products' magnitudes Z.  Its distance to the maximum (and 15, and the v scale's logarithm) is at most 300 where
-    the weight counts: 300 U, its power of two 2 U: rho = (2 d + 310) U max(Z, 1).  A weight is rounded to fp16 by 2^-11, or by
-    2^-25 2^-15 of the largest weight where small, in units of the largest v scale.  Weights and their sum share rho; the sums over n tokens round 2 n U.  Then the
+    the weight counts: 300 U, its power of two 2 U: rho = (2 d + 310) U max(Z, 1).  A weight is
+    rounded to fp16 by 2^-11, or where small by half of fp16's least step, 2^-25, of a value that stands for at least 2^-4 of a reference not above
+    the largest weight: 2^-29 of it, in units of the largest v scale.  Weights and their sum share rho; the sums over n tokens round 2 n U.  Then the
     division, the gate (exp, sum, division: 8 U), and one rounding to bf16, 2^-8."""
     rows, hq, d = q.shape
     y, bound = np.full(q.shape, np.nan), np.full(q.shape, np.nan)
@@ -150,7 +151,7 @@ def attention(c, q, start, lens, scale, gate):
                     w /= w.sum()
                     o, mag = w @ vv, w @ np.abs(vv)
                     rho = (2 * d + 310) * U * max(1, (abs(scale) * (np.abs(kk) @ np.abs(qq))).max())
-                    e = mag * (2.0 ** -11 + 2 * rho + (2 * len(kk) + 20) * U) + len(kk) * 2.0 ** -40 * unit
+                    e = mag * (2.0 ** -11 + 2 * rho + (2 * len(kk) + 20) * U) + len(kk) * 2.0 ** -29 * unit
                     if gate is not None:
                         s = 1 / (1 + np.exp(-gate[row, a]))
                         o, e = o * s, e * s
