@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   // those of O += V P of block k and of S = K Q of block k + 1 alternate.
   enum { WEIGH = 1, SCORE = 2 };
   auto products = [&](auto what, int k, int n) {
-    constexpr int M = decltype(what)::value, N = M == 3 ? 8 * DC : 4 * DC, T = N / 4, PT = T > 2 ? T - 2 : 1;
+    constexpr int M = decltype(what)::value, N = M == 3 ? 8 * DC : 4 * DC, T = N / 4;
     const half8* vf = vb + (k & 1) * 2 * F * WAVE + l;
     const half8* kf = kb + ((k + 1) & 1) * 2 * F * WAVE + l;
     auto is_score = [](int x) { return M == SCORE || (M == 3 && (x & 1)); };
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
       if (n >= 0 && M == 3) {
 #pragma unroll
         for (int f = 0; f < 4 * PER; ++f)
-          if (f * PT / (4 * PER) == c) put_part(n, f);
+          if (T - 1 - (4 * PER - f) * (T - 2) / (4 * PER + 2) == c) put_part(n, f);
         if (c == T - 1) put_loads(n);
       }
 #pragma unroll
@@ -639,7 +639,9 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   int k = 0;
   for (; k + 1 < mine_cnt; ++k) {
     soft(k);
+    __builtin_amdgcn_s_setprio(3);  // the products' few issues before the other wave's vector work: 342 us for 366
     products(both, k, k + 1);
+    __builtin_amdgcn_s_setprio(0);
   }
   for (; k < cnt; ++k) {
     soft(k);
