@@ -57,15 +57,18 @@ DEV float quad_sum(float v) { return xsum_step<32>(xsum_step<16>(v)); }
 DEV float lane_f(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
 // Four elements e .. of column p (row `row` of the call, query `head`): the finished output, or a part of it to be joined.
-// o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor; no token seen: o = l = 0.
-DEV void emit(const Attn& a, int split, size_t row, int head, int e, const f32x4& o, float l, float m) {
+// o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor; no token seen: o = l = 0.  alone: there is no other part, which
+// an l of kAlone tells the launch that joins.
+constexpr float kAlone = -1.f;
+DEV void emit(const Attn& a, bool alone, int split, size_t row, int head, int e, const f32x4& o, float l, float m) {
   const int d = a.c.d;
-  if (a.splits > 1) {
-    const size_t at = ((size_t)split * a.c.rows + row) * a.hq + head;
+  const size_t at = ((size_t)split * a.c.rows + row) * a.hq + head;
+  if (!alone) {
     *reinterpret_cast<f32x4*>(a.part + at * d + e) = o;
     if (e == 0) a.ml[2 * at] = m, a.ml[2 * at + 1] = l;
     return;
   }
+  if (a.splits > 1 && e == 0) a.ml[2 * at + 1] = kAlone;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float v[4];
 #pragma unroll
@@ -154,8 +157,8 @@ struct Pages {
   int page, ve;          // v's scale is a fraction in [1/2, 1) times 2^ve,
   float ks, lv, rv;      // the fraction's log2 and reciprocal
   unsigned long long have, num;  // blocks in the cache; those whose scales are numbers
-  DEV void fetch(const Attn& a, int seq, int h, int block, bool on) {
-    const int p = on ? page_of(a.c, seq, block) : -1;
+  DEV void fetch(const Attn& a, int seq, int h, int block, bool on) { fetch(a, h, on ? page_of(a.c, seq, block) : -1, on); }
+  DEV void fetch(const Attn& a, int h, int p, bool on) {
     have = __ballot(p >= 0);
     page = p >= 0 ? p : 0;
     ks = 0.f;
@@ -240,10 +243,11 @@ DEV void soften(Cols<DC, MT>& w, f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], const P
   }
 }
 
-// The blocks [b0, b1) of a sequence that split sp takes of the nb blocks that its columns see.
-DEV void share(const Attn& a, int nb, int sp, int& b0, int& b1) {
+// The blocks [b0, b1) of a sequence that split sp takes of the nb blocks that its columns see; true where the first takes all.
+DEV bool share(const Attn& a, int nb, int sp, int& b0, int& b1) {
   const int each = (nb + a.splits - 1) / a.splits, n = each > a.chunk ? each : a.chunk;
-  b0 = sp * n < nb ? sp * n : nb, b1 = b0 + n < nb ? b0 + n : nb;
+  b0 = (long long)sp * n < nb ? sp * n : nb, b1 = nb - b0 > n ? b0 + n : nb;
+  return nb <= n;
 }
 
 // A split without blocks leaves word of that for its columns [c0, c1).
@@ -262,7 +266,11 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
   __shared__ __align__(16) float sm[W * 16 * LD];
   __shared__ float sml[W * 32];
   const int l = lane_id(), j = l >> 4, wv = __builtin_amdgcn_readfirstlane(wave_id());
-  const int i = blockIdx.x, h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
+  // Consecutive blocks go to the eight dies in turn: heads first, and each split one sequence further, so that no die gets the long
+  // sequences (48 ragged ones: 81 us with the sequences in turn, 53).
+  const int h = blockIdx.x % a.c.hkv, sp = blockIdx.y, i = (int)((blockIdx.x / a.c.hkv + sp) % a.c.seqs), d = a.c.d, d16 = d >> 4, g = a.g;
+  // the table's entries as the host's word for the lengths has it, beside the sequence's length itself
+  const int ahead = page_of(a.c, i, (int)((long long)sp * a.chunk + wv + W * l < a.c.maxp ? sp * a.chunk + wv + W * l : -1));
   const Seq s = seq_of(a.c, i);
   const int np = s.n * g < TP ? s.n * g : TP;
   if (np == 0) return;
@@ -270,8 +278,11 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
   const int p_lo = s.first, p_end = s.first + (np - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
   const int nb = p_hi < 0 ? 0 : (p_hi >> 6) + 1;
   int b0, b1;
-  share(a, nb, sp, b0, b1);
-  if (b0 == b1 && sp > 0) return emit_none(a, s, h, sp, 0, np, threadIdx.x, NT);
+  const bool alone = share(a, nb, sp, b0, b1);
+  if (b0 == b1 && sp > 0) {
+    if (!alone) emit_none(a, s, h, sp, 0, np, threadIdx.x, NT);
+    return;
+  }
   const int cnt = (b1 - b0 - wv + W - 1) / W;  // the wave's blocks b0 + wv, b0 + wv + W ..
 
   int koff[DC];
@@ -295,7 +306,8 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
   Pages pg;
   Cols<DC, MT> w;
   // the first block's bytes are on their way while the queries arrive
-  pg.fetch(a, i, h, b0 + wv + W * l, l < cnt);
+  if (b0 == sp * a.chunk) pg.fetch(a, h, l < cnt ? ahead : -1, l < cnt);
+  else pg.fetch(a, i, h, b0 + wv + W * l, l < cnt);
   if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
   begin(w, a, s, h, 0, np);
   for (int k0 = 0; k0 < cnt; k0 += WAVE) {
@@ -359,7 +371,7 @@ __global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < W; ++z) v += wt[z] * *reinterpret_cast<const f32x4*>(sm + (z * 16 + col) * LD + e);
-        emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, e, v, ll, mm);
+        emit(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, e, v, ll, mm);
       }
   }
 }
@@ -510,8 +522,11 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   const long long cap = (long long)a.c.maxp * KB - 1;
   const int p_end = s.first + (c1 - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
   int b0, b1;
-  share(a, p_hi < 0 ? 0 : (p_hi >> 6) + 1, sp, b0, b1);
-  if (b0 == b1 && sp > 0) return emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);
+  const bool alone = share(a, p_hi < 0 ? 0 : (p_hi >> 6) + 1, sp, b0, b1);
+  if (b0 == b1 && sp > 0) {
+    if (!alone) emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);
+    return;
+  }
   const int cnt = b1 - b0;
   // the wave's columns and how many of the blocks they see
   const int w0 = c0 + 32 * wv, w1 = w0 + 32 < c1 ? w0 + 32 : c1;
@@ -660,49 +675,50 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
       for (int r = 0; r < 16; r += 4) {
         const int e = 32 * u + 2 * r + 4 * (z >> 5);
         if (e < d)
-          emit(a, sp, (size_t)s.r0 + row, h * g + p - row * g, e, f32x4{w.o[u][r] * us, w.o[u][r + 1] * us, w.o[u][r + 2] * us, w.o[u][r + 3] * us}, sum, w.m);
+          emit(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, e, f32x4{w.o[u][r] * us, w.o[u][r + 1] * us, w.o[u][r + 2] * us, w.o[u][r + 3] * us}, sum, w.m);
       }
 }
 
-// Joins the parts of 64 elements of a row's query: 16 groups of 16 lanes take every 16th part, all their loads together.
+// Joins the parts of a row's query, or of 64 elements of it where the queries are few: LE lanes of four elements, each group of them every
+// NT / LE'th part, four at a time in flight, with a maximum of its own; the groups meet in LDS.
 constexpr int kSplits = 128;  // at most
-__global__ void __launch_bounds__(NT) k_attn_join(Attn a) {
-  __shared__ __align__(16) f32x4 sm[NT];
-  __shared__ float wt[kSplits], red[2 * W];
-  const int head = blockIdx.x % a.hq, row = blockIdx.x / a.hq;
-  if (row < a.c.start[0] || row >= a.c.start[a.c.seqs]) return;
-  const int t = threadIdx.x, grp = t >> 4, e = 64 * blockIdx.y + 4 * (t & 15), d = a.c.d;
+__global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
+  __shared__ __align__(16) f32x4 so[NT];
+  __shared__ float sm[NT / 16], sl[NT / 16];
+  const int head = blockIdx.x % a.hq, row = blockIdx.x / a.hq, t = threadIdx.x, G = NT / LE, grp = t / LE, d = a.c.d;
+  const int e = 4 * (LE * blockIdx.y + (t & (LE - 1)));
   const size_t at = (size_t)row * a.hq + head, step = (size_t)a.c.rows * a.hq;
   float m = -kInf, s = 0.f;
-  if (t < a.splits) m = a.ml[2 * (at + t * step)], s = a.ml[2 * (at + t * step) + 1];
-  float mm = wave_max(m);
-  if (lane_id() == 0) red[wave_id()] = mm;
-  __syncthreads();
-  mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float p = m == -kInf && mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - mm);
-  if (t < a.splits) wt[t] = s == 0.f ? 0.f : p;  // a part that saw no token has no sums
-  s = wave_sum(s * p);
-  if (lane_id() == 0) red[W + wave_id()] = s;
-  __syncthreads();
-  f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f}, r[kSplits / 16];
+  f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = grp; s0 < a.splits; s0 += 4 * G) {
+    uint2 w[4];
+    f32x4 r[4];
 #pragma unroll
-  for (int k = 0; k < kSplits / 16; ++k) {
-    const int sp = grp + 16 * k;
-    r[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (sp < a.splits && wt[sp] != 0.f && e < d) r[k] = *reinterpret_cast<const f32x4*>(a.part + (at + sp * step) * d + e);
+    for (int k = 0; k < 4; ++k) {
+      const int sp = s0 + G * k < a.splits ? s0 + G * k : s0;
+      w[k] = ld8(a.ml + 2 * (at + sp * step));
+      r[k] = gld<f32x4>(a.part + (at + sp * step) * d + (e < d ? e : 0));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float pm = __uint_as_float(w[k].x), pl = __uint_as_float(w[k].y);
+      if (s0 + G * k >= a.splits || pl == 0.f) continue;  // a part that saw no token has no sums
+      if (s0 + k == 0 && pl == kAlone) s = kAlone;
+      const float mn = fmaxf(m, pm), c0 = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - mn), c1 = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f(pm - mn);
+      if (s != kAlone) v = c0 * v + c1 * r[k], s = c0 * s + c1 * pl, m = mn;
+    }
   }
-#pragma unroll
-  for (int k = 0; k < kSplits / 16; ++k)
-    if (grp + 16 * k < a.splits) v += wt[grp + 16 * k] * r[k];
-  sm[t] = v;
+  so[t] = v;
+  if ((t & (LE - 1)) == 0) sm[grp] = m, sl[grp] = s;
   __syncthreads();
-  if (t < 16 && e < d) {
-#pragma unroll
-    for (int k = 1; k < 16; ++k) v += sm[16 * k + t];
-    Attn o = a;
-    o.splits = 1;
-    emit(o, 0, row, head, e, v, red[W] + red[W + 1] + red[W + 2] + red[W + 3], 0.f);
+  if (grp || sl[0] == kAlone || row < a.c.start[0] || row >= a.c.start[a.c.seqs] || e >= d) return;
+  for (int k = 1; k < G; ++k) {
+    if (sl[k] == 0.f) continue;
+    const float mn = fmaxf(m, sm[k]), c0 = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - mn), c1 = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f(sm[k] - mn);
+    v = c0 * v + c1 * so[k * LE + t], s = c0 * s + c1 * sl[k], m = mn;
   }
+  a.splits = 1;
+  emit(a, true, 0, row, head, e, v, s, 0.f);
 }
 
 // How a call is cut: by its sizes alone, so that the workspace is known before.
@@ -723,7 +739,7 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   p.nw = p.few || d > 128 ? 4 : 8;
   cut(p.few ? 16 * p.mt : 32 * p.nw);
   if (p.nw == 8 && p.tiles * hkv < 256) p.nw = 4, cut(32 * p.nw);
-  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = p.few ? 2048 : 512;
+  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = p.few && p.mt == 1 ? 2048 : 512;
   long long s = units >= want / 2 && !p.few ? 1 : (want + units - 1) / units;
   const long long most = (blocks + W - 1) / W;
   s = s > most ? most : s;
@@ -764,7 +780,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
                (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan};
   const dim3 grid((unsigned)p.tiles, hkv, p.splits);
   auto few = [&](auto dc, auto mt) {
-    hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), grid, dim3(NT), 0, st, a);
+    hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), dim3((unsigned)(seqs * hkv), p.splits), dim3(NT), 0, st, a);
   };
   auto tiles = [&](auto dc) {
     constexpr int DC = decltype(dc)::value;
@@ -790,6 +806,11 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
     else if (d <= 128) tiles(i4);
     else d <= 192 ? tiles(i6) : tiles(i8);
   }
-  if (p.splits > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(rows * hq), (d + 63) / 64), dim3(NT), 0, st, a);
+  if (p.splits > 1) {
+    int le = 16;
+    if ((long long)rows * hq >= 512)
+      while (4 * le < d) le <<= 1;
+    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(rows * hq), (d + 4 * le - 1) / (4 * le)), dim3(NT), 0, st, a, le);
+  }
   return 0;
 }
