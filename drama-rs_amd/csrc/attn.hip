@@ -56,7 +56,20 @@ DEV float quad_max(float v) { return xmax_step<32>(xmax_step<16>(v)); }
 DEV float quad_sum(float v) { return xsum_step<32>(xsum_step<16>(v)); }
 DEV float lane_f(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
-// Four elements e .. of column p (row `row` of the call, query `head`): the finished output, or a part of it to be joined.
+// Four elements e .. of the output of a row's query `head`: o / l (0 where no token was seen), its gate, bf16.
+DEV void finish(const Attn& a, size_t row, int head, int e, const f32x4& o, float l, const float4& g) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = o[i] * inv;
+  if (a.gate) v[0] /= 1.f + expf(-g.x), v[1] /= 1.f + expf(-g.y), v[2] /= 1.f + expf(-g.z), v[3] /= 1.f + expf(-g.w);
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = to_bf16(v[i]);
+  *reinterpret_cast<uint2*>(a.y + row * a.ldy + (size_t)head * a.c.d + e) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+}
+
+// The same, or a part of it to be joined.
 // o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor; no token seen: o = l = 0.  alone: there is no other part, which
 // an l of kAlone tells the launch that joins.
 constexpr float kAlone = -1.f;
@@ -69,18 +82,7 @@ DEV void emit(const Attn& a, bool alone, int split, size_t row, int head, int e,
     return;
   }
   if (a.splits > 1 && e == 0) a.ml[2 * at + 1] = kAlone;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = o[i] * inv;
-  if (a.gate) {
-    const float4 g = ldf4(a.gate + row * a.ldg + head * a.hsg + e);
-    v[0] /= 1.f + expf(-g.x), v[1] /= 1.f + expf(-g.y), v[2] /= 1.f + expf(-g.z), v[3] /= 1.f + expf(-g.w);
-  }
-  uint32_t b[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) b[i] = to_bf16(v[i]);
-  *reinterpret_cast<uint2*>(a.y + row * a.ldy + (size_t)head * d + e) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+  finish(a, row, head, e, o, l, a.gate ? ldf4(a.gate + row * a.ldg + head * a.hsg + e) : make_float4(0.f, 0.f, 0.f, 0.f));
 }
 
 // A wave's columns: MT tiles of 16, lane l holds column l & 15 of each.  DC: 64-element chunks of a head.
@@ -261,7 +263,7 @@ DEV void emit_none(const Attn& a, const Seq& s, int h, int sp, int c0, int c1, i
 // Few columns: the four waves of a block of threads hold the same MT tiles of them and take every fourth cached block.  The last chunk of a
 // head may be part of one: what lies past d is loaded from inside the head, times zero queries, and not stored.
 template <int DC, int MT>
-__global__ void __launch_bounds__(NT) k_attn_few(Attn a) {
+__global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   constexpr int TP = 16 * MT, LD = 64 * DC + 4;
   __shared__ __align__(16) float sm[W * 16 * LD];
   __shared__ float sml[W * 32];
@@ -680,45 +682,60 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
 }
 
 // Joins the parts of a row's query, or of 64 elements of it where the queries are few: LE lanes of four elements, each group of them every
-// NT / LE'th part, four at a time in flight, with a maximum of its own; the groups meet in LDS.
+// NT / LE'th part, eight at a time in flight, with a maximum of its own; the groups meet in LDS.
 constexpr int kSplits = 128;  // at most
 __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
+  constexpr int P = 8;
   __shared__ __align__(16) f32x4 so[NT];
   __shared__ float sm[NT / 16], sl[NT / 16];
   const int head = blockIdx.x % a.hq, row = blockIdx.x / a.hq, t = threadIdx.x, G = NT / LE, grp = t / LE, d = a.c.d;
   const int e = 4 * (LE * blockIdx.y + (t & (LE - 1)));
   const size_t at = (size_t)row * a.hq + head, step = (size_t)a.c.rows * a.hq;
+  float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (a.gate && grp == 0 && e < d) gate = ldf4(a.gate + row * a.ldg + head * a.hsg + e);
   float m = -kInf, s = 0.f;
   f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s0 = grp; s0 < a.splits; s0 += 4 * G) {
-    uint2 w[4];
-    f32x4 r[4];
+  bool whole = false;
+  for (int s0 = grp; s0 < a.splits; s0 += P * G) {
+    uint2 w[P];
+    f32x4 r[P];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int sp = s0 + G * k < a.splits ? s0 + G * k : s0;
-      w[k] = ld8(a.ml + 2 * (at + sp * step));
-      r[k] = gld<f32x4>(a.part + (at + sp * step) * d + (e < d ? e : 0));
+    for (int k = 0; k < P; ++k) {
+      const size_t sp = at + (s0 + G * k) * step;
+      w[k] = make_uint2(0, 0), r[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (s0 + G * k < a.splits) w[k] = ld8(a.ml + 2 * sp), r[k] = gld<f32x4>(a.part + sp * d + (e < d ? e : 0));
     }
+    float mn = m;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float pm = __uint_as_float(w[k].x), pl = __uint_as_float(w[k].y);
-      if (s0 + G * k >= a.splits || pl == 0.f) continue;  // a part that saw no token has no sums
-      if (s0 + k == 0 && pl == kAlone) s = kAlone;
-      const float mn = fmaxf(m, pm), c0 = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - mn), c1 = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f(pm - mn);
-      if (s != kAlone) v = c0 * v + c1 * r[k], s = c0 * s + c1 * pl, m = mn;
+    for (int k = 0; k < P; ++k)
+      if (w[k].y != 0) mn = fmaxf(mn, __uint_as_float(w[k].x));  // a part that saw no token (l = 0) has no sums
+    if (s0 == 0) whole = __uint_as_float(w[0].y) == kAlone;
+    const float ms = mn == -kInf ? 0.f : mn, c0 = __builtin_amdgcn_exp2f(m - ms);
+    v *= c0, s *= c0, m = mn;
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      if (w[k].y == 0) continue;
+      const float c = __builtin_amdgcn_exp2f(__uint_as_float(w[k].x) - ms);
+      v += c * r[k], s += c * __uint_as_float(w[k].y);
     }
   }
   so[t] = v;
-  if ((t & (LE - 1)) == 0) sm[grp] = m, sl[grp] = s;
+  if ((t & (LE - 1)) == 0) sm[grp] = m, sl[grp] = whole ? kAlone : s;
   __syncthreads();
   if (grp || sl[0] == kAlone || row < a.c.start[0] || row >= a.c.start[a.c.seqs] || e >= d) return;
-  for (int k = 1; k < G; ++k) {
-    if (sl[k] == 0.f) continue;
-    const float mn = fmaxf(m, sm[k]), c0 = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - mn), c1 = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f(sm[k] - mn);
-    v = c0 * v + c1 * so[k * LE + t], s = c0 * s + c1 * sl[k], m = mn;
-  }
-  a.splits = 1;
-  emit(a, true, 0, row, head, e, v, s, 0.f);
+  float mn = -kInf;
+#pragma unroll
+  for (int k = 0; k < NT / 16; ++k)
+    if (k < G) mn = fmaxf(mn, sm[k]);
+  const float ms = mn == -kInf ? 0.f : mn;
+  s = 0.f, v = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < NT / 16; ++k)
+    if (k < G) {
+      const float c = __builtin_amdgcn_exp2f(sm[k] - ms);
+      v += c * so[k * LE + t], s += c * sl[k];
+    }
+  finish(a, row, head, e, v, s, gate);
 }
 
 // How a call is cut: by its sizes alone, so that the workspace is known before.

@@ -50,6 +50,12 @@ DEV void ld_x(const void* x, size_t at, float (&o)[V]) {
   }
 }
 
+// two fp32 to bf16, nearest even, in one instruction
+DEV uint32_t pack_bf16(float a, float b) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, bf2{(__bf16)a, (__bf16)b});
+}
+
 template <int V>
 DEV void st_y(const Rope& a, size_t row, int at, const float (&o)[V]) {
   if (a.y) {
@@ -59,11 +65,8 @@ DEV void st_y(const Rope& a, size_t row, int at, const float (&o)[V]) {
   }
   if (a.yb) {
     uint16_t* p = a.yb + row * a.ldb + at;
-    uint32_t q[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) q[v] = to_bf16(o[v]);
-    if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
-    else *p = (uint16_t)q[0];
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+    else *p = to_bf16(o[0]);
   }
 }
 
@@ -78,42 +81,50 @@ DEV float head_sum(float v, int L) {
   return v;
 }
 
-// V elements a load (4, or 1 where sizes, strides or addresses allow no more); a unit is two vectors: partners of V pairs, or
-// elements behind rot.  L lanes a head, up to PER units a lane; RB rows a block.
-template <bool B16, int V, int PER>
-__global__ void __launch_bounds__(NT) k_rope(Rope a, int L, int RB) {
+// V elements a load (4, or 1 where sizes, strides or addresses allow no more).  A unit is a vector of the first half of the turned elements and
+// its counterpart in the second (the partners, or V / 2 pairs each), or two vectors of the elements behind rot likewise: lanes beside each other
+// load and store beside each other.  2^LS lanes a head, up to PER units a lane; RB rows a block; U heads a lane at a time.
+template <bool B16, int V, int PER, int U>
+__global__ void __launch_bounds__(NT) k_rope(Rope a, int LS, int RB) {
   extern __shared__ float2 cs[];  // [RB][rot / 2]
-  const int half = a.rot >> 1, turned = half / V, units = turned + (a.d - a.rot + 2 * V - 1) / (2 * V);
+  const int half = a.rot >> 1, turned = half / V, tail = (a.d - a.rot + 2 * V - 1) / (2 * V), units = turned + tail;
   const long long r0 = (long long)blockIdx.x * RB;
-  const int nr = a.rows - r0 < RB ? (int)(a.rows - r0) : RB, items = nr * a.heads * L;
+  const int nr = a.rows - r0 < RB ? (int)(a.rows - r0) : RB, items = (nr * a.heads) << LS, l = threadIdx.x & ((1 << LS) - 1);
+  int e0[PER], e1[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int k = l + (u << LS);
+    e0[u] = k < turned ? V * k : a.rot + V * (k - turned);
+    e1[u] = k < turned ? e0[u] + half : e0[u] + V * tail;
+    if (V == 1 && a.pairs && k < turned) e0[u] = 2 * k, e1[u] = 2 * k + 1;  // a unit is one pair
+    if (k >= units) e0[u] = e1[u] = a.d;
+  }
   bool ready = false;
-  for (int w0 = 0; w0 < items; w0 += NT) {
-    const int w = w0 + threadIdx.x, l = w & (L - 1), hr = w / L, rl = hr / a.heads, h = hr - rl * a.heads;
-    const bool on = w < items;
-    const size_t r = (size_t)r0 + rl, xb = r * a.ldx + (size_t)h * a.hsx;
-    float p[PER][2][V], nw[PER][2][V];
-    int e0[PER], e1[PER];
+  for (int w0 = threadIdx.x; w0 - (int)threadIdx.x < items; w0 += U * NT) {
+    float p[U][PER][2][V], nw[U][PER][2][V];
+    int h[U], rl[U];
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int k = l + L * u;
-      // the two vectors' first elements
-      if (k >= turned) e0[u] = a.rot + 2 * V * (k - turned), e1[u] = e0[u] + V;
-      else if (a.pairs) e0[u] = 2 * V * k, e1[u] = e0[u] + V;
-      else e0[u] = V * k, e1[u] = e0[u] + half;
-      if (!on || k >= units) e0[u] = e1[u] = a.d;
+    for (int x = 0; x < U; ++x) {
+      const int w = w0 + NT * x, hr = w >> LS;
+      rl[x] = RB == 1 ? 0 : hr / a.heads, h[x] = hr - rl[x] * a.heads;
+      const size_t xb = (size_t)(r0 + rl[x]) * a.ldx + (size_t)h[x] * a.hsx;
 #pragma unroll
-      for (int v = 0; v < V; ++v) p[u][0][v] = p[u][1][v] = 0.f, nw[u][0][v] = nw[u][1][v] = 1.f;
-      if (e0[u] < a.d) ld_x<B16, V>(a.x, xb + e0[u], p[u][0]);
-      if (e1[u] < a.d) ld_x<B16, V>(a.x, xb + e1[u], p[u][1]);
-      if (a.nw) {
-        if (e0[u] < a.d) ld_x<false, V>(a.nw, h * a.ldn + e0[u], nw[u][0]);
-        if (e1[u] < a.d) ld_x<false, V>(a.nw, h * a.ldn + e1[u], nw[u][1]);
-      }
+      for (int u = 0; u < PER; ++u)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int e = b ? e1[u] : e0[u];
+#pragma unroll
+          for (int v = 0; v < V; ++v) p[x][u][b][v] = 0.f, nw[x][u][b][v] = 1.f;
+          if (w < items && e < a.d) {
+            ld_x<B16, V>(a.x, xb + e, p[x][u][b]);
+            if (a.nw) ld_x<false, V>(a.nw, h[x] * a.ldn + e, nw[x][u][b]);
+          }
+        }
     }
     if (!ready) {
       // behind the first loads, which are on their way meanwhile
       for (int t = threadIdx.x; t < nr * half; t += NT) {
-        const int tr = t / half;
+        const int tr = RB == 1 ? 0 : t / half;
         double turns = (double)a.pos[r0 + tr] * (double)a.freq[t - tr * half] * 0.15915494309189533577;
         turns -= rint(turns);
         float sn, cn;
@@ -123,36 +134,47 @@ __global__ void __launch_bounds__(NT) k_rope(Rope a, int L, int RB) {
       __syncthreads();
       ready = true;
     }
-    if (a.nw) {
-      float ss = 0.f;
 #pragma unroll
-      for (int u = 0; u < PER; ++u)
+    for (int x = 0; x < U; ++x) {
+      if (a.nw) {
+        float ss = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) ss += p[u][0][v] * p[u][0][v] + p[u][1][v] * p[u][1][v];
-      const float inv = rsqrtf(head_sum(ss, L) / (float)a.d + a.eps);
+        for (int u = 0; u < PER; ++u)
 #pragma unroll
-      for (int u = 0; u < PER; ++u)
+          for (int v = 0; v < V; ++v) ss += p[x][u][0][v] * p[x][u][0][v] + p[x][u][1][v] * p[x][u][1][v];
+        const float inv = rsqrtf(head_sum(ss, 1 << LS) / (float)a.d + a.eps);
 #pragma unroll
-        for (int v = 0; v < V; ++v) p[u][0][v] *= inv * nw[u][0][v], p[u][1][v] *= inv * nw[u][1][v];
-    }
+        for (int u = 0; u < PER; ++u)
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int k = l + L * u;
-      if (e0[u] >= a.d) continue;
-      if (k < turned) {
-        const float2* c = cs + rl * half + V * k;
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          // in pairs the 2 V elements are a, b, a, b, ..
-          float& x0 = a.pairs && V > 1 ? (v < V / 2 ? p[u][0][(2 * v) % V] : p[u][1][(2 * v) % V]) : p[u][0][v];
-          float& x1 = a.pairs && V > 1 ? (v < V / 2 ? p[u][0][(2 * v + 1) % V] : p[u][1][(2 * v + 1) % V]) : p[u][1][v];
-          const float2 t = c[v];
-          const float x = x0 * t.x - x1 * t.y, y = x1 * t.x + x0 * t.y;
-          x0 = x, x1 = y;
-        }
+            for (int v = 0; v < V; ++v) p[x][u][b][v] *= inv * nw[x][u][b][v];
       }
-      st_y<V>(a, r, h * a.d + e0[u], p[u][0]);
-      if (e1[u] < a.d) st_y<V>(a, r, h * a.d + e1[u], p[u][1]);
+      if (w0 + NT * x >= items) continue;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        if (e0[u] >= a.d) continue;
+        if (e0[u] < a.rot) {
+          const float2* c = cs + rl[x] * half;
+          auto turn = [](float& m, float& n, const float2& t) {
+            const float y = m * t.x - n * t.y;
+            n = n * t.x + m * t.y, m = y;
+          };
+          if (!a.pairs) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) turn(p[x][u][0][v], p[x][u][1][v], c[e0[u] + v]);
+          } else if constexpr (V == 1) {
+            turn(p[x][u][0][0], p[x][u][1][0], c[e0[u] >> 1]);
+          } else {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int v = 0; v < V; v += 2) turn(p[x][u][b][v], p[x][u][b][(v + 1) % V], c[(b ? e1[u] : e0[u]) / 2 + v / 2]);
+          }
+        }
+        st_y<V>(a, (size_t)(r0 + rl[x]), h[x] * a.d + e0[u], p[x][u][0]);
+        if (e1[u] < a.d) st_y<V>(a, (size_t)(r0 + rl[x]), h[x] * a.d + e1[u], p[x][u][1]);
+      }
     }
   }
 }
@@ -169,14 +191,15 @@ int rope(const Rope& a, int ldx, int hsx, int ldn, int ldy, int ldb, hipStream_t
   const bool vec = a.d % 4 == 0 && a.rot % 8 == 0 && al(a.x, B16 ? 8 : 16) && ldx % 4 == 0 && hsx % 4 == 0 && al(a.nw, 16) && ldn % 4 == 0 &&
                    (!a.y || (al(a.y, 16) && ldy % 4 == 0)) && (!a.yb || (al(a.yb, 8) && ldb % 4 == 0));
   const int V = vec ? 4 : 1, units = (a.rot >> 1) / V + (a.d - a.rot + 2 * V - 1) / (2 * V);
-  int L = 1;
-  while (L < units && L < WAVE) L <<= 1;
-  const int per_row = a.heads * L, RB = per_row >= NT ? 1 : NT / per_row;
+  int LS = 0;
+  while ((1 << LS) < units && LS < 6) ++LS;
+  const int per_row = a.heads << LS, RB = per_row >= NT ? 1 : NT / per_row;
   const dim3 g((unsigned)(((long long)a.rows + RB - 1) / RB)), b(NT);
   const size_t lds = (size_t)RB * (a.rot >> 1) * sizeof(float2);
-  if (vec) hipLaunchKernelGGL((k_rope<B16, 4, 1>), g, b, lds, st, a, L, RB);
-  else if (units <= L) hipLaunchKernelGGL((k_rope<B16, 1, 1>), g, b, lds, st, a, L, RB);
-  else hipLaunchKernelGGL((k_rope<B16, 1, 4>), g, b, lds, st, a, L, RB);
+  if (vec && per_row > NT) hipLaunchKernelGGL((k_rope<B16, 4, 1, 2>), g, b, lds, st, a, LS, RB);
+  else if (vec) hipLaunchKernelGGL((k_rope<B16, 4, 1, 1>), g, b, lds, st, a, LS, RB);
+  else if (units <= 1 << LS) hipLaunchKernelGGL((k_rope<B16, 1, 1, 1>), g, b, lds, st, a, LS, RB);
+  else hipLaunchKernelGGL((k_rope<B16, 1, 4, 1>), g, b, lds, st, a, LS, RB);
   return 0;
 }
 
