@@ -515,10 +515,10 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   const bool late = NW == 8 && wv >= 4;
   const int h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
   int at = gridDim.x - 1 - blockIdx.x, i = at;  // the last rows, which see most, first
-  if (a.scan) i = find_item(a.c, at, [g](const Seq& s) { return (s.n * g + TP - 1) / TP; });
-  else at = 0;
+  Seq s;
+  if (a.scan) i = find_item(a.c, at, s, [g](const Seq& q) { return (q.n * g + TP - 1) / TP; });
+  else at = 0, s = seq_of(a.c, i);
   if (i < 0) return;
-  const Seq s = seq_of(a.c, i);
   const int np = a.scan || s.n * g < TP ? s.n * g : TP, c0 = at * TP, c1 = c0 + TP < np ? c0 + TP : np;
   if (c0 >= np) return;
   const long long cap = (long long)a.c.maxp * KB - 1;

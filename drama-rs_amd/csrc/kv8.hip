@@ -12,8 +12,8 @@ using namespace drm;
 
 namespace {
 
-constexpr int NT = 256;
-constexpr int VROW = KB + 16;  // LDS row of v's 64 bytes: 16-byte pieces, four banks further each row
+constexpr int NT = 512;
+constexpr int UNITS = 1024 / NT;  // of 4 tokens x 4 elements a thread: 64 tokens of up to 256 elements
 
 struct Append {
   Kv8 c;
@@ -21,24 +21,36 @@ struct Append {
   size_t ldk, ldv;
 };
 
-template <bool B16>
-DEV void ld_elems(const void* p, size_t at, float (&o)[16]) {
-  if constexpr (B16) {
-    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at);
+// Unit n of a block (16 d / 4 of them) is four dwords of it.  k: elements e .. e + 3 of tokens t + 16 i, a dword a token; v: tokens t .. t + 3 of
+// elements e + i, a dword an element.  Either way a wave's dwords lie beside each other in runs of 64 bytes or more, and the 16-byte pieces
+// of the rows outside in runs of 64.
+struct Unit {
+  int t, e;
+  size_t at[4];  // of the dwords in the block
+};
+DEV Unit unit_of(bool isv, int n) {
+  Unit u;
+  if (isv) {
+    const int m = n & 15;  // dword of a row: tokens 16 (m & 3) + 4 (m >> 2) ..
+    u.t = 16 * (m & 3) + 4 * (m >> 2), u.e = n >> 4 << 2;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 w = ld16(q + i);
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[8 * i + 2 * e] = bf16_lo(ww[e]), o[8 * i + 2 * e + 1] = bf16_hi(ww[e]);
-    }
+    for (int i = 0; i < 4; ++i) u.at[i] = (size_t)(u.e + i) * KB + 4 * m;
   } else {
-    const float* q = reinterpret_cast<const float*>(p) + at;
+    u.t = n >> 2 & 15, u.e = (n >> 6) * 16 + 4 * (n & 3);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 w = ldf4(q + 4 * i);
-      o[4 * i] = w.x, o[4 * i + 1] = w.y, o[4 * i + 2] = w.z, o[4 * i + 3] = w.w;
-    }
+    for (int i = 0; i < 4; ++i) u.at[i] = ((size_t)(n >> 6) * KB + u.t + 16 * i) * 16 + 4 * (n & 3);
+  }
+  return u;
+}
+DEV int token_of(bool isv, const Unit& u, int i) { return isv ? u.t + i : u.t + 16 * i; }
+
+template <bool B16>
+DEV float4 ld4_elems(const void* p, size_t at) {
+  if constexpr (B16) {
+    const uint2 w = ld8(reinterpret_cast<const uint16_t*>(p) + at);
+    return make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
+  } else {
+    return ldf4(reinterpret_cast<const float*>(p) + at);
   }
 }
 
@@ -65,130 +77,195 @@ DEV uint32_t shrink4(uint32_t w, int j) {
   return o;
 }
 
-DEV int v_at(int t) { return 16 * ((t >> 2) & 3) + 4 * (t >> 4) + (t & 3); }
+// A block's scale s with tokens of largest magnitude `top` (infinity: some are no numbers) in it, 2^grow times s_old; first: its first token is
+// among them.
+struct Scale {
+  float s, lift, sl, inv;
+  int grow;
+  bool none;
+  DEV uint32_t byte(float v) const { return (uint32_t)((none ? 0 : quant(v * lift, sl, inv)) + 128); }
+};
+DEV Scale scale_of(float top, float s_old, bool first) {
+  Scale q;
+  q.grow = 0;
+  if (!(top < __builtin_inff()) || (!first && !(s_old < __builtin_inff()))) {
+    q.s = __builtin_nanf("");  // the block stands for no numbers
+  } else if (first || s_old == 0.f) {
+    q.s = (float)((double)top / 127.0);
+  } else {
+    // 127 s_old and the comparisons are exact in 64 bits
+    const double most = 127.0 * (double)s_old;
+    if ((double)top > most) {
+      int e;
+      const double m = frexp((double)top / most, &e);
+      q.grow = m == 0.5 ? e - 1 : e;
+    }
+    q.s = __builtin_ldexpf(s_old, q.grow);
+  }
+  // tiny scales are lifted by a power of two, so that their reciprocal is a normal number
+  q.none = !(q.s > 0.f);
+  q.lift = q.s < 0x1p-90f ? 0x1p90f : 1.f, q.sl = q.s * q.lift, q.inv = q.none ? 0.f : 1.f / q.sl;
+  return q;
+}
+DEV bool finite4(const float4& v) {
+  return fabsf(v.x) < __builtin_inff() && fabsf(v.y) < __builtin_inff() && fabsf(v.z) < __builtin_inff() && fabsf(v.w) < __builtin_inff();
+}
+DEV float top4(const float4& v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
+// A few tokens a sequence (decode steps): a wave owns a head's k or v of a block, a lane four elements of each token; tokens past the fourth
+// are loaded again.  Bound by its chain of loads (sequence, rows beside the table, scale): XXX
 template <bool B16>
-__global__ void __launch_bounds__(NT) k_kv8_append(Append a) {
-  __shared__ float red[NT / WAVE + 1];
-  __shared__ __align__(16) uint8_t vt[256 * VROW];
+__global__ void __launch_bounds__(256) k_kv8_append_few(Append a) {
   int at = blockIdx.x;
-  const int i = find_item(a.c, at, seq_blocks);
-  if (i < 0) return;
-  const Seq s = seq_of(a.c, i);
-  const int b = (s.first >> 6) + at, page = page_of(a.c, i, b);
-  if (page < 0) return;
-  const int h = blockIdx.y >> 1, d = a.c.d, d16 = d >> 4;
-  const bool isv = blockIdx.y & 1;
-  // the block's places [t0, t1) get rows r .. of the call
+  Seq s;
+  const int i = find_item(a.c, at, s, seq_blocks);
+  const int y = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+  if (i < 0 || y >= 2 * a.c.hkv) return;
+  const int b = (s.first >> 6) + at, h = y >> 1, d = a.c.d, l = lane_id(), e = 4 * l;
+  const bool isv = y & 1, on = e < d;
   const int t0 = s.first > b * KB ? s.first - b * KB : 0, t1 = s.len - b * KB < KB ? s.len - b * KB : KB;
-  const size_t r = (size_t)s.r0 + (b * KB + t0 - s.first), ld = isv ? a.ldv : a.ldk;
+  const size_t ld = isv ? a.ldv : a.ldk, r = ((size_t)s.r0 + (b * KB + t0 - s.first)) * ld + (size_t)h * d + e;
   const void* src = isv ? a.v : a.k;
+  float4 x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on && t0 + k < t1) x[k] = ld4_elems<B16>(src, r + k * ld);
+  }
+  const int page = page_of(a.c, i, b);
+  if (page < 0) return;
   const size_t ph = (size_t)page * a.c.hkv + h;
   uint8_t* blk = (isv ? a.c.vq : a.c.kq) + ph * KB * d;
   float* scale = (isv ? a.c.vs : a.c.ks) + ph;
-  if (threadIdx.x == 0) red[NT / WAVE] = *scale;  // read by the thread that writes it
-  const int units = (t1 - t0) * d16;
-  float x[4][16];
+  const float s_old = *scale;
   float top = 0.f;
   bool fine = true;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int w = threadIdx.x + NT * u;
-    if (w >= units) break;
-    const int t = w / d16, c = w - t * d16;
-    ld_elems<B16>(src, (r + t) * ld + (size_t)h * d + 16 * c, x[u]);
+  for (int k = 0; k < 4; ++k) top = fmaxf(top, top4(x[k])), fine = fine && finite4(x[k]);
+  for (int t = t0 + 4; t < t1; ++t) {
+    if (!on) continue;
+    const float4 v = ld4_elems<B16>(src, r + (t - t0) * ld);
+    top = fmaxf(top, top4(v)), fine = fine && finite4(v);
   }
+  top = wave_max(fine ? top : __builtin_inff());
+  const Scale q = scale_of(top, s_old, t0 == 0);
+  if (q.grow && t0 > 0) {
+    // 16 bytes are 16 elements of a token (k: the lane's token), or of an element 16 tokens, new ones among them that are written below
+    for (int n = l; n < 4 * d; n += WAVE) {
+      if (!isv && (n & (KB - 1)) >= t0) continue;
+      uint4* p = reinterpret_cast<uint4*>(blk) + n;
+      uint4 o = *p;
+      o.x = shrink4(o.x, q.grow), o.y = shrink4(o.y, q.grow), o.z = shrink4(o.z, q.grow), o.w = shrink4(o.w, q.grow);
+      *p = o;
+    }
+    // the new tokens' bytes come from other lanes than these
+    __builtin_amdgcn_s_waitcnt(0);
+  }
+  auto put = [&](int t, const float4& v) {
+    const uint32_t w = q.byte(v.x) | q.byte(v.y) << 8 | q.byte(v.z) << 16 | q.byte(v.w) << 24;
+    if (isv) {
+      uint8_t* p = blk + (size_t)e * KB + 16 * (t >> 2 & 3) + 4 * (t >> 4) + (t & 3);
+      p[0] = (uint8_t)w, p[KB] = (uint8_t)(w >> 8), p[2 * KB] = (uint8_t)(w >> 16), p[3 * KB] = (uint8_t)(w >> 24);
+    } else {
+      *reinterpret_cast<uint32_t*>(blk + ((size_t)(e >> 4) * KB + t) * 16 + (e & 15)) = w;
+    }
+  };
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    if ((int)threadIdx.x + NT * u >= units) break;
+  for (int k = 0; k < 4; ++k)
+    if (on && t0 + k < t1) put(t0 + k, x[k]);
+  for (int t = t0 + 4; t < t1; ++t)
+    if (on) put(t, ld4_elems<B16>(src, r + (t - t0) * ld));
+  if (l == 0) *scale = q.s;
+}
+
+template <bool B16>
+__global__ void __launch_bounds__(NT) k_kv8_append(Append a) {
+  constexpr int NW = NT / WAVE;
+  __shared__ float red[NW + 1];
+  int at = blockIdx.x;
+  Seq s;
+  const int i = find_item(a.c, at, s, seq_blocks);
+  if (i < 0) return;
+  const int b = (s.first >> 6) + at, h = blockIdx.y >> 1, d = a.c.d;
+  const bool isv = blockIdx.y & 1;
+  // the block's places [t0, t1) get rows r .. of the call
+  const int t0 = s.first > b * KB ? s.first - b * KB : 0, t1 = s.len - b * KB < KB ? s.len - b * KB : KB;
+  const size_t ld = isv ? a.ldv : a.ldk, r = ((size_t)s.r0 + (b * KB + t0 - s.first)) * ld + (size_t)h * d;
+  const void* src = isv ? a.v : a.k;
+  // the rows are on their way while the table says where they go
+  float4 x[UNITS][4];
+  Unit u[UNITS];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      top = fmaxf(top, fabsf(x[u][e]));
-      fine = fine && fabsf(x[u][e]) < __builtin_inff();
+  for (int n = 0; n < UNITS; ++n) {
+    u[n] = unit_of(isv, threadIdx.x + NT * n);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = token_of(isv, u[n], k);
+      x[n][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (u[n].e < d && t >= t0 && t < t1) x[n][k] = ld4_elems<B16>(src, r + (size_t)(t - t0) * ld + u[n].e);
     }
   }
+  const int page = page_of(a.c, i, b);
+  if (page < 0) return;
+  const size_t ph = (size_t)page * a.c.hkv + h;
+  uint8_t* blk = (isv ? a.c.vq : a.c.kq) + ph * KB * d;
+  float* scale = (isv ? a.c.vs : a.c.ks) + ph;
+  if (threadIdx.x == 0) red[NW] = *scale;  // read by the thread that writes it
+  float top = 0.f;
+  bool fine = true;
+#pragma unroll
+  for (int n = 0; n < UNITS; ++n)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, top4(x[n][k])), fine = fine && finite4(x[n][k]);
   top = wave_max(fine ? top : __builtin_inff());  // an infinity or NaN among them: infinity
   if (lane_id() == 0) red[wave_id()] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float s_old = red[NT / WAVE];
+  top = red[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) top = fmaxf(top, red[w]);
+  const float s_old = red[NW];
 
-  const bool fresh = t0 == 0 || s_old == 0.f;
-  float sc;
-  int grow = 0;
-  if (!(top < __builtin_inff()) || (t0 > 0 && !(s_old < __builtin_inff()))) {
-    sc = __builtin_nanf("");  // the block stands for no numbers
-  } else if (fresh) {
-    sc = (float)((double)top / 127.0);
-  } else {
-    const double ratio = (double)top / (127.0 * (double)s_old);
-    if (ratio > 1.0) {
-      int e;
-      const double m = frexp(ratio, &e);
-      grow = m == 0.5 ? e - 1 : e;
+  const Scale q = scale_of(top, s_old, t0 == 0);
+  const int grow = q.grow;
+  // dword o of the block: those of its bytes that `now` says are new
+  auto put = [&](size_t o, uint32_t w, int now, bool old) {
+    if (now == 15) {
+      *reinterpret_cast<uint32_t*>(blk + o) = w;
+    } else if (grow && old) {
+      // places that keep what they held are rewritten only where the scale grew
+      uint32_t p = shrink4(*reinterpret_cast<const uint32_t*>(blk + o), grow);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (now >> k & 1) p = (p & ~(255u << 8 * k)) | (w & (255u << 8 * k));
+      *reinterpret_cast<uint32_t*>(blk + o) = p;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (now >> k & 1) blk[o + k] = (uint8_t)(w >> 8 * k);
     }
-    sc = __builtin_ldexpf(s_old, grow);
-  }
-  // tiny scales are lifted by a power of two, so that their reciprocal is a normal number
-  const bool none = !(sc > 0.f);
-  const float lift = sc < 0x1p-90f ? 0x1p90f : 1.f, sl = sc * lift, inv = none ? 0.f : 1.f / sl;
-  // places that keep what they held are rewritten only where the scale grew
-  const bool keep = t0 > 0 && grow > 0;
-  if (!isv) {
+  };
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int w = threadIdx.x + NT * u;
-      if (w >= units) break;
-      const int t = w / d16, c = w - t * d16;
-      uint32_t o[4];
+  for (int n = 0; n < UNITS; ++n) {
+    if (u[n].e >= d) break;
+    const float* f = reinterpret_cast<const float*>(x[n]);
+    if (isv) {
+      int now = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[e] = 0;
+      for (int k = 0; k < 4; ++k) now |= (int)(u[n].t + k >= t0 && u[n].t + k < t1) << k;
+      if (!now && !(grow && u[n].t < t0)) continue;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) o[e] |= (uint32_t)((none ? 0 : quant(x[u][4 * e + f] * lift, sl, inv)) + 128) << (8 * f);
+      for (int e = 0; e < 4; ++e)
+        put(u[n].at[e], q.byte(f[e]) | q.byte(f[4 + e]) << 8 | q.byte(f[8 + e]) << 16 | q.byte(f[12 + e]) << 24, now, u[n].t < t0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = u[n].t + 16 * k;
+        if (t < t1 && (t >= t0 || grow))
+          put(u[n].at[k], q.byte(f[4 * k]) | q.byte(f[4 * k + 1]) << 8 | q.byte(f[4 * k + 2]) << 16 | q.byte(f[4 * k + 3]) << 24, t >= t0 ? 15 : 0, t < t0);
       }
-      *reinterpret_cast<uint4*>(blk + ((size_t)c * KB + t0 + t) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    if (keep)
-      for (int w = threadIdx.x; w < t0 * d16; w += NT) {
-        uint4* p = reinterpret_cast<uint4*>(blk + ((size_t)(w / t0) * KB + w % t0) * 16);
-        uint4 o = *p;
-        o.x = shrink4(o.x, grow), o.y = shrink4(o.y, grow), o.z = shrink4(o.z, grow), o.w = shrink4(o.w, grow);
-        *p = o;
-      }
-  } else {
-    // whole rows where every place is written or the call began the block, the new bytes alone otherwise
-    const bool rows = keep || t0 == 0;
-    if (rows && (keep || t1 < KB)) {
-      for (int w = threadIdx.x; w < d * 4; w += NT) {
-        uint4 o = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        if (keep) {
-          o = *reinterpret_cast<const uint4*>(blk + (size_t)w * 16);
-          o.x = shrink4(o.x, grow), o.y = shrink4(o.y, grow), o.z = shrink4(o.z, grow), o.w = shrink4(o.w, grow);
-        }
-        *reinterpret_cast<uint4*>(vt + (w >> 2) * VROW + (w & 3) * 16) = o;
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int w = threadIdx.x + NT * u;
-      if (w >= units) break;
-      const int t = w / d16, c = w - t * d16, p = v_at(t0 + t);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint8_t q = (uint8_t)((none ? 0 : quant(x[u][e] * lift, sl, inv)) + 128);
-        if (rows) vt[(16 * c + e) * VROW + p] = q;
-        else blk[(size_t)(16 * c + e) * KB + p] = q;
-      }
-    }
-    if (rows) {
-      __syncthreads();
-      for (int w = threadIdx.x; w < d * 4; w += NT)
-        *reinterpret_cast<uint4*>(blk + (size_t)w * 16) = *reinterpret_cast<const uint4*>(vt + (w >> 2) * VROW + (w & 3) * 16);
     }
   }
-  if (threadIdx.x == 0) *scale = sc;
+  if (threadIdx.x == 0) *scale = q.s;
 }
 
 struct Read {
@@ -197,42 +274,39 @@ struct Read {
   size_t ldk, ldv;
 };
 
-__global__ void __launch_bounds__(NT) k_kv8_read(Read a) {
-  __shared__ __align__(16) uint8_t vt[256 * VROW];
+constexpr int RT = 256;
+__global__ void __launch_bounds__(RT) k_kv8_read(Read a) {
   int at = blockIdx.x;
-  const int i = find_item(a.c, at, seq_blocks);
+  Seq s;
+  const int i = find_item(a.c, at, s, seq_blocks);
   if (i < 0) return;
-  const Seq s = seq_of(a.c, i);
-  const int b = (s.first >> 6) + at, page = page_of(a.c, i, b);
-  const int h = blockIdx.y >> 1, d = a.c.d;
+  const int b = (s.first >> 6) + at, page = page_of(a.c, i, b), h = blockIdx.y >> 1, d = a.c.d;
   const bool isv = blockIdx.y & 1;
   const int t0 = s.first > b * KB ? s.first - b * KB : 0, t1 = s.len - b * KB < KB ? s.len - b * KB : KB;
-  const size_t r = (size_t)s.r0 + (b * KB + t0 - s.first), ld = isv ? a.ldv : a.ldk;
-  float* dst = (isv ? a.v : a.k) + r * ld + (size_t)h * d;
+  const size_t ld = isv ? a.ldv : a.ldk;
+  float* dst = (isv ? a.v : a.k) + ((size_t)s.r0 + (b * KB + t0 - s.first)) * ld + (size_t)h * d;
   const size_t ph = (size_t)(page < 0 ? 0 : page) * a.c.hkv + h;
   const uint8_t* blk = (isv ? a.c.vq : a.c.kq) + ph * KB * d;
-  const float sc = page < 0 ? 0.f : (isv ? a.c.vs : a.c.ks)[ph];
-  if (isv && page >= 0) {
-    for (int w = threadIdx.x; w < d * 4; w += NT) *reinterpret_cast<uint4*>(vt + (w >> 2) * VROW + (w & 3) * 16) = ld16(blk + (size_t)w * 16);
-    __syncthreads();
-  }
-  // four elements a thread, a token's elements beside each other
-  const int d4 = d >> 2;
-  for (int w = threadIdx.x; w < (t1 - t0) * d4; w += NT) {
-    const int t = w / d4, e = 4 * (w - t * d4);
-    uint32_t q = 0x80808080u;
-    if (page >= 0) {
-      if (isv) {
-        const uint8_t* p = vt + e * VROW + v_at(t0 + t);
-        q = p[0] | p[VROW] << 8 | p[2 * VROW] << 16 | (uint32_t)p[3 * VROW] << 24;
-      } else {
-        q = ld4(blk + ((size_t)(e >> 4) * KB + t0 + t) * 16 + (e & 15));
+  const float sc = (isv ? a.c.vs : a.c.ks)[ph];
+#pragma unroll
+  for (int n = 0; n < 1024 / RT; ++n) {
+    const Unit u = unit_of(isv, threadIdx.x + RT * n);
+    if (u.e >= d) break;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = ld4(blk + u.at[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = token_of(isv, u, k);
+      if (t < t0 || t >= t1) continue;
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int q = (int)(isv ? w[e] >> 8 * k : w[k] >> 8 * e) & 255;
+        o[e] = page < 0 ? 0.f : sc * (float)(q - 128);
       }
+      *reinterpret_cast<float4*>(dst + (size_t)(t - t0) * ld + u.e) = make_float4(o[0], o[1], o[2], o[3]);
     }
-    float4 o;
-    o.x = sc * (float)((int)(q & 255) - 128), o.y = sc * (float)((int)((q >> 8) & 255) - 128);
-    o.z = sc * (float)((int)((q >> 16) & 255) - 128), o.w = sc * (float)((int)(q >> 24) - 128);
-    *reinterpret_cast<float4*>(dst + t * ld + e) = o;
   }
 }
 
@@ -242,7 +316,9 @@ int append(const Append& a, int ldk, int ldv, hipStream_t st) {
   if (!kv8_ok(a.c) || ldk < n || ldv < n || ldk % per || ldv % per) return -1;
   if (a.c.rows == 0 || a.c.seqs == 0) return 0;
   if (!kv8_buffers_ok(a.c) || !a.k || !a.v || ((uintptr_t)a.k & 15) || ((uintptr_t)a.v & 15)) return -1;
-  hipLaunchKernelGGL((k_kv8_append<B16>), dim3((unsigned)max_blocks(a.c.rows, a.c.seqs), 2 * a.c.hkv), dim3(NT), 0, st, a);
+  const unsigned nb = (unsigned)max_blocks(a.c.rows, a.c.seqs);
+  if (a.c.rows <= 4ll * a.c.seqs) hipLaunchKernelGGL((k_kv8_append_few<B16>), dim3(nb, (2 * a.c.hkv + 3) / 4), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_kv8_append<B16>), dim3(nb, 2 * a.c.hkv), dim3(NT), 0, st, a);
   return 0;
 }
 
@@ -271,6 +347,6 @@ API int dr_kv8_read(const int* start, const int* len, const int* table, int maxp
   if (rows == 0 || seqs == 0) return 0;
   if (!kv8_buffers_ok(c) || !k || !v || ((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return -1;
   const Read a{c, k, v, (size_t)ldk, (size_t)ldv};
-  hipLaunchKernelGGL(k_kv8_read, dim3((unsigned)max_blocks(rows, seqs), 2 * hkv), dim3(NT), 0, st, a);
+  hipLaunchKernelGGL(k_kv8_read, dim3((unsigned)max_blocks(rows, seqs), 2 * hkv), dim3(RT), 0, st, a);
   return 0;
 }

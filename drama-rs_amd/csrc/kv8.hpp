@@ -51,26 +51,30 @@ DEV int page_of(const Kv8& a, int i, int b) {
   return p >= 0 && p < a.pages ? p : -1;
 }
 
-// Item `at` of the items of all sequences in order, count(sequence) of each: its sequence, and its number there in `at`; -1
-// where there are fewer.  64 sequences a step, all lanes of the wave together.
+// Item `at` of the items of all sequences in order, count(sequence) of each: its sequence (s: what seq_of gives for it), and its number there in
+// `at`; -1 where there are fewer.  64 sequences a step, all lanes of the wave together.
 template <class Count>
-DEV int find_item(const Kv8& a, int& at, Count count) {
+DEV int find_item(const Kv8& a, int& at, Seq& s, Count count) {
   const int l = lane_id();
   for (int i0 = 0; i0 < a.seqs; i0 += WAVE) {
-    const int c = i0 + l < a.seqs ? count(seq_of(a, i0 + l)) : 0;
-    int s = c;
+    Seq q{0, 0, 0, 0};
+    if (i0 + l < a.seqs) q = seq_of(a, i0 + l);
+    const int c = i0 + l < a.seqs ? count(q) : 0;
+    int n = c;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) {
-      const int t = __shfl_up(s, o);
-      s += l >= o ? t : 0;
+      const int t = __shfl_up(n, o);
+      n += l >= o ? t : 0;
     }
-    const unsigned long long behind = __ballot(s > at);
+    const unsigned long long behind = __ballot(n > at);
     if (behind) {
       const int w = __builtin_ctzll(behind);
-      at -= __builtin_amdgcn_readlane(s - c, w);
+      at -= __builtin_amdgcn_readlane(n - c, w);
+      s = Seq{__builtin_amdgcn_readlane(q.r0, w), __builtin_amdgcn_readlane(q.n, w), __builtin_amdgcn_readlane(q.first, w),
+              __builtin_amdgcn_readlane(q.len, w)};
       return i0 + w;
     }
-    at -= __builtin_amdgcn_readlane(s, WAVE - 1);
+    at -= __builtin_amdgcn_readlane(n, WAVE - 1);
   }
   return -1;
 }

@@ -71,6 +71,7 @@ CASES = [
     ([1], [1], 1, 16, 0, 0.0), ([1], [64], 2, 64, 0, 1.0), ([1], [65], 2, 64, 0, 1.0), ([64], [64], 1, 128, 0, 0.0), ([63], [63], 3, 48, 0, 1.0),
     ([65], [65], 2, 80, 0, 1.0), ([200], [333], 2, 256, 0, 1.0), ([1] * 70, [1 + 7 * i for i in range(70)], 2, 32, 3, 2.0),
     ([3, 0, 5, 129, 0, 1], [3, 100, 64, 140, 0, 700], 4, 96, 2, 2.0), ([2, 4, 3], [0, 2, 3], 2, 64, 1, 1.0),
+    ([9, 0, 0, 70, 0, 0] + [1] * 20, [9, 5, 0, 200, 1, 0] + [64 * i for i in range(1, 21)], 2, 128, 1, 2.0), ([13, 0, 0, 0], [50, 9, 0, 0], 3, 256, 0, 1.0),
     ([130], [130], 1, 240, 0, 3.0), ([17] * 9, [17 + 61 * i for i in range(9)], 5, 112, 0, 2.0),
 ]
 
