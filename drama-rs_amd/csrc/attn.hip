@@ -73,7 +73,7 @@ DEV void finish(const Attn& a, size_t row, int head, int e, const f32x4& o, floa
 // o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor; no token seen: o = l = 0.  alone: there is no other part, which
 // an l of kAlone tells the launch that joins.
 constexpr float kAlone = -1.f;
-DEV void emit(const Attn& a, bool alone, int split, size_t row, int head, int e, const f32x4& o, float l, float m) {
+DEV void emit(const Attn& a, bool alone, int split, size_t row, int head, int e, const f32x4& o, float l, float m, const float4& gate) {
   const int d = a.c.d;
   const size_t at = ((size_t)split * a.c.rows + row) * a.hq + head;
   if (!alone) {
@@ -82,7 +82,13 @@ DEV void emit(const Attn& a, bool alone, int split, size_t row, int head, int e,
     return;
   }
   if (a.splits > 1 && e == 0) a.ml[2 * at + 1] = kAlone;
-  finish(a, row, head, e, o, l, a.gate ? ldf4(a.gate + row * a.ldg + head * a.hsg + e) : make_float4(0.f, 0.f, 0.f, 0.f));
+  finish(a, row, head, e, o, l, gate);
+}
+// The gate's logits of those elements (an output waits for memory once where all of a lane's are asked for together).
+DEV float4 gate_of(const Attn& a, bool on, size_t row, int head, int e) {
+  float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (a.gate && on) g = ldf4(a.gate + row * a.ldg + head * a.hsg + e);
+  return g;
 }
 
 // A wave's columns: MT tiles of 16, lane l holds column l & 15 of each.  DC: 64-element chunks of a head.
@@ -354,12 +360,15 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
     w.sum[x] = quad_sum(w.sum[x]) * 0x1p-16f;
+    const int col = threadIdx.x >> 4, p = 16 * x + col, row = p / g, e0 = 4 * (threadIdx.x & 15);
+    float4 gate[DC];
+#pragma unroll
+    for (int c = 0; c < DC; ++c) gate[c] = gate_of(a, alone && p < np && e0 + 64 * c < d, (size_t)s.r0 + row, h * g + p - row * g, e0 + 64 * c);
     if (x) __syncthreads();
     if (j == 0) sml[wv * 32 + 2 * l] = w.m[x], sml[wv * 32 + 2 * l + 1] = w.sum[x];
 #pragma unroll
     for (int u = 0; u < 4 * DC; ++u) *reinterpret_cast<f32x4*>(sm + (wv * 16 + (l & 15)) * LD + 16 * u + 4 * j) = w.o[x][u] * us;
     __syncthreads();
-    const int col = threadIdx.x >> 4, p = 16 * x + col, row = p / g;
     float wt[W], mm = -kInf, ll = 0.f;
 #pragma unroll
     for (int v = 0; v < W; ++v) mm = fmaxf(mm, sml[v * 32 + 2 * col]);
@@ -369,11 +378,14 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
       ll += wt[v] * sml[v * 32 + 2 * col + 1];
     }
     if (p < np)
-      for (int e = 4 * (threadIdx.x & 15); e < d; e += 64) {
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        const int e = e0 + 64 * c;
+        if (e >= d) break;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < W; ++z) v += wt[z] * *reinterpret_cast<const f32x4*>(sm + (z * 16 + col) * LD + e);
-        emit(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, e, v, ll, mm);
+        emit(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, e, v, ll, mm, gate[c]);
       }
   }
 }
@@ -397,20 +409,23 @@ struct Cols32 {
 constexpr float kBase = 4.f;      // a weight is 2^kBase times its ratio to the reference's: 2^11 above it before fp16 ends,
 constexpr float kMost = 40000.f;  // which a lane's sum of weights up to kMost rules out
 
+// A lane's share of the queries of columns c0 .. of the np pairs of sequence s and cached head h; begin32 makes columns of them.
 template <int DC>
-DEV void begin32(Cols32<DC>& w, const Attn& a, const Seq& s, int h, int c0, int np) {
-  const int l = lane_id(), hh = l >> 5, d = a.c.d, g = a.g;
-  const long long cap = (long long)a.c.maxp * KB - 1;
-  const int p = c0 + (l & 31), row = p / g;
-  const bool on = p < np;
+DEV void load_q32(const Attn& a, const Seq& s, int h, int c0, int np, uint4 (&r)[2 * DC]) {
+  const int l = lane_id(), hh = l >> 5, d = a.c.d, g = a.g, p = c0 + (l & 31), row = p / g;
   const uint16_t* src = a.q + (size_t)(s.r0 + row) * a.ldq + (size_t)(h * g + p - row * g) * d;
-  uint4 r[2 * DC];
 #pragma unroll
   for (int i = 0; i < 2 * DC; ++i) {
     const int e = 32 * (i >> 1) + 16 * hh + 8 * (i & 1);
     r[i] = make_uint4(0, 0, 0, 0);
-    if (on && e < d) r[i] = ld16(src + e);
+    if (p < np && e < d) r[i] = ld16(src + e);
   }
+}
+template <int DC>
+DEV void begin32(Cols32<DC>& w, const Attn& a, const Seq& s, int c0, int np, const uint4 (&r)[2 * DC]) {
+  const long long cap = (long long)a.c.maxp * KB - 1;
+  const int p = c0 + (lane_id() & 31), row = p / a.g;
+  const bool on = p < np;
   float top = 0.f;
   bool num = true;
 #pragma unroll
@@ -559,6 +574,8 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   };
 
   Pages pg, px;  // of 64 blocks, and of the 64 behind them
+  uint4 qr[2 * DC];
+  load_q32<DC>(a, s, h, w0, c1, qr);
   pg.fetch(a, i, h, b0 + l, l < cnt);
   if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
   px.fetch(a, i, h, b0 + WAVE + l, WAVE + l < cnt);
@@ -586,7 +603,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
     put_loads(n);
   };
   Cols32<DC> w;
-  begin32(w, a, s, h, w0, c1);
+  begin32(w, a, s, w0, c1, qr);
   if (cnt > 0) {
 #pragma unroll
     for (int f = 2 * PER; f < 4 * PER; ++f) put_part(-1, f);
@@ -669,16 +686,25 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   const float us = __builtin_ldexpf(1.f, w.unit - 16), sum = xsum_step<32>(w.sum) * 0x1p-16f;
   int z = threadIdx.x & 63;  // worked out again: values kept from begin32() would cost registers through the loop
   asm volatile("" : "+v"(z));
-  const int p = w0 + (z & 31), row = p / g;
-  if (p < c1)
+  const int p = w0 + (z & 31), row = p / g, head = h * g + p - row * g;
+  if (p >= c1) return;
+  const size_t rw = (size_t)s.r0 + row;
+  float4 gate[DC][4];
 #pragma unroll
-    for (int u = 0; u < DC; ++u)
+  for (int u = 0; u < DC; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int e = 32 * u + 2 * r + 4 * (z >> 5);
-        if (e < d)
-          emit(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, e, f32x4{w.o[u][r] * us, w.o[u][r + 1] * us, w.o[u][r + 2] * us, w.o[u][r + 3] * us}, sum, w.m);
-      }
+    for (int r = 0; r < 4; ++r) {
+      const int e = 32 * u + 8 * r + 4 * (z >> 5);
+      gate[u][r] = gate_of(a, alone && e < d, rw, head, e);
+    }
+#pragma unroll
+  for (int u = 0; u < DC; ++u)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int e = 32 * u + 8 * r + 4 * (z >> 5);
+      const f32x4 o = {w.o[u][4 * r] * us, w.o[u][4 * r + 1] * us, w.o[u][4 * r + 2] * us, w.o[u][4 * r + 3] * us};
+      if (e < d) emit(a, alone, sp, rw, head, e, o, sum, w.m, gate[u][r]);
+    }
 }
 
 // Joins the parts of a row's query, or of 64 elements of it where the queries are few: LE lanes of four elements, each group of them every
@@ -691,8 +717,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
   const int head = blockIdx.x % a.hq, row = blockIdx.x / a.hq, t = threadIdx.x, G = NT / LE, grp = t / LE, d = a.c.d;
   const int e = 4 * (LE * blockIdx.y + (t & (LE - 1)));
   const size_t at = (size_t)row * a.hq + head, step = (size_t)a.c.rows * a.hq;
-  float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (a.gate && grp == 0 && e < d) gate = ldf4(a.gate + row * a.ldg + head * a.hsg + e);
+  const float4 gate = gate_of(a, grp == 0 && e < d, row, head, e);
   float m = -kInf, s = 0.f;
   f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
   bool whole = false;
