@@ -56,34 +56,32 @@ DEV float quad_max(float v) { return xmax_step<32>(xmax_step<16>(v)); }
 DEV float quad_sum(float v) { return xsum_step<32>(xsum_step<16>(v)); }
 DEV float lane_f(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
-// Four elements e .. of the output of a row's query `head`: o / l (0 where no token was seen), its gate, bf16.
-DEV void finish(const Attn& a, size_t row, int head, int e, const f32x4& o, float l, const float4& g) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = o[i] * inv;
-  if (a.gate) v[0] /= 1.f + expf(-g.x), v[1] /= 1.f + expf(-g.y), v[2] /= 1.f + expf(-g.z), v[3] /= 1.f + expf(-g.w);
-  uint32_t b[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) b[i] = to_bf16(v[i]);
-  *reinterpret_cast<uint2*>(a.y + row * a.ldy + (size_t)head * a.c.d + e) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-}
-
-// The same, or a part of it to be joined.
-// o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor; no token seen: o = l = 0.  alone: there is no other part, which
-// an l of kAlone tells the launch that joins.
+// What becomes of a row's query `head`: elements e .. e + 3, o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor (no token seen:
+// both 0).  The finished output, or, not alone, a part of it to be joined; alone, an l of kAlone tells the launch that joins.
 constexpr float kAlone = -1.f;
-DEV void emit(const Attn& a, bool alone, int split, size_t row, int head, int e, const f32x4& o, float l, float m, const float4& gate) {
-  const int d = a.c.d;
-  const size_t at = ((size_t)split * a.c.rows + row) * a.hq + head;
-  if (!alone) {
-    *reinterpret_cast<f32x4*>(a.part + at * d + e) = o;
-    if (e == 0) a.ml[2 * at] = m, a.ml[2 * at + 1] = l;
-    return;
+struct Out {
+  uint16_t* y;
+  float *part, inv;
+  bool alone, gated;
+  DEV Out(const Attn& a, bool alone, int split, size_t row, int head, float l, float m, bool first) : alone(alone), gated(a.gate != nullptr) {
+    const size_t at = ((size_t)split * a.c.rows + row) * a.hq + head;
+    y = a.y + row * a.ldy + (size_t)head * a.c.d, part = a.part + at * a.c.d;
+    inv = l == 0.f ? 0.f : 1.f / l;
+    if (first && !alone) a.ml[2 * at] = m;
+    if (first && (!alone || a.splits > 1)) a.ml[2 * at + 1] = alone ? kAlone : l;
   }
-  if (a.splits > 1 && e == 0) a.ml[2 * at + 1] = kAlone;
-  finish(a, row, head, e, o, l, gate);
-}
+  // sigmoid by the hardware's exp2 and reciprocal (1 ulp each): far below the output's rounding to bf16
+  DEV static float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g)); }
+  DEV void put(int e, const f32x4& o, const float4& g) const {
+    if (!alone) {
+      *reinterpret_cast<f32x4*>(part + e) = o;
+      return;
+    }
+    f32x4 v = o * inv;
+    if (gated) v[0] *= sigmoid(g.x), v[1] *= sigmoid(g.y), v[2] *= sigmoid(g.z), v[3] *= sigmoid(g.w);
+    *reinterpret_cast<uint2*>(y + e) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+  }
+};
 // The gate's logits of those elements (an output waits for memory once where all of a lane's are asked for together).
 DEV float4 gate_of(const Attn& a, bool on, size_t row, int head, int e) {
   float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -377,7 +375,8 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
       wt[v] = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(sml[v * 32 + 2 * col] - mm);
       ll += wt[v] * sml[v * 32 + 2 * col + 1];
     }
-    if (p < np)
+    if (p < np) {
+      const Out out(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, ll, mm, e0 == 0);
 #pragma unroll
       for (int c = 0; c < DC; ++c) {
         const int e = e0 + 64 * c;
@@ -385,8 +384,9 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < W; ++z) v += wt[z] * *reinterpret_cast<const f32x4*>(sm + (z * 16 + col) * LD + e);
-        emit(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, e, v, ll, mm, gate[c]);
+        out.put(e, v, gate[c]);
       }
+    }
   }
 }
 
@@ -697,13 +697,14 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
       const int e = 32 * u + 8 * r + 4 * (z >> 5);
       gate[u][r] = gate_of(a, alone && e < d, rw, head, e);
     }
+  const Out out(a, alone, sp, rw, head, sum, w.m, z < 32);
 #pragma unroll
   for (int u = 0; u < DC; ++u)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int e = 32 * u + 8 * r + 4 * (z >> 5);
       const f32x4 o = {w.o[u][4 * r] * us, w.o[u][4 * r + 1] * us, w.o[u][4 * r + 2] * us, w.o[u][4 * r + 3] * us};
-      if (e < d) emit(a, alone, sp, rw, head, e, o, sum, w.m, gate[u][r]);
+      if (e < d) out.put(e, o, gate[u][r]);
     }
 }
 
@@ -760,7 +761,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
       const float c = __builtin_amdgcn_exp2f(sm[k] - ms);
       v += c * so[k * LE + t], s += c * sl[k];
     }
-  finish(a, row, head, e, v, s, gate);
+  Out(a, true, 0, row, head, s, 0.f, false).put(e, v, gate);
 }
 
 // How a call is cut: by its sizes alone, so that the workspace is known before.

@@ -74,6 +74,12 @@ DEV uint16_t to_bf16(float f) {
   return (uint16_t)(u >> 16);
 }
 
+// Two fp32 to a word of bf16, nearest even, in one instruction.
+DEV uint32_t pack_bf16(float a, float b) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, bf2{(__bf16)a, (__bf16)b});
+}
+
 // Cross-lane exchange for the ascending xor butterfly o = 1, 2, 4, 8, 16, 32.
 //   o = 1, 2: DPP quad_perm, the exact xor partner;
 //   o = 4, 8: DPP row_half_mirror / row_mirror (lane 7 - i, 15 - i); after the lower steps every

@@ -50,12 +50,6 @@ DEV void ld_x(const void* x, size_t at, float (&o)[V]) {
   }
 }
 
-// two fp32 to bf16, nearest even, in one instruction
-DEV uint32_t pack_bf16(float a, float b) {
-  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, bf2{(__bf16)a, (__bf16)b});
-}
-
 template <int V>
 DEV void st_y(const Rope& a, size_t row, int at, const float (&o)[V]) {
   if (a.y) {
