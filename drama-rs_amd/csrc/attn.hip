@@ -528,8 +528,9 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   __shared__ __align__(16) half8 kb[2 * 2 * F * WAVE], vb[2 * 2 * F * WAVE];  // [2][F][2][64]
   const int l = lane_id(), hh = l >> 5, wv = __builtin_amdgcn_readfirstlane(wave_id());
   const bool late = NW == 8 && wv >= 4;
-  const int h = blockIdx.y, sp = blockIdx.z, d = a.c.d, d16 = d >> 4, g = a.g;
-  int at = gridDim.x - 1 - blockIdx.x, i = at;  // the last rows, which see most, first
+  // the last rows of all heads, which see most, first; heads beside each other, so that a die's share of the blocks is of few heads
+  const int h = blockIdx.x % a.c.hkv, sp = blockIdx.y, d = a.c.d, d16 = d >> 4, g = a.g;
+  int at = (gridDim.x - 1 - blockIdx.x) / a.c.hkv, i = at;
   Seq s;
   if (a.scan) i = find_item(a.c, at, s, [g](const Seq& q) { return (q.n * g + TP - 1) / TP; });
   else at = 0, s = seq_of(a.c, i);
@@ -668,7 +669,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
       px.fetch(a, i, h, b0 + k + WAVE + l, k + WAVE + l < cnt);
     }
     if (k < mine_cnt) soften32(w, sc, pf, pg, k - base, (b0 + k) * KB, w_lo);
-    lds_barrier();
+    if (NW == 8) lds_barrier();  // four waves are not out of step: what their products read was written before the barrier above
   };
   int k = 0;
   for (; k + 1 < mine_cnt; ++k) {
@@ -782,7 +783,7 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   p.nw = p.few || d > 128 ? 4 : 8;
   cut(p.few ? 16 * p.mt : 32 * p.nw);
   if (p.nw == 8 && p.tiles * hkv < 256) p.nw = 4, cut(32 * p.nw);
-  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = p.few && p.mt == 1 ? 2048 : 512;
+  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = p.few && p.mt == 1 && d <= 128 ? 2048 : 512;
   long long s = units >= want / 2 && !p.few ? 1 : (want + units - 1) / units;
   const long long most = (blocks + W - 1) / W;
   s = s > most ? most : s;
@@ -821,9 +822,9 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   float* part = reinterpret_cast<float*>(ws);
   const Attn a{c, q, gate, y, part, part + (size_t)p.splits * rows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
                (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan};
-  const dim3 grid((unsigned)p.tiles, hkv, p.splits);
+  const dim3 grid((unsigned)(p.tiles * hkv), p.splits);
   auto few = [&](auto dc, auto mt) {
-    hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), dim3((unsigned)(seqs * hkv), p.splits), dim3(NT), 0, st, a);
+    hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), grid, dim3(NT), 0, st, a);
   };
   auto tiles = [&](auto dc) {
     constexpr int DC = decltype(dc)::value;
