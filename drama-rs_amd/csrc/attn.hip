@@ -782,8 +782,12 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   };
   p.nw = p.few || d > 128 ? 4 : 8;
   cut(p.few ? 16 * p.mt : 32 * p.nw);
+  // eight waves only where their tiles fill the card: 1000 rows of 32 heads 30.2 us with four, 35.8 with eight; 4096 behind 8192 tokens 465 and 344
   if (p.nw == 8 && p.tiles * hkv < 256) p.nw = 4, cut(32 * p.nw);
-  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = p.few && p.mt == 1 && d <= 128 ? 2048 : 512;
+  // Blocks of threads to fill the card with.  Few columns: a CU holds two up to d 128 (one with two tiles of columns or wider heads), and with lengths
+  // apart a long sequence needs many (48 ragged sequences: 2048 57.5 us, 1024 75; 32 of 8000 tokens with heads of 256: 512 62 us, 2048 104).
+  // Many columns: 64 rows on 30000 tokens 38.8 us with 256, 42.3 with 512 (more parts to join), 51.6 with 128.
+  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = !p.few ? 256 : p.mt == 1 && d <= 128 ? 2048 : 512;
   long long s = units >= want / 2 && !p.few ? 1 : (want + units - 1) / units;
   const long long most = (blocks + W - 1) / W;
   s = s > most ? most : s;
