@@ -1,11 +1,16 @@
 // Tokens into and out of the cache in 8 bits (layout: kv8.hpp).
 //
-// A block of threads owns one head's k or v of one cached block: it takes the call's tokens of that block into registers, reduces their largest
-// magnitude A, and stores round(x / s).  With the block's first token in the call s = fl(A / 127); otherwise s is the
-// block's scale, doubled until A <= 127 s, and where it grew by 2^j the block's earlier integers become round(q / 2^j).  Growth by
-// powers of two bounds what repeated rounding adds: every earlier rounding is worth at most half of the next one's step, so an element is
-// never off by a whole step of the block's present scale, however often single tokens made it grow.  Integers are exact roundings of
-// the quotient (half to even): x - q s needs at most 24 bits where q is next to x / s, so one fma tells on which side x lies.
+// One owner (a block of threads, or a wave where few tokens come) takes one head's k or v of one cached block: the call's tokens of that block go
+// into registers, their largest magnitude A is reduced, and round(x / s) is stored.  With the block's first token in the call s = fl(A / 127);
+// otherwise s is the block's scale, doubled until A <= 127 s, and where it grew by 2^j the block's earlier integers become round(q / 2^j).
+// Growth by powers of two bounds what repeated rounding adds: every earlier rounding is worth at most half of the next one's step, so an element
+// is never off by a whole step of the block's present scale, however often single tokens made it grow.  Integers are exact roundings of the
+// quotient (half to even): |x - q s| below half a step says that q = round(x / s), and one fma compares it without an error that counts.
+//
+// Nothing is read or written twice, so memory bounds the large calls and a chain of loads (where a sequence's rows are, the table, the scale)
+// the small ones.  Kernels alone: 4844 rows of 4 heads of 128 in fp32, 9 sequences: 9.9 us into the cache (2.5 TB/s of rows and bytes; 2.7 us
+// more with every integer by quant()) and 7.8 us out of it (3.2 TB/s); 63 sequences with one token of 8 heads of 128 in bf16 5.9 us,
+// their last blocks out 8.5 us; one token 3.7 us.
 #include "kv8.hpp"
 
 using namespace drm;
@@ -84,6 +89,21 @@ struct Scale {
   int grow;
   bool none;
   DEV uint32_t byte(float v) const { return (uint32_t)((none ? 0 : quant(v * lift, sl, inv)) + 128); }
+  // Four bytes by the reciprocal alone, and in `off` the largest distance of an element to its integer's value: right where that is
+  // below half a step (and never past 127, but for scales that are subnormal or no numbers).
+  DEV uint32_t guess(float a, float b, float c, float e, float& off) const {
+    uint32_t w = 0;
+    const float v[4] = {a, b, c, e};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float q = rintf(v[k] * inv);
+      off = fmaxf(off, fabsf(__builtin_fmaf(-q, s, v[k])));
+      w = __builtin_amdgcn_cvt_pk_u8_f32(q + 128.f, k, w);
+    }
+    return w;
+  }
+  DEV bool sure(float off) const { return lift == 1.f && !none && off < 0.5f * s; }
+  DEV uint32_t exact(float a, float b, float c, float e) const { return byte(a) | byte(b) << 8 | byte(c) << 16 | byte(e) << 24; }
 };
 DEV Scale scale_of(float top, float s_old, bool first) {
   Scale q;
@@ -91,7 +111,7 @@ DEV Scale scale_of(float top, float s_old, bool first) {
   if (!(top < __builtin_inff()) || (!first && !(s_old < __builtin_inff()))) {
     q.s = __builtin_nanf("");  // the block stands for no numbers
   } else if (first || s_old == 0.f) {
-    q.s = (float)((double)top / 127.0);
+    q.s = top / 127.f;  // rounded correctly
   } else {
     // 127 s_old and the comparisons are exact in 64 bits
     const double most = 127.0 * (double)s_old;
@@ -113,7 +133,8 @@ DEV bool finite4(const float4& v) {
 DEV float top4(const float4& v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
 // A few tokens a sequence (decode steps): a wave owns a head's k or v of a block, a lane four elements of each token; tokens past the fourth
-// are loaded again.  Bound by its chain of loads (sequence, rows beside the table, scale): XXX
+// are loaded again.  Bound by its chain of loads (sequence, rows beside the table, scale): 3.7 us for one
+// token and 5.9 us for 63 sequences with one of 8 heads of 128, where k_kv8_append takes 7.4 and 13.9.
 template <bool B16>
 __global__ void __launch_bounds__(256) k_kv8_append_few(Append a) {
   int at = blockIdx.x;
@@ -162,7 +183,7 @@ __global__ void __launch_bounds__(256) k_kv8_append_few(Append a) {
     __builtin_amdgcn_s_waitcnt(0);
   }
   auto put = [&](int t, const float4& v) {
-    const uint32_t w = q.byte(v.x) | q.byte(v.y) << 8 | q.byte(v.z) << 16 | q.byte(v.w) << 24;
+    const uint32_t w = q.exact(v.x, v.y, v.z, v.w);
     if (isv) {
       uint8_t* p = blk + (size_t)e * KB + 16 * (t >> 2 & 3) + 4 * (t >> 4) + (t & 3);
       p[0] = (uint8_t)w, p[KB] = (uint8_t)(w >> 8), p[2 * KB] = (uint8_t)(w >> 16), p[3 * KB] = (uint8_t)(w >> 24);
@@ -178,6 +199,8 @@ __global__ void __launch_bounds__(256) k_kv8_append_few(Append a) {
   if (l == 0) *scale = q.s;
 }
 
+// Many tokens a sequence: a block of threads owns a head's k or v of a block, and a thread loads all of its rows' pieces before it needs the
+// first.  512 threads hold 64 tokens of 256 elements in 32 registers each; 256 took 12.4 us where these take 10.9.
 template <bool B16>
 __global__ void __launch_bounds__(NT) k_kv8_append(Append a) {
   constexpr int NW = NT / WAVE;
@@ -248,20 +271,28 @@ __global__ void __launch_bounds__(NT) k_kv8_append(Append a) {
   for (int n = 0; n < UNITS; ++n) {
     if (u[n].e >= d) break;
     const float* f = reinterpret_cast<const float*>(x[n]);
+    // dword k is elements of token k, or tokens of element k
+    uint32_t w[4];
+    float off = 0.f;
+    auto all = [&](auto how) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = isv ? how(f[k], f[4 + k], f[8 + k], f[12 + k]) : how(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+    };
+    all([&](float a, float b, float c, float e) { return q.guess(a, b, c, e, off); });
+    if (!q.sure(off)) all([&](float a, float b, float c, float e) { return q.exact(a, b, c, e); });
     if (isv) {
       int now = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) now |= (int)(u[n].t + k >= t0 && u[n].t + k < t1) << k;
       if (!now && !(grow && u[n].t < t0)) continue;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        put(u[n].at[e], q.byte(f[e]) | q.byte(f[4 + e]) << 8 | q.byte(f[8 + e]) << 16 | q.byte(f[12 + e]) << 24, now, u[n].t < t0);
+      for (int e = 0; e < 4; ++e) put(u[n].at[e], w[e], now, u[n].t < t0);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int t = u[n].t + 16 * k;
-        if (t < t1 && (t >= t0 || grow))
-          put(u[n].at[k], q.byte(f[4 * k]) | q.byte(f[4 * k + 1]) << 8 | q.byte(f[4 * k + 2]) << 16 | q.byte(f[4 * k + 3]) << 24, t >= t0 ? 15 : 0, t < t0);
+        if (t < t1 && (t >= t0 || grow)) put(u[n].at[k], w[k], t >= t0 ? 15 : 0, t < t0);
       }
     }
   }
@@ -274,6 +305,7 @@ struct Read {
   size_t ldk, ldv;
 };
 
+// Out of the cache: the reverse, each thread's dwords loaded together.  512 threads are as fast (within 0.5 us either way).
 constexpr int RT = 256;
 __global__ void __launch_bounds__(RT) k_kv8_read(Read a) {
   int at = blockIdx.x;
@@ -317,6 +349,7 @@ int append(const Append& a, int ldk, int ldv, hipStream_t st) {
   if (a.c.rows == 0 || a.c.seqs == 0) return 0;
   if (!kv8_buffers_ok(a.c) || !a.k || !a.v || ((uintptr_t)a.k & 15) || ((uintptr_t)a.v & 15)) return -1;
   const unsigned nb = (unsigned)max_blocks(a.c.rows, a.c.seqs);
+  // a wave walks four rows at a time: more than four a sequence are left to a block of threads
   if (a.c.rows <= 4ll * a.c.seqs) hipLaunchKernelGGL((k_kv8_append_few<B16>), dim3(nb, (2 * a.c.hkv + 3) / 4), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((k_kv8_append<B16>), dim3(nb, 2 * a.c.hkv), dim3(NT), 0, st, a);
   return 0;
