@@ -93,10 +93,11 @@ DEV float4 gate_of(const Attn& a, bool on, size_t row, int head, int e) {
 template <int DC, int MT>
 struct Cols {
   half8 q[MT][DC][2];      // elements 64 c + 16 (l >> 4) + 8 x + (0 .. 7), times a power of two
-  f32x4 o[MT][4 * DC];     // O^T, elements 16 u + 4 (l >> 4) + (0 .. 3), over 2^(unit - 15)
+  f32x4 o[MT][4 * DC];     // O^T, elements 16 u + 4 (l >> 4) + (0 .. 3), over 2^(unit - below - 15)
   float m[MT], sum[MT], qm[MT];  // maximum of the log2 scores, the lane's share of the sum, log2 score of a unit of S and of k's scale
   int pos[MT];             // the columns' positions, -1 where there is none
   int unit;                // 2^unit: a power of two not below any v scale so far
+  int below[MT];           // by how much it rose for blocks that a column does not see: all that it sees lie before them
 };
 
 // Columns c0 .. of the np pairs (row, query) of sequence s and cached head h.
@@ -152,7 +153,7 @@ DEV void begin(Cols<DC, MT>& w, const Attn& a, const Seq& s, int h, int c0, int 
     w.qm[t] = __builtin_ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
     const int ps = s.first + row;
     w.pos[t] = on ? (ps < cap ? ps : (int)cap) : -1;
-    w.m[t] = -kInf, w.sum[t] = 0.f;
+    w.m[t] = -kInf, w.sum[t] = 0.f, w.below[t] = 0;
 #pragma unroll
     for (int u = 0; u < 4 * DC; ++u) w.o[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -173,8 +174,8 @@ struct Pages {
     const bool ok = vs >= 0.f && vs < kInf && ks >= 0.f && ks < kInf;
     num = __ballot(ok);
     if (!ok) ks = 0.f;
-    // a scale of 0 weighs nothing, by an exponent far below any
-    const bool pos = ok && vs > 0.f;
+    // a scale of 0 weighs nothing, by an exponent far below any; nor does a block that is not there
+    const bool pos = ok && p >= 0 && vs > 0.f;
     ve = pos ? __builtin_amdgcn_frexp_expf(vs) : -200;
     const float fr = pos ? __builtin_amdgcn_frexp_mantf(vs) : 0.5f;
     lv = __builtin_amdgcn_logf(fr), rv = 1.f / fr;
@@ -219,7 +220,9 @@ DEV void soften(Cols<DC, MT>& w, f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], const P
   if (__any(up)) {
 #pragma unroll
     for (int x = 0; x < MT; ++x) {
-      const float al = mnew[x] == -kInf ? 0.f : __builtin_amdgcn_exp2f(w.m[x] - mnew[x]), ao = __builtin_ldexpf(al, w.unit - unew);
+      const bool seen = w.pos[x] >= b0;
+      if (!seen) w.below[x] += unew - w.unit;
+      const float al = mnew[x] == -kInf ? 0.f : __builtin_amdgcn_exp2f(w.m[x] - mnew[x]), ao = __builtin_ldexpf(al, seen ? w.unit - unew : 0);
       w.sum[x] *= al;
 #pragma unroll
       for (int u = 0; u < 4 * DC; ++u) w.o[x][u] *= ao;
@@ -354,9 +357,9 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   }
 
   // the waves' sums joined in LDS, both less 2^16 so that a v scale next to fp32's largest does not leave it
-  const float us = __builtin_ldexpf(1.f, w.unit - 16);
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
+    const float us = __builtin_ldexpf(1.f, w.unit - w.below[x] - 16);
     w.sum[x] = quad_sum(w.sum[x]) * 0x1p-16f;
     const int col = threadIdx.x >> 4, p = 16 * x + col, row = p / g, e0 = 4 * (threadIdx.x & 15);
     float4 gate[DC];
@@ -402,9 +405,9 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 template <int DC>
 struct Cols32 {
   half8 q[2 * DC];   // 32-element chunk i, half y: elements 32 i + 16 (l >> 5) + 8 y + (0 .. 7), times a power of two
-  f32x16 o[DC];      // O^T: elements 32 u + 8 (r >> 2) + 4 (l >> 5) + (r & 3), over 2^(unit - kBase)
+  f32x16 o[DC];      // O^T: elements 32 u + 8 (r >> 2) + 4 (l >> 5) + (r & 3), over 2^(unit - below - kBase)
   float m, sum, qm;  // reference of the log2 scores, the lane's share of the sum, log2 score of a unit of S and of k's scale
-  int pos, unit;
+  int pos, unit, below;  // as in Cols
 };
 constexpr float kBase = 4.f;      // a weight is 2^kBase times its ratio to the reference's: 2^11 above it before fp16 ends,
 constexpr float kMost = 40000.f;  // which a lane's sum of weights up to kMost rules out
@@ -454,7 +457,7 @@ DEV void begin32(Cols32<DC>& w, const Attn& a, const Seq& s, int c0, int np, con
   w.qm = __builtin_ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
   const int ps = s.first + row;
   w.pos = on ? (ps < cap ? ps : (int)cap) : -1;
-  w.m = -kInf, w.sum = 0.f, w.unit = -200;
+  w.m = -kInf, w.sum = 0.f, w.unit = -200, w.below = 0;
 #pragma unroll
   for (int u = 0; u < DC; ++u)
 #pragma unroll
@@ -478,7 +481,8 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
   const float f = fmaxf(w.qm * Pages::lane(pg.ks, k), 0x1p-126f), iw = __builtin_ldexpf(Pages::lane(pg.rv, k), -dv);  // as in soften()
   float at = kBase + Pages::lane(pg.lv, k) + (float)dv - (w.m == -kInf ? 0.f : w.m);
   if (unew > w.unit) {
-    const int sh = w.unit - unew;
+    const int sh = lim >= 0 ? w.unit - unew : 0;
+    if (lim < 0) w.below += unew - w.unit;
 #pragma unroll
     for (int u = 0; u < DC; ++u)
 #pragma unroll
@@ -684,7 +688,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
     if (k + 1 < cnt) put(k + 1);
   }
   if (NW == 8 && !late) lds_barrier();
-  const float us = __builtin_ldexpf(1.f, w.unit - 16), sum = xsum_step<32>(w.sum) * 0x1p-16f;
+  const float us = __builtin_ldexpf(1.f, w.unit - w.below - 16), sum = xsum_step<32>(w.sum) * 0x1p-16f;
   int z = threadIdx.x & 63;  // worked out again: values kept from begin32() would cost registers through the loop
   asm volatile("" : "+v"(z));
   const int p = w0 + (z & 31), row = p / g, head = h * g + p - row * g;
@@ -716,8 +720,9 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
   constexpr int P = 8;
   __shared__ __align__(16) f32x4 so[NT];
   __shared__ float sm[NT / 16], sl[NT / 16];
-  const int head = blockIdx.x % a.hq, row = blockIdx.x / a.hq, t = threadIdx.x, G = NT / LE, grp = t / LE, d = a.c.d;
-  const int e = 4 * (LE * blockIdx.y + (t & (LE - 1)));
+  const int head = blockIdx.y % a.hq, row = blockIdx.x, t = threadIdx.x, G = NT / LE, grp = t / LE, d = a.c.d;
+  if (row < a.c.start[0] || row >= a.c.start[a.c.seqs]) return;
+  const int e = 4 * (LE * (blockIdx.y / a.hq) + (t & (LE - 1)));
   const size_t at = (size_t)row * a.hq + head, step = (size_t)a.c.rows * a.hq;
   const float4 gate = gate_of(a, grp == 0 && e < d, row, head, e);
   float m = -kInf, s = 0.f;
@@ -749,7 +754,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
   so[t] = v;
   if ((t & (LE - 1)) == 0) sm[grp] = m, sl[grp] = whole ? kAlone : s;
   __syncthreads();
-  if (grp || sl[0] == kAlone || row < a.c.start[0] || row >= a.c.start[a.c.seqs] || e >= d) return;
+  if (grp || sl[0] == kAlone || e >= d) return;
   float mn = -kInf;
 #pragma unroll
   for (int k = 0; k < NT / 16; ++k)
@@ -803,12 +808,16 @@ bool attn_shape_ok(int rows, int seqs, int max_rows, int max_len, int hq, int hk
          hq <= 1024 && hq % hkv == 0 && d >= 16 && d <= 256 && d % 16 == 0;
 }
 
+// A launch has fewer than 2^32 threads in a dimension.
+bool too_many(const Plan& p, int hkv) { return p.tiles * hkv >= 1 << 23; }
+
 }  // namespace
 
 API size_t dr_attn_kv8_ws(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d) {
   if (!attn_shape_ok(rows, seqs, max_rows, max_len, hq, hkv, d)) return 0;
   if (rows == 0 || seqs == 0 || max_rows == 0) return 256;
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
+  if (too_many(p, hkv)) return 0;
   return p.splits > 1 ? ((size_t)p.splits * rows * hq * (d + 2) * sizeof(float) + 255) & ~(size_t)255 : 256;
 }
 
@@ -826,6 +835,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   float* part = reinterpret_cast<float*>(ws);
   const Attn a{c, q, gate, y, part, part + (size_t)p.splits * rows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
                (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan};
+  if (too_many(p, hkv)) return -1;
   const dim3 grid((unsigned)(p.tiles * hkv), p.splits);
   auto few = [&](auto dc, auto mt) {
     hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), grid, dim3(NT), 0, st, a);
@@ -858,7 +868,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
     int le = 16;
     if ((long long)rows * hq >= 512)
       while (4 * le < d) le <<= 1;
-    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(rows * hq), (d + 4 * le - 1) / (4 * le)), dim3(NT), 0, st, a, le);
+    hipLaunchKernelGGL(k_attn_join, dim3(rows, hq * ((d + 4 * le - 1) / (4 * le))), dim3(NT), 0, st, a, le);
   }
   return 0;
 }

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(NT) k_rope(Rope a, int LS, int RB) {
 template <bool B16>
 int rope(const Rope& a, int ldx, int hsx, int ldn, int ldy, int ldb, hipStream_t st) {
   const long long n = (long long)a.heads * a.d;
-  if (a.rows < 0 || a.heads < 1 || a.heads > 4096 || a.d < 1 || a.d > 512 || a.rot < 0 || a.rot > a.d || a.rot % 2 || a.pairs < 0 || a.pairs > 1) return -1;
+  if (a.rows < 0 || a.rows > 1 << 23 || a.heads < 1 || a.heads > 4096 || a.d < 1 || a.d > 512 || a.rot < 0 || a.rot > a.d || a.rot % 2 || a.pairs < 0 || a.pairs > 1) return -1;
   if (hsx < a.d || ldx < (long long)(a.heads - 1) * hsx + a.d || (a.nw && ldn != 0 && ldn < a.d) || (!a.y && !a.yb) || (a.y && ldy < n) ||
       (a.yb && ldb < n) || (a.rot && (!a.pos || !a.freq)) || !a.x)
     return -1;

@@ -479,7 +479,7 @@ int dr_moe_layer_rows_fp8_bf16s(const dr_bf16* router, const uint8_t* gu_w, cons
  * drama-rs_amd/kvcache.py); both may be NULL where rot is 0.  y f32 and yb bf16: either may be NULL; head h of row r at r * ldy (ldb) + h * d.
  * y may be an f32 x, and yb a bf16 x, at the same strides with hsx = d.  Angles are formed in 64 bits, all else in fp32.  16-byte addresses
  * and strides of whole 16 bytes (8 for bf16) with d a multiple of 4 and rot of 8 take the wide path; any others work.
- * Unsupported: rows < 0, heads < 1 or > 4096, d < 1 or > 512, rot odd, < 0 or > d, an unknown layout, a missing x, neither y nor
+ * Unsupported: rows < 0 or > 8388608, heads < 1 or > 4096, d < 1 or > 512, rot odd, < 0 or > d, an unknown layout, a missing x, neither y nor
  * yb, rot without pos or freq, hsx < d, rows that overlap (ldx < (heads - 1) hsx + d; ldy, ldb < heads d), ldn between 1 and d - 1 or
  * negative -> -1.  rows == 0 does nothing. */
 int dr_rope(const float* x, int ldx, int hsx, const float* nw, int ldn, float eps, const int* pos, const float* freq, float mscale,
@@ -520,12 +520,15 @@ int dr_kv8_read(const int* start, const int* len, const int* table, int maxp, co
  *   y = bf16(sigmoid(gate) * sum_t softmax_t(scale * q . k_t) v_t), queries h (hq / hkv) .. of cached head h.
  * q bf16 and y bf16: query h of row r at r * ldq (ldy) + h * d; gate f32, NULL for none: at r * ldg + h * hsg.  y may be q at the same stride.  A row that
  * sees no token (a negative position, blocks that are not there) gets zeros; rows of no sequence are left as they were.  A query
- * with an infinity or NaN, or a block of scale NaN among what it sees, gives NaN to that row's query alone.
- * max_rows: no sequence has more rows (rows past it are not computed); max_len: the longest sequence, as far as the host knows it (a longer one
+ * with an infinity or NaN, or a block with a scale that is negative, infinite or NaN among what it sees, gives NaN to that row's query alone;
+ * blocks that a row does not see have no part in its result, whatever their scales.
+ * max_rows: no sequence has more rows (what y then holds for rows past it is undefined); max_len: the longest sequence, as far as the host knows it (a longer one
  * is computed as well).  The cut into blocks goes by these, so a graph that is replayed for growing sequences takes their final values.
- * Scores, softmax and sums are fp32; weights enter the product with v in fp16 (2^-11 of each).
+ * Scores, softmax and sums are fp32; weights, times their block's v scale, enter the product with v in fp16: 2^-11 of each, and at most 2^-29
+ * of the largest weight times the largest v scale that the row sees.
  * ws: dr_attn_kv8_ws(same sizes) bytes of scratch, holding anything, a multiple of 16 bytes.  Calls that share ws must not overlap (two graphs that may run at once need one each).
- * Unsupported: as above, and hq > 1024 or no multiple of hkv, max_rows or max_len < 0, ldq < hq d or no multiple of 8, ldy < hq d or
+ * Unsupported: as above, and a scale that is infinite or NaN, hq > 1024 or no multiple of hkv, max_rows or max_len < 0, 2^23 or more tiles of (rows, queries) of a cached
+ * head and sequence (at least one for each of them), ldq < hq d or no multiple of 8, ldy < hq d or
  * no multiple of 4, hsg < d, ldg < (hq - 1) hsg + d, either no multiple of 4, a missing q, y or ws, q, gate or ws no multiple of 16 bytes, y none of 8 -> -1 (ws size: 0). */
 size_t dr_attn_kv8_ws(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d);
 int dr_attn_kv8(const dr_bf16* q, int ldq, const int* start, const int* len, const int* table, int maxp, const uint8_t* kq,

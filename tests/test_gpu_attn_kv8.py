@@ -175,6 +175,31 @@ def test_what_is_not_seen_has_no_part():
         t.copy_(old)
 
 
+@pytest.mark.parametrize("rows,lens,hq,d", [([3, 1], [257, 60], 4, 64), ([3], [257], 12, 128), ([2], [1025], 8, 256), ([300], [300], 4, 64), ([90], [257], 4, 128), ([130], [200], 4, 256)])
+@pytest.mark.parametrize("far", [2.0 ** 60, 1e38])
+def test_later_blocks_of_huge_scale(rows, lens, hq, d, far):
+    """The rows of a call that see less keep their bits, however large the numbers are that only rows beside them see, and where a block is not there."""
+    import torch
+
+    c = cache(23, lens, 2, d)
+    last = (lens[0] - 1) // 64
+    call = Call(c, rows, lens, hq)
+    y = call.run()
+    first = lens[0] - rows[0]
+    before = last * 64 - first  # rows of sequence 0 that do not see its last block
+    assert 0 < before < rows[0]
+    call.dc.vs[int(c.table[0, last])] = far
+    z = call.run()
+    torch.cuda.synchronize()
+    assert torch.equal(z[:before], y[:before]) and torch.equal(z[rows[0]:], y[rows[0]:]) and not torch.equal(z[before:rows[0]], y[before:rows[0]])
+    # the page that an entry outside the pages stands in for has no part either
+    call.dc.table[0, last] = -1
+    call.dc.vs[0] = far if 0 not in c.table[:, :last].ravel().tolist() else call.dc.vs[0]
+    z = call.run()
+    torch.cuda.synchronize()
+    assert torch.equal(z[:before], y[:before])
+
+
 def test_queries_that_are_no_numbers():
     import torch
 
