@@ -27,6 +27,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int W = 4, NT = W * WAVE;
 constexpr float kInf = __builtin_inff();
+constexpr int kUnit = -200;  // an exponent below that of any scale
 
 struct Attn {
   Kv8 c;
@@ -77,10 +78,10 @@ struct Out {
       *reinterpret_cast<f32x4*>(part + e) = o;
       return;
     }
-    f32x4 v = o * inv;
-    if (gated) v[0] *= sigmoid(g.x), v[1] *= sigmoid(g.y), v[2] *= sigmoid(g.z), v[3] *= sigmoid(g.w);
-    *reinterpret_cast<uint2*>(y + e) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    store(e, gated ? gate(o * inv, g) : o * inv);
   }
+  DEV static f32x4 gate(const f32x4& v, const float4& g) { return v * f32x4{sigmoid(g.x), sigmoid(g.y), sigmoid(g.z), sigmoid(g.w)}; }
+  DEV void store(int e, const f32x4& v) const { *reinterpret_cast<uint2*>(y + e) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); }
 };
 // The gate's logits of those elements (an output waits for memory once where all of a lane's are asked for together).
 DEV float4 gate_of(const Attn& a, bool on, size_t row, int head, int e) {
@@ -105,7 +106,7 @@ template <int DC, int MT>
 DEV void begin(Cols<DC, MT>& w, const Attn& a, const Seq& s, int h, int c0, int np) {
   const int l = lane_id(), j = l >> 4, d = a.c.d, g = a.g;
   const long long cap = (long long)a.c.maxp * KB - 1;
-  w.unit = -200;
+  w.unit = kUnit;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int p = c0 + 16 * t + (l & 15), row = p / g;
@@ -176,7 +177,7 @@ struct Pages {
     if (!ok) ks = 0.f;
     // a scale of 0 weighs nothing, by an exponent far below any; nor does a block that is not there
     const bool pos = ok && p >= 0 && vs > 0.f;
-    ve = pos ? __builtin_amdgcn_frexp_expf(vs) : -200;
+    ve = pos ? __builtin_amdgcn_frexp_expf(vs) : kUnit;
     const float fr = pos ? __builtin_amdgcn_frexp_mantf(vs) : 0.5f;
     lv = __builtin_amdgcn_logf(fr), rv = 1.f / fr;
   }
@@ -281,15 +282,16 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   // the table's entries as the host's word for the lengths has it, beside the sequence's length itself
   const int ahead = page_of(a.c, i, (int)((long long)sp * a.chunk + wv + W * l < a.c.maxp ? sp * a.chunk + wv + W * l : -1));
   const Seq s = seq_of(a.c, i);
-  const int np = s.n * g < TP ? s.n * g : TP;
-  if (np == 0) return;
+  const int c0 = blockIdx.z * TP;
+  if (s.n * g <= c0) return;
+  const int np = s.n * g - c0 < TP ? s.n * g : c0 + TP;
   const long long cap = (long long)a.c.maxp * KB - 1;
-  const int p_lo = s.first, p_end = s.first + (np - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
+  const int p_lo = s.first + c0 / g, p_end = s.first + (np - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
   const int nb = p_hi < 0 ? 0 : (p_hi >> 6) + 1;
   int b0, b1;
   const bool alone = share(a, nb, sp, b0, b1);
   if (b0 == b1 && sp > 0) {
-    if (!alone) emit_none(a, s, h, sp, 0, np, threadIdx.x, NT);
+    if (!alone) emit_none(a, s, h, sp, c0, np, threadIdx.x, NT);
     return;
   }
   const int cnt = (b1 - b0 - wv + W - 1) / W;  // the wave's blocks b0 + wv, b0 + wv + W ..
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   if (b0 == sp * a.chunk) pg.fetch(a, h, l < cnt ? ahead : -1, l < cnt);
   else pg.fetch(a, i, h, b0 + wv + W * l, l < cnt);
   if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
-  begin(w, a, s, h, 0, np);
+  begin(w, a, s, h, c0, np);
   for (int k0 = 0; k0 < cnt; k0 += WAVE) {
     const int n = cnt - k0 < WAVE ? cnt - k0 : WAVE;
     if (k0) {
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   for (int x = 0; x < MT; ++x) {
     const float us = __builtin_ldexpf(1.f, w.unit - w.below[x] - 16);
     w.sum[x] = quad_sum(w.sum[x]) * 0x1p-16f;
-    const int col = threadIdx.x >> 4, p = 16 * x + col, row = p / g, e0 = 4 * (threadIdx.x & 15);
+    const int col = threadIdx.x >> 4, p = c0 + 16 * x + col, row = p / g, e0 = 4 * (threadIdx.x & 15);
     float4 gate[DC];
 #pragma unroll
     for (int c = 0; c < DC; ++c) gate[c] = gate_of(a, alone && p < np && e0 + 64 * c < d, (size_t)s.r0 + row, h * g + p - row * g, e0 + 64 * c);
@@ -457,7 +459,7 @@ DEV void begin32(Cols32<DC>& w, const Attn& a, const Seq& s, int c0, int np, con
   w.qm = __builtin_ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
   const int ps = s.first + row;
   w.pos = on ? (ps < cap ? ps : (int)cap) : -1;
-  w.m = -kInf, w.sum = 0.f, w.unit = -200, w.below = 0;
+  w.m = -kInf, w.sum = 0.f, w.unit = kUnit, w.below = 0;
 #pragma unroll
   for (int u = 0; u < DC; ++u)
 #pragma unroll
@@ -483,10 +485,12 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
   if (unew > w.unit) {
     const int sh = lim >= 0 ? w.unit - unew : 0;
     if (lim < 0) w.below += unew - w.unit;
+    if (w.unit > kUnit) {  // before there are no sums
 #pragma unroll
-    for (int u = 0; u < DC; ++u)
+      for (int u = 0; u < DC; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) w.o[u][r] = __builtin_ldexpf(w.o[u][r], sh);
+        for (int r = 0; r < 16; ++r) w.o[u][r] = __builtin_ldexpf(w.o[u][r], sh);
+    }
     w.unit = unew;
   }
   if (!(pg.num >> k & 1) && lim >= 0) w.sum = __builtin_nanf("");  // scales that are no numbers
@@ -694,112 +698,156 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   const int p = w0 + (z & 31), row = p / g, head = h * g + p - row * g;
   if (p >= c1) return;
   const size_t rw = (size_t)s.r0 + row;
-  float4 gate[DC][4];
-#pragma unroll
-  for (int u = 0; u < DC; ++u)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int e = 32 * u + 8 * r + 4 * (z >> 5);
-      gate[u][r] = gate_of(a, alone && e < d, rw, head, e);
-    }
   const Out out(a, alone, sp, rw, head, sum, w.m, z < 32);
+  const float fin = __builtin_ldexpf(out.inv, w.unit - w.below - 16);
+  // A block runs through this once, and what it costs is the fetch of its code: few branches (d ends on a multiple of 16), gates of as many
+  // elements at a time as registers allow.
+  auto each = [&](int u0, int n, auto f) {
 #pragma unroll
-  for (int u = 0; u < DC; ++u)
+    for (int u = 0; u < n; ++u)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int e = 32 * u + 8 * r + 4 * (z >> 5);
-      const f32x4 o = {w.o[u][4 * r] * us, w.o[u][4 * r + 1] * us, w.o[u][4 * r + 2] * us, w.o[u][4 * r + 3] * us};
-      if (e < d) out.put(e, o, gate[u][r]);
+      for (int x = 0; x < 2; ++x) {
+        if (32 * (u0 + u) + 16 * x >= d) break;
+#pragma unroll
+        for (int r = 2 * x; r < 2 * x + 2; ++r) f(u0 + u, r, 32 * (u0 + u) + 8 * r + 4 * (z >> 5));
+      }
+  };
+  auto o4 = [&](int u, int r, float s) { return f32x4{w.o[u][4 * r] * s, w.o[u][4 * r + 1] * s, w.o[u][4 * r + 2] * s, w.o[u][4 * r + 3] * s}; };
+  if (!alone) {
+    each(0, DC, [&](int u, int r, int e) { *reinterpret_cast<f32x4*>(out.part + e) = o4(u, r, us); });
+  } else if (!a.gate) {
+    each(0, DC, [&](int u, int r, int e) { out.store(e, o4(u, r, fin)); });
+  } else {
+    constexpr int GU = DC > 4 ? DC / 2 : DC;
+#pragma unroll
+    for (int u0 = 0; u0 < DC; u0 += GU) {
+      float4 gate[GU][4];
+      each(u0, GU, [&](int u, int r, int e) { gate[u - u0][r] = gate_of(a, true, rw, head, e); });
+      each(u0, GU, [&](int u, int r, int e) { out.store(e, Out::gate(o4(u, r, fin), gate[u - u0][r])); });
     }
+  }
 }
 
-// Joins the parts of a row's query, or of 64 elements of it where the queries are few: LE lanes of four elements, each group of them every
-// NT / LE'th part, eight at a time in flight, with a maximum of its own; the groups meet in LDS.
+// Joins the parts of a row's query, or of 4 LE elements of it where the queries are few: G groups of LE lanes of four elements, each group every
+// G'th part, eight at a time in flight, with a maximum of its own; the groups meet in LDS.  As many queries a block as that leaves room for.
 constexpr int kSplits = 128;  // at most
-__global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE) {
-  constexpr int P = 8;
+constexpr int kJoin = 8;      // parts of a group in flight
+__global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
   __shared__ __align__(16) f32x4 so[NT];
   __shared__ float sm[NT / 16], sl[NT / 16];
-  const int head = blockIdx.y % a.hq, row = blockIdx.x, t = threadIdx.x, G = NT / LE, grp = t / LE, d = a.c.d;
-  if (row < a.c.start[0] || row >= a.c.start[a.c.seqs]) return;
-  const int e = 4 * (LE * (blockIdx.y / a.hq) + (t & (LE - 1)));
-  const size_t at = (size_t)row * a.hq + head, step = (size_t)a.c.rows * a.hq;
-  const float4 gate = gate_of(a, grp == 0 && e < d, row, head, e);
+  const int t = threadIdx.x, gi = t / LE, grp = gi & (G - 1), d = a.c.d, n = a.c.rows * a.hq;
+  const int item = blockIdx.x * (NT / (LE * G)) + gi / G, at = item < n ? item : n - 1, row = at / a.hq, head = at - row * a.hq;
+  const int e = 4 * (LE * blockIdx.y + (t & (LE - 1)));
+  const bool on = item < n && e < d && row >= a.c.start[0] && row < a.c.start[a.c.seqs];
+  const size_t step = n;
+  const float4 gate = gate_of(a, on && grp == 0, row, head, e);
   float m = -kInf, s = 0.f;
   f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
   bool whole = false;
-  for (int s0 = grp; s0 < a.splits; s0 += P * G) {
-    uint2 w[P];
-    f32x4 r[P];
+  for (int s0 = grp; s0 < a.splits; s0 += kJoin * G) {
+    uint2 w[kJoin];
+    f32x4 r[kJoin];
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
+    for (int k = 0; k < kJoin; ++k) {
       const size_t sp = at + (s0 + G * k) * step;
       w[k] = make_uint2(0, 0), r[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (s0 + G * k < a.splits) w[k] = ld8(a.ml + 2 * sp), r[k] = gld<f32x4>(a.part + sp * d + (e < d ? e : 0));
+      if (on && s0 + G * k < a.splits) w[k] = ld8(a.ml + 2 * sp), r[k] = gld<f32x4>(a.part + sp * d + e);
     }
     float mn = m;
 #pragma unroll
-    for (int k = 0; k < P; ++k)
+    for (int k = 0; k < kJoin; ++k)
       if (w[k].y != 0) mn = fmaxf(mn, __uint_as_float(w[k].x));  // a part that saw no token (l = 0) has no sums
     if (s0 == 0) whole = __uint_as_float(w[0].y) == kAlone;
     const float ms = mn == -kInf ? 0.f : mn, c0 = __builtin_amdgcn_exp2f(m - ms);
     v *= c0, s *= c0, m = mn;
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
+    for (int k = 0; k < kJoin; ++k) {
       if (w[k].y == 0) continue;
       const float c = __builtin_amdgcn_exp2f(__uint_as_float(w[k].x) - ms);
       v += c * r[k], s += c * __uint_as_float(w[k].y);
     }
   }
-  so[t] = v;
-  if ((t & (LE - 1)) == 0) sm[grp] = m, sl[grp] = whole ? kAlone : s;
-  __syncthreads();
-  if (grp || sl[0] == kAlone || e >= d) return;
-  float mn = -kInf;
+  if (G > 1) {
+    so[t] = v;
+    if ((t & (LE - 1)) == 0) sm[gi] = m, sl[gi] = s;
+    __syncthreads();
+    float mn = -kInf;
 #pragma unroll
-  for (int k = 0; k < NT / 16; ++k)
-    if (k < G) mn = fmaxf(mn, sm[k]);
-  const float ms = mn == -kInf ? 0.f : mn;
-  s = 0.f, v = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < NT / 16; ++k)
+      if (k < G) mn = fmaxf(mn, sm[gi - grp + k]);
+    const float ms = mn == -kInf ? 0.f : mn;
+    s = 0.f, v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < NT / 16; ++k)
-    if (k < G) {
-      const float c = __builtin_amdgcn_exp2f(sm[k] - ms);
-      v += c * so[k * LE + t], s += c * sl[k];
-    }
-  Out(a, true, 0, row, head, s, 0.f, false).put(e, v, gate);
+    for (int k = 0; k < NT / 16; ++k)
+      if (k < G) {
+        const float c = __builtin_amdgcn_exp2f(sm[gi - grp + k] - ms);
+        v += c * so[t + (k - grp) * LE], s += c * sl[gi - grp + k];
+      }
+  }
+  if (on && grp == 0 && !whole) Out(a, true, 0, row, head, s, 0.f, false).put(e, v, gate);
 }
 
 // How a call is cut: by its sizes alone, so that the workspace is known before.
 struct Plan {
   bool few, scan;
-  int mt, nw, splits, chunk;
+  int mt, cols, nw, splits, chunk;
   long long tiles;
 };
 Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d) {
   Plan p;
-  const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g;
-  p.few = pairs <= 16 || (d <= 128 && pairs <= 32);
-  p.mt = pairs <= 16 ? 1 : 2;
-  auto cut = [&](long long tp) {
-    const long long per = (pairs + tp - 1) / tp, all = rows * g / tp + seqs;
-    p.scan = per > 1, p.tiles = per > 1 && all < per * seqs ? all : per * seqs;
+  const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g, blocks = ((long long)max_len + KB - 1) / KB, items = (long long)rows * hq;
+  // Few columns: each block of threads 16 or 32 pairs of a cached head and sequence.
+  p.mt = pairs <= 16 || d > 128 ? 1 : 2;
+  const long long cols = (pairs + 16 * p.mt - 1) / (16 * p.mt), few = cols * seqs * hkv;
+  // Many: tiles of 128 or 256 pairs; where sequences have several, of all rows together.  Eight waves only where a tile fills them and the tiles the
+  // card: 1000 rows of 32 heads 30.2 us with four, 35.8 with eight; 4096 behind 8192 tokens 465 and 344.
+  auto cut = [&](int nw) {
+    const long long tp = 32 * nw, per = (pairs + tp - 1) / tp, all = rows * g / tp + seqs;
+    p.nw = nw, p.scan = per > 1, p.tiles = per > 1 && all < per * seqs ? all : per * seqs;
   };
-  p.nw = p.few || d > 128 ? 4 : 8;
-  cut(p.few ? 16 * p.mt : 32 * p.nw);
-  // eight waves only where their tiles fill the card: 1000 rows of 32 heads 30.2 us with four, 35.8 with eight; 4096 behind 8192 tokens 465 and 344
-  if (p.nw == 8 && p.tiles * hkv < 256) p.nw = 4, cut(32 * p.nw);
-  // Blocks of threads to fill the card with.  Few columns: a CU holds two up to d 128 (one with two tiles of columns or wider heads), and with lengths
-  // apart a long sequence needs many (48 ragged sequences: 2048 57.5 us, 1024 75; 32 of 8000 tokens with heads of 256: 512 62 us, 2048 104).
-  // Many columns: 64 rows on 30000 tokens 38.8 us with 256, 42.3 with 512 (more parts to join), 51.6 with 128.
-  const long long blocks = ((long long)max_len + KB - 1) / KB, units = p.tiles * hkv, want = !p.few ? 256 : p.mt == 1 && d <= 128 ? 2048 : 512;
-  long long s = units >= want / 2 && !p.few ? 1 : (want + units - 1) / units;
-  const long long most = (blocks + W - 1) / W;
-  s = s > most ? most : s;
-  s = s > kSplits ? kSplits : s;
-  p.splits = s < 1 || blocks <= 16 ? 1 : (int)s;
+  cut(8);
+  if (d > 128 || pairs <= 128 || p.tiles * hkv < 256) cut(4);
+  // us: rounds of the blocks that the card holds, each a start and its steps, `at` cached blocks a step; with splits a launch that joins, and the
+  // parts out and back.  The constants are what single rounds took.  What the rule gives and the other side: 3 sequences of 1000 tokens with 72 pairs
+  // of d 256 14.7 us in few columns, 26 in split tiles, 58 in whole ones; 8 of 500 with 192 pairs of d 64 9.1, 15.6; 49 of 2000 with 122 pairs of
+  // d 128 25 in tiles, 30 in few columns; 30 of 40 tokens with 120 pairs of d 256 21 in tiles, 32 in few columns.
+  struct Cut {
+    long long s;
+    float us;
+  };
+  const float part = (float)items * d * 8 / 3e6f;
+  auto best = [&](long long units, int holds, int at, float start, float step) {
+    Cut c{1, 3e38f};
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
+      if (s > 1 && s * at > blocks) break;
+      const float us = (float)((units * s + holds - 1) / holds) * (start + step * (float)((blocks + s * at - 1) / (s * at))) + (s > 1 ? 3.f + s * part : 0.f);
+      if (us < c.us) c = Cut{s, us};
+    }
+    return c;
+  };
+  Cut c;
+  if (pairs <= 64) {
+    // With lengths apart a long sequence needs many splits (48 ragged sequences: blocks of threads up to 2048 57.5 us, to 1024 75; 32 of 8000
+    // tokens with heads of 256: to 512 62 us, to 2048 104).  Four waves walk over 16 blocks in less than a launch that joins takes.
+    const long long want = p.mt == 1 && d <= 128 ? 2048 : 512, most = (blocks + W - 1) / W;
+    p.few = true;
+    c.s = blocks <= 16 ? 1 : (want + few - 1) / few;
+    c.s = c.s > most ? most : c.s;
+    c.s = c.s > kSplits ? kSplits : c.s;
+  } else {
+    const float step = p.nw == 8 ? 1.6f : d <= 64 ? 1.f : d <= 128 ? 1.2f : d <= 192 ? 2.f : 2.8f;
+    c = best(p.tiles * hkv, 256, 1, d <= 128 ? 5.f : d <= 192 ? 8.f : 15.f, step);
+    const Cut f = best(few, d <= 128 ? 512 : 256, W, d <= 64 ? 4.f : 5.f, d <= 64 ? .7f : d <= 128 ? 1.8f : 2.9f);
+    // what either asks of L2, which the rounds leave out
+    const float each = blocks * KB * 2 * d / 8e6f;
+    p.few = pairs <= 2048 && f.us + each * few < c.us + each * p.tiles * hkv;
+    if (p.few) c = f;
+  }
+  if (p.few) p.scan = false, p.tiles = seqs;
+  p.cols = p.few ? (int)cols : 1;
+  p.splits = c.s < 1 || items >= 1 << 22 ? 1 : (int)c.s;  // with so many rows most are of no sequence, or there are blocks enough
   p.chunk = (int)((blocks + p.splits - 1) / p.splits);
-  if (p.chunk < W) p.chunk = W;
+  if (p.chunk < (p.few ? W : 1)) p.chunk = p.few ? W : 1;
   return p;
 }
 
@@ -836,7 +884,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   const Attn a{c, q, gate, y, part, part + (size_t)p.splits * rows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
                (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan};
   if (too_many(p, hkv)) return -1;
-  const dim3 grid((unsigned)(p.tiles * hkv), p.splits);
+  const dim3 grid((unsigned)(p.tiles * hkv), p.splits, p.cols);
   auto few = [&](auto dc, auto mt) {
     hipLaunchKernelGGL((k_attn_few<decltype(dc)::value, decltype(mt)::value>), grid, dim3(NT), 0, st, a);
   };
@@ -865,10 +913,13 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
     else d <= 192 ? tiles(i6) : tiles(i8);
   }
   if (p.splits > 1) {
-    int le = 16;
-    if ((long long)rows * hq >= 512)
+    int le = 16, grps = 1;
+    const long long items = (long long)rows * hq;
+    if (items >= 512)
       while (4 * le < d) le <<= 1;
-    hipLaunchKernelGGL(k_attn_join, dim3(rows, hq * ((d + 4 * le - 1) / (4 * le))), dim3(NT), 0, st, a, le);
+    while (grps * kJoin < p.splits && 2 * grps * le <= NT) grps <<= 1;
+    const int per = NT / (le * grps);
+    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)((items + per - 1) / per), (d + 4 * le - 1) / (4 * le)), dim3(NT), 0, st, a, le, grps);
   }
   return 0;
 }

@@ -106,6 +106,26 @@ def test_attention(rows, lens, hq, hkv, d, gate, behind, pad):
         assert torch.equal(call.q[:n], y[:n])
 
 
+# every way to cut a call: few columns in one block of threads or several, whole or split, and tiles of four and eight waves, whole or split
+CUTS = [
+    ([3], [40], 40, 2, 64, True), ([3], [3000], 40, 2, 64, False), ([8], [1500], 12, 2, 128, True), ([5, 2], [1300, 70], 20, 4, 256, True), ([9], [9], 16, 4, 192, False),
+    ([30, 7, 0, 12], [30, 7, 5, 900], 8, 2, 128, False), ([30, 7, 0, 12], [30, 7, 5, 900], 8, 2, 256, True), ([100], [100], 8, 2, 256, False), ([140], [700], 4, 1, 64, False),
+    ([300], [1000], 8, 2, 64, True), ([300], [1000], 8, 2, 128, False), ([300], [700], 8, 1, 256, True), ([600], [600], 8, 1, 160, False), ([700, 20], [900, 20], 8, 1, 128, False),
+    ([20] * 40, [20 + i for i in range(40)], 32, 8, 64, False), ([4] * 300, [1 + i % 9 for i in range(300)], 16, 1, 32, True),
+    ([2100], [2100], 8, 1, 96, False), ([64] * 9, [64 + 300 * i for i in range(9)], 8, 4, 128, False),
+]
+
+
+@pytest.mark.parametrize("rows,lens,hq,hkv,d,gate", CUTS)
+def test_every_cut(rows, lens, hq, hkv, d, gate):
+    import torch
+
+    call = Call(cache(31, lens, hkv, d), rows, lens, hq, gate=gate, behind=1, seed=4)
+    y = call.run()
+    torch.cuda.synchronize()
+    call.check(y)
+
+
 @pytest.mark.parametrize("rows,lens,hq,hkv,d", [([1], [900], 8, 2, 128), ([70], [300], 4, 2, 64), ([1, 3], [2000, 100], 4, 1, 256)])
 @pytest.mark.parametrize("max_len", [0, 1, 100000])
 def test_any_cut_is_right(rows, lens, hq, hkv, d, max_len):
