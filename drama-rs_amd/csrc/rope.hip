@@ -3,11 +3,15 @@
 //   th = pos freq[j], c = mscale cos th, s = mscale sin th,  j < rot / 2
 //   (a, b) = (n[j], n[j + rot/2]) or, in pairs, (n[2 j], n[2 j + 1]) -> (a c - b s, b c + a s); elements from rot on stay n.
 //
-// A block takes a row, or as many rows as give its lanes work: it requests its elements, works out the rows' cosines and
+// A block takes a row (or a share of its heads, or as many rows as give its lanes work): it requests its elements, works out the rows' cosines and
 // sines once for all heads (LDS), and turns.  The lanes of a head (a power of two within a wave) hold both partners of
 // each pair, so the norm is a butterfly and nothing else crosses lanes, and y may be x.  Angles: the product of a position
 // and a frequency in 64 bits, its whole turns taken off there (at position 10^6 fp32 would be 0.06 rad off), the
 // sine and cosine of the rest in fp32.
+//
+// Every element is loaded once and stored once, so memory bounds large calls: 8192 rows of 16 heads of 256 (64 turned, gates between the heads, fp32
+// in, bf16 out) 38.4 us, 5.24 TB/s.  Small ones are a launch and one chain of loads, sums and stores: one row of 20 heads of 128 3.5 us; 777 rows of
+// 15 heads of 80, 36 turned in pairs (a load an element), 5.4 us.
 #include "common.hpp"
 
 using namespace drm;
@@ -83,7 +87,8 @@ __global__ void __launch_bounds__(NT) k_rope(Rope a, int LS, int RB) {
   extern __shared__ float2 cs[];  // [RB][rot / 2]
   const int half = a.rot >> 1, turned = half / V, tail = (a.d - a.rot + 2 * V - 1) / (2 * V), units = turned + tail;
   const long long r0 = (long long)blockIdx.x * RB;
-  const int nr = a.rows - r0 < RB ? (int)(a.rows - r0) : RB, items = (nr * a.heads) << LS, l = threadIdx.x & ((1 << LS) - 1);
+  const int hb = (a.heads + gridDim.y - 1) / gridDim.y, h0 = blockIdx.y * hb, nh = a.heads - h0 < hb ? a.heads - h0 : hb;
+  const int nr = a.rows - r0 < RB ? (int)(a.rows - r0) : RB, items = (nr * nh) << LS, l = threadIdx.x & ((1 << LS) - 1);
   int e0[PER], e1[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
@@ -100,7 +105,7 @@ __global__ void __launch_bounds__(NT) k_rope(Rope a, int LS, int RB) {
 #pragma unroll
     for (int x = 0; x < U; ++x) {
       const int w = w0 + NT * x, hr = w >> LS;
-      rl[x] = RB == 1 ? 0 : hr / a.heads, h[x] = hr - rl[x] * a.heads;
+      rl[x] = RB == 1 ? 0 : hr / nh, h[x] = h0 + hr - rl[x] * nh;
       const size_t xb = (size_t)(r0 + rl[x]) * a.ldx + (size_t)h[x] * a.hsx;
 #pragma unroll
       for (int u = 0; u < PER; ++u)
@@ -188,9 +193,12 @@ int rope(const Rope& a, int ldx, int hsx, int ldn, int ldy, int ldb, hipStream_t
   int LS = 0;
   while ((1 << LS) < units && LS < 6) ++LS;
   const int per_row = a.heads << LS, RB = per_row >= NT ? 1 : NT / per_row;
-  const dim3 g((unsigned)(((long long)a.rows + RB - 1) / RB)), b(NT);
+  // rows that do not fill the card share their heads out to several blocks: 67 rows of 39 heads of 219 4.3 us (15.4 with a block a row), one of 40
+  // heads of 256 3.8 (6.2)
+  const int loops = (per_row + NT - 1) / NT, U = vec && loops > 1 ? 2 : 1, room = a.rows < 2048 ? 2048 / a.rows : 1, most = (loops + U - 1) / U;
+  const dim3 g((unsigned)(((long long)a.rows + RB - 1) / RB), most < room ? most : room), b(NT);
   const size_t lds = (size_t)RB * (a.rot >> 1) * sizeof(float2);
-  if (vec && per_row > NT) hipLaunchKernelGGL((k_rope<B16, 4, 1, 2>), g, b, lds, st, a, LS, RB);
+  if (U == 2) hipLaunchKernelGGL((k_rope<B16, 4, 1, 2>), g, b, lds, st, a, LS, RB);
   else if (vec) hipLaunchKernelGGL((k_rope<B16, 4, 1, 1>), g, b, lds, st, a, LS, RB);
   else if (units <= 1 << LS) hipLaunchKernelGGL((k_rope<B16, 1, 1, 1>), g, b, lds, st, a, LS, RB);
   else hipLaunchKernelGGL((k_rope<B16, 1, 4, 1>), g, b, lds, st, a, LS, RB);

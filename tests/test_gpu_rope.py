@@ -38,6 +38,9 @@ CASES = [
     (4, 2, 3, 2, True, True, 1, 3, 1), (3, 7, 33, 20, False, True, 2, 5, 3), (2, 2, 512, 512, True, True, 0, 0, 0), (2, 1, 511, 510, False, True, 1, 1, 1),
     (300, 4, 96, 0, False, True, 0, 0, 0), (1000, 1, 8, 8, False, True, 0, 0, 0), (129, 3, 100, 24, True, True, 0, 0, 0), (64, 40, 64, 32, False, False, 0, 0, 2),
     (2, 130, 192, 192, False, True, 0, 0, 0),
+    # few rows whose heads several blocks share, evenly and not
+    (1, 40, 256, 256, False, True, 0, 0, 0), (3, 37, 128, 64, True, True, 4, 8, 0), (5, 39, 219, 108, True, True, 1, 3, 1), (2, 130, 33, 32, False, False, 0, 0, 0),
+    (300, 30, 223, 160, False, True, 0, 0, 0),
 ]
 
 
