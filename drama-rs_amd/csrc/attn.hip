@@ -1,19 +1,20 @@
 // Attention over the cache in 8 bits (layout: kv8.hpp): row r at position p of sequence i sees the sequence's tokens 0 .. p,
 //   z_t = scale q . k_t,  w_t = exp(z_t) / sum exp(z),  y = sigmoid(gate) sum_t w_t v_t.
 //
-// The g = hq / hkv queries of a cached head and a sequence's rows make the columns (pairs) of both products, which run on
-// v_mfma_f32_16x16x32_f16 with the cache as the row operand: S^T = K Q^T, O^T = V^T P^T.  A lane then holds 16 scores of one
-// column and every block of 64 tokens, the maximum of a column is 15 fmaxf and two cross-lane steps, and the weights are the second
-// product's operand as they stand.  Stored bytes become fp16 exactly: byte u beside 0x64 is 1024 + u, less 1152 is q.  A query
+// The g = hq / hkv queries of a cached head and a sequence's rows make the columns (pairs) of both products, which run on the fp16 matrix
+// instructions with the cache as the row operand: S^T = K Q^T, O^T = V^T P^T.  A lane then holds scores of one column only, a column's maximum
+// and sum are a lane's own and one or two cross-lane steps, and the weights are the second product's operand as they stand.
+// Stored bytes become fp16 exactly: byte u beside 0x64 is 1024 + u, less 1152 is q.  A query
 // (bf16) is fp16 times a power of two of its own that brings its largest element into [2^12, 2^13): exact down to 2^-29 of that
-// element, below it rounded by 2^-37 of it.  Weights are rounded to fp16 (2^-11 of each; the bf16 output is rounded
-// by 2^-8) as 2^15 exp(z - max), so that those down to 2^-29 of the largest keep all their bits.  Running maximum, sums and both products
+// element, below it rounded by 2^-37 of it.  Weights are rounded to fp16 (2^-11 of each; the bf16 output is rounded by 2^-8) as
+// 2^15 exp(z - max) with few columns, 2^4 exp(z - reference) with many, so that at least those down to 2^-18 of the largest keep all their
+// bits and smaller ones are rounded by 2^-29 of it.  Running maximum, sums and both products
 // are fp32; a block's k scale multiplies its scores, its v scale joins the exponent, relative to a
 // power of two that no scale so far exceeds (a row's bits then do not turn on the scale of a block that it does not see).
 //
 // Two kernels.  Few columns (a decode step): a wave walks over cached blocks by itself with no barrier, the next block's bytes requested as soon
 // as this one's are used.  Many (prompts): a block's bytes are converted once for all waves, in LDS.  Where the columns alone leave CUs
-// idle the cached blocks are split over blocks of threads, whose sums (fp32) a second launch joins.
+// idle the cached blocks are split over blocks of threads, whose sums (fp32) a second launch joins.  plan() chooses.
 #include "kv8.hpp"
 
 using namespace drm;
@@ -269,7 +270,11 @@ DEV void emit_none(const Attn& a, const Seq& s, int h, int sp, int c0, int c1, i
 }
 
 // Few columns: the four waves of a block of threads hold the same MT tiles of them and take every fourth cached block.  The last chunk of a
-// head may be part of one: what lies past d is loaded from inside the head, times zero queries, and not stored.
+// head may be part of one: what lies past d is loaded from inside the head, times zero queries, and not stored.  More pairs than a block of threads
+// holds are several blocks (z), which find the cache in L2.
+// Memory bounds it where sequences are long: 48 ragged sequences of 115191 tokens in all, 8 cached heads of 128, 216 MB in 53 us (4.1 TB/s), 32 of 8000
+// in 104 with the join (5.07 TB/s of 5.12 that a copy reaches); one of 60001 tokens with 2 heads of 256 is two to three blocks a wave,
+// 61 MB in 18.  Short ones are a chain of loads (length and table, scales and bytes, LDS): 300 tokens 7.4 us, of which 3 to 4 are the launch.
 template <int DC, int MT>
 __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   constexpr int TP = 16 * MT, LD = 64 * DC + 4;
@@ -404,6 +409,12 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 // What bounds it is the vector unit, which a product keeps for 10 to 12 cycles whatever its size: hence 32 x 32 x 16 products, and a
 // softmax without a maximum where it can be: a column's reference is the maximum of an earlier block, and only where a lane's sum says that a
 // weight may have passed fp16 (or the column has no reference yet) is the block's maximum taken, O rescaled and the weights formed again.
+// 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 343 to 358 us, 0.96 to 1.0 PFLOP/s (a large library product in fp16: 1.33); the matrix
+// unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 548 us (1.0),
+// heads of 64 111 us (0.62: the softmax is as long for half the products), of 256 262 us for 2048 rows on 6144 (0.65: four waves a CU,
+// no other wave's products beside a softmax, and 90 of a lane's registers in memory, which are read where a turn or the epilogue starts).
+// Short prompts are steps of 1 to 1.2 us (2.8 with heads of 256) behind a start of 5 (15), most of it the fetch of code that runs once: 7 prompts
+// of 33 to 373 rows, 12 heads of 64, 13.3 us.
 template <int DC>
 struct Cols32 {
   half8 q[2 * DC];   // 32-element chunk i, half y: elements 32 i + 16 (l >> 5) + 8 y + (0 .. 7), times a power of two
@@ -729,7 +740,8 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
 }
 
 // Joins the parts of a row's query, or of 4 LE elements of it where the queries are few: G groups of LE lanes of four elements, each group every
-// G'th part, eight at a time in flight, with a maximum of its own; the groups meet in LDS.  As many queries a block as that leaves room for.
+// G'th part, eight at a time in flight, with a maximum of its own; the groups meet in LDS.  As many queries a block as that
+// leaves room for.  A launch and two rounds of loads: 4 to 5 us for all of the above.
 constexpr int kSplits = 128;  // at most
 constexpr int kJoin = 8;      // parts of a group in flight
 __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
