@@ -38,7 +38,7 @@ struct Attn {
   float *part, *ml;  // [splits, rows, hq, d] and [splits, rows, hq, 2]
   size_t ldq, ldg, hsg, ldy;
   float scale;
-  int hq, g, splits, chunk, scan;
+  int hq, g, splits, chunk, scan, fold;
 };
 
 DEV half8 to_half8(uint32_t a, uint32_t b) {
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 // What bounds it is the vector unit, which a product keeps for 10 to 12 cycles whatever its size: hence 32 x 32 x 16 products, and a
 // softmax without a maximum where it can be: a column's reference is the maximum of an earlier block, and only where a lane's sum says that a
 // weight may have passed fp16 (or the column has no reference yet) is the block's maximum taken, O rescaled and the weights formed again.
-// 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 343 to 358 us, 0.96 to 1.0 PFLOP/s (a large library product in fp16: 1.33); the matrix
+// 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 341 us, 1.01 PFLOP/s (a large library product in fp16: 1.33); the matrix
 // unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 548 us (1.0),
 // heads of 64 111 us (0.62: the softmax is as long for half the products), of 256 262 us for 2048 rows on 6144 (0.65: four waves a CU,
 // no other wave's products beside a softmax, and 90 of a lane's registers in memory, which are read where a turn or the epilogue starts).
@@ -554,19 +554,26 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   if (a.scan) i = find_item(a.c, at, s, [g](const Seq& q) { return (q.n * g + TP - 1) / TP; });
   else at = 0, s = seq_of(a.c, i);
   if (i < 0) return;
-  const int np = a.scan || s.n * g < TP ? s.n * g : TP, c0 = at * TP, c1 = c0 + TP < np ? c0 + TP : np;
-  if (c0 >= np) return;
+  const int np = a.scan || s.n * g < TP ? s.n * g : TP;
+  // folded: the first four waves have a half tile, the others (none in the middle one) its mirror image in the sequence, which ends later
+  const bool fold = NW == 8 && a.fold;
+  const int half = fold ? TP / 2 : TP, c0 = at * half, m0 = fold ? ((np - 1) / half - at) * half : c0;
+  if (c0 >= np || m0 < c0) return;
+  const int c1 = m0 + half < np ? m0 + half : np;
   const long long cap = (long long)a.c.maxp * KB - 1;
   const int p_end = s.first + (c1 - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
   int b0, b1;
   const bool alone = share(a, p_hi < 0 ? 0 : (p_hi >> 6) + 1, sp, b0, b1);
   if (b0 == b1 && sp > 0) {
-    if (!alone) emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);
+    if (!alone) {
+      emit_none(a, s, h, sp, c0, c0 + half < np ? c0 + half : np, threadIdx.x, 64 * NW);
+      if (m0 > c0) emit_none(a, s, h, sp, m0, c1, threadIdx.x, 64 * NW);
+    }
     return;
   }
   const int cnt = b1 - b0;
   // the wave's columns and how many of the blocks they see
-  const int w0 = c0 + 32 * wv, w1 = w0 + 32 < c1 ? w0 + 32 : c1;
+  const int w0 = !fold || wv < 4 ? c0 + 32 * wv : m0 > c0 ? m0 + 32 * (wv - 4) : np, w1 = w0 + 32 < c1 ? w0 + 32 : c1;
   const int w_lo = s.first + w0 / g, w_end = s.first + (w1 - 1) / g, w_cnt = w0 < c1 && w_end >= 0 ? (w_end >> 6) + 1 - b0 : 0;
 
   // load f of the wave: k of 32 tokens (tile t) and of 32 elements (chunk c), 16 of them a lane; v of 32 elements (tile) and of the tokens
@@ -801,7 +808,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
 
 // How a call is cut: by its sizes alone, so that the workspace is known before.
 struct Plan {
-  bool few, scan;
+  bool few, scan, fold;
   int mt, cols, nw, splits, chunk;
   long long tiles;
 };
@@ -811,14 +818,14 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   // Few columns: each block of threads 16 or 32 pairs of a cached head and sequence.
   p.mt = pairs <= 16 || d > 128 ? 1 : 2;
   const long long cols = (pairs + 16 * p.mt - 1) / (16 * p.mt), few = cols * seqs * hkv;
-  // Many: tiles of 128 or 256 pairs; where sequences have several, of all rows together.  Eight waves only where a tile fills them and the tiles the
-  // card: 1000 rows of 32 heads 30.2 us with four, 35.8 with eight; 4096 behind 8192 tokens 465 and 344.
+  // Many: tiles of 128 or 256 pairs; where sequences have several, of all rows together.  Eight waves only where a tile fills them and the tiles
+  // most of the card (16 heads of 128, 2 cached; behind 8192 tokens 2800 rows 254 us with eight, 283 with four, 2100 215 and 203).
   auto cut = [&](int nw) {
     const long long tp = 32 * nw, per = (pairs + tp - 1) / tp, all = rows * g / tp + seqs;
     p.nw = nw, p.scan = per > 1, p.tiles = per > 1 && all < per * seqs ? all : per * seqs;
   };
   cut(8);
-  if (d > 128 || pairs <= 128 || p.tiles * hkv < 256) cut(4);
+  if (d > 128 || pairs <= 128 || p.tiles * hkv < 176) cut(4);
   // us: rounds of the blocks that the card holds, each a start and its steps, `at` cached blocks a step; with splits a launch that joins, and the
   // parts out and back.  The constants are what single rounds took.  What the rule gives and the other side: 3 sequences of 1000 tokens with 72 pairs
   // of d 256 14.7 us in few columns, 26 in split tiles, 58 in whole ones; 8 of 500 with 192 pairs of d 64 9.1, 15.6; 49 of 2000 with 122 pairs of
@@ -860,6 +867,9 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   p.splits = c.s < 1 || items >= 1 << 22 ? 1 : (int)c.s;  // with so many rows most are of no sequence, or there are blocks enough
   p.chunk = (int)((blocks + p.splits - 1) / p.splits);
   if (p.chunk < (p.few ? W : 1)) p.chunk = p.few ? W : 1;
+  // Where all tiles run at once the last rows' take longest: folding gives each as many steps as the next (4096 rows of 16 heads behind 8192 tokens
+  // 341 us, 352 without; 98 and 109 behind none).  With more tiles than that the next ones fill the gaps (8192 rows of 32 heads 538 without, 634 folded).
+  p.fold = !p.few && p.nw == 8 && p.tiles * hkv * p.splits <= 256;
   return p;
 }
 
@@ -894,7 +904,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
   float* part = reinterpret_cast<float*>(ws);
   const Attn a{c, q, gate, y, part, part + (size_t)p.splits * rows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
-               (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan};
+               (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan, p.fold};
   if (too_many(p, hkv)) return -1;
   const dim3 grid((unsigned)(p.tiles * hkv), p.splits, p.cols);
   auto few = [&](auto dc, auto mt) {

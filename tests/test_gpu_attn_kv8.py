@@ -112,7 +112,7 @@ CUTS = [
     ([30, 7, 0, 12], [30, 7, 5, 900], 8, 2, 128, False), ([30, 7, 0, 12], [30, 7, 5, 900], 8, 2, 256, True), ([100], [100], 8, 2, 256, False), ([140], [700], 4, 1, 64, False),
     ([300], [1000], 8, 2, 64, True), ([300], [1000], 8, 2, 128, False), ([300], [700], 8, 1, 256, True), ([600], [600], 8, 1, 160, False), ([700, 20], [900, 20], 8, 1, 128, False),
     ([20] * 40, [20 + i for i in range(40)], 32, 8, 64, False), ([4] * 300, [1 + i % 9 for i in range(300)], 16, 1, 32, True),
-    ([2100], [2100], 8, 1, 96, False), ([64] * 9, [64 + 300 * i for i in range(9)], 8, 4, 128, False),
+    ([2100], [2100], 8, 1, 96, False), ([1500], [1600], 32, 1, 64, True), ([700, 300, 701], [1000, 300, 701], 32, 1, 128, False), ([1430], [1430], 32, 1, 32, False), ([64] * 9, [64 + 300 * i for i in range(9)], 8, 4, 128, False),
 ]
 
 
