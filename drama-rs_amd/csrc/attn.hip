@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 // softmax without a maximum where it can be: a column's reference is the maximum of an earlier block, and only where a lane's sum says that a
 // weight may have passed fp16 (or the column has no reference yet) is the block's maximum taken, O rescaled and the weights formed again.
 // 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 341 us, 1.01 PFLOP/s (a large library product in fp16: 1.33); the matrix
-// unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 548 us (1.0),
+// unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 538 us (1.0),
 // heads of 64 111 us (0.62: the softmax is as long for half the products), of 256 262 us for 2048 rows on 6144 (0.65: four waves a CU,
 // no other wave's products beside a softmax, and 90 of a lane's registers in memory, which are read where a turn or the epilogue starts).
 // Short prompts are steps of 1 to 1.2 us (2.8 with heads of 256) behind a start of 5 (15), most of it the fetch of code that runs once: 7 prompts
@@ -829,7 +829,8 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   // us: rounds of the blocks that the card holds, each a start and its steps, `at` cached blocks a step; with splits a launch that joins, and the
   // parts out and back.  The constants are what single rounds took.  What the rule gives and the other side: 3 sequences of 1000 tokens with 72 pairs
   // of d 256 14.7 us in few columns, 26 in split tiles, 58 in whole ones; 8 of 500 with 192 pairs of d 64 9.1, 15.6; 49 of 2000 with 122 pairs of
-  // d 128 25 in tiles, 30 in few columns; 30 of 40 tokens with 120 pairs of d 256 21 in tiles, 32 in few columns.
+  // d 128 25 in tiles, 30 in few columns; 30 of 40 tokens with 120 pairs of d 256 21 in tiles, 32 in few columns;
+  // 63 of 10 with 40 pairs of d 112 9.5 in tiles, 15.7 in few columns.
   struct Cut {
     long long s;
     float us;
@@ -845,7 +846,8 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
     return c;
   };
   Cut c;
-  if (pairs <= 64) {
+  const int holds = d <= 128 ? 512 : 256;  // blocks of few columns
+  if (pairs <= 32 || (pairs <= 64 && (blocks > 16 || 2 * few <= 3 * holds))) {
     // With lengths apart a long sequence needs many splits (48 ragged sequences: blocks of threads up to 2048 57.5 us, to 1024 75; 32 of 8000
     // tokens with heads of 256: to 512 62 us, to 2048 104).  Four waves walk over 16 blocks in less than a launch that joins takes.
     const long long want = p.mt == 1 && d <= 128 ? 2048 : 512, most = (blocks + W - 1) / W;
@@ -856,7 +858,7 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   } else {
     const float step = p.nw == 8 ? 1.6f : d <= 64 ? 1.f : d <= 128 ? 1.2f : d <= 192 ? 2.f : 2.8f;
     c = best(p.tiles * hkv, 256, 1, d <= 128 ? 5.f : d <= 192 ? 8.f : 15.f, step);
-    const Cut f = best(few, d <= 128 ? 512 : 256, W, d <= 64 ? 4.f : 5.f, d <= 64 ? .7f : d <= 128 ? 1.8f : 2.9f);
+    const Cut f = best(few, holds, W, d <= 64 ? 4.f : 5.f, d <= 64 ? .7f : d <= 128 ? 1.8f : 2.9f);
     // what either asks of L2, which the rounds leave out
     const float each = blocks * KB * 2 * d / 8e6f;
     p.few = pairs <= 2048 && f.us + each * few < c.us + each * p.tiles * hkv;
