@@ -565,10 +565,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   int b0, b1;
   const bool alone = share(a, p_hi < 0 ? 0 : (p_hi >> 6) + 1, sp, b0, b1);
   if (b0 == b1 && sp > 0) {
-    if (!alone) {
-      emit_none(a, s, h, sp, c0, c0 + half < np ? c0 + half : np, threadIdx.x, 64 * NW);
-      if (m0 > c0) emit_none(a, s, h, sp, m0, c1, threadIdx.x, 64 * NW);
-    }
+    if (!alone) emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);  // not folded: that is without splits
     return;
   }
   const int cnt = b1 - b0;
@@ -871,7 +868,7 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   if (p.chunk < (p.few ? W : 1)) p.chunk = p.few ? W : 1;
   // Where all tiles run at once the last rows' take longest: folding gives each as many steps as the next (4096 rows of 16 heads behind 8192 tokens
   // 341 us, 352 without; 98 and 109 behind none).  With more tiles than that the next ones fill the gaps (8192 rows of 32 heads 538 without, 634 folded).
-  p.fold = !p.few && p.nw == 8 && p.tiles * hkv * p.splits <= 256;
+  p.fold = !p.few && p.nw == 8 && p.splits == 1 && p.tiles * hkv <= 256;
   return p;
 }
 

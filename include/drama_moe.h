@@ -496,7 +496,8 @@ int dr_rope_bf16(const dr_bf16* x, int ldx, int hsx, const float* nw, int ldn, f
  *   vq u8 [pages, hkv, d, 64]: token 16 a + 4 b + c of element x at [.., x, 16 b + 4 a + c];  both hold q + 128, -127 <= q <= 127;
  *   ks, vs f32 [pages, hkv]: an element is q * scale.
  * table i32 [seqs, maxp] names the page of each block of a sequence: block b holds tokens 64 b .. 64 b + 63.  An entry outside 0 .. pages - 1
- * (or a token past 64 maxp): that block is not there.  The same page may stand for several sequences as long as no call appends to it.
+ * (or a token past 64 maxp): that block is not there.  The same page may stand for several blocks, of one sequence or more, as long as no
+ * call appends to it.
  * start i32 [seqs + 1], ascending: rows start[i] .. start[i + 1] - 1 of a call belong to sequence i.  len i32 [seqs]: its tokens with
  * those rows, so that its first row has position len[i] - (start[i + 1] - start[i]); a row of negative position is no token.  Rows before start[0] and
  * from start[seqs] on belong to none: nothing of theirs is read or written.  All of these are read on the device.  kq and vq are multiples of 16 bytes.

@@ -166,6 +166,25 @@ def test_peaked_and_flat_weights():
         call.check(y)
 
 
+@pytest.mark.parametrize("rows,lens,hq,hkv,d", [([1], [4000], 4, 1, 64), ([3], [2000], 16, 1, 256), ([300], [4000], 8, 1, 128), ([600], [2500], 8, 1, 64), ([400], [1500], 8, 1, 256)])
+@pytest.mark.parametrize("octaves", [17.5, 21.5, 26.5])
+def test_small_weights_add_up(rows, lens, hq, hkv, d, octaves):
+    """One token without a value of its own outweighs all others together or nearly, which decide the result: fp16's subnormals count."""
+    import torch
+
+    c = cache(25, lens, hkv, d)
+    first = int(c.table[0, 0])
+    c.k[:], c.v[:] = -60, np.minimum(np.abs(c.v) + 1, 127)
+    c.k[first, :, 0], c.v[first, :, 0] = 60, 0
+    c.ks[:], c.vs[:] = 2.0 ** -4, 0.02
+    call = Call(c, rows, lens, hq, scale=octaves * np.log(2) / (120 * 2.0 ** -4 * d))
+    call.q[:, :hq * d] = 1.0
+    y = call.run()
+    torch.cuda.synchronize()
+    call.check(y)
+    assert (y[:, :hq * d] != 0).all()
+
+
 def test_what_is_not_seen_has_no_part():
     """Scales that are no numbers and full-size integers in places behind a row's position, in blocks of no sequence and behind the last token."""
     import torch
