@@ -524,7 +524,8 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
-    const float top = xmax_step<32>(mx) * f;
+    // a column's own lanes alone decide, so that what is in the other columns has no part in its bits (2% of a long chunk's time)
+    const float most = xmax_step<32>(add), high = xmax_step<32>(mx) * f, top = !(most <= kMost) || w.m == -kInf ? high : w.m;
     if (top > w.m) {
       // less than the reference stays as it is; without one (m -infinity) there are no sums to scale
       const float al = w.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(w.m - top);

@@ -521,7 +521,7 @@ int dr_kv8_read(const int* start, const int* len, const int* table, int maxp, co
  *   y = bf16(sigmoid(gate) * sum_t softmax_t(scale * q . k_t) v_t), queries h (hq / hkv) .. of cached head h.
  * q bf16 and y bf16: query h of row r at r * ldq (ldy) + h * d; gate f32, NULL for none: at r * ldg + h * hsg.  y may be q at the same stride.  A row that
  * sees no token (a negative position, blocks that are not there) gets zeros; rows of no sequence are left as they were.  A query
- * with an infinity or NaN, or a block with a scale that is negative, infinite or NaN among what it sees, gives NaN to that row's query alone;
+ * with an infinity or NaN, or a block with a scale that is negative, infinite or NaN among what it sees, gives NaN to that row's query alone (the others keep their bits);
  * blocks that a row does not see have no part in its result, whatever their scales.
  * max_rows: no sequence has more rows (what y then holds for rows past it is undefined); max_len: the longest sequence, as far as the host knows it (a longer one
  * is computed as well).  The cut into blocks goes by these, so a graph that is replayed for growing sequences takes their final values.
