@@ -127,10 +127,13 @@ def lib() -> Lib:
 
 
 def stream_ptr(stream=None) -> int:
+    """Handle of a torch stream, of the current device's current one by default."""
     import torch
 
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # torch.cuda.current_stream().cuda_stream without the object in between: 0.4 us for 2.8, of the 8 that a small call took
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def ptr(t) -> int | None:
