@@ -102,26 +102,34 @@ struct Cols {
   int below[MT];           // by how much it rose for blocks that a column does not see: all that it sees lie before them
 };
 
-// Columns c0 .. of the np pairs (row, query) of sequence s and cached head h.
+// A lane's share of the queries of columns c0 .. of the np pairs (row, query) of sequence s and cached head h; begin makes columns of them.
 template <int DC, int MT>
-DEV void begin(Cols<DC, MT>& w, const Attn& a, const Seq& s, int h, int c0, int np) {
+DEV void load_q(const Attn& a, const Seq& s, int h, int c0, int np, uint4 (&q)[MT][DC][2]) {
   const int l = lane_id(), j = l >> 4, d = a.c.d, g = a.g;
-  const long long cap = (long long)a.c.maxp * KB - 1;
-  w.unit = kUnit;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int p = c0 + 16 * t + (l & 15), row = p / g;
-    const bool on = p < np;
     const uint16_t* src = a.q + (size_t)(s.r0 + row) * a.ldq + (size_t)(h * g + p - row * g) * d;
-    uint4 r[DC][2];
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int e = 64 * c + 16 * j + 8 * x;
-        r[c][x] = make_uint4(0, 0, 0, 0);
-        if (on && e < d) r[c][x] = ld16(src + e);
+        q[t][c][x] = make_uint4(0, 0, 0, 0);
+        if (p < np && e < d) q[t][c][x] = ld16(src + e);
       }
+  }
+}
+template <int DC, int MT>
+DEV void begin(Cols<DC, MT>& w, const Attn& a, const Seq& s, int c0, int np, const uint4 (&q)[MT][DC][2]) {
+  const int l = lane_id();
+  const long long cap = (long long)a.c.maxp * KB - 1;
+  w.unit = kUnit;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int p = c0 + 16 * t + (l & 15), row = p / a.g;
+    const bool on = p < np;
+    const uint4(&r)[DC][2] = q[t];
     float top = 0.f;
     bool num = true;
 #pragma unroll
@@ -166,18 +174,21 @@ struct Pages {
   int page, ve;          // v's scale is a fraction in [1/2, 1) times 2^ve,
   float ks, lv, rv;      // the fraction's log2 and reciprocal
   unsigned long long have, num;  // blocks in the cache; those whose scales are numbers
-  DEV void fetch(const Attn& a, int seq, int h, int block, bool on) { fetch(a, h, on ? page_of(a.c, seq, block) : -1, on); }
-  DEV void fetch(const Attn& a, int h, int p, bool on) {
+  // ask() asks for the scales, behind which blocks can be asked for; take() waits for them
+  DEV void ask(const Attn& a, int seq, int h, int block, bool on) { ask(a, h, on ? page_of(a.c, seq, block) : -1, on); }
+  DEV void ask(const Attn& a, int h, int p, bool on) {
     have = __ballot(p >= 0);
     page = p >= 0 ? p : 0;
-    ks = 0.f;
-    float vs = 0.f;
-    if (on) ks = a.c.ks[(size_t)page * a.c.hkv + h], vs = a.c.vs[(size_t)page * a.c.hkv + h];
+    ks = lv = 0.f;
+    if (on) ks = a.c.ks[(size_t)page * a.c.hkv + h], lv = a.c.vs[(size_t)page * a.c.hkv + h];
+  }
+  DEV void take() {
+    const float vs = lv;
     const bool ok = vs >= 0.f && vs < kInf && ks >= 0.f && ks < kInf;
     num = __ballot(ok);
     if (!ok) ks = 0.f;
     // a scale of 0 weighs nothing, by an exponent far below any; nor does a block that is not there
-    const bool pos = ok && p >= 0 && vs > 0.f;
+    const bool pos = ok && (have >> lane_id() & 1) && vs > 0.f;
     ve = pos ? __builtin_amdgcn_frexp_expf(vs) : kUnit;
     const float fr = pos ? __builtin_amdgcn_frexp_mantf(vs) : 0.5f;
     lv = __builtin_amdgcn_logf(fr), rv = 1.f / fr;
@@ -321,16 +332,20 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 
   Pages pg;
   Cols<DC, MT> w;
-  // the first block's bytes are on their way while the queries arrive
-  if (b0 == sp * a.chunk) pg.fetch(a, h, l < cnt ? ahead : -1, l < cnt);
-  else pg.fetch(a, i, h, b0 + wv + W * l, l < cnt);
+  // loads come back in order: the queries are converted while the first block's bytes are on their way
+  uint4 qr[MT][DC][2];
+  load_q<DC, MT>(a, s, h, c0, np, qr);
+  if (b0 == sp * a.chunk) pg.ask(a, h, l < cnt ? ahead : -1, l < cnt);
+  else pg.ask(a, i, h, b0 + wv + W * l, l < cnt);
   if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
-  begin(w, a, s, h, c0, np);
+  begin(w, a, s, c0, np, qr);
+  pg.take();
   for (int k0 = 0; k0 < cnt; k0 += WAVE) {
     const int n = cnt - k0 < WAVE ? cnt - k0 : WAVE;
     if (k0) {
-      pg.fetch(a, i, h, b0 + wv + W * (k0 + l), l < n);
+      pg.ask(a, i, h, b0 + wv + W * (k0 + l), l < n);
       load_k(pg.at(0)), load_v(pg.at(0));
+      pg.take();
     }
     for (int k = 0; k < n; ++k) {
       const int b = b0 + wv + W * (k0 + k), nx = pg.at(k + 1 < n ? k + 1 : k);
@@ -601,9 +616,10 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   Pages pg, px;  // of 64 blocks, and of the 64 behind them
   uint4 qr[2 * DC];
   load_q32<DC>(a, s, h, w0, c1, qr);
-  pg.fetch(a, i, h, b0 + l, l < cnt);
+  pg.ask(a, i, h, b0 + l, l < cnt);
   if (cnt > 0) load_k(pg.at(0)), load_v(pg.at(0));
-  px.fetch(a, i, h, b0 + WAVE + l, WAVE + l < cnt);
+  px.ask(a, i, h, b0 + WAVE + l, WAVE + l < cnt);
+  pg.take();
   int base = 0;
   auto page = [&](int n) {
     const int p = pg.at((n - base) & (WAVE - 1)), x = px.at((n - base) & (WAVE - 1));  // no branch
@@ -690,7 +706,8 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
     lds_barrier();
     if (k - base == WAVE) {
       pg = px, base = k;
-      px.fetch(a, i, h, b0 + k + WAVE + l, k + WAVE + l < cnt);
+      pg.take();
+      px.ask(a, i, h, b0 + k + WAVE + l, k + WAVE + l < cnt);
     }
     if (k < mine_cnt) soften32(w, sc, pf, pg, k - base, (b0 + k) * KB, w_lo);
     if (NW == 8) lds_barrier();  // four waves are not out of step: what their products read was written before the barrier above
