@@ -832,7 +832,7 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g, blocks = ((long long)max_len + KB - 1) / KB, items = (long long)rows * hq;
   // Few columns: each block of threads 16 or 32 pairs of a cached head and sequence.
   p.mt = pairs <= 16 || d > 128 ? 1 : 2;
-  const long long cols = (pairs + 16 * p.mt - 1) / (16 * p.mt), few = cols * seqs * hkv;
+  const long long cols = (pairs + 16 * p.mt - 1) / (16 * p.mt), room = rows * g / (16 * p.mt) + seqs, few = (cols * seqs < room ? cols * seqs : room) * hkv;
   // Many: tiles of 128 or 256 pairs; where sequences have several, of all rows together.  Eight waves only where a tile fills them and the tiles
   // most of the card (16 heads of 128, 2 cached; behind 8192 tokens 2800 rows 254 us with eight, 283 with four, 2100 215 and 203).
   auto cut = [&](int nw) {
@@ -843,8 +843,8 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   if (d > 128 || pairs <= 128 || p.tiles * hkv < 176) cut(4);
   // us: rounds of the blocks that the card holds, each a start and its steps, `at` cached blocks a step; with splits a launch that joins, and the
   // parts out and back.  The constants are what single rounds took.  What the rule gives and the other side: 3 sequences of 1000 tokens with 72 pairs
-  // of d 256 14.7 us in few columns, 26 in split tiles, 58 in whole ones; 8 of 500 with 192 pairs of d 64 9.1, 15.6; 49 of 2000 with 122 pairs of
-  // d 128 25 in tiles, 30 in few columns; 30 of 40 tokens with 120 pairs of d 256 21 in tiles, 32 in few columns;
+  // of d 256 14.7 us in few columns, 26 in split tiles, 58 in whole ones; 8 of 500 with 192 pairs of d 64 9.1, 15.6; 7 of 33 to 373 with as many pairs
+  // of d 64 10.8, 13.2; 49 of 2000 with 122 pairs of d 128 25 in tiles, 30 in few columns; 12 of 420 to 3900 with 318 pairs of d 96 65, 94; 30 of 40 tokens with 120 pairs of d 256 21 in tiles, 32 in few columns;
   // 63 of 10 with 40 pairs of d 112 9.5 in tiles, 15.7 in few columns.
   struct Cut {
     long long s;
@@ -855,7 +855,9 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
     Cut c{1, 3e38f};
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
       if (s > 1 && s * at > blocks) break;
-      const float us = (float)((units * s + holds - 1) / holds) * (start + step * (float)((blocks + s * at - 1) / (s * at))) + (s > 1 ? 3.f + s * part : 0.f);
+      // up to d 128 a CU takes a second block beside the first, so that half rounds count
+      const float rounds = d > 128 ? (float)((units * s + holds - 1) / holds) : units * s > holds ? .5f * (float)((2 * units * s + holds - 1) / holds) : 1.f;
+      const float us = rounds * (start + step * (float)((blocks + s * at - 1) / (s * at))) + (s > 1 ? 3.f + s * part : 0.f);
       if (us < c.us) c = Cut{s, us};
     }
     return c;
