@@ -285,7 +285,7 @@ DEV void emit_none(const Attn& a, const Seq& s, int h, int sp, int c0, int c1, i
 // holds are several blocks (z), which find the cache in L2.
 // Memory bounds it where sequences are long: 48 ragged sequences of 115191 tokens in all, 8 cached heads of 128, 216 MB in 53 us (4.1 TB/s), 32 of 8000
 // in 104 with the join (5.07 TB/s of 5.12 that a copy reaches); one of 60001 tokens with 2 heads of 256 is two to three blocks a wave,
-// 61 MB in 18.  Short ones are a chain of loads (length and table, scales and bytes, LDS): 300 tokens 7.4 us, of which 3 to 4 are the launch.
+// 61 MB in 18.  7 prompts of 33 to 373 rows, 12 heads of 64: 10.8.  Short ones are a chain of loads (length and table, scales and bytes, LDS): 300 tokens 7.4 us, of which 3 to 4 are the launch.
 template <int DC, int MT>
 __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   constexpr int TP = 16 * MT, LD = 64 * DC + 4;
@@ -424,12 +424,12 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 // What bounds it is the vector unit, which a product keeps for 10 to 12 cycles whatever its size: hence 32 x 32 x 16 products, and a
 // softmax without a maximum where it can be: a column's reference is the maximum of an earlier block, and only where a lane's sum says that a
 // weight may have passed fp16 (or the column has no reference yet) is the block's maximum taken, O rescaled and the weights formed again.
-// 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 341 us, 1.01 PFLOP/s (a large library product in fp16: 1.33); the matrix
-// unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 538 us (1.0),
-// heads of 64 111 us (0.62: the softmax is as long for half the products), of 256 262 us for 2048 rows on 6144 (0.65: four waves a CU,
-// no other wave's products beside a softmax, and 90 of a lane's registers in memory, which are read where a turn or the epilogue starts).
-// Short prompts are steps of 1 to 1.2 us (2.8 with heads of 256) behind a start of 5 (15), most of it the fetch of code that runs once: 7 prompts
-// of 33 to 373 rows, 12 heads of 64, 13.3 us.
+// 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 330 to 341 us, 1.01 to 1.04 PFLOP/s (a large library product in fp16: 1.33); the matrix
+// unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 515 us (1.06),
+// heads of 64 108 us (0.64: the softmax is as long for half the products), of 256 256 us for 2048 rows on 6144 (0.67: four waves a CU,
+// no other wave's products beside a softmax, and 142 of a lane's registers in memory, which are read where a turn or the epilogue starts).
+// Short prompts are steps of 1 to 1.2 us (2.8 with heads of 256) behind a start of 5 (15), most of it the fetch of code that runs once: 1000 rows
+// of 32 heads of 128 28.7 us.
 template <int DC>
 struct Cols32 {
   half8 q[2 * DC];   // 32-element chunk i, half y: elements 32 i + 16 (l >> 5) + 8 y + (0 .. 7), times a power of two
@@ -842,10 +842,11 @@ Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d)
   cut(8);
   if (d > 128 || pairs <= 128 || p.tiles * hkv < 176) cut(4);
   // us: rounds of the blocks that the card holds, each a start and its steps, `at` cached blocks a step; with splits a launch that joins, and the
-  // parts out and back.  The constants are what single rounds took.  What the rule gives and the other side: 3 sequences of 1000 tokens with 72 pairs
-  // of d 256 14.7 us in few columns, 26 in split tiles, 58 in whole ones; 8 of 500 with 192 pairs of d 64 9.1, 15.6; 7 of 33 to 373 with as many pairs
-  // of d 64 10.8, 13.2; 49 of 2000 with 122 pairs of d 128 25 in tiles, 30 in few columns; 12 of 420 to 3900 with 318 pairs of d 96 65, 94; 30 of 40 tokens with 120 pairs of d 256 21 in tiles, 32 in few columns;
-  // 63 of 10 with 40 pairs of d 112 9.5 in tiles, 15.7 in few columns.
+  // parts out and back.  The constants are what single rounds took.  What the rule gives, and the other side:
+  //   in few columns  3 sequences of 1000 tokens with 72 pairs of d 256 14.7 us (split tiles 26, whole ones 58), 8 of 500 with 192 pairs of d 64
+  //                   9.1 (15.6), 7 of 33 to 373 with as many pairs of d 64 10.8 (13.2);
+  //   in tiles        49 of 2000 with 122 pairs of d 128 25 (30), 12 of 420 to 3900 with 318 pairs of d 96 65 (94), 30 of 40 with 120 pairs of d 256
+  //                   21 (32), 63 of 10 with 40 pairs of d 112 9.5 (15.7).
   struct Cut {
     long long s;
     float us;
