@@ -126,6 +126,17 @@ def test_every_cut(rows, lens, hq, hkv, d, gate):
     call.check(y)
 
 
+@pytest.mark.parametrize("rows,lens,hq,hkv,d,gate", CUTS)
+def test_output_in_the_queries_place(rows, lens, hq, hkv, d, gate):
+    import torch
+
+    call = Call(cache(51, lens, hkv, d), rows, lens, hq, gate=gate, seed=6)
+    y = call.run()
+    call.run(y=call.q)
+    torch.cuda.synchronize()
+    assert torch.equal(call.q, y)
+
+
 @pytest.mark.parametrize("rows,lens,hq,hkv,d", [([1], [900], 8, 2, 128), ([70], [300], 4, 2, 64), ([1, 3], [2000, 100], 4, 1, 256)])
 @pytest.mark.parametrize("max_len", [0, 1, 100000])
 def test_any_cut_is_right(rows, lens, hq, hkv, d, max_len):
