@@ -11,7 +11,7 @@
 //
 // Every element is loaded once and stored once, so memory bounds large calls: 8192 rows of 16 heads of 256 (64 turned, gates between the heads, fp32
 // in, bf16 out) 38.4 us, 5.24 TB/s.  Small ones are a launch and one chain of loads, sums and stores: one row of 20 heads of 128 3.5 us; 777 rows of
-// 15 heads of 80, 36 turned in pairs (a load an element), 5.4 us.
+// 15 heads of 80 in bf16, 36 turned in pairs, 3.9 us (5.4 with a load an element).
 #include "common.hpp"
 
 using namespace drm;
@@ -80,12 +80,13 @@ DEV float head_sum(float v, int L) {
 }
 
 // V elements a load (4, or 1 where sizes, strides or addresses allow no more).  A unit is a vector of the first half of the turned elements and
-// its counterpart in the second (the partners, or V / 2 pairs each), or two vectors of the elements behind rot likewise: lanes beside each other
-// load and store beside each other.  2^LS lanes a head, up to PER units a lane; RB rows a block; U heads a lane at a time.
+// its counterpart in the second (the partners), or two vectors of the elements behind rot likewise; in pairs a vector of the first half
+// of the head and one of the second, as each holds both partners: lanes beside each other load and store beside each other.  2^LS lanes a head, up to PER units a lane; RB rows a block; U heads a lane at a time.
 template <bool B16, int V, int PER, int U>
 __global__ void __launch_bounds__(NT) k_rope(Rope a, int LS, int RB) {
   extern __shared__ float2 cs[];  // [RB][rot / 2]
-  const int half = a.rot >> 1, turned = half / V, tail = (a.d - a.rot + 2 * V - 1) / (2 * V), units = turned + tail;
+  const bool whole = V > 1 && a.pairs;
+  const int half = a.rot >> 1, turned = whole ? 0 : half / V, tail = (a.d - (whole ? 0 : a.rot) + 2 * V - 1) / (2 * V), units = turned + tail;
   const long long r0 = (long long)blockIdx.x * RB;
   const int hb = (a.heads + gridDim.y - 1) / gridDim.y, h0 = blockIdx.y * hb, nh = a.heads - h0 < hb ? a.heads - h0 : hb;
   const int nr = a.rows - r0 < RB ? (int)(a.rows - r0) : RB, items = (nr * nh) << LS, l = threadIdx.x & ((1 << LS) - 1);
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(NT) k_rope(Rope a, int LS, int RB) {
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int k = l + (u << LS);
-    e0[u] = k < turned ? V * k : a.rot + V * (k - turned);
+    e0[u] = k < turned ? V * k : (whole ? 0 : a.rot) + V * (k - turned);
     e1[u] = k < turned ? e0[u] + half : e0[u] + V * tail;
     if (V == 1 && a.pairs && k < turned) e0[u] = 2 * k, e1[u] = 2 * k + 1;  // a unit is one pair
     if (k >= units) e0[u] = e1[u] = a.d;
@@ -153,23 +154,22 @@ __global__ void __launch_bounds__(NT) k_rope(Rope a, int LS, int RB) {
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         if (e0[u] >= a.d) continue;
-        if (e0[u] < a.rot) {
-          const float2* c = cs + rl[x] * half;
-          auto turn = [](float& m, float& n, const float2& t) {
-            const float y = m * t.x - n * t.y;
-            n = n * t.x + m * t.y, m = y;
-          };
-          if (!a.pairs) {
+        const float2* c = cs + rl[x] * half;
+        auto turn = [](float& m, float& n, const float2& t) {
+          const float y = m * t.x - n * t.y;
+          n = n * t.x + m * t.y, m = y;
+        };
+        if (whole) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) turn(p[x][u][0][v], p[x][u][1][v], c[e0[u] + v]);
-          } else if constexpr (V == 1) {
-            turn(p[x][u][0][0], p[x][u][1][0], c[e0[u] >> 1]);
-          } else {
+          for (int b = 0; b < 2; ++b) {
+            const int e = b ? e1[u] : e0[u];
+            if (e >= a.rot) continue;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-              for (int v = 0; v < V; v += 2) turn(p[x][u][b][v], p[x][u][b][(v + 1) % V], c[(b ? e1[u] : e0[u]) / 2 + v / 2]);
+            for (int v = 0; v < V; v += 2) turn(p[x][u][b][v], p[x][u][b][(v + 1) % V], c[(e + v) >> 1]);
           }
+        } else if (e0[u] < a.rot) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) turn(p[x][u][0][v], p[x][u][1][v], c[V == 1 && a.pairs ? e0[u] >> 1 : e0[u] + v]);
         }
         st_y<V>(a, (size_t)(r0 + rl[x]), h[x] * a.d + e0[u], p[x][u][0]);
         if (e1[u] < a.d) st_y<V>(a, (size_t)(r0 + rl[x]), h[x] * a.d + e1[u], p[x][u][1]);
@@ -187,9 +187,9 @@ int rope(const Rope& a, int ldx, int hsx, int ldn, int ldy, int ldb, hipStream_t
     return -1;
   if (a.rows == 0) return 0;
   auto al = [](const void* p, uintptr_t m) { return ((uintptr_t)p & (m - 1)) == 0; };
-  const bool vec = a.d % 4 == 0 && a.rot % 8 == 0 && al(a.x, B16 ? 8 : 16) && ldx % 4 == 0 && hsx % 4 == 0 && al(a.nw, 16) && ldn % 4 == 0 &&
+  const bool vec = a.d % 4 == 0 && a.rot % (a.pairs ? 4 : 8) == 0 && al(a.x, B16 ? 8 : 16) && ldx % 4 == 0 && hsx % 4 == 0 && al(a.nw, 16) && ldn % 4 == 0 &&
                    (!a.y || (al(a.y, 16) && ldy % 4 == 0)) && (!a.yb || (al(a.yb, 8) && ldb % 4 == 0));
-  const int V = vec ? 4 : 1, units = (a.rot >> 1) / V + (a.d - a.rot + 2 * V - 1) / (2 * V);
+  const int V = vec ? 4 : 1, units = vec && a.pairs ? (a.d + 7) / 8 : (a.rot >> 1) / V + (a.d - a.rot + 2 * V - 1) / (2 * V);
   int LS = 0;
   while ((1 << LS) < units && LS < 6) ++LS;
   const int per_row = a.heads << LS, RB = per_row >= NT ? 1 : NT / per_row;

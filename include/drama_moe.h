@@ -478,7 +478,7 @@ int dr_moe_layer_rows_fp8_bf16s(const dr_bf16* router, const uint8_t* gu_w, cons
  * pos i32 [rows]; freq f32 [rot / 2], radians per position, scaled for long contexts as the model asks (rope_freq of
  * drama-rs_amd/kvcache.py); both may be NULL where rot is 0.  y f32 and yb bf16: either may be NULL; head h of row r at r * ldy (ldb) + h * d.
  * y may be an f32 x, and yb a bf16 x, at the same strides with hsx = d.  Angles are formed in 64 bits, all else in fp32.  16-byte addresses
- * and strides of whole 16 bytes (8 for bf16) with d a multiple of 4 and rot of 8 take the wide path; any others work.
+ * and strides of whole 16 bytes (8 for bf16) with d a multiple of 4 and rot of 8 (in pairs of 4) take the wide path; any others work.
  * Unsupported: rows < 0 or > 8388608, heads < 1 or > 4096, d < 1 or > 512, rot odd, < 0 or > d, an unknown layout, a missing x, neither y nor
  * yb, rot without pos or freq, hsx < d, rows that overlap (ldx < (heads - 1) hsx + d; ldy, ldb < heads d), ldn between 1 and d - 1 or
  * negative -> -1.  rows == 0 does nothing. */

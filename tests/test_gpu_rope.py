@@ -41,6 +41,8 @@ CASES = [
     # few rows whose heads several blocks share, evenly and not
     (1, 40, 256, 256, False, True, 0, 0, 0), (3, 37, 128, 64, True, True, 4, 8, 0), (5, 39, 219, 108, True, True, 1, 3, 1), (2, 130, 33, 32, False, False, 0, 0, 0),
     (300, 30, 223, 160, False, True, 0, 0, 0),
+    # pairs whose turned elements end inside a wide load's half
+    (9, 5, 20, 4, True, True, 0, 0, 0), (4, 3, 76, 76, True, True, 4, 0, 4), (2, 2, 508, 500, True, False, 0, 4, 0), (3, 1, 4, 4, True, True, 0, 0, 0), (5, 2, 12, 0, True, True, 0, 0, 0),
 ]
 
 
