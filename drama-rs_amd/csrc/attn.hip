@@ -29,6 +29,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int W = 4, NT = W * WAVE;
 constexpr float kInf = __builtin_inff();
 constexpr int kUnit = -200;  // an exponent below that of any scale
+constexpr float kFar = 0x1p20f;  // log2 scores from here on: see is_far()
 
 struct Attn {
   Kv8 c;
@@ -197,6 +198,17 @@ struct Pages {
   DEV int at(int k) const { return __builtin_amdgcn_readlane(page, k); }
 };
 
+// The common weight, 2^fma(score, f, base) with base = lw - m (m: the maximum, lw: a weight at it), keeps the exact product beside a rounded m and
+// rounds lw - m once more: 2 2^-24 |m| in all, an eighth up to kFar, but octaves from 2^24 on, which lift weights past fp16 or sink the
+// largest to zero.  From kFar on a column's scores become their distances to m first, the product rounded as m was (0 at the maximum).  What that
+// costs the calls that never get there: nothing with few columns, 1 to 2% in tiles, 5% with heads of 256 (six more registers in memory).
+DEV bool is_far(float m) { return fabsf(m) >= kFar && m > -kInf; }
+DEV float distance(float sc, float f, float m) {
+#pragma clang fp contract(off)
+  const float z = sc * f;
+  return z - m;
+}
+
 // One step of the softmax: the scores sc of block k of pg, its first place at position b0, become fp16 weights.
 // lo: every column sees the places up to lo.
 template <int DC, int MT>
@@ -216,7 +228,7 @@ DEV void soften(Cols<DC, MT>& w, f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], const P
   // v's scale enters relative to 2^unit.  f > 0, so that what is hidden (-infinity) stays it with a k scale of 0
   const float ks = Pages::lane(pg.ks, k);
   const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
-  const float lw = 15.f + Pages::lane(pg.lv, k) + (float)dv, iw = __builtin_ldexpf(Pages::lane(pg.rv, k), -dv);
+  const float lw = 15.f + Pages::lane(pg.lv, k) + (float)dv;
   float f[MT], mnew[MT];
   bool up = unew > w.unit;
 #pragma unroll
@@ -249,9 +261,25 @@ DEV void soften(Cols<DC, MT>& w, f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], const P
     for (int x = 0; x < MT; ++x)
       if (there && w.pos[x] >= b0) w.sum[x] = __builtin_nanf("");
   }
+  bool any_far = false;
+#pragma unroll
+  for (int x = 0; x < MT; ++x) any_far = any_far || is_far(w.m[x]);
+  if (__any(any_far)) {
+    // by columns, so that no other has a part in a column's bits
+#pragma unroll
+    for (int x = 0; x < MT; ++x) {
+      if (!is_far(w.m[x])) continue;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[x][t][e] = distance(sc[x][t][e], f[x], w.m[x]);
+      f[x] = 1.f;
+    }
+  }
+  const float iw = __builtin_ldexpf(Pages::lane(pg.rv, k), -dv);
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
-    const float base = lw - (w.m[x] == -kInf ? 0.f : w.m[x]);
+    const float base = lw - (fabsf(w.m[x]) >= kFar ? 0.f : w.m[x]);
     float add = 0.f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -506,8 +534,8 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
       for (int r = 0; r < 16; ++r) sc[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) > mine ? -kInf : sc[t][r];
   }
   const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
-  const float f = fmaxf(w.qm * Pages::lane(pg.ks, k), 0x1p-126f), iw = __builtin_ldexpf(Pages::lane(pg.rv, k), -dv);  // as in soften()
-  float at = kBase + Pages::lane(pg.lv, k) + (float)dv - (w.m == -kInf ? 0.f : w.m);
+  float f = fmaxf(w.qm * Pages::lane(pg.ks, k), 0x1p-126f);  // as in soften()
+  const float lw = lane_f(kBase + Pages::lane(pg.lv, k) + (float)dv, 0);  // a scalar register
   if (unew > w.unit) {
     const int sh = lim >= 0 ? w.unit - unew : 0;
     if (lim < 0) w.below += unew - w.unit;
@@ -520,7 +548,7 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
     w.unit = unew;
   }
   if (!(pg.num >> k & 1) && lim >= 0) w.sum = __builtin_nanf("");  // scales that are no numbers
-  float add = 0.f;
+  float add = 0.f, at = lw - (fabsf(w.m) >= kFar ? 0.f : w.m);
   auto form = [&]() {
     add = 0.f;
 #pragma unroll
@@ -533,28 +561,35 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
       }
   };
   form();
-  if (__any(!(add <= kMost) || (w.m == -kInf && lim >= 0))) {
+  // without a reference yet, or with one far from zero, the block's maximum is taken in any case
+  if (__any(!(add <= kMost) || (lim >= 0 && fabsf(w.m) >= kFar))) {
     float mx = -kInf;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
     // a column's own lanes alone decide, so that what is in the other columns has no part in its bits (2% of a long chunk's time)
-    const float most = xmax_step<32>(add), high = xmax_step<32>(mx) * f, top = !(most <= kMost) || w.m == -kInf ? high : w.m;
+    const float most = xmax_step<32>(add), high = xmax_step<32>(mx) * f, top = !(most <= kMost) || fabsf(w.m) >= kFar ? high : w.m;
     if (top > w.m) {
       // less than the reference stays as it is; without one (m -infinity) there are no sums to scale
       const float al = w.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(w.m - top);
-      at -= top - (w.m == -kInf ? 0.f : w.m);
-      w.m = top;
+      w.m = top, at = lw - top;
       w.sum *= al;
 #pragma unroll
       for (int u = 0; u < DC; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) w.o[u][r] *= al;
     }
+    if (is_far(w.m)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[t][r] = distance(sc[t][r], f, w.m);
+      f = 1.f, at = lw;
+    }
     form();
   }
-  w.sum += add * iw;
+  w.sum += add * __builtin_ldexpf(Pages::lane(pg.rv, k), -dv);
 }
 
 template <int DC, int NW, int OCC>
