@@ -28,6 +28,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int W = 4, NT = W * WAVE;
 constexpr float kInf = __builtin_inff();
+constexpr float kLow = -__FLT_MAX__;  // the maximum of scores that all lie below fp32's range (none seen: -infinity)
 constexpr int kUnit = -200;  // an exponent below that of any scale
 constexpr float kFar = 0x1p20f;  // log2 scores from here on: see is_far()
 
@@ -61,6 +62,8 @@ DEV float lane_f(float v, int l) { return __int_as_float(__builtin_amdgcn_readla
 
 // What becomes of a row's query `head`: elements e .. e + 3, o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor (no token seen:
 // both 0).  The finished output, or, not alone, a part of it to be joined; alone, an l of kAlone tells the launch that joins.
+// Scores past fp32's range count as infinities of their sign, whichever way a call is cut: one of +infinity leaves NaN sums by itself; all of
+// -infinity (m kLow) weigh nothing in a part, which stays a part that saw tokens, and are no number where they are all that there is.
 constexpr float kAlone = -1.f;
 struct Out {
   uint16_t* y;
@@ -69,6 +72,7 @@ struct Out {
   DEV Out(const Attn& a, bool alone, int split, size_t row, int head, float l, float m, bool first) : alone(alone), gated(a.gate != nullptr) {
     const size_t at = ((size_t)split * a.c.rows + row) * a.hq + head;
     y = a.y + row * a.ldy + (size_t)head * a.c.d, part = a.part + at * a.c.d;
+    if (m == kLow) l = alone ? __builtin_nanf("") : l == 0.f ? 1.f : l;
     inv = l == 0.f ? 0.f : 1.f / l;
     if (first && !alone) a.ml[2 * at] = m;
     if (first && (!alone || a.splits > 1)) a.ml[2 * at + 1] = alone ? kAlone : l;
@@ -203,6 +207,11 @@ struct Pages {
 // largest to zero.  From kFar on a column's scores become their distances to m first, the product rounded as m was (0 at the maximum).  What that
 // costs the calls that never get there: nothing with few columns, 1 to 2% in tiles, 5% with heads of 256 (six more registers in memory).
 DEV bool is_far(float m) { return fabsf(m) >= kFar && m > -kInf; }
+// A score's factor: above 0, so that what is hidden (-infinity) stays it with a k scale of 0, and below infinity, so that a product of nothing
+// stays 0.  The words of positive floats are in their order.
+DEV float factor_of(float f) { return __uint_as_float(min(__float_as_uint(fmaxf(f, 0x1p-126f)), 0x7f7fffffu)); }
+// The maximum of scores from that of their products (-infinity: none is seen).
+DEV float top_of(float mx, float f) { return mx > -kInf ? fmaxf(mx * f, kLow) : -kInf; }
 DEV float distance(float sc, float f, float m) {
 #pragma clang fp contract(off)
   const float z = sc * f;
@@ -225,7 +234,7 @@ DEV void soften(Cols<DC, MT>& w, f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], const P
         for (int e = 0; e < 4; ++e) sc[x][t][e] = 16 * t + e > lim ? -kInf : sc[x][t][e];
     }
   }
-  // v's scale enters relative to 2^unit.  f > 0, so that what is hidden (-infinity) stays it with a k scale of 0
+  // v's scale enters relative to 2^unit
   const float ks = Pages::lane(pg.ks, k);
   const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
   const float lw = 15.f + Pages::lane(pg.lv, k) + (float)dv;
@@ -233,13 +242,13 @@ DEV void soften(Cols<DC, MT>& w, f32x4 (&sc)[MT][4], half8 (&pf)[MT][2], const P
   bool up = unew > w.unit;
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
-    f[x] = fmaxf(w.qm[x] * ks, 0x1p-126f);
+    f[x] = factor_of(w.qm[x] * ks);
     float mx = -kInf;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[x][t][e]);
-    mnew[x] = fmaxf(w.m[x], quad_max(mx) * f[x]);
+    mnew[x] = fmaxf(w.m[x], top_of(quad_max(mx), f[x]));
     up = up || mnew[x] > w.m[x];
   }
   if (__any(up)) {
@@ -534,7 +543,7 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
       for (int r = 0; r < 16; ++r) sc[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) > mine ? -kInf : sc[t][r];
   }
   const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
-  float f = fmaxf(w.qm * Pages::lane(pg.ks, k), 0x1p-126f);  // as in soften()
+  float f = factor_of(w.qm * Pages::lane(pg.ks, k));  // as in soften()
   const float lw = lane_f(kBase + Pages::lane(pg.lv, k) + (float)dv, 0);  // a scalar register
   if (unew > w.unit) {
     const int sh = lim >= 0 ? w.unit - unew : 0;
@@ -569,7 +578,7 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
     // a column's own lanes alone decide, so that what is in the other columns has no part in its bits (2% of a long chunk's time)
-    const float most = xmax_step<32>(add), high = xmax_step<32>(mx) * f, top = !(most <= kMost) || fabsf(w.m) >= kFar ? high : w.m;
+    const float most = xmax_step<32>(add), high = top_of(xmax_step<32>(mx), f), top = !(most <= kMost) || fabsf(w.m) >= kFar ? high : w.m;
     if (top > w.m) {
       // less than the reference stays as it is; without one (m -infinity) there are no sums to scale
       const float al = w.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(w.m - top);
@@ -852,8 +861,9 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
         const float c = __builtin_amdgcn_exp2f(sm[gi - grp + k] - ms);
         v += c * so[t + (k - grp) * LE], s += c * sl[gi - grp + k];
       }
+    m = mn;
   }
-  if (on && grp == 0 && !whole) Out(a, true, 0, row, head, s, 0.f, false).put(e, v, gate);
+  if (on && grp == 0 && !whole) Out(a, true, 0, row, head, s, m, false).put(e, v, gate);
 }
 
 // How a call is cut: by its sizes alone, so that the workspace is known before.

@@ -522,7 +522,8 @@ int dr_kv8_read(const int* start, const int* len, const int* table, int maxp, co
  * q bf16 and y bf16: query h of row r at r * ldq (ldy) + h * d; gate f32, NULL for none: at r * ldg + h * hsg.  y may be q at the same stride.  A row that
  * sees no token (a negative position, blocks that are not there) gets zeros; rows of no sequence are left as they were.  A query
  * with an infinity or NaN, or a block with a scale that is negative, infinite or NaN among what it sees, gives NaN to that row's query alone (the others keep their bits);
- * blocks that a row does not see have no part in its result, whatever their scales.
+ * blocks that a row does not see have no part in its result, whatever their scales.  A score whose magnitude passes fp32 (2.3e38) counts as an
+ * infinity of its sign: NaN for the row's query where one is positive or all that it sees are negative.
  * max_rows: no sequence has more rows (what y then holds for rows past it is undefined); max_len: the longest sequence, as far as the host knows it (a longer one
  * is computed as well).  The cut into blocks goes by these, so a graph that is replayed for growing sequences takes their final values.
  * Scores, softmax and sums are fp32; weights, times their block's v scale, enter the product with v in fp16: 2^-11 of each, and at most 2^-29

@@ -84,3 +84,67 @@ def test_far_columns_leave_the_others_alone(rows, lens, hq, hkv, d):
     torch.cuda.synchronize()
     z[at] = y[at]
     assert torch.equal(z, y)
+
+
+def overflow(rows, lens, hq, hkv, d, blocks, sign):
+    """A call in which every score of `blocks` of sequence 0 passes fp32 with the given sign, (row, query) alike, and others are of the common size."""
+    c = cache(71, lens, hkv, d)
+    call = Call(c, rows, lens, hq, scale=0.1)
+    call.q[:, :hq * d] = call.q[:, :hq * d].abs() + 1
+    import torch
+
+    for b in blocks:
+        p = int(c.table[0, b])
+        call.dc.ks[p] = 1e38
+        # all of a block's k of one sign, 3 or more (stored with 128 added)
+        k = call.dc.kq[p].to(torch.int32) - 128
+        call.dc.kq[p] = (sign * k.abs().clamp(min=3) + 128).to(torch.uint8)
+    return c, call
+
+
+@pytest.mark.parametrize("rows,lens,hq,hkv,d", SHAPES)
+def test_scores_past_fp32(rows, lens, hq, hkv, d):
+    """A block of scores that are +infinity in fp32: NaN for the rows that see it.  Of -infinity: as if the block was not there.  Nothing but such scores: NaN.
+    The others keep their bits."""
+    import torch
+
+    n = hq * d
+    blocks = sorted({0, (lens[0] - 1) // 128, (lens[0] - 1) // 64})
+    plain = overflow(rows, lens, hq, hkv, d, [], 1)[1].run()
+    for b in blocks:
+        c, call = overflow(rows, lens, hq, hkv, d, [b], 1)
+        y = call.run()
+        torch.cuda.synchronize()
+        seen = min(max(b * 64 - (lens[0] - rows[0]), 0), rows[0])
+        assert torch.isnan(y[seen:rows[0], :n]).all() and torch.equal(y[:seen], plain[:seen]) and torch.equal(y[rows[0]:], plain[rows[0]:])
+        c, call = overflow(rows, lens, hq, hkv, d, [b], -1)
+        y = call.run()
+        torch.cuda.synchronize()
+        assert torch.equal(y[:seen], plain[:seen]) and torch.equal(y[rows[0]:], plain[rows[0]:])
+        alone = max(0, min(rows[0], 64 - (lens[0] - rows[0]))) if b == 0 else 0  # rows that see that block only
+        assert torch.isnan(y[:alone, :n]).all()
+        page, c.table[0, b] = int(c.table[0, b]), -1
+        want, bound = call.reference()
+        c.table[0, b] = page
+        got = y[:, :n].double().cpu().numpy().reshape(want.shape)
+        own = slice(alone, call.start[-1])
+        assert (np.abs(got[own] - want[own]) <= bound[own]).all()
+    c, call = overflow(rows, lens, hq, hkv, d, range((lens[0] + 63) // 64), -1)
+    y = call.run()
+    torch.cuda.synchronize()
+    assert torch.isnan(y[:rows[0], :n]).all() and torch.equal(y[rows[0]:], plain[rows[0]:])
+
+
+@pytest.mark.parametrize("rows,lens,hq,hkv,d", SHAPES)
+def test_products_of_nothing(rows, lens, hq, hkv, d):
+    """Queries of zeros on k scales next to fp32's largest, and a scale for the scores that is: all weights alike."""
+    import torch
+
+    c = cache(73, lens, hkv, d)
+    c.ks[::2] = 3.4e38
+    for scale in (3.4e38, 1.0):
+        call = Call(c, rows, lens, hq, scale=scale)
+        call.q[:, :hq * d] = 0
+        y = call.run()
+        torch.cuda.synchronize()
+        call.check(y)
