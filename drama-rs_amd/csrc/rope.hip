@@ -182,10 +182,9 @@ template <bool B16>
 int rope(const Rope& a, int ldx, int hsx, int ldn, int ldy, int ldb, hipStream_t st) {
   const long long n = (long long)a.heads * a.d;
   if (a.rows < 0 || a.rows > 1 << 23 || a.heads < 1 || a.heads > 4096 || a.d < 1 || a.d > 512 || a.rot < 0 || a.rot > a.d || a.rot % 2 || a.pairs < 0 || a.pairs > 1) return -1;
-  if (hsx < a.d || ldx < (long long)(a.heads - 1) * hsx + a.d || (a.nw && ldn != 0 && ldn < a.d) || (!a.y && !a.yb) || (a.y && ldy < n) ||
-      (a.yb && ldb < n) || (a.rot && (!a.pos || !a.freq)) || !a.x)
-    return -1;
-  if (a.rows == 0) return 0;
+  if (hsx < a.d || ldx < (long long)(a.heads - 1) * hsx + a.d || (a.nw && ldn != 0 && ldn < a.d) || (a.y && ldy < n) || (a.yb && ldb < n)) return -1;
+  if (a.rows == 0) return 0;  // before the buffers: an empty one may have no address
+  if ((!a.y && !a.yb) || (a.rot && (!a.pos || !a.freq)) || !a.x) return -1;
   auto al = [](const void* p, uintptr_t m) { return ((uintptr_t)p & (m - 1)) == 0; };
   const bool vec = a.d % 4 == 0 && a.rot % (a.pairs ? 4 : 8) == 0 && al(a.x, B16 ? 8 : 16) && ldx % 4 == 0 && hsx % 4 == 0 && al(a.nw, 16) && ldn % 4 == 0 &&
                    (!a.y || (al(a.y, 16) && ldy % 4 == 0)) && (!a.yb || (al(a.yb, 8) && ldb % 4 == 0));
