@@ -40,8 +40,11 @@ struct Attn {
   float *part, *ml;  // [splits, rows, hq, d] and [splits, rows, hq, 2]
   size_t ldq, ldg, hsg, ldy;
   float scale;
-  int hq, g, splits, chunk, scan, fold;
+  int hq, g, splits, chunk, scan, fold, most;  // most: rows of a sequence that the cut has room for
 };
+
+// The rows of a sequence that the call computes.  More than the host said are left out here: their tiles and columns would be others'.
+DEV int rows_of(const Attn& a, const Seq& s) { return s.n < a.most ? s.n : a.most; }
 
 DEV half8 to_half8(uint32_t a, uint32_t b) {
   const half2v off = {(_Float16)1152.f, (_Float16)1152.f};
@@ -335,9 +338,9 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   // the table's entries as the host's word for the lengths has it, beside the sequence's length itself
   const int ahead = page_of(a.c, i, (int)((long long)sp * a.chunk + wv + W * l < a.c.maxp ? sp * a.chunk + wv + W * l : -1));
   const Seq s = seq_of(a.c, i);
-  const int c0 = blockIdx.z * TP;
-  if (s.n * g <= c0) return;
-  const int np = s.n * g - c0 < TP ? s.n * g : c0 + TP;
+  const int c0 = blockIdx.z * TP, all = rows_of(a, s) * g;
+  if (all <= c0) return;
+  const int np = all - c0 < TP ? all : c0 + TP;
   const long long cap = (long long)a.c.maxp * KB - 1;
   const int p_lo = s.first + c0 / g, p_end = s.first + (np - 1) / g, p_hi = p_end < cap ? p_end : (int)cap;
   const int nb = p_hi < 0 ? 0 : (p_hi >> 6) + 1;
@@ -611,9 +614,11 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   const int h = blockIdx.x % a.c.hkv, sp = blockIdx.y, d = a.c.d, d16 = d >> 4, g = a.g;
   int at = (gridDim.x - 1 - blockIdx.x) / a.c.hkv, i = at;
   Seq s;
-  if (a.scan) i = find_item(a.c, at, s, [g](const Seq& q) { return (q.n * g + TP - 1) / TP; });
+  const int most = a.most;
+  if (a.scan) i = find_item(a.c, at, s, [g, most](const Seq& q) { return ((q.n < most ? q.n : most) * g + TP - 1) / TP; });
   else at = 0, s = seq_of(a.c, i);
   if (i < 0) return;
+  s.n = rows_of(a, s);
   const int np = a.scan || s.n * g < TP ? s.n * g : TP;
   // folded: the first four waves have a half tile, the others (none in the middle one) its mirror image in the sequence, which ends later
   const bool fold = NW == 8 && a.fold;
@@ -974,7 +979,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
   float* part = reinterpret_cast<float*>(ws);
   const Attn a{c, q, gate, y, part, part + (size_t)p.splits * rows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
-               (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan, p.fold};
+               (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan, p.fold, max_rows};
   if (too_many(p, hkv)) return -1;
   const dim3 grid((unsigned)(p.tiles * hkv), p.splits, p.cols);
   auto few = [&](auto dc, auto mt) {
