@@ -9,7 +9,9 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("rows,lens,hq,hkv,d,most", [([20, 3, 9, 1], [300, 90, 9, 70], 4, 2, 64, 5), ([20, 3, 9], [3000, 900, 700], 8, 2, 128, 4), ([700, 40, 701, 130], [900, 40, 701, 200], 8, 1, 128, 150),
-                                                     ([300, 40, 130], [300, 700, 200], 8, 2, 256, 100), ([700, 300, 701, 9], [1000, 300, 701, 60], 64, 1, 128, 500), ([100, 60, 130], [100, 60, 200], 2, 1, 64, 64)])
+                                                     ([300, 40, 130], [300, 700, 200], 8, 2, 256, 100), ([100, 60, 130], [100, 60, 200], 2, 1, 64, 64),
+                                                     # tiles that the first sequence's surplus would take from the others; a sequence folded at an end that is not the host's
+                                                     ([600, 40], [700, 60], 32, 1, 64, 70), ([1700], [1700], 32, 1, 32, 1500)])
 def test_more_rows_than_the_host_says(rows, lens, hq, hkv, d, most):
     """The rows past the limit are undefined; those before it, and the other sequences', are right."""
     import torch
