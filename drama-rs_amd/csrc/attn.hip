@@ -37,14 +37,18 @@ struct Attn {
   const uint16_t* q;
   const float* gate;
   uint16_t* y;
-  float *part, *ml;  // [splits, rows, hq, d] and [splits, rows, hq, 2]
+  float *part, *ml;  // [splits, prows, hq, d] and [splits, prows, hq, 2]: see part_rows()
   size_t ldq, ldg, hsg, ldy;
   float scale;
-  int hq, g, splits, chunk, scan, fold, most;  // most: rows of a sequence that the cut has room for
+  int hq, g, splits, chunk, scan, fold, most, prows, by_seq;  // most: rows of a sequence that the cut has room for
 };
 
 // The rows of a sequence that the call computes.  More than the host said are left out here: their tiles and columns would be others'.
 DEV int rows_of(const Attn& a, const Seq& s) { return s.n < a.most ? s.n : a.most; }
+
+// The part of sequence i's first row: parts are a row each, or, where rows of no sequence outnumber what the sequences can have, `most` a
+// sequence, so that neither the workspace nor the launch that joins is sized by the rows of none.
+DEV size_t part_of(const Attn& a, const Seq& s, int i) { return a.by_seq ? (size_t)i * a.most : (size_t)s.r0; }
 
 DEV half8 to_half8(uint32_t a, uint32_t b) {
   const half2v off = {(_Float16)1152.f, (_Float16)1152.f};
@@ -72,8 +76,8 @@ struct Out {
   uint16_t* y;
   float *part, inv;
   bool alone, gated;
-  DEV Out(const Attn& a, bool alone, int split, size_t row, int head, float l, float m, bool first) : alone(alone), gated(a.gate != nullptr) {
-    const size_t at = ((size_t)split * a.c.rows + row) * a.hq + head;
+  DEV Out(const Attn& a, bool alone, int split, size_t row, size_t prow, int head, float l, float m, bool first) : alone(alone), gated(a.gate != nullptr) {
+    const size_t at = ((size_t)split * a.prows + prow) * a.hq + head;
     y = a.y + row * a.ldy + (size_t)head * a.c.d, part = a.part + at * a.c.d;
     if (m == kLow) l = alone ? __builtin_nanf("") : l == 0.f ? 1.f : l;
     inv = l == 0.f ? 0.f : 1.f / l;
@@ -313,9 +317,9 @@ DEV bool share(const Attn& a, int nb, int sp, int& b0, int& b1) {
 }
 
 // A split without blocks leaves word of that for its columns [c0, c1).
-DEV void emit_none(const Attn& a, const Seq& s, int h, int sp, int c0, int c1, int t, int nt) {
+DEV void emit_none(const Attn& a, size_t part, int h, int sp, int c0, int c1, int t, int nt) {
   for (int p = c0 + t; p < c1; p += nt) {
-    const size_t r = ((size_t)sp * a.c.rows + s.r0 + p / a.g) * a.hq + h * a.g + p % a.g;
+    const size_t r = ((size_t)sp * a.prows + part + p / a.g) * a.hq + h * a.g + p % a.g;
     a.ml[2 * r] = -kInf, a.ml[2 * r + 1] = 0.f;
   }
 }
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   int b0, b1;
   const bool alone = share(a, nb, sp, b0, b1);
   if (b0 == b1 && sp > 0) {
-    if (!alone) emit_none(a, s, h, sp, c0, np, threadIdx.x, NT);
+    if (!alone) emit_none(a, part_of(a, s, i), h, sp, c0, np, threadIdx.x, NT);
     return;
   }
   const int cnt = (b1 - b0 - wv + W - 1) / W;  // the wave's blocks b0 + wv, b0 + wv + W ..
@@ -441,7 +445,7 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
       ll += wt[v] * sml[v * 32 + 2 * col + 1];
     }
     if (p < np) {
-      const Out out(a, alone, sp, (size_t)s.r0 + row, h * g + p - row * g, ll, mm, e0 == 0);
+      const Out out(a, alone, sp, (size_t)s.r0 + row, part_of(a, s, i) + row, h * g + p - row * g, ll, mm, e0 == 0);
 #pragma unroll
       for (int c = 0; c < DC; ++c) {
         const int e = e0 + 64 * c;
@@ -630,7 +634,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   int b0, b1;
   const bool alone = share(a, p_hi < 0 ? 0 : (p_hi >> 6) + 1, sp, b0, b1);
   if (b0 == b1 && sp > 0) {
-    if (!alone) emit_none(a, s, h, sp, c0, c1, threadIdx.x, 64 * NW);  // not folded: that is without splits
+    if (!alone) emit_none(a, part_of(a, s, i), h, sp, c0, c1, threadIdx.x, 64 * NW);  // not folded: that is without splits
     return;
   }
   const int cnt = b1 - b0;
@@ -780,7 +784,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   const int p = w0 + (z & 31), row = p / g, head = h * g + p - row * g;
   if (p >= c1) return;
   const size_t rw = (size_t)s.r0 + row;
-  const Out out(a, alone, sp, rw, head, sum, w.m, z < 32);
+  const Out out(a, alone, sp, rw, part_of(a, s, i) + row, head, sum, w.m, z < 32);
   const float fin = __builtin_ldexpf(out.inv, w.unit - w.below - 16);
   // A block runs through this once, and what it costs is the fetch of its code: few branches (d ends on a multiple of 16), gates of as many
   // elements at a time as registers allow.
@@ -818,10 +822,19 @@ constexpr int kJoin = 8;      // parts of a group in flight
 __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
   __shared__ __align__(16) f32x4 so[NT];
   __shared__ float sm[NT / 16], sl[NT / 16];
-  const int t = threadIdx.x, gi = t / LE, grp = gi & (G - 1), d = a.c.d, n = a.c.rows * a.hq;
-  const int item = blockIdx.x * (NT / (LE * G)) + gi / G, at = item < n ? item : n - 1, row = at / a.hq, head = at - row * a.hq;
+  const int t = threadIdx.x, gi = t / LE, grp = gi & (G - 1), d = a.c.d, n = a.prows * a.hq;
+  const int item = blockIdx.x * (NT / (LE * G)) + gi / G, at = item < n ? item : n - 1, pr = at / a.hq, head = at - pr * a.hq;
   const int e = 4 * (LE * blockIdx.y + (t & (LE - 1)));
-  const bool on = item < n && e < d && row >= a.c.start[0] && row < a.c.start[a.c.seqs];
+  int row = pr;
+  bool own;
+  if (a.by_seq) {
+    const int i = pr / a.most;
+    const Seq s = seq_of(a.c, i);
+    row = s.r0 + (pr - i * a.most), own = pr - i * a.most < s.n;
+  } else {
+    own = row >= a.c.start[0] && row < a.c.start[a.c.seqs];
+  }
+  const bool on = item < n && e < d && own;
   const size_t step = n;
   const float4 gate = gate_of(a, on && grp == 0, row, head, e);
   float m = -kInf, s = 0.f;
@@ -868,8 +881,11 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
       }
     m = mn;
   }
-  if (on && grp == 0 && !whole) Out(a, true, 0, row, head, s, m, false).put(e, v, gate);
+  if (on && grp == 0 && !whole) Out(a, true, 0, row, 0, head, s, m, false).put(e, v, gate);
 }
+
+// Rows of a part (part_of()).
+int part_rows(int rows, int seqs, int max_rows) { return (long long)seqs * max_rows < rows ? seqs * max_rows : rows; }
 
 // How a call is cut: by its sizes alone, so that the workspace is known before.
 struct Plan {
@@ -879,7 +895,7 @@ struct Plan {
 };
 Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d) {
   Plan p;
-  const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g, blocks = ((long long)max_len + KB - 1) / KB, items = (long long)rows * hq;
+  const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g, blocks = ((long long)max_len + KB - 1) / KB, items = (long long)part_rows(rows, seqs, max_rows) * hq;
   // Few columns: each block of threads 16 or 32 pairs of a cached head and sequence.
   p.mt = pairs <= 16 || d > 128 ? 1 : 2;
   const long long cols = (pairs + 16 * p.mt - 1) / (16 * p.mt), room = rows * g / (16 * p.mt) + seqs, few = (cols * seqs < room ? cols * seqs : room) * hkv;
@@ -963,7 +979,7 @@ API size_t dr_attn_kv8_ws(int rows, int seqs, int max_rows, int max_len, int hq,
   if (rows == 0 || seqs == 0 || max_rows == 0) return 256;
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
   if (too_many(p, hkv)) return 0;
-  return p.splits > 1 ? ((size_t)p.splits * rows * hq * (d + 2) * sizeof(float) + 255) & ~(size_t)255 : 256;
+  return p.splits > 1 ? ((size_t)p.splits * part_rows(rows, seqs, max_rows) * hq * (d + 2) * sizeof(float) + 255) & ~(size_t)255 : 256;
 }
 
 API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len, const int* table, int maxp, const uint8_t* kq, const float* ks,
@@ -977,9 +993,10 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   if (rows == 0 || seqs == 0 || max_rows == 0) return 0;
   if (!kv8_buffers_ok(c) || !q || !y || !ws || ((uintptr_t)q & 15) || ((uintptr_t)y & 7) || ((uintptr_t)ws & 15)) return -1;
   const Plan p = plan(rows, seqs, max_rows, max_len, hq, hkv, d);
+  const int prows = part_rows(rows, seqs, max_rows);
   float* part = reinterpret_cast<float*>(ws);
-  const Attn a{c, q, gate, y, part, part + (size_t)p.splits * rows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
-               (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan, p.fold, max_rows};
+  const Attn a{c, q, gate, y, part, part + (size_t)p.splits * prows * hq * d, (size_t)ldq, (size_t)(gate ? ldg : 0), (size_t)(gate ? hsg : 0),
+               (size_t)ldy, scale, hq, hq / hkv, p.splits, p.chunk, p.scan, p.fold, max_rows, prows, prows < rows};
   if (too_many(p, hkv)) return -1;
   const dim3 grid((unsigned)(p.tiles * hkv), p.splits, p.cols);
   auto few = [&](auto dc, auto mt) {
@@ -1011,7 +1028,7 @@ API int dr_attn_kv8(const uint16_t* q, int ldq, const int* start, const int* len
   }
   if (p.splits > 1) {
     int le = 16, grps = 1;
-    const long long items = (long long)rows * hq;
+    const long long items = (long long)prows * hq;
     if (items >= 512)
       while (4 * le < d) le <<= 1;
     while (grps * kJoin < p.splits && 2 * grps * le <= NT) grps <<= 1;
