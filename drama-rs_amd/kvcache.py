@@ -61,6 +61,7 @@ class Batch:
         self.pos = torch.tensor([m - n + r for n, m in zip(rows, lens) for r in range(n)], dtype=torch.int32, device=device)
         self.start = torch.tensor(start, dtype=torch.int32, device=device)
         self.len = torch.tensor(list(lens), dtype=torch.int32, device=device)
+        self.seqs, self.device = len(start) - 1, self.start.device
 
 
 class KvCache:
@@ -133,6 +134,11 @@ class KvCache:
         if t.device != self.device or t.dtype not in dtypes or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != width or t.stride(1) != 1:
             raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device}, expected [{rows}, {width}] of {dtypes} on {self.device}")
 
+    def _check_batch(self, batch):
+        # the kernels read start and len of every sequence of the cache
+        if batch.seqs != self.seqs or batch.device != self.device:
+            raise ValueError(f"a batch of {batch.seqs} sequences on {batch.device}, expected {self.seqs} on {self.device}")
+
     def _cache(self, layer):
         P = dramamoe.ptr
         return (P(self.table), self.maxp, P(self.kq[layer]), P(self.ks[layer]), P(self.vq[layer]), P(self.vs[layer]), self.pages)
@@ -147,6 +153,7 @@ class KvCache:
         import torch
 
         n = self.hkv * self.d
+        self._check_batch(batch)
         for t, what in ((k, "k"), (v, "v")):
             self._check(t, batch.total, n, (torch.float32, torch.bfloat16), what)
         if k.dtype != v.dtype:
@@ -161,6 +168,7 @@ class KvCache:
         import torch
 
         n, P = self.hkv * self.d, dramamoe.ptr
+        self._check_batch(batch)
         with self._on_device():
             k, v = (torch.empty(batch.total, n, device=self.device) for _ in range(2))
             self.lib.dr_kv8_read(P(batch.start), P(batch.len), *self._cache(layer), P(k), n, P(v), n, batch.total, self.seqs, self.hkv, self.d,
@@ -175,6 +183,7 @@ class KvCache:
         import torch
 
         n, P = self.hq * self.d, dramamoe.ptr
+        self._check_batch(batch)
         self._check(q, batch.total, n, (torch.bfloat16,), "q")
         if gate is not None:
             self._check(gate, batch.total, n, (torch.float32,), "gate")
