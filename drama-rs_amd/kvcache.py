@@ -106,16 +106,19 @@ class KvCache:
             need.append((self.lens[i] + n + BLOCK - 1) // BLOCK - len(self.held[i]))
         if sum(need) > len(self.free_pages):
             raise MemoryError(f"{sum(need)} pages needed, {len(self.free_pages)} free")
-        at, new = [], []
-        for i, k in enumerate(need):
-            for _ in range(k):
-                at.append(i * self.maxp + len(self.held[i]))
-                self.held[i].append(self.free_pages.pop())
-                new.append(self.held[i][-1])
-            self.lens[i] += rows[i]
+        # what can fail comes before what is counted
+        lens = [m + n for m, n in zip(self.lens, rows)]
+        batch = Batch(rows, lens, self.device)
+        new = self.free_pages[len(self.free_pages) - sum(need):][::-1]
+        at = [i * self.maxp + len(self.held[i]) + k for i in range(self.seqs) for k in range(need[i])]
         if at:
             self.table.view(-1)[torch.tensor(at, device=self.device)] = torch.tensor(new, dtype=torch.int32, device=self.device)
-        return Batch(rows, self.lens, self.device)
+            del self.free_pages[-len(new):]
+        pages = iter(new)
+        for i, k in enumerate(need):
+            self.held[i] += [next(pages) for _ in range(k)]
+        self.lens = lens
+        return batch
 
     def truncate(self, seq: int, length: int) -> None:
         """Keeps the first ``length`` tokens of a sequence and gives back the pages behind them (0: all; drafted tokens that were refused).

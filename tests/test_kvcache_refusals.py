@@ -14,3 +14,25 @@ def test_batch_of_another_cache():
         for call in (lambda: c.append(0, kv, kv, other), lambda: c.read(0, other), lambda: c.attend(0, q, other)):
             with pytest.raises(ValueError, match="batch"):
                 call()
+
+
+@pytest.mark.parametrize("fails", ["Batch", "table"])
+def test_step_that_fails_leaves_the_cache_as_it_was(monkeypatch, fails):
+    """No memory for what a step makes on the device: no token is counted and no page taken."""
+    c = cache()
+    c.step([65, 0, 1])
+    before = (list(c.lens), c.table.clone(), list(c.free_pages), [list(h) for h in c.held])
+
+    def full(*a, **k):
+        raise MemoryError("no room")
+
+    with monkeypatch.context() as m:
+        if fails == "Batch":
+            m.setattr(K, "Batch", full)
+        else:
+            m.setattr(torch, "tensor", full)
+        with pytest.raises(MemoryError, match="no room"):
+            c.step([10, 64, 70])
+    assert (c.lens, c.free_pages, c.held) == (before[0], before[2], before[3]) and torch.equal(c.table, before[1])
+    b = c.step([10, 64, 70])
+    assert b.len.tolist() == [75, 64, 71] and c.table.tolist() == [[0, 1, -1, -1], [3, -1, -1, -1], [2, 4, -1, -1]]
