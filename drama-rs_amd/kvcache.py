@@ -48,6 +48,11 @@ def rope_freq(rot: int, theta: float = 10000.0, scaling: str | None = None, fact
     return f.float().to(device or "cpu"), mscale
 
 
+def _check_rows(t, rows, width, dtypes, device, what):
+    if t.device != device or t.dtype not in dtypes or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != width or t.stride(1) != 1:
+        raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device}, expected [{rows}, {width}] of {dtypes} on {device}")
+
+
 class Batch:
     """New rows of a call: sequence i has rows start[i] .. start[i + 1] - 1, len[i] tokens with them, row r the position pos[r]."""
 
@@ -134,8 +139,7 @@ class KvCache:
     # ---- what runs on the device ----
 
     def _check(self, t, rows, width, dtypes, what):
-        if t.device != self.device or t.dtype not in dtypes or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != width or t.stride(1) != 1:
-            raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device}, expected [{rows}, {width}] of {dtypes} on {self.device}")
+        _check_rows(t, rows, width, dtypes, self.device, what)
 
     def _check_batch(self, batch):
         # the kernels read start and len of every sequence of the cache
@@ -178,9 +182,12 @@ class KvCache:
                                  dramamoe.stream_ptr())
         return k, v
 
-    def attend(self, layer: int, q, batch: Batch, scale: float | None = None, gate=None, out=None, max_len: int | None = None):
+    def attend(self, layer: int, q, batch: Batch, scale: float | None = None, gate=None, out=None, max_len: int | None = None,
+               gate_stride: int | None = None):
         """Attention of the batch's rows (their tokens appended before) over ``layer``: q bf16 [batch.total, hq * d], gate None or f32 of
-        that shape, -> bf16 of that shape (``out``, which may be q).  scale: d ** -0.5.  max_len: a captured call that is replayed while the
+        that shape, -> bf16 of that shape (``out``, which may be q).  scale: d ** -0.5.  gate_stride: elements from a head's gate to the next
+        one's, d where the heads' gates lie side by side; 2 * d where each lies beside its query: gate is then the projection's [batch.total, (2 hq - 1) d]
+        from the first gate on.  max_len: a captured call that is replayed while the
         sequences grow takes their final length here.  Captured calls keep the stream's workspace: graphs that may run at the same
         time are captured on streams of their own."""
         import torch
@@ -189,7 +196,8 @@ class KvCache:
         self._check_batch(batch)
         self._check(q, batch.total, n, (torch.bfloat16,), "q")
         if gate is not None:
-            self._check(gate, batch.total, n, (torch.float32,), "gate")
+            hsg = self.d if gate_stride is None else gate_stride
+            self._check(gate, batch.total, (self.hq - 1) * hsg + self.d, (torch.float32,), "gate")
         if out is not None:
             self._check(out, batch.total, n, (torch.bfloat16,), "out")
         longest = batch.max_len if max_len is None else max_len
@@ -208,14 +216,15 @@ class KvCache:
                     self._old.append(ws)
                 ws = self._ws[st] = torch.empty(size, dtype=torch.uint8, device=self.device)
             self.lib.dr_attn_kv8(q.data_ptr(), q.stride(0), P(batch.start), P(batch.len), *self._cache(layer), self.d ** -0.5 if scale is None else scale,
-                                 None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), self.d, P(ws), out.data_ptr(),
+                                 None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), 0 if gate is None else hsg, P(ws), out.data_ptr(),
                                  out.stride(0), batch.total, self.seqs, batch.max_rows, longest, self.hq, self.hkv, self.d, st)
         return out
 
 
 def rope(x, heads: int, d: int, pos, freq, mscale: float = 1.0, layout: int = HALF, nw=None, eps: float = 1e-6, head_stride: int | None = None,
-         f32: bool = False):
-    """dr_rope on x (f32 or bf16, rows of ``heads`` heads head_stride or d elements apart): bf16 [rows, heads * d], f32 where ``f32``.  nw
+         f32: bool = False, out=None):
+    """dr_rope on x (f32 or bf16, rows of ``heads`` heads head_stride or d elements apart): bf16 [rows, heads * d], f32 where ``f32``, or into ``out`` (f32
+    or bf16 of that shape; x itself where its heads lie side by side and the types are the same).  nw
     None, or f32 [d] or [heads, d]; freq f32 [rot / 2], of which the first rot elements of a head are turned."""
     import torch
 
@@ -228,10 +237,15 @@ def rope(x, heads: int, d: int, pos, freq, mscale: float = 1.0, layout: int = HA
         raise ValueError("nw f32 [d] or [heads, d]")
     if any(t is not None and t.device != x.device for t in (pos, freq, nw)):
         raise ValueError("pos, freq and nw on the device of x")
+    if out is not None:
+        _check_rows(out, x.shape[0], n, (torch.float32, torch.bfloat16), x.device, "out")
+        f32 = out.dtype == torch.float32
     lib = dramamoe.lib()
     f = lib.dr_rope_bf16 if x.dtype == torch.bfloat16 else lib.dr_rope
     with torch.cuda.device(x.device):
-        out = torch.empty(x.shape[0], n, dtype=torch.float32 if f32 else torch.bfloat16, device=x.device)
+        if out is None:
+            out = torch.empty(x.shape[0], n, dtype=torch.float32 if f32 else torch.bfloat16, device=x.device)
+        y, ldy = out.data_ptr(), out.stride(0)
         f(x.data_ptr(), x.stride(0), hs, P(nw), 0 if nw is None or nw.numel() == d else d, eps, P(pos), P(freq), mscale, layout,
-          P(out) if f32 else None, n, None if f32 else P(out), n, x.shape[0], heads, d, 2 * freq.numel(), dramamoe.stream_ptr())
+          y if f32 else None, ldy, None if f32 else y, ldy, x.shape[0], heads, d, 2 * freq.numel(), dramamoe.stream_ptr())
     return out

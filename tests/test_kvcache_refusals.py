@@ -36,3 +36,15 @@ def test_step_that_fails_leaves_the_cache_as_it_was(monkeypatch, fails):
     assert (c.lens, c.free_pages, c.held) == (before[0], before[2], before[3]) and torch.equal(c.table, before[1])
     b = c.step([10, 64, 70])
     assert b.len.tolist() == [75, 64, 71] and c.table.tolist() == [[0, 1, -1, -1], [3, -1, -1, -1], [2, 4, -1, -1]]
+
+
+def test_outputs_and_gates_that_do_not_fit():
+    c = cache()
+    b = c.step([2, 1, 0])
+    q, x = torch.zeros(3, 128, dtype=torch.bfloat16), torch.zeros(3, 64)
+    for gate, stride in ((torch.zeros(3, 256), 64), (torch.zeros(3, 223), 64), (torch.zeros(3, 224), None), (torch.zeros(2, 224), 64), (torch.zeros(3, 224).double(), 64), (torch.zeros(224, 3).t(), 64)):
+        with pytest.raises(ValueError, match="gate"):
+            c.attend(0, q, b, gate=gate, gate_stride=stride)
+    for out in (torch.zeros(2, 64), torch.zeros(3, 63), torch.zeros(3, 64).half(), torch.zeros(64, 3).t(), torch.zeros(3, 1, 64)):
+        with pytest.raises(ValueError, match="out"):
+            K.rope(x, 2, 32, b.pos, torch.zeros(8), out=out)
