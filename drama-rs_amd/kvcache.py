@@ -213,7 +213,9 @@ class KvCache:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("call attend once on this stream, with as many rows and tokens, before capturing it")
                 if ws is not None:
+                    # at least doubled, so that all that were outgrown together are smaller than the one in use
                     self._old.append(ws)
+                    size = max(size, 2 * ws.numel())
                 ws = self._ws[st] = torch.empty(size, dtype=torch.uint8, device=self.device)
             self.lib.dr_attn_kv8(q.data_ptr(), q.stride(0), P(batch.start), P(batch.len), *self._cache(layer), self.d ** -0.5 if scale is None else scale,
                                  None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), 0 if gate is None else hsg, P(ws), out.data_ptr(),

@@ -113,3 +113,20 @@ def test_captured_step_of_an_attention_layer():
         torch.cuda.synchronize()
         for g, w in zip(got, (q, k, y, e.kq, e.vq, e.ks, e.vs)):
             assert torch.equal(g, w), n
+
+
+def test_outgrown_workspaces_stay_small():
+    """Captured calls may use them, so they are kept: all together they are smaller than the one in use, however slowly the calls grow."""
+    import torch
+
+    c = K.KvCache(1, 70, 64, 5000, 16, 1, 64)
+    sizes = set()
+    for n in range(1, 65):
+        b = c.step([int(i < n) for i in range(64)])
+        q = torch.randn(b.total, 16 * 64, device="cuda").to(torch.bfloat16)
+        c.attend(0, q, b, max_len=5000)
+        ws = c._ws[torch.cuda.current_stream().cuda_stream]
+        sizes.add(ws.numel())
+        assert sum(o.numel() for o in c._old) < ws.numel(), n
+    assert len(c._old) >= 3 and len(sizes) == len(c._old) + 1
+    torch.cuda.synchronize()
