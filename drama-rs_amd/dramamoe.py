@@ -126,14 +126,21 @@ def lib() -> Lib:
     return _lib
 
 
+_raw_stream = None
+
+
 def stream_ptr(stream=None) -> int:
     """Handle of a torch stream, of the current device's current one by default."""
     import torch
 
     if stream is not None:
         return stream.cuda_stream
-    # torch.cuda.current_stream().cuda_stream without the object in between: 0.4 us for 2.8, of the 8 that a small call took
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    # torch.cuda.current_stream().cuda_stream without the object in between: 0.4 us for 2.8, of the 8 that a small call took.  torch does not
+    # promise the direct call, so the object stands in where it is gone.
+    global _raw_stream
+    if _raw_stream is None:
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return _raw_stream(torch.cuda.current_device())
 
 
 def ptr(t) -> int | None:
