@@ -15,6 +15,7 @@
 // Two kernels.  Few columns (a decode step): a wave walks over cached blocks by itself with no barrier, the next block's bytes requested as soon
 // as this one's are used.  Many (prompts): a block's bytes are converted once for all waves, in LDS.  Where the columns alone leave CUs
 // idle the cached blocks are split over blocks of threads, whose sums (fp32) a second launch joins.  plan() chooses.
+#include "attn_plan.hpp"
 #include "kv8.hpp"
 
 using namespace drm;
@@ -26,7 +27,8 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int W = 4, NT = W * WAVE;
+constexpr int W = kPlanWaves, NT = W * WAVE;
+static_assert(KB == kPlanBlock, "the plan's blocks are the cache's");
 constexpr float kInf = __builtin_inff();
 constexpr float kLow = -__FLT_MAX__;  // the maximum of scores that all lie below fp32's range (none seen: -infinity)
 constexpr int kUnit = -200;  // an exponent below that of any scale
@@ -817,7 +819,6 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
 // Joins the parts of a row's query, or of 4 LE elements of it where the queries are few: G groups of LE lanes of four elements, each group every
 // G'th part, eight at a time in flight, with a maximum of its own; the groups meet in LDS.  As many queries a block as that
 // leaves room for.  A launch and two rounds of loads: 4 to 5 us for all of the above.
-constexpr int kSplits = 128;  // at most
 constexpr int kJoin = 8;      // parts of a group in flight
 __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
   __shared__ __align__(16) f32x4 so[NT];
@@ -882,86 +883,6 @@ __global__ void __launch_bounds__(NT) k_attn_join(Attn a, int LE, int G) {
     m = mn;
   }
   if (on && grp == 0 && !whole) Out(a, true, 0, row, 0, head, s, m, false).put(e, v, gate);
-}
-
-// Rows of a part (part_of()).
-int part_rows(int rows, int seqs, int max_rows) { return (long long)seqs * max_rows < rows ? seqs * max_rows : rows; }
-
-// How a call is cut: by its sizes alone, so that the workspace is known before.
-struct Plan {
-  bool few, scan, fold;
-  int mt, cols, nw, splits, chunk;
-  long long tiles;
-};
-Plan plan(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d) {
-  Plan p;
-  const long long g = hq / hkv, pairs = (max_rows < rows ? max_rows : rows) * g, blocks = ((long long)max_len + KB - 1) / KB, items = (long long)part_rows(rows, seqs, max_rows) * hq;
-  // Few columns: each block of threads 16 or 32 pairs of a cached head and sequence.
-  p.mt = pairs <= 16 || d > 128 ? 1 : 2;
-  const long long cols = (pairs + 16 * p.mt - 1) / (16 * p.mt), room = rows * g / (16 * p.mt) + seqs, few = (cols * seqs < room ? cols * seqs : room) * hkv;
-  // Many: tiles of 128 or 256 pairs; where sequences have several, of all rows together.  Eight waves only where a tile fills them and the tiles
-  // most of the card (16 heads of 128, 2 cached; behind 8192 tokens 2800 rows 254 us with eight, 283 with four, 2100 215 and 203).
-  auto cut = [&](int nw) {
-    const long long tp = 32 * nw, per = (pairs + tp - 1) / tp, all = rows * g / tp + seqs;
-    p.nw = nw, p.scan = per > 1, p.tiles = per > 1 && all < per * seqs ? all : per * seqs;
-  };
-  cut(8);
-  if (d > 128 || pairs <= 128 || p.tiles * hkv < 176) cut(4);
-  // us: rounds of the blocks that the card holds, each a start and its steps, `at` cached blocks a step; with splits a launch that joins, and the
-  // parts out and back.  The constants are what single rounds took.  What the rule gives, and the other side:
-  //   in few columns  3 sequences of 1000 tokens with 72 pairs of d 256 14.7 us (split tiles 26, whole ones 58), 8 of 500 with 192 pairs of d 64
-  //                   9.1 (15.6), 7 of 33 to 373 with as many pairs of d 64 10.8 (13.2);
-  //   in tiles        49 of 2000 with 122 pairs of d 128 25 (30), 12 of 420 to 3900 with 318 pairs of d 96 65 (94), 30 of 40 with 120 pairs of d 256
-  //                   21 (32), 63 of 10 with 40 pairs of d 112 9.5 (15.7).
-  struct Cut {
-    long long s;
-    float us;
-  };
-  const float part = (float)items * d * 8 / 3e6f;
-  auto best = [&](long long units, int holds, int at, float start, float step) {
-    Cut c{1, 3e38f};
-    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
-      if (s > 1 && s * at > blocks) break;
-      // up to d 128 a CU takes a second block beside the first, so that half rounds count
-      const float rounds = d > 128 ? (float)((units * s + holds - 1) / holds) : units * s > holds ? .5f * (float)((2 * units * s + holds - 1) / holds) : 1.f;
-      const float us = rounds * (start + step * (float)((blocks + s * at - 1) / (s * at))) + (s > 1 ? 3.f + s * part : 0.f);
-      if (us < c.us) c = Cut{s, us};
-    }
-    return c;
-  };
-  Cut c;
-  const int holds = d <= 128 ? 512 : 256;  // blocks of few columns
-  if (pairs <= 32 || (pairs <= 64 && (blocks > 16 || 2 * few <= 3 * holds))) {
-    // With lengths apart a long sequence needs many splits (48 ragged sequences: blocks of threads up to 2048 57.5 us, to 1024 75; 32 of 8000
-    // tokens with heads of 256: to 512 62 us, to 2048 104).  Four waves walk over 16 blocks in less than a launch that joins takes.
-    const long long want = p.mt == 1 && d <= 128 ? 2048 : 512, most = (blocks + W - 1) / W;
-    p.few = true;
-    c.s = blocks <= 16 ? 1 : (want + few - 1) / few;
-    c.s = c.s > most ? most : c.s;
-    c.s = c.s > kSplits ? kSplits : c.s;
-  } else {
-    const float step = p.nw == 8 ? 1.6f : d <= 64 ? 1.f : d <= 128 ? 1.2f : d <= 192 ? 2.f : 2.8f;
-    c = best(p.tiles * hkv, 256, 1, d <= 128 ? 5.f : d <= 192 ? 8.f : 15.f, step);
-    const Cut f = best(few, holds, W, d <= 64 ? 4.f : 5.f, d <= 64 ? .7f : d <= 128 ? 1.8f : 2.9f);
-    // what either asks of L2, which the rounds leave out
-    const float each = blocks * KB * 2 * d / 8e6f;
-    p.few = pairs <= 2048 && f.us + each * few < c.us + each * p.tiles * hkv;
-    if (p.few) c = f;
-  }
-  if (p.few) p.scan = false, p.tiles = seqs;
-  p.cols = p.few ? (int)cols : 1;
-  p.splits = c.s < 1 || items >= 1 << 22 ? 1 : (int)c.s;  // with so many rows most are of no sequence, or there are blocks enough
-  p.chunk = (int)((blocks + p.splits - 1) / p.splits);
-  if (p.few) {
-    // as many blocks for each of the waves (16 sequences of 1000 to 5000 tokens, 8 heads of 128: 24.6 us, 29.6 with chunks of any number)
-    p.chunk = p.chunk < W ? W : (p.chunk + W - 1) / W * W;
-    p.splits = blocks > p.chunk ? (int)((blocks + p.chunk - 1) / p.chunk) : 1;
-  }
-  if (p.chunk < 1) p.chunk = 1;
-  // Where all tiles run at once the last rows' take longest: folding gives each as many steps as the next (4096 rows of 16 heads behind 8192 tokens
-  // 341 us, 352 without; 98 and 109 behind none).  With more tiles than that the next ones fill the gaps (8192 rows of 32 heads 538 without, 634 folded).
-  p.fold = !p.few && p.nw == 8 && p.splits == 1 && p.tiles * hkv <= 256;
-  return p;
 }
 
 bool attn_shape_ok(int rows, int seqs, int max_rows, int max_len, int hq, int hkv, int d) {
