@@ -67,7 +67,6 @@ DEV half8 to_half8(uint32_t a, uint32_t b) {
 
 DEV float quad_max(float v) { return xmax_step<32>(xmax_step<16>(v)); }
 DEV float quad_sum(float v) { return xsum_step<32>(xsum_step<16>(v)); }
-DEV float lane_f(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
 // What becomes of a row's query `head`: elements e .. e + 3, o: sum of exp(z - m) v, l: sum of exp(z - m), up to a common factor (no token seen:
 // both 0).  The finished output, or, not alone, a part of it to be joined; alone, an l of kAlone tells the launch that joins.
@@ -553,7 +552,7 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
   }
   const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
   float f = factor_of(w.qm * Pages::lane(pg.ks, k));  // as in soften()
-  const float lw = lane_f(kBase + Pages::lane(pg.lv, k) + (float)dv, 0);  // a scalar register
+  const float lw = Pages::lane(kBase + Pages::lane(pg.lv, k) + (float)dv, 0);  // a scalar register
   if (unew > w.unit) {
     const int sh = lim >= 0 ? w.unit - unew : 0;
     if (lim < 0) w.below += unew - w.unit;
