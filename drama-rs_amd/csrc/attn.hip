@@ -213,7 +213,8 @@ struct Pages {
 // The common weight, 2^fma(score, f, base) with base = lw - m (m: the maximum, lw: a weight at it), keeps the exact product beside a rounded m and
 // rounds lw - m once more: 2 2^-24 |m| in all, an eighth up to kFar, but octaves from 2^24 on, which lift weights past fp16 or sink the
 // largest to zero.  From kFar on a column's scores become their distances to m first, the product rounded as m was (0 at the maximum).  What that
-// costs the calls that never get there: nothing with few columns, 1 to 2% in tiles, 5% with heads of 256 (six more registers in memory).
+// costs the calls that never get there: nothing with few columns, up to 1% in tiles, 2% with
+// heads of 192 and 4% with heads of 256 (more registers in memory).
 DEV bool is_far(float m) { return fabsf(m) >= kFar && m > -kInf; }
 // A score's factor: above 0, so that what is hidden (-infinity) stays it with a k scale of 0, and below infinity, so that a product of nothing
 // stays 0.  The words of positive floats are in their order.
@@ -552,7 +553,6 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
   }
   const int ve = __builtin_amdgcn_readlane(pg.ve, k), unew = w.unit > ve ? w.unit : ve, dv = ve - unew > -40 ? ve - unew : -40;
   float f = factor_of(w.qm * Pages::lane(pg.ks, k));  // as in soften()
-  const float lw = Pages::lane(kBase + Pages::lane(pg.lv, k) + (float)dv, 0);  // a scalar register
   if (unew > w.unit) {
     const int sh = lim >= 0 ? w.unit - unew : 0;
     if (lim < 0) w.below += unew - w.unit;
@@ -565,7 +565,7 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
     w.unit = unew;
   }
   if (!(pg.num >> k & 1) && lim >= 0) w.sum = __builtin_nanf("");  // scales that are no numbers
-  float add = 0.f, at = lw - (fabsf(w.m) >= kFar ? 0.f : w.m);
+  float add = 0.f, at = kBase + Pages::lane(pg.lv, k) + (float)dv - (fabsf(w.m) >= kFar ? -kInf : w.m);
   auto form = [&]() {
     add = 0.f;
 #pragma unroll
@@ -578,8 +578,8 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
       }
   };
   form();
-  // without a reference yet, or with one far from zero, the block's maximum is taken in any case
-  if (__any(!(add <= kMost) || (lim >= 0 && fabsf(w.m) >= kFar))) {
+  // without a reference yet, or with one far from zero, the weights above are infinite and the block's maximum is taken in any case
+  if (__any(!(add <= kMost))) {
     float mx = -kInf;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -590,19 +590,22 @@ DEV void soften32(Cols32<DC>& w, f32x16 (&sc)[2], half8 (&pf)[2][2], const Pages
     if (top > w.m) {
       // less than the reference stays as it is; without one (m -infinity) there are no sums to scale
       const float al = w.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(w.m - top);
-      w.m = top, at = lw - top;
+      w.m = top;
       w.sum *= al;
 #pragma unroll
       for (int u = 0; u < DC; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) w.o[u][r] *= al;
     }
+    int k2 = k, d2 = dv;  // worked out again: a value kept from above costs a register where there is none (heads of 256: 267 us, 274)
+    asm volatile("" : "+s"(k2), "+s"(d2));
+    at = kBase + Pages::lane(pg.lv, k2) + (float)d2 - (fabsf(w.m) >= kFar ? 0.f : w.m);
     if (is_far(w.m)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[t][r] = distance(sc[t][r], f, w.m);
-      f = 1.f, at = lw;
+      f = 1.f;
     }
     form();
   }
@@ -699,6 +702,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) k_attn_tiles(Attn a) {
   };
   Cols32<DC> w;
   begin32(w, a, s, w0, c1, qr);
+  if (w.pos < b0 * KB) w.m = 0.f;  // a column that sees none of the blocks asks for no reference
   if (cnt > 0) {
 #pragma unroll
     for (int f = 2 * PER; f < 4 * PER; ++f) put_part(-1, f);
