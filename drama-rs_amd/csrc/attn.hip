@@ -7,8 +7,8 @@
 // Stored bytes become fp16 exactly: byte u beside 0x64 is 1024 + u, less 1152 is q.  A query
 // (bf16) is fp16 times a power of two of its own that brings its largest element into [2^12, 2^13): exact down to 2^-29 of that
 // element, below it rounded by 2^-37 of it.  Weights are rounded to fp16 (2^-11 of each; the bf16 output is rounded by 2^-8) as
-// 2^15 exp(z - max) with few columns, 2^4 exp(z - reference) with many, so that at least those down to 2^-18 of the largest keep all their
-// bits and smaller ones are rounded by 2^-29 of it.  Running maximum, sums and both products
+// 2^15 exp(z - max) with few columns, 2^4 exp(z - reference) with many, so that at least those down to 2^-29 and 2^-18 of the largest keep all their
+// bits and smaller ones are rounded by 2^-40 and 2^-29 of it; in units of a power of two up to twice the largest v scale so far.  Running maximum, sums and both products
 // are fp32; a block's k scale multiplies its scores, its v scale joins the exponent, relative to a
 // power of two that no scale so far exceeds (a row's bits then do not turn on the scale of a block that it does not see).
 //
@@ -330,8 +330,8 @@ DEV void emit_none(const Attn& a, size_t part, int h, int sp, int c0, int c1, in
 // head may be part of one: what lies past d is loaded from inside the head, times zero queries, and not stored.  More pairs than a block of threads
 // holds are several blocks (z), which find the cache in L2.
 // Memory bounds it where sequences are long: 48 ragged sequences of 115191 tokens in all, 8 cached heads of 128, 216 MB in 53 us (4.1 TB/s), 32 of 8000
-// in 104 with the join (5.07 TB/s of 5.12 that a copy reaches); one of 60001 tokens with 2 heads of 256 is two to three blocks a wave,
-// 61 MB in 18.  7 prompts of 33 to 373 rows, 12 heads of 64: 10.8.  Short ones are a chain of loads (length and table, scales and bytes, LDS): 300 tokens 7.4 us, of which 3 to 4 are the launch.
+// in 104 with the join (5.07 TB/s of 5.12 that a copy reaches); one of 60001 tokens with 2 heads of 256 is two blocks a wave,
+// 61 MB in 18.  7 prompts of 33 to 373 rows, 12 heads of 64: 11.4.  Short ones are a chain of loads (length and table, scales and bytes, LDS): 300 tokens 7.4 us, of which 3 to 4 are the launch.
 template <int DC, int MT>
 __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
   constexpr int TP = 16 * MT, LD = 64 * DC + 4;
@@ -470,12 +470,12 @@ __global__ void __launch_bounds__(NT, DC <= 2 ? 2 : 1) k_attn_few(Attn a) {
 // What bounds it is the vector unit, which a product keeps for 10 to 12 cycles whatever its size: hence 32 x 32 x 16 products, and a
 // softmax without a maximum where it can be: a column's reference is the maximum of an earlier block, and only where a lane's sum says that a
 // weight may have passed fp16 (or the column has no reference yet) is the block's maximum taken, O rescaled and the weights formed again.
-// 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 330 to 341 us, 1.01 to 1.04 PFLOP/s (a large library product in fp16: 1.33); the matrix
-// unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 515 us (1.06),
-// heads of 64 108 us (0.64: the softmax is as long for half the products), of 256 256 us for 2048 rows on 6144 (0.67: four waves a CU,
-// no other wave's products beside a softmax, and 142 of a lane's registers in memory, which are read where a turn or the epilogue starts).
+// 4096 rows of 16 heads of 128 behind 8192 tokens (2 cached heads): 335 to 346 us, 0.99 to 1.03 PFLOP/s (a large library product in fp16: 1.33); the matrix
+// unit is busy 40% of the time, the vector unit's own instructions and what products keep it for take the rest.  8192 rows of 32 heads 533 us (1.03),
+// heads of 64 108 us (0.64: the softmax is as long for half the products), of 256 267 us for 2048 rows on 6144 (0.64: four waves a CU,
+// no other wave's products beside a softmax, and 147 of a lane's registers in memory, which are read where a turn or the epilogue starts).
 // Short prompts are steps of 1 to 1.2 us (2.8 with heads of 256) behind a start of 5 (15), most of it the fetch of code that runs once: 1000 rows
-// of 32 heads of 128 28.7 us.
+// of 32 heads of 128 29.8 us.
 template <int DC>
 struct Cols32 {
   half8 q[2 * DC];   // 32-element chunk i, half y: elements 32 i + 16 (l >> 5) + 8 y + (0 .. 7), times a power of two

@@ -349,7 +349,10 @@ int append(const Append& a, int ldk, int ldv, hipStream_t st) {
   if (a.c.rows == 0 || a.c.seqs == 0) return 0;
   if (!kv8_buffers_ok(a.c) || !a.k || !a.v || ((uintptr_t)a.k & 15) || ((uintptr_t)a.v & 15)) return -1;
   const unsigned nb = (unsigned)max_blocks(a.c.rows, a.c.seqs);
-  // a wave walks four rows at a time: more than four a sequence are left to a block of threads
+  // A wave walks four rows at a time: more than four a sequence are left to a block of threads.  Kernels alone, us, a wave and (a block of threads), 8 heads of
+  // 128 in bf16: 64 tokens of as many sequences 4.5 (12.8), 32 x 4 5.7 (11.5), 32 x 6 7.2 (11.6), 1 x 5 5.8 (7.8), 1 x 20 14.6 (7.3); 2 heads of 256 in fp32: 32 x 4 5.1
+  // (6.4), 32 x 6 7.0 (6.6), 16 x 8 8.7 (6.5).  The rule knows the average alone: a prompt of 512 rows beside 63 single tokens takes a block of threads, 15.4
+  // (53), beside 200 a wave, 56 (44; 2 heads of 256 60, 16), where a choice by each block of the cache would take both.
   if (a.c.rows <= 4ll * a.c.seqs) hipLaunchKernelGGL((k_kv8_append_few<B16>), dim3(nb, (2 * a.c.hkv + 3) / 4), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((k_kv8_append<B16>), dim3(nb, 2 * a.c.hkv), dim3(NT), 0, st, a);
   return 0;

@@ -127,7 +127,9 @@ class KvCache:
 
     def truncate(self, seq: int, length: int) -> None:
         """Keeps the first ``length`` tokens of a sequence and gives back the pages behind them (0: all; drafted tokens that were refused).
-        Pages given back may be taken by the next ``step``: calls over them must have been issued to the same stream."""
+        Pages given back may be taken by the next ``step``: calls over them must have been issued to the same stream.  A block that is kept in
+        part keeps what the tokens taken back made of it: a scale that they made grow, with the kept tokens' integers rounded to it, and NaN where
+        one of them was no number.  Where that matters, drafts are kept from the cache until they are accepted."""
         if not 0 <= length <= self.lens[seq]:
             raise ValueError(f"sequence {seq} has {self.lens[seq]} tokens, not {length}")
         keep = (length + BLOCK - 1) // BLOCK

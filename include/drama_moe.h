@@ -505,7 +505,8 @@ int dr_rope_bf16(const dr_bf16* x, int ldx, int hsx, const float* nw, int ldn, f
  * dr_kv8_append: the rows' k and v (f32, or bf16 for _bf16; head h of row r at r * ldk + h * d) become their tokens.  A block whose first
  * token is in the call gets the scale fl(A / 127), A the largest magnitude of the call's tokens in it; one that holds tokens
  * already keeps its scale, doubled as often as A > 127 scale asks, its integers then rounded to the new step (together less
- * than one step off, however often that happens).  Integers are round(x / scale), half to even, from the exact quotient.  An infinity or NaN gives the block, all its
+ * than one step off, however often that happens).  That holds for tokens that a caller then takes back (refused drafts, other rows at the same
+ * positions) too: the block keeps the scale that they made it grow to, or their NaN, until a call begins it anew.  Integers are round(x / scale), half to even, from the exact quotient.  An infinity or NaN gives the block, all its
  * tokens, the scale NaN.  Appending the same rows again changes nothing.  Places of a block behind its last token hold nothing of use.
  * dr_kv8_read: the reverse, k and v f32 of the rows' tokens (0 for a row that is none or whose block is not there).
  * Unsupported: rows or seqs < 0 or > 1048576, hkv < 1 or > 1024, d < 16, > 256 or no multiple of 16, maxp < 1 or >= 33554432, pages < 1, ldk or ldv below hkv d or
@@ -526,8 +527,8 @@ int dr_kv8_read(const int* start, const int* len, const int* table, int maxp, co
  * infinity of its sign: NaN for the row's query where one is positive or all that it sees are negative.
  * max_rows: no sequence has more rows (what y then holds for rows past it is undefined); max_len: the longest sequence, as far as the host knows it (a longer one
  * is computed as well).  The cut into blocks goes by these, so a graph that is replayed for growing sequences takes their final values.
- * Scores, softmax and sums are fp32; weights, times their block's v scale, enter the product with v in fp16: 2^-11 of each, and at most 2^-29
- * of the largest weight times the largest v scale that the row sees.
+ * Scores, softmax and sums are fp32; weights, times their block's v scale, enter the product with v in fp16: 2^-11 of each, and at most 2^-28
+ * (2^-39 with few rows) of the largest weight times the largest v scale that the row sees, for each token and unit of its integer.
  * ws: dr_attn_kv8_ws(same sizes) bytes of scratch, holding anything, a multiple of 16 bytes.  Calls that share ws must not overlap (two graphs that may run at once need one each).
  * Unsupported: as above, and a scale that is infinite or NaN, hq > 1024 or no multiple of hkv, max_rows or max_len < 0, 2^23 or more tiles of (rows, queries) of a cached
  * head and sequence (at least one for each of them), ldq < hq d or no multiple of 8, ldy < hq d or
