@@ -228,8 +228,7 @@ class KvCache:
 def rope(x, heads: int, d: int, pos, freq, mscale: float = 1.0, layout: int = HALF, nw=None, eps: float = 1e-6, head_stride: int | None = None,
          f32: bool = False, out=None):
     """dr_rope on x (f32 or bf16, rows of ``heads`` heads head_stride or d elements apart): bf16 [rows, heads * d], f32 where ``f32``, or into ``out`` (f32
-    or bf16 of that shape; x itself where its heads lie side by side and the types are the same).  nw
-    None, or f32 [d] or [heads, d]; freq f32 [rot / 2], of which the first rot elements of a head are turned."""
+    or bf16 of that shape; x itself where its heads lie side by side and the types are the same).  nw None, or f32 [d] or [heads, d]; freq f32 [rot / 2], of which the first rot elements of a head are turned."""
     import torch
 
     P, hs, n = dramamoe.ptr, head_stride or d, heads * d
